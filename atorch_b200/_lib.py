@@ -52,12 +52,15 @@ SIGNATURES = {
     "atb_moe_gather_sum": "pppipiiip",
     "atb_moe_ungather": "ppppippiiip",
     "atb_row_intervals": "pppiiiipipiippiip",
+    "atb_kv4_append": "pppppppppiiiiiiiiillipp",
+    "atb_kv4_read": "pppppppiiiiiiilipp",
+    "atb_kv4_attention": "ppppppppiiiiiiiiilllfipp",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 _ctypes_launches = 0
 _NOT_LAUNCHES = {"atb_norm_bwd_parts", "atb_sumsq_parts", "atb_set_comm_wait_ns", "atb_noalloc_max_n",
-                 "atb_embedding_bwd_scratch"}
+                 "atb_embedding_bwd_scratch", "atb_kv4_partial_rows"}
 
 
 def __getattr__(name):
@@ -199,7 +202,8 @@ def check_status(device: torch.device) -> None:
     v = int(t.item())
     if v != 0:
         t.zero_()
-        raise KernelError(f"kernel status {v} (1 = wait timeout, 3 = TMEM allocation, 4 = peer timeout)")
+        raise KernelError(f"kernel status {v} (1 = wait timeout, 3 = TMEM allocation, 4 = peer timeout, "
+                          "5 = an index in device memory out of range)")
 
 
 DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}

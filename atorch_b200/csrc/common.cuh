@@ -26,6 +26,7 @@ enum AtbStatus : int {
   ATB_ERR_BAD_ARG = 2,        // launcher rejected the arguments
   ATB_ERR_TMEM_ALLOC = 3,
   ATB_ERR_PEER_TIMEOUT = 4,   // a peer flag was never set
+  ATB_ERR_BAD_INDEX = 5,      // an index in device memory (page, position, parent) is out of range
 };
 
 namespace atb {

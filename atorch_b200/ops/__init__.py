@@ -11,6 +11,8 @@ from .embedding import embedding
 from .cross_entropy import cross_entropy, cross_entropy_reference
 from .optim import (adamw_step, adamw_reference, agd_step, agd_reference, sum_squares, outer_sgd_step,
                     outer_sgd_reference)
+from .kv4 import (KV4Cache, kv4_append, kv4_append_reference, kv4_attention, kv4_attention_reference, kv4_read,
+                  kv4_read_reference)
 from .attention import attention, attention_reference, build_dense_mask
 
 __all__ = [n for n in dir() if not n.startswith("_")]
