@@ -52,6 +52,8 @@ SIGNATURES = {
     "atb_moe_gather_sum": "pppipiiip",
     "atb_moe_ungather": "ppppippiiip",
     "atb_row_intervals": "pppiiiipipiippiip",
+    "atb_w4_linear": "pppppiiiiliipp",
+    "atb_w4_expand": "pppiiiip",
     "atb_kv4_append": "pppppppppiiiiiiiiillipp",
     "atb_kv4_read": "pppppppiiiiiiilipp",
     "atb_kv4_attention": "ppppppppiiiiiiiiilllfipp",
