@@ -54,6 +54,8 @@ SIGNATURES = {
     "atb_row_intervals": "pppiiiipipiippiip",
     "atb_w4_linear": "pppppiiiiliipp",
     "atb_w4_expand": "pppiiiip",
+    "atb_beam_select": "ppppppppiiiliiiipp",
+    "atb_beam_reorder": "pppppiiiliiiiipp",
     "atb_kv4_append": "pppppppppiiiiiiiiillipp",
     "atb_kv4_read": "pppppppiiiiiiilipp",
     "atb_kv4_attention": "ppppppppiiiiiiiiilllfipp",

@@ -14,6 +14,7 @@ from .optim import (adamw_step, adamw_reference, agd_step, agd_reference, sum_sq
 from .kv4 import (KV4Cache, kv4_append, kv4_append_reference, kv4_attention, kv4_attention_reference, kv4_read,
                   kv4_read_reference)
 from .w4 import w4_dequantize, w4_linear, w4_linear_reference, w4_quantize
+from .beam import beam_reorder, beam_reorder_reference, beam_select, beam_select_reference
 from .attention import attention, attention_reference, build_dense_mask
 
 __all__ = [n for n in dir() if not n.startswith("_")]

@@ -1,0 +1,67 @@
+"""4-bit weights and beam search without a GPU: the plain implementations and the refusals."""
+import math
+
+import pytest
+import torch
+
+from atorch_b200 import ops
+
+
+@pytest.mark.parametrize("N,K,group", [(5, 64, 32), (3, 100, 64), (2, 1, 128), (7, 257, 128)])
+def test_weights_come_back_and_multiply(N, K, group):
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(K))
+    codes, scales = ops.w4_quantize(w, group)
+    assert codes.shape == (N, -(-K // 32) * 16) and scales.shape == (N, -(-K // group))
+    got = ops.w4_dequantize(codes, scales, K, group)
+    assert ((got - w).abs() <= scales.float().repeat_interleave(group, 1)[:, :K] * (0.5 + 7 / 256)).all()
+    x, b = torch.randn(2, 3, K).half(), torch.randn(N).half()
+    y = ops.w4_linear(x, codes, scales, group, b)
+    assert torch.allclose(y.float(), x.float() @ got.t() + b.float(), atol=2e-2, rtol=2e-3)
+    with pytest.raises(ValueError):
+        ops.w4_linear(x.float(), codes, scales, group)
+    with pytest.raises(RuntimeError):
+        ops.w4_linear(x.clone().requires_grad_(), codes, scales, group)
+
+
+def test_select_is_a_sort_of_all_continuations():
+    g = torch.Generator().manual_seed(0)
+    logits, scores = torch.randn(3, 4, 50, generator=g), torch.randn(3, 4, generator=g)
+    finished = torch.tensor([[False, True, False, False]] * 3)
+    got, tokens, parents, ended = ops.beam_select(logits, scores, finished, 7, 6)
+    for b in range(3):
+        every = []
+        lse = torch.logsumexp(logits[b].double(), -1)
+        for w in range(4):
+            for v in range(50):
+                f = scores[b, w].double() + (logits[b, w, v].double() - lse[w])
+                if finished[b, w]:
+                    f = scores[b, w].double() if v == 7 else torch.tensor(-math.inf)
+                every.append((-float(f), w, v))
+        every.sort()
+        assert [(w, v) for _, w, v in every[:6]] == list(zip(parents[b].tolist(), tokens[b].tolist()))
+        assert [v == 7 or w == 1 for _, w, v in every[:6]] == ended[b].tolist()
+        assert all(abs(f + s) < 1e-5 for (f, _, _), s in zip(every, got[b].tolist()))
+    with pytest.raises(ValueError):
+        ops.beam_select(logits, scores, finished)
+
+
+def test_reorder_moves_what_the_beams_hold():
+    """Before and after: row w reads what its parent read."""
+    cache = ops.KV4Cache(2, 12, 16, 1, 32)
+    g = torch.Generator().manual_seed(1)
+    table = torch.tensor([[0, 1, 5], [0, 2, 6], [0, 3, 7]], dtype=torch.int32)
+    n = 41
+    for i in range(2):
+        for w in range(3):
+            ops.kv4_append(cache.layer(i), table, torch.full((n,), w), torch.arange(n), torch.randn(n, 64, generator=g), 0)
+    pos = torch.arange(n)
+    held = [[ops.kv4_read(cache.layer(i), table, torch.full((n,), w), pos) for w in range(3)] for i in range(2)]
+    parents = torch.tensor([[2, 0, 0]], dtype=torch.int32)
+    ops.beam_reorder(cache.codes, cache.scales, table, torch.full((3,), n, dtype=torch.int32), parents)
+    assert table[:, 2].tolist() == [5, 6, 7]
+    for i in range(2):
+        for w in range(3):
+            k, v = ops.kv4_read(cache.layer(i), table, torch.full((n,), w), pos)
+            assert torch.equal(k, held[i][parents[0, w]][0]) and torch.equal(v, held[i][parents[0, w]][1])
+    with pytest.raises(IndexError):
+        ops.beam_reorder(cache.codes, cache.scales, table, torch.full((3,), n, dtype=torch.int32), parents + 1)
