@@ -58,13 +58,13 @@ SIGNATURES = {
     "atb_beam_reorder": "pppppiiiliiiiipp",
     "atb_kv4_append": "pppppppppiiiiiiiiillipp",
     "atb_kv4_read": "pppppppiiiiiiilipp",
-    "atb_kv4_attention": "ppppppppiiiiiiiiilllfipp",
+    "atb_kv4_attention": "ppppppppiiiiiiiilllfipp",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 _ctypes_launches = 0
 _NOT_LAUNCHES = {"atb_norm_bwd_parts", "atb_sumsq_parts", "atb_set_comm_wait_ns", "atb_noalloc_max_n",
-                 "atb_embedding_bwd_scratch", "atb_kv4_partial_rows"}
+                 "atb_embedding_bwd_scratch", "atb_kv4_attention_scratch"}
 
 
 def __getattr__(name):

@@ -5,6 +5,8 @@
 //   scales bf16  [pages][kv heads][page size][4]           scale and minimum of the key, scale and minimum of the value
 // A value is code * scale + minimum, one scale and minimum per token, head and tensor: (D + 8) bytes a token and head where
 // bf16 keeps 4 D. Sequence b's token p lies in page table[b][p / page size], place p % page size.
+#include <atomic>
+#include <type_traits>
 #include "common.cuh"
 
 namespace {
@@ -198,76 +200,75 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(T* k, T* v, Cache c, cons
 // Attention
 // ----------------------------------------------------------------------------------
 // Query i of sequence b's S newest tokens sees its keys j < lengths[b] - S + i + 1. The g query heads of a key/value head times
-// the S tokens are the columns of one matrix product: n = i g + h, in tiles of 8.
+// the S tokens are the columns of one matrix product: n = i g + h, in tiles of 8 or 16.
 //
-// The sequences are cut into chunks of equal length, as many as fill the GPU, by every block for itself from the lengths on the
-// device (they need not be known on the host); a block takes chunks of a head until there are none left. Sequences of one chunk
-// are finished in place, the others leave sums, maximum and denominator per chunk, which a second kernel joins in their order.
-constexpr int WARPS = 4, MIN_CHUNK = 64, TILE = 16;
+// The work is one row of units: the tiles of 32 tokens of a sequence, once per head and column tile, one sequence behind another.
+// Every block takes an equal run of it, which it finds for itself from the lengths on the device (they need not be known on the
+// host), so that long and short sequences fill the GPU alike. A run is cut into segments where a sequence (of a head) ends;
+// what a segment costs beside its tiles counts as START units before the first. A segment that is a whole sequence is finished
+// in place; of the others, the run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins in
+// the order of the blocks.
+constexpr int WARPS = 4, TILE = 32, START = 8;
 
-struct Plan {
-  int chunk;             // tokens, a multiple of MIN_CHUNK
-  long long chunks;      // of all sequences
-};
 ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
   const int n = lengths[b], most = c.width << c.page_shift;
   if (n > most) atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
   return max(0, min(n, most));
 }
-ATB_DEVICE int chunks_of(int n, int chunk) { return max(1, (n + chunk - 1) / chunk); }
+ATB_DEVICE int tiles_of(int n) { return max(1, (n + TILE - 1) / TILE); }     // an empty sequence has its zeros written
 ATB_DEVICE long long warp_sum_ll(long long v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-// `per`: blocks that a chunk occupies (heads x column tiles); `ctas`: blocks that the GPU is to be filled with
+
+struct Plan {
+  long long units;
+  int ctas;              // blocks with a run: run k is [k units / ctas, (k + 1) units / ctas)
+  ATB_DEVICE long long begin(long long k) const { return k * units / ctas; }
+  ATB_DEVICE int owner(long long u) const { return (int)(((u + 1) * ctas - 1) / units); }
+};
+// `per`: heads x column tiles. A run has a unit for every warp where there are enough.
 ATB_DEVICE Plan make_plan(const Cache& c, const int* lengths, int per, int ctas, int* status) {
-  const int lane = threadIdx.x & 31;
   long long total = 0;
-  for (int b = lane; b < c.rows; b += 32) total += seen_length(c, lengths, b, status);
-  total = warp_sum_ll(total);
-  const long long want = (total * per + ctas - 1) / ctas;
+  for (int b = threadIdx.x & 31; b < c.rows; b += 32) total += START + tiles_of(seen_length(c, lengths, b, status));
   Plan p;
-  p.chunk = (int)max((long long)MIN_CHUNK, (want + MIN_CHUNK - 1) / MIN_CHUNK * MIN_CHUNK);
-  long long n = 0;
-  for (int b = lane; b < c.rows; b += 32) n += chunks_of(seen_length(c, lengths, b, status), p.chunk);
-  p.chunks = warp_sum_ll(n);
+  p.units = warp_sum_ll(total) * per;
+  p.ctas = (int)max(1LL, min((long long)ctas, p.units / WARPS));
   return p;
 }
-// Sequence b of chunk number `w`, the chunk's place in it, and the number of the first partial result of b (only sequences of
-// several chunks have any). Computed by a whole warp.
-ATB_DEVICE void find_chunk(const Cache& c, const int* lengths, const Plan& p, long long w, int& b, int& place, int& of,
-                           int& len, long long& partial, int* status) {
+// Sequence of unit u, its length and its first unit. Computed by a whole warp.
+ATB_DEVICE void find_sequence(const Cache& c, const int* lengths, int per, long long u, int& b, int& len, long long& first,
+                              int* status) {
   const int lane = threadIdx.x & 31;
-  long long before = 0, before_partial = 0;
+  long long before = 0;
   for (int b0 = 0; b0 < c.rows; b0 += 32) {
     const int n = b0 + lane < c.rows ? seen_length(c, lengths, b0 + lane, status) : 0;
-    const int k = b0 + lane < c.rows ? chunks_of(n, p.chunk) : 0;
-    int sum = k, sum_partial = k > 1 ? k : 0;
+    const long long mine = b0 + lane < c.rows ? (long long)(START + tiles_of(n)) * per : 0;
+    long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, sum, o), y = __shfl_up_sync(0xffffffffu, sum_partial, o);
-      if (lane >= o) {
-        sum += x;
-        sum_partial += y;
-      }
+      const long long x = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += x;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, w < before + sum);
+    const unsigned hit = __ballot_sync(0xffffffffu, u < before + sum);
     if (hit) {
       const int src = __ffs(hit) - 1;
       b = b0 + src;
-      of = __shfl_sync(0xffffffffu, k, src);
       len = __shfl_sync(0xffffffffu, n, src);
-      place = (int)(w - before) - __shfl_sync(0xffffffffu, sum - k, src);
-      partial = before_partial + __shfl_sync(0xffffffffu, sum_partial, src) - (of > 1 ? of : 0);
+      first = before + __shfl_sync(0xffffffffu, sum - mine, src);
       return;
     }
     before += __shfl_sync(0xffffffffu, sum, 31);
-    before_partial += __shfl_sync(0xffffffffu, sum_partial, 31);
   }
-  b = -1;
 }
 
+// 16-byte pieces from global to shared memory by the copy unit (both addresses and the size multiples of 16)
+ATB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 ATB_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -297,12 +298,9 @@ ATB_DEVICE Words<WORDS> load_words(const void* p) {
     const uint2 u = *reinterpret_cast<const uint2*>(p);
     r.w[0] = u.x; r.w[1] = u.y;
   }
-  if constexpr (WORDS >= 4) {
-#pragma unroll
-    for (int i = 0; i < WORDS / 4; ++i) {
-      const uint4 u = reinterpret_cast<const uint4*>(p)[i];
-      r.w[4 * i] = u.x; r.w[4 * i + 1] = u.y; r.w[4 * i + 2] = u.z; r.w[4 * i + 3] = u.w;
-    }
+  if constexpr (WORDS == 4) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w;
   }
   return r;
 }
@@ -313,8 +311,8 @@ struct AttnArgs {
   const void* q;
   void* out;
   float* lse;                 // [rows][heads][S] or nullptr
-  float* partial;             // sums [..][D], then maximum and denominator [..][2]
-  long long partial_rows;
+  float* partial;             // sums [2 ctas][columns of a tile][D], then maximum and denominator [2 ctas][columns][2]
+  int2* owners;               // first and last block of each [row][head and column tile]
   long long q_batch, q_token; // strides of q, elements
   int S, heads, group;
   float scale_log2;           // softmax scale * log2(e)
@@ -330,35 +328,110 @@ struct AttnArgs {
 // q is scaled by a power of two to at most 2^15 before it is rounded to fp16 (bf16 and fp16 values stay exact down to 2^-29 of
 // the largest), p vs by 2^(15 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
 // 11 bits of it are kept, which is what the products with 4-bit codes can use. Sums, maxima and denominators are fp32.
+//
+// A warp has every fourth tile of a segment. Its tiles come through a ring of its own in shared memory, filled by the copy unit
+// STAGES tiles ahead. What bounds the kernel beside memory is the integer pipe: 5 operations for 8 codes of a key, 6 of a value.
+// So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and
+// only the tiles at a sequence's end are masked. Row i of 16 tokens' products is token order(i): a lane then reads its values'
+// words without a bank conflict worse than two ways.
+template <int D, int NT>
+struct Shape {
+  static constexpr int COLS = 8 * NT, STAGE = TILE * D + TILE * 8, STAGES = NT == 1 ? 2 : 4, RING = WARPS * STAGES * STAGE;
+  static constexpr int BLOCKS = NT == 1 ? 4 : 2;       // of an SM: 128 or 255 registers
+};
+ATB_DEVICE int order(int i) {
+  const int k = (i & 7) >> 1;
+  return (i & 8) + ((i & 1) ? (k ^ 1) + 4 : k);
+}
+
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
-  constexpr int KW = D / 32, VW = D / 64, COLS = 8 * NT, MT = D / 16;
-  __shared__ float sh_o[WARPS][COLS][D + 4];
+__global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attention_kernel(AttnArgs a) {
+  using Sh = Shape<D, NT>;
+  constexpr int KW = D / 32, VW = D / 64, COLS = Sh::COLS, MT = D / 16, STAGES = Sh::STAGES;
+  static_assert(WARPS * COLS * (D + 4) * 4 <= Sh::RING, "the warps' sums lie in the place of the ring");
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sh_m[WARPS][COLS], sh_l[WARPS][COLS];
+  __shared__ uint64_t bars[WARPS][STAGES];
+  __shared__ int abort_flag;
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
+  uint8_t* const ring = smem + warp * (STAGES * Sh::STAGE);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < STAGES) mbar_init(&bars[warp][lane], 1);
+  mbar_fence_init();
   grid_go();
   grid_wait();
   if (__syncthreads_or(threadIdx.x == 0 && *a.status != 0)) return;    // one answer for the block: others may fail meanwhile
-  const Cache& c = a.c;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
-  const int columns = a.S * a.group, tiles = (columns + COLS - 1) / COLS, per = tiles * c.kv_heads;
+  const int columns = a.S * a.group, col_tiles = (columns + COLS - 1) / COLS, per = col_tiles * c.kv_heads;
   const Plan plan = make_plan(c, a.lengths, per, a.ctas, a.status);
-  const int page_mask = (1 << c.page_shift) - 1;
+  if ((int)blockIdx.x >= plan.ctas) return;
+  const long long run = plan.begin(blockIdx.x), run_end = plan.begin(blockIdx.x + 1);
+  uint32_t loads = 0;            // tiles that this warp has taken from its ring
 
-  for (long long item = blockIdx.x; item < plan.chunks * per; item += gridDim.x) {
-    const long long w = item / per;
-    const int head = (int)(item - w * per) % c.kv_heads, tile = (int)(item - w * per) / c.kv_heads;
-    int b, place, of, len;
-    long long first_partial;
-    find_chunk(c, a.lengths, plan, w, b, place, of, len, first_partial, a.status);
-    const int t_begin = place * plan.chunk, t_end = min(len, t_begin + plan.chunk);
+  // A tile is two pieces of 16 tokens, each in one page, of three copies: keys, values, scales. Lane 3 p + x has copy x of piece p.
+  const int piece = lane / 3, what = lane - 3 * piece;
+  const bool copies = lane < 6;
+  const long long page_stride = ((what < 2 ? (long long)c.kv_heads * D : c.kv_heads * 8LL) << c.page_shift);
+  const int token_bytes = what < 2 ? D / 2 : 8;
+  const int dst_at = (what < 2 ? what * (TILE * D / 2) : TILE * D) + piece * 16 * token_bytes;
 
-    // queries: column 8 j + r, this lane's quarter of the dims; class-1 dims (odd places of a word) carry 2^-4
+  for (long long u = run; u < run_end;) {
+    int b, len;
+    long long first;
+    find_sequence(c, a.lengths, per, u, b, len, first, a.status);
+    const int tiles = tiles_of(len), hc = (int)((u - first) / (START + tiles));
+    const int head = hc % c.kv_heads, col_tile = hc / c.kv_heads;
+    const long long begin = first + (long long)hc * (START + tiles);       // of the sequence, for this head
+    const int t_first = max(0, (int)(u - begin) - START);                  // tiles of this segment
+    const int t_last = (int)min(run_end - begin - START, (long long)tiles);
+    u = begin + START + t_last;
+    if (t_last <= t_first) {      // the run ends before the first tile
+      u = run_end;
+      continue;
+    }
+    const bool whole = t_first == 0 && t_last == tiles;
+    if (t_first == 0 && threadIdx.x == 0)
+      a.owners[(long long)b * per + hc] = make_int2(blockIdx.x, plan.owner(begin + START + tiles - 1));
+    const int mine = len == 0 ? 0 : max(0, (t_last - t_first - warp + WARPS - 1) / WARPS);
+    const int* const row = c.table + b * c.table_stride;
+    const uint8_t* const src_at = what < 2 ? codes_at<D>(c, 0, what, head, 0) : reinterpret_cast<uint8_t*>(scales_at(c, 0, head, 0));
+
+    // pages of the warp's pieces 2 j to 2 j + 31: two of each tile
+    auto pages_from = [&](int j) {
+      const int t = (t_first + warp + (j + (lane >> 1)) * WARPS) * TILE + (lane & 1) * 16;
+      int page = 0;
+      if (j + (lane >> 1) < mine && t < len) {
+        page = row[t >> c.page_shift];
+        if (page < 0 || page >= c.pages) {
+          atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+          page = 0;
+        }
+      }
+      return page;
+    };
+    int pages = pages_from(0);
+    auto fetch = [&](int j) {      // by the whole warp: tile j into the ring
+      if (j >= mine) return;
+      if (j > 0 && (j & 15) == 0) pages = pages_from(j);
+      const int page = __shfl_sync(0xffffffffu, pages, (2 * j + piece) & 31);
+      const int t = (t_first + warp + j * WARPS) * TILE + piece * 16;
+      const uint32_t s = (loads + j) % STAGES;
+      const bool both = t - piece * 16 + 16 < len;         // the second piece may lie behind the sequence, and have no page
+      if (lane == 0) mbar_expect_tx(&bars[warp][s], both ? Sh::STAGE : Sh::STAGE / 2);
+      __syncwarp();
+      if (copies && t < len)
+        bulk_load(ring + s * Sh::STAGE + dst_at, src_at + page * page_stride + (t & ((1 << c.page_shift) - 1)) * token_bytes,
+                  16 * token_bytes, &bars[warp][s]);
+    };
+    for (int j = 0; j < STAGES; ++j) fetch(j);
+
+    // queries: column 8 j + r, this lane's quarter of the dims; odd places of a word carry 2^-4
     uint32_t qf[NT][KW][4];
     float cs[NT][2], bs[NT][2];      // factors of the products and sum(q) of the columns 8 j + 2 q4 + {0, 1}
     int limit[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      const int n = tile * COLS + 8 * j + r;
+      const int n = col_tile * COLS + 8 * j + r;
       const bool live = n < columns;
       const int i = live ? n / a.group : 0, h = live ? n - i * a.group : 0;
       const T* q = reinterpret_cast<const T*>(a.q) + b * a.q_batch + i * a.q_token +
@@ -398,12 +471,15 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
       for (int o = 0; o < 2; ++o) {
         cs[j][o] = __shfl_sync(0xffffffffu, back, (2 * q4 + o) * 4);
         bs[j][o] = __shfl_sync(0xffffffffu, sum, (2 * q4 + o) * 4);
-        const int col = tile * COLS + 8 * j + 2 * q4 + o;
-        limit[j][o] = min(t_end, len - a.S + col / a.group + 1);
+        const int col = col_tile * COLS + 8 * j + 2 * q4 + o;
+        limit[j][o] = min(len, len - a.S + col / a.group + 1);
       }
     }
+    const int all_see = len - a.S + col_tile * COLS / a.group + 1;      // tokens that every column of the tile sees
 
-    float o_acc[NT][MT][4], m[NT][2], l[NT][2], z[NT][2];
+    // running maximum of the scores (m), sums of p, of p times the values' minima and of p times their scaled codes; `ref` is what
+    // scores are taken relative to: m, or 0 where there is none yet
+    float o_acc[NT][MT][4], m[NT][2], ref[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -413,131 +489,148 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
         m[j][o] = -INFINITY;
-        l[j][o] = z[j][o] = 0.f;
+        ref[j][o] = l[j][o] = z[j][o] = 0.f;
       }
     }
     int top_e = 16;        // exponent field of the largest value scale so far
+    bool unset = true;     // whether a column has no maximum yet
 
-    for (int t0 = t_begin + warp * TILE; t0 < t_end; t0 += WARPS * TILE) {
-      int page = c.table[b * c.table_stride + (t0 >> c.page_shift)];
-      if (page < 0 || page >= c.pages) {
-        if (lane == 0) atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
-        page = 0;
-      }
-      const int slot = t0 & page_mask;
-      Words<KW> kc[2];
-      Words<VW> vc[4];
-      uint2 sc[2];
+    auto tile = [&](const uint8_t* src, int t0, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+      float s[2][NT][4];
+      float2 vs[4];
+      float over = 0.f;
+      int e_new = 0;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kc[i] = load_words<KW>(codes_at<D>(c, page, 0, head, slot + r + 8 * i) + q4 * (KW * 4));
-        sc[i] = *reinterpret_cast<const uint2*>(scales_at(c, page, head, slot + r + 8 * i));
-      }
+      for (int p = 0; p < 2; ++p) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vc[i] = load_words<VW>(codes_at<D>(c, page, 1, head, slot + 2 * q4 + (i & 1) + 8 * (i >> 1)) + r * (VW * 4));
-
-      float s[NT][4];
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+          for (int e = 0; e < 4; ++e) s[p][n][e] = 0.f;
+        const Words<KW> x = load_words<KW>(src + (16 * p + order(r)) * (D / 2) + q4 * (KW * 4));
+        const Words<KW> y = load_words<KW>(src + (16 * p + order(r) + 8) * (D / 2) + q4 * (KW * 4));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[j][e] = 0.f;
+        for (int k = 0; k < KW; ++k) {
+          const uint32_t xs = x.w[k] >> 8, ys = y.w[k] >> 8;
 #pragma unroll
-      for (int k = 0; k < KW; ++k) {
-        const uint32_t x = kc[0].w[k], y = kc[1].w[k], xs = x >> 8, ys = y >> 8;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          mma_f16(s[j], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, qf[j][k][0], qf[j][k][1]);
-          mma_f16(s[j], xs & 0x000F000Fu, ys & 0x000F000Fu, xs & 0x00F000F0u, ys & 0x00F000F0u, qf[j][k][2], qf[j][k][3]);
-        }
-      }
-
-      float2 ks[2], vs[2];
-      int e_new = top_e;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const bool in = t0 + r + 8 * i < t_end;       // places behind the last token hold anything
-        ks[i] = unpack_bf16x2(in ? sc[i].x : 0u);
-        vs[i] = unpack_bf16x2(in ? sc[i].y : 0u);
-        const int e = (__float_as_int(vs[i].x) >> 23) & 255;
-        e_new = max(e_new, e == 255 ? 0 : e);         // an infinity is not for the queries that do not see it
-      }
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
-
-      float m_new[NT][2];
-      bool moved = e_new != top_e;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          m_new[j][o] = m[j][o];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            float& x = s[j][2 * i + o];
-            x = t0 + r + 8 * i < limit[j][o] ? fmaf(ks[i].x, x * cs[j][o], ks[i].y * bs[j][o]) : -INFINITY;
-            m_new[j][o] = fmaxf(m_new[j][o], x);
+          for (int n = 0; n < NT; ++n) {
+            mma_f16(s[p][n], x.w[k] & 0x000F000Fu, y.w[k] & 0x000F000Fu, x.w[k] & 0x00F000F0u, y.w[k] & 0x00F000F0u,
+                    qf[n][k][0], qf[n][k][1]);
+            mma_f16(s[p][n], xs & 0x000F000Fu, ys & 0x000F000Fu, xs & 0x00F000F0u, ys & 0x00F000F0u, qf[n][k][2], qf[n][k][3]);
           }
+        }
 #pragma unroll
-          for (int k = 4; k < 32; k <<= 1) m_new[j][o] = fmaxf(m_new[j][o], __shfl_xor_sync(0xffffffffu, m_new[j][o], k));
-          moved = moved || m_new[j][o] != m[j][o];
+        for (int i = 0; i < 2; ++i) {
+          const int t = 16 * p + order(r) + 8 * i;
+          uint2 sc = *reinterpret_cast<const uint2*>(src + TILE * D + t * 8);
+          if (MASK && t0 + t >= len) sc = make_uint2(0u, 0u);           // places behind the last token hold anything
+          const float2 ks = unpack_bf16x2(sc.x);
+          vs[2 * p + i] = unpack_bf16x2(sc.y);
+          const int e = (sc.y >> 7) & 255;
+          e_new = max(e_new, e == 255 ? 0 : e);       // an infinity is not for the queries that do not see it
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              float& v = s[p][n][2 * i + o];
+              v = fmaf(ks.x * cs[n][o], v, fmaf(ks.y, bs[n][o], -ref[n][o]));
+              if (MASK && t0 + t >= limit[n][o]) v = -INFINITY;
+              over = fmaxf(over, v);
+            }
         }
       }
-      if (__any_sync(0xffffffffu, moved)) {
-        const float down = __int_as_float((127 + max(top_e - e_new, -126)) << 23);
+      if (__any_sync(0xffffffffu, over > 0.f || e_new > top_e || unset)) {
+        e_new = max(e_new, top_e);
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
+        const float down = __int_as_float((127 + max(top_e - e_new, -126)) << 23);
+        top_e = e_new;
+        unset = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
           float f[2];
 #pragma unroll
           for (int o = 0; o < 2; ++o) {
-            f[o] = m[j][o] == -INFINITY ? 0.f : fast_exp2(m[j][o] - m_new[j][o]);
-            l[j][o] *= f[o];
-            z[j][o] *= f[o];
-            m[j][o] = m_new[j][o];
+            float most = -INFINITY;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) most = fmaxf(most, fmaxf(s[p][n][o], s[p][n][2 + o]));
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
+            const float to = fmaxf(m[n][o], ref[n][o] + most), by = (to == -INFINITY ? 0.f : to) - ref[n][o];
+            f[o] = m[n][o] == -INFINITY ? 0.f : fast_exp2(-by);
+            m[n][o] = to;
+            ref[n][o] += by;
+            unset = unset || to == -INFINITY;
+            l[n][o] *= f[o];
+            z[n][o] *= f[o];
             f[o] *= down;
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {
+              s[p][n][o] -= by;
+              s[p][n][2 + o] -= by;
+            }
           }
 #pragma unroll
           for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o_acc[j][i][e] *= f[e & 1];
+            for (int e = 0; e < 4; ++e) o_acc[n][i][e] *= f[e & 1];
         }
-        top_e = e_new;
       }
       const float up = __int_as_float((268 - top_e) << 23);      // 2^15 / 2^(exponent + 1)
-      uint32_t pf[NT][2];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const float ref[2] = {m[j][0] == -INFINITY ? 0.f : m[j][0], m[j][1] == -INFINITY ? 0.f : m[j][1]};
+      for (int p = 0; p < 2; ++p) {
+        uint32_t pf[NT][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float pv[2];
+          const int t = 16 * p + order(r) + 8 * i;
+          const float scale = vs[2 * p + i].x * up, low = vs[2 * p + i].y;
 #pragma unroll
-          for (int o = 0; o < 2; ++o) {
-            const bool seen = t0 + r + 8 * i < limit[j][o];
-            const float p = fast_exp2(s[j][2 * i + o] - ref[o]);
-            l[j][o] += p;
-            z[j][o] += seen ? p * vs[i].y : 0.f;
-            pv[o] = seen ? p * (vs[i].x * up) : 0.f;
+          for (int n = 0; n < NT; ++n) {
+            float pv[2];
+#pragma unroll
+            for (int o = 0; o < 2; ++o) {
+              const float w = fast_exp2(s[p][n][2 * i + o]);
+              const bool seen = !MASK || t0 + t < limit[n][o];
+              l[n][o] += w;
+              z[n][o] = seen ? fmaf(w, low, z[n][o]) : z[n][o];
+              pv[o] = seen ? w * scale : 0.f;
+            }
+            pf[n][i] = transpose_8x8(pack_f16x2(pv[0], pv[1]));
           }
-          pf[j][i] = transpose_8x8(pack_f16x2(pv[0], pv[1]));
         }
-      }
-#pragma unroll
-      for (int k = 0; k < VW; ++k) {
-        // words of two neighbouring tokens side by side: places 0 to 3 of both, then 4 to 7
-        const uint32_t lo0 = __byte_perm(vc[0].w[k], vc[1].w[k], 0x5410), hi0 = __byte_perm(vc[0].w[k], vc[1].w[k], 0x7632);
-        const uint32_t lo1 = __byte_perm(vc[2].w[k], vc[3].w[k], 0x5410), hi1 = __byte_perm(vc[2].w[k], vc[3].w[k], 0x7632);
-        const uint32_t x[4] = {lo0, lo0 >> 8, hi0, hi0 >> 8}, y[4] = {lo1, lo1 >> 8, hi1, hi1 >> 8};
+        Words<VW> vc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
+          vc[i] = load_words<VW>(src + TILE * D / 2 + (16 * p + order(2 * q4 + (i & 1) + 8 * (i >> 1))) * (D / 2) + r * (VW * 4));
 #pragma unroll
-          for (int j = 0; j < NT; ++j)
-            mma_f16(o_acc[j][4 * k + i], x[i] & 0x000F000Fu, x[i] & 0x00F000F0u, y[i] & 0x000F000Fu, y[i] & 0x00F000F0u,
-                    pf[j][0], pf[j][1]);
+        for (int k = 0; k < VW; ++k) {
+          // words of two tokens side by side: places 0 to 3 of both, then 4 to 7
+          const uint32_t lo0 = __byte_perm(vc[0].w[k], vc[1].w[k], 0x5410), hi0 = __byte_perm(vc[0].w[k], vc[1].w[k], 0x7632);
+          const uint32_t lo1 = __byte_perm(vc[2].w[k], vc[3].w[k], 0x5410), hi1 = __byte_perm(vc[2].w[k], vc[3].w[k], 0x7632);
+          const uint32_t x[4] = {lo0, lo0 >> 8, hi0, hi0 >> 8}, y[4] = {lo1, lo1 >> 8, hi1, hi1 >> 8};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+              mma_f16(o_acc[n][4 * k + i], x[i] & 0x000F000Fu, x[i] & 0x00F000F0u, y[i] & 0x000F000Fu, y[i] & 0x00F000F0u,
+                      pf[n][0], pf[n][1]);
+        }
       }
-    }
+    };
 
-    // the warps' sums, in their order
+    for (int j = 0; j < mine; ++j) {
+      const uint32_t stage = (loads + j) % STAGES, phase = ((loads + j) / STAGES) & 1;
+      const int t0 = (t_first + warp + j * WARPS) * TILE;
+      mbar_wait_warp(&bars[warp][stage], phase, &abort_flag, a.status);
+      if (t0 + TILE <= all_see) tile(ring + stage * Sh::STAGE, t0, std::false_type());
+      else tile(ring + stage * Sh::STAGE, t0, std::true_type());
+      __syncwarp();
+      fetch(j + STAGES);
+    }
+    loads += mine;
+
+    // the warps' sums, in their order, in the place of the rings: every copy has arrived and been read
+    float (*const sh_o)[COLS][D + 4] = reinterpret_cast<float (*)[COLS][D + 4]>(smem);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
@@ -553,17 +646,17 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
           sh_m[warp][col] = m[j][o];
           sh_l[warp][col] = l[j][o];
         }
-        const float f = pow2(min(top_e - 121, 127));           // 2^20 / (2^15 / 2^(exponent + 1)) of the odd places
+        const float f = pow2(min(top_e - 121, 127));          // 2^20 / (2^15 / 2^(exponent + 1)) of the odd places
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          sh_o[warp][col][r * (D / 8) + 2 * i] = o_acc[j][i][o] * (16.f * f) + z[j][o];
-          sh_o[warp][col][r * (D / 8) + 2 * i + 1] = o_acc[j][i][2 + o] * f + z[j][o];
-        }
+        for (int i = 0; i < MT; ++i)
+          *reinterpret_cast<float2*>(&sh_o[warp][col][r * (D / 8) + 2 * i]) =
+              make_float2(o_acc[j][i][o] * (16.f * f) + z[j][o], o_acc[j][i][2 + o] * f + z[j][o]);
       }
     }
     __syncthreads();
+    const long long slot = 2LL * blockIdx.x + (t_first == 0);        // a sequence that goes on, or one that begins, in this block
     for (int x = threadIdx.x; x < COLS * (D / 4); x += WARPS * 32) {
-      const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = tile * COLS + col;
+      const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
       if (n >= columns) continue;
       float top = sh_m[0][col];
 #pragma unroll
@@ -572,16 +665,19 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
 #pragma unroll
       for (int k = 0; k < WARPS; ++k) {
         const float f = sh_m[k][col] == -INFINITY ? (sh_l[k][col] == 0.f ? 0.f : 1.f) : fast_exp2(sh_m[k][col] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&sh_o[k][col][d]);
         sum += f * sh_l[k][col];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] += f * sh_o[k][col][d + e];
+        o[0] += f * v.x;
+        o[1] += f * v.y;
+        o[2] += f * v.z;
+        o[3] += f * v.w;
       }
-      const int i = n / a.group, h = head * a.group + n - i * a.group;
-      if (of > 1) {
-        const long long row = (first_partial + place) * ((long long)a.heads * a.S) + (long long)h * a.S + i;
-        *reinterpret_cast<float4*>(a.partial + row * D + d) = make_float4(o[0], o[1], o[2], o[3]);
-        if (d == 0) *reinterpret_cast<float2*>(a.partial + a.partial_rows * D + row * 2) = make_float2(top, sum);
+      if (!whole) {
+        *reinterpret_cast<float4*>(a.partial + (slot * COLS + col) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (d == 0)
+          *reinterpret_cast<float2*>(a.partial + 2LL * a.ctas * COLS * D + (slot * COLS + col) * 2) = make_float2(top, sum);
       } else {
+        const int i = n / a.group, h = head * a.group + n - i * a.group;
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T y[4];
 #pragma unroll
@@ -591,50 +687,69 @@ __global__ void __launch_bounds__(WARPS * 32) kv4_attention_kernel(AttnArgs a) {
         if (d == 0 && a.lse) a.lse[((long long)b * a.heads + h) * a.S + i] = (top + log2f(sum)) * 0.69314718056f;
       }
     }
+    if (u < run_end) {
+      fence_proxy_async_smem();      // the sums were written by the threads, the next tiles come by the copy unit
+      __syncthreads();
+    }
   }
 }
 
-// Sequences of several chunks: one warp per row of the output.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_join_kernel(AttnArgs a, int per) {
+// Sequences (of a head and a column tile: a block) that several blocks worked on. Bound by latency: the blocks' results are read
+// eight at a time, independent of one another.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kv4_join_kernel(AttnArgs a, int per) {
+  constexpr int COLS = 8 * NT, EACH = 8;
   grid_go();
   grid_wait();
-  if (warp_uniform(*a.status) != 0) return;
-  const int lane = threadIdx.x & 31;
-  const long long row = blockIdx.x * 4ll + (threadIdx.x >> 5);      // (b, h, i)
-  if (row >= (long long)a.c.rows * a.heads * a.S) return;
-  const int b = (int)(row / ((long long)a.heads * a.S)), hi = (int)(row - (long long)b * a.heads * a.S);
-  const Plan plan = make_plan(a.c, a.lengths, per, a.ctas, a.status);
-  const int of = chunks_of(seen_length(a.c, a.lengths, b, a.status), plan.chunk);
-  if (of == 1) return;
-  long long first = 0;
-  for (int x = lane; x < b; x += 32) {
-    const int k = chunks_of(seen_length(a.c, a.lengths, x, a.status), plan.chunk);
-    first += k > 1 ? k : 0;
+  const int2 own = a.owners[blockIdx.x];
+  const bool failed = *a.status != 0;
+  // (behind a kernel that left early there may be anything)
+  if (__syncthreads_or(failed) || own.x < 0 || own.y >= a.ctas || own.x >= own.y) return;
+  const int columns = a.S * a.group, b = blockIdx.x / per, hc = blockIdx.x - b * per;
+  const int head = hc % a.c.kv_heads, col_tile = hc / a.c.kv_heads;
+  const float* const stats = a.partial + 2LL * a.ctas * COLS * D;
+  for (int x = threadIdx.x; x < COLS * (D / 4); x += 256) {
+    const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
+    if (n >= columns) continue;
+    float top = -INFINITY, sum = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = own.x; k0 <= own.y; k0 += EACH) {
+      float2 ml[EACH];
+      float4 v[EACH];
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const int at = (2 * min(k0 + k, own.y) + (k0 + k == own.x)) * COLS + col;
+        ml[k] = *reinterpret_cast<const float2*>(stats + 2LL * at);
+        v[k] = *reinterpret_cast<const float4*>(a.partial + (long long)at * D + d);
+        if (k0 + k > own.y) ml[k] = make_float2(-INFINITY, 0.f);
+      }
+      float to = top;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) to = fmaxf(to, ml[k].x);
+      const float down = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : fast_exp2(top - to);
+      sum *= down;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= down;
+      top = to;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        if (k0 + k > own.y) continue;
+        const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : fast_exp2(ml[k].x - top);
+        sum += f * ml[k].y;
+        o[0] += f * v[k].x;
+        o[1] += f * v[k].y;
+        o[2] += f * v[k].z;
+        o[3] += f * v[k].w;
+      }
+    }
+    const int i = n / a.group, h = head * a.group + n - i * a.group;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[e] * inv);
+    *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (((long long)b * a.S + i) * a.heads + h) * D + d) =
+        *reinterpret_cast<const uint2*>(y);
+    if (d == 0 && a.lse) a.lse[((long long)b * a.heads + h) * a.S + i] = (top + log2f(sum)) * 0.69314718056f;
   }
-  first = warp_sum_ll(first);
-  const float* stats = a.partial + a.partial_rows * D;
-  const long long step = (long long)a.heads * a.S, at = first * step + hi;
-  float top = -INFINITY;
-  for (int k = lane; k < of; k += 32) top = fmaxf(top, stats[(at + k * step) * 2]);
-  top = warp_max(top);
-  float sum = 0.f, o[D / 32];
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e) o[e] = 0.f;
-#pragma unroll 4
-  for (int k = 0; k < of; ++k) {
-    const float2 ml = *reinterpret_cast<const float2*>(stats + (at + k * step) * 2);
-    const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - top);
-    sum += f * ml.y;
-#pragma unroll
-    for (int e = 0; e < D / 32; ++e) o[e] += f * a.partial[(at + k * step) * D + lane + 32 * e];
-  }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int h = hi / a.S, i = hi - h * a.S;
-#pragma unroll
-  for (int e = 0; e < D / 32; ++e)
-    reinterpret_cast<T*>(a.out)[(((long long)b * a.S + i) * a.heads + h) * D + lane + 32 * e] = from_f32<T>(o[e] * inv);
-  if (lane == 0 && a.lse) a.lse[row] = (top + log2f(sum)) * 0.69314718056f;
 }
 
 Cache cache_of(void* codes, void* scales, const void* table, long long table_stride, int rows, int width, int pages,
@@ -659,20 +774,28 @@ int launch_read(void* k, void* v, const Cache& c, const void* seq, const void* p
                       (const int*)pos, units, status) == cudaSuccess ? 0 : -5;
 }
 
-constexpr int CTAS = 148 * 4;
-
 template <typename T, int D, int NT>
-int launch_attention(const AttnArgs& a, bool join, cudaStream_t st) {
-  const int tiles = (a.S * a.group + 8 * NT - 1) / (8 * NT), per = tiles * a.c.kv_heads;
-  // no more blocks than chunks there can be
-  const long long of = (((long long)a.c.width << a.c.page_shift) + MIN_CHUNK - 1) / MIN_CHUNK;
-  const long long most = (of > 1 ? of : 1) * a.c.rows * per;
-  const unsigned grid = (unsigned)(most < CTAS ? most : (long long)CTAS);
-  if (launch_after(kv4_attention_kernel<T, D, NT>, dim3(grid), WARPS * 32, 0, st, 1, a) != cudaSuccess) return -5;
-  if (!join) return 0;
-  const long long rows = (long long)a.c.rows * a.heads * a.S, blocks = (rows + 3) / 4;
-  if (blocks > 0x7fffffffLL) return -2;
-  return launch_after(kv4_join_kernel<T, D>, dim3((unsigned)blocks), 128, 0, st, 1, a, per) == cudaSuccess ? 0 : -5;
+int launch_attention(AttnArgs a, cudaStream_t st) {
+  using Sh = Shape<D, NT>;
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return -5;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::RING) != cudaSuccess)
+      return -4;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const long long per = (a.S * a.group + Sh::COLS - 1) / Sh::COLS * (long long)a.c.kv_heads;
+  const long long room = ((long long)a.c.width << a.c.page_shift) / TILE;       // tiles that a sequence can have
+  const long long most = (START + (room > 1 ? room : 1)) * a.c.rows * per, runs = a.c.rows * per;
+  if (runs > 0x7fffffffLL) return -2;
+  a.ctas = 148 * Sh::BLOCKS;
+  a.owners = reinterpret_cast<int2*>(a.partial + 2LL * a.ctas * Sh::COLS * (D + 2));
+  const unsigned grid = (unsigned)(most < a.ctas ? most : a.ctas);
+  if (launch_after(kv4_attention_kernel<T, D, NT>, dim3(grid), WARPS * 32, Sh::RING, st, 1, a) != cudaSuccess) return -5;
+  if (room <= 1) return 0;                                                         // nothing to cut
+  return launch_after(kv4_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per) == cudaSuccess ? 0 : -5;
 }
 }  // namespace
 
@@ -709,16 +832,15 @@ extern "C" int atb_kv4_read(void* k, void* v, void* codes, void* scales, const v
   return -1;
 }
 
-// Rows of the workspace of partial results ((D + 2) floats each): a sequence of several chunks has fewer than twice as many as
-// its length in chunks, and all lengths together make no more chunks than the blocks that the GPU is filled with.
-extern "C" int atb_kv4_partial_rows(int heads, int kv_heads, int S) {
-  const int columns = S * (heads / kv_heads), nt = columns > 8 ? 2 : 1, per = (columns + 8 * nt - 1) / (8 * nt) * kv_heads;
-  return (2 * (CTAS / per) + 2) * heads * S;
+// Floats of the workspace of atb_kv4_attention: two segments a block, and two numbers a sequence.
+extern "C" long long atb_kv4_attention_scratch(int rows, int heads, int kv_heads, int S, int head_dim) {
+  const int columns = S * (heads / kv_heads), cols = columns > 8 ? 16 : 8, blocks = columns > 8 ? Shape<128, 2>::BLOCKS : Shape<128, 1>::BLOCKS;
+  return 2LL * 148 * blocks * cols * (head_dim + 2) + 2LL * rows * kv_heads * ((columns + cols - 1) / cols);
 }
 
 extern "C" int atb_kv4_attention(const void* q, void* out, void* lse, void* codes, void* scales, const void* table,
-                                 const void* lengths, void* partial, int partial_rows, int S, int heads, int kv_heads,
-                                 int head_dim, int page_shift, int pages, int rows, int width, long long table_stride,
+                                 const void* lengths, void* partial, int S, int heads, int kv_heads, int head_dim,
+                                 int page_shift, int pages, int rows, int width, long long table_stride,
                                  long long q_batch, long long q_token, float scale, int dtype, void* stream, void* status) {
   if (rows <= 0 || S <= 0) return 0;
   AttnArgs a;
@@ -728,20 +850,16 @@ extern "C" int atb_kv4_attention(const void* q, void* out, void* lse, void* code
   a.out = out;
   a.lse = (float*)lse;
   a.partial = (float*)partial;
-  a.partial_rows = partial_rows;
   a.q_batch = q_batch;
   a.q_token = q_token;
   a.S = S;
   a.heads = heads;
   a.group = heads / kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
-  a.ctas = CTAS;
   a.status = (int*)status;
-  const bool join = partial != nullptr;
-  if (!join && ((long long)width << page_shift) > MIN_CHUNK) return -1;
   const bool two = S * a.group > 8;
 #define ATTN(T, D) \
-  return two ? launch_attention<T, D, 2>(a, join, (cudaStream_t)stream) : launch_attention<T, D, 1>(a, join, (cudaStream_t)stream)
+  return two ? launch_attention<T, D, 2>(a, (cudaStream_t)stream) : launch_attention<T, D, 1>(a, (cudaStream_t)stream)
   if (dtype == 0 && head_dim == 64) ATTN(__nv_bfloat16, 64);
   if (dtype == 0 && head_dim == 128) ATTN(__nv_bfloat16, 128);
   if (dtype == 1 && head_dim == 64) ATTN(__half, 64);

@@ -13,6 +13,8 @@ These operators serve generation: they have no gradient, and refuse tensors that
 """
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 from typing import Optional, Tuple
 
@@ -22,7 +24,6 @@ from .. import _lib
 
 Layer = Tuple[torch.Tensor, torch.Tensor]
 HEAD_DIMS = (64, 128)          # of the kernels; the CPU path takes any even one
-MIN_CHUNK = 64                 # csrc/kv4.cu: a sequence of so many tokens is never cut
 
 
 class KV4Cache:
@@ -52,8 +53,8 @@ def _sizes(layer: Layer, page_table: torch.Tensor) -> Tuple[int, int, int, int]:
     pages, two, kv_heads, page_size, half = codes.shape
     if two != 2 or tuple(scales.shape) != (pages, kv_heads, page_size, 4) or pages == 0 or kv_heads == 0 or half == 0:
         raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not one cache")
-    if not (codes.is_contiguous() and scales.is_contiguous()):
-        raise ValueError("the cache has to be contiguous")
+    if not (codes.is_contiguous() and scales.is_contiguous()) or (codes.data_ptr() | scales.data_ptr()) % 16:
+        raise ValueError("the cache has to be contiguous and begin on 16 bytes")
     _check_page_size(page_size)
     if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
         raise ValueError("page_table is int32 [sequences, pages], its rows contiguous")
@@ -232,6 +233,14 @@ def kv4_attention_reference(q, layer, page_table, lengths, softmax_scale=None):
     return out.to(q.dtype), lse
 
 
+@functools.lru_cache(maxsize=256)
+def _scratch(*sizes: int) -> int:
+    """Floats of the attention kernels' workspace."""
+    fn = _lib.lib().atb_kv4_attention_scratch
+    fn.restype = ctypes.c_longlong
+    return fn(*sizes)
+
+
 def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengths: torch.Tensor,
                   softmax_scale: Optional[float] = None, return_lse: bool = False):
     """Attention of the newest tokens over the cache. ``q`` ``[sequences, S, n_q, head_dim]`` (bf16 or fp16) are the queries of
@@ -256,14 +265,10 @@ def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengt
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
     lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if return_lse else None
-    L = _lib.lib()
-    partial, rows = None, 0
-    if page_table.shape[1] * page_size > MIN_CHUNK:
-        rows = L.atb_kv4_partial_rows(H, KV, S)
-        partial = torch.empty(rows * (D + 2), dtype=torch.float32, device=q.device)
-    rc = L.atb_kv4_attention(
+    partial = torch.empty(_scratch(B, H, KV, S, D), dtype=torch.float32, device=q.device)
+    rc = _lib.lib().atb_kv4_attention(
         q.data_ptr(), out.data_ptr(), _lib.addr(lse), layer[0].data_ptr(), layer[1].data_ptr(), page_table.data_ptr(),
-        lengths.data_ptr(), _lib.addr(partial), rows, S, H, KV, D, page_size.bit_length() - 1, pages, B, page_table.shape[1],
+        lengths.data_ptr(), partial.data_ptr(), S, H, KV, D, page_size.bit_length() - 1, pages, B, page_table.shape[1],
         page_table.stride(0), q.stride(0), q.stride(1), softmax_scale if softmax_scale is not None else D ** -0.5,
         _lib.DT[q.dtype], _lib.stream(), _lib.status_addr(q))
     _lib.check(rc, "atb_kv4_attention")
