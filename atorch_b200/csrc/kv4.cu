@@ -209,6 +209,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(T* k, T* v, Cache c, cons
 // in place; of the others, the run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins in
 // the order of the blocks.
 constexpr int WARPS = 4, TILE = 32, START = 8;
+constexpr float SLACK = 8.f;       // powers of two by which a score may exceed the maximum that is kept
 
 ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
   const int n = lengths[b], most = c.width << c.page_shift;
@@ -270,10 +271,16 @@ ATB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* 
                : "memory");
 }
 ATB_DEVICE void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero.
+ATB_DEVICE void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 ATB_DEVICE uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -326,13 +333,14 @@ struct AttnArgs {
 // else that a value has:
 //   s[t, n]  = ks[t] (q[n] . code[t]) + km[t] sum(q[n])        o[d, n] = sum_t (p[t, n] vs[t]) code[t, d] + sum_t p[t, n] vm[t]
 // q is scaled by a power of two to at most 2^15 before it is rounded to fp16 (bf16 and fp16 values stay exact down to 2^-29 of
-// the largest), p vs by 2^(15 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
+// the largest), p vs by 2^(7 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
 // 11 bits of it are kept, which is what the products with 4-bit codes can use. Sums, maxima and denominators are fp32.
 //
 // A warp has every fourth tile of a segment. Its tiles come through a ring of its own in shared memory, filled by the copy unit
 // STAGES tiles ahead. What bounds the kernel beside memory is the integer pipe: 5 operations for 8 codes of a key, 6 of a value.
 // So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and
-// only the tiles at a sequence's end are masked. Row i of 16 tokens' products is token order(i): a lane then reads its values'
+// only the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by
+// 2^8 before everything is rescaled: a warp sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its values'
 // words without a bank conflict worse than two ways.
 template <int D, int NT>
 struct Shape {
@@ -492,7 +500,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
         ref[j][o] = l[j][o] = z[j][o] = 0.f;
       }
     }
-    int top_e = 16;        // exponent field of the largest value scale so far
+    int top_e = 24;        // exponent field of the largest value scale so far
     bool unset = true;     // whether a column has no maximum yet
 
     auto tile = [&](const uint8_t* src, int t0, auto masked) {
@@ -500,13 +508,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
       float s[2][NT][4];
       float2 vs[4];
       float over = 0.f;
-      int e_new = 0;
+      uint32_t most_scale = 0;       // bf16 bits
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[p][n][e] = 0.f;
         const Words<KW> x = load_words<KW>(src + (16 * p + order(r)) * (D / 2) + q4 * (KW * 4));
         const Words<KW> y = load_words<KW>(src + (16 * p + order(r) + 8) * (D / 2) + q4 * (KW * 4));
 #pragma unroll
@@ -514,8 +518,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           const uint32_t xs = x.w[k] >> 8, ys = y.w[k] >> 8;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            mma_f16(s[p][n], x.w[k] & 0x000F000Fu, y.w[k] & 0x000F000Fu, x.w[k] & 0x00F000F0u, y.w[k] & 0x00F000F0u,
-                    qf[n][k][0], qf[n][k][1]);
+            if (k == 0)
+              mma_f16_first(s[p][n], x.w[k] & 0x000F000Fu, y.w[k] & 0x000F000Fu, x.w[k] & 0x00F000F0u, y.w[k] & 0x00F000F0u,
+                            qf[n][k][0], qf[n][k][1]);
+            else
+              mma_f16(s[p][n], x.w[k] & 0x000F000Fu, y.w[k] & 0x000F000Fu, x.w[k] & 0x00F000F0u, y.w[k] & 0x00F000F0u,
+                      qf[n][k][0], qf[n][k][1]);
             mma_f16(s[p][n], xs & 0x000F000Fu, ys & 0x000F000Fu, xs & 0x00F000F0u, ys & 0x00F000F0u, qf[n][k][2], qf[n][k][3]);
           }
         }
@@ -526,8 +534,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           if (MASK && t0 + t >= len) sc = make_uint2(0u, 0u);           // places behind the last token hold anything
           const float2 ks = unpack_bf16x2(sc.x);
           vs[2 * p + i] = unpack_bf16x2(sc.y);
-          const int e = (sc.y >> 7) & 255;
-          e_new = max(e_new, e == 255 ? 0 : e);       // an infinity is not for the queries that do not see it
+          most_scale = max(most_scale, sc.y & 0x7fffu);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -539,8 +546,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
             }
         }
       }
-      if (__any_sync(0xffffffffu, over > 0.f || e_new > top_e || unset)) {
-        e_new = max(e_new, top_e);
+      if (__any_sync(0xffffffffu, over > SLACK || (int)(most_scale >> 7) > top_e || unset)) {
+        int e_new = top_e;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = (__float_as_int(vs[i].x) >> 23) & 255;
+          e_new = max(e_new, e == 255 ? 0 : e);       // an infinity is not for the queries that do not see it
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
         const float down = __int_as_float((127 + max(top_e - e_new, -126)) << 23);
@@ -576,7 +588,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
             for (int e = 0; e < 4; ++e) o_acc[n][i][e] *= f[e & 1];
         }
       }
-      const float up = __int_as_float((268 - top_e) << 23);      // 2^15 / 2^(exponent + 1)
+      const float up = __int_as_float((268 - (int)SLACK - top_e) << 23);      // 2^(15 - SLACK) / 2^(exponent + 1)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         uint32_t pf[NT][2];
@@ -646,7 +658,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           sh_m[warp][col] = m[j][o];
           sh_l[warp][col] = l[j][o];
         }
-        const float f = pow2(min(top_e - 121, 127));          // 2^20 / (2^15 / 2^(exponent + 1)) of the odd places
+        const float f = pow2(min(top_e - 121 + (int)SLACK, 127));      // of the odd places: 2^20 over what p was scaled by
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           *reinterpret_cast<float2*>(&sh_o[warp][col][r * (D / 8) + 2 * i]) =
