@@ -4,41 +4,53 @@
 //   scales bf16  [N][ceil(K / G)]       G = 32, 64 or 128 columns share a scale
 //
 // Bound by the codes, N K / 2 bytes, for as many rows as a decode step has. The products run on the warp's matrix instruction
-// (16 x 8 x 16) with 16 weight rows as its tall operand and 8 rows of x as the other. A code becomes code - 8 in the type of x
-// by one AND-OR and one packed subtraction for two of them, exactly: 128 + code and 1024 + code are bf16 and fp16 numbers with
-// the code in their last bits. The products with x are exact in fp32, sums of a group are fp32, and the scale, one per row and
-// group, multiplies the sum of the group.
+// (16 x 8 x 16, fp32 sums) with 16 weight rows as its tall operand and 8 rows of x as the other. Two codes become code - 8 in the
+// type of x by one AND-OR and one packed operation, exactly: 128 + code is a bf16 number with the code in its last bits, 1024 +
+// code and 1024 + 16 code are such fp16 numbers. Products are exact in fp32, sums are fp32, and the scale of a row and group
+// multiplies the sum of the group.
+#include <atomic>
+#include <cooperative_groups.h>
 #include "common.cuh"
 
 namespace {
 using namespace atb;
+namespace cg = cooperative_groups;
 
-constexpr int WARPS = 8;
+constexpr int WARPS = 8, AHEAD = 3;      // groups of codes asked for ahead
 
 template <typename T>
 ATB_DEVICE void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2 && __is_same(T, __half))
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  if constexpr (__is_same(T, __half))
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// codes at places p and p + 4 of a word, less 8, as two numbers of T
+ATB_DEVICE uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+ATB_DEVICE uint32_t bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// The codes of a word less 8: pair p holds places p and p + 4.
 template <typename T>
-ATB_DEVICE uint32_t weights_of(uint32_t w, int p) {
+ATB_DEVICE void weights_of(uint32_t w, uint32_t (&f)[4]) {
   if constexpr (__is_same(T, __half)) {
-    const uint32_t u = ((w >> (4 * p)) & 0x000F000Fu) | 0x64006400u, eight = 0x64086408u;
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&eight));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const uint32_t magic = 0x64006400u, eight = 0x64086408u, by16 = 0x2c002c00u, less72 = 0xd480d480u;      // 1024, 1032, 1 / 16, -72
+    const uint32_t hi = w >> 8;
+    const uint32_t u[4] = {(w & 0x000F000Fu) | magic, (w & 0x00F000F0u) | magic, (hi & 0x000F000Fu) | magic, (hi & 0x00F000F0u) | magic};
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const __half2 h = *reinterpret_cast<const __half2*>(&u[p]);
+      f[p] = bits(p & 1 ? __hfma2(h, *reinterpret_cast<const __half2*>(&by16), *reinterpret_cast<const __half2*>(&less72))
+                        : __hsub2(h, *reinterpret_cast<const __half2*>(&eight)));
+    }
   } else {
-    const uint32_t u = ((w >> (4 * p)) & 0x000F000Fu) | 0x43004300u, eight = 0x43084308u;
-    const __nv_bfloat162 h = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&eight));
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const uint32_t magic = 0x43004300u, eight = 0x43084308u;                                                // 128, 136
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      const uint32_t u = ((w >> (4 * p)) & 0x000F000Fu) | magic;
+      f[p] = bits(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&eight)));
+    }
   }
 }
 
@@ -51,6 +63,7 @@ struct Args {
   int M, N, K, row_bytes, groups;
   long long x_stride;
   int wide;          // rows of x can be read in 16-byte pieces
+  int round;         // groups of x that shared memory holds
   const int* status;
 };
 
@@ -64,90 +77,141 @@ ATB_DEVICE uint4 load_x(const Args& a, const T* row, int k) {
   for (int i = 0; i < 8; ++i) h[i] = k + i < a.K ? row[k + i] : from_f32<T>(0.f);
   return u;
 }
+template <int V, int R>
+struct Codes {
+  uint32_t w[2 * R][V];
+};
 
-// A block has 16 R rows of the weights and 8 NT rows of x; its warps take the groups in turn. A lane (r, q) reads the quarter q of
-// a group of weight rows r and r + 8, V words (8 codes each), and of row r of x.
+// A block has 128 R rows of the weights, 16 R a warp, and 8 NT rows of x; the blocks of a cluster have equal shares of the groups
+// and add up their sums through each other's shared memory, in their order. A lane (r, q) reads the quarter q of a group of weight
+// rows r + 8 i, V words (8 codes each), AHEAD groups ahead. What a block needs of x goes through shared memory in rounds of `round`
+// groups, in the order in which the lanes need it: [group][word][row of x][quarter] pieces of 16 bytes, places p and p + 4 paired.
 template <typename T, int V, int NT, int R>
-__global__ void __launch_bounds__(WARPS * 32) w4_kernel(Args a) {
-  constexpr int G = 32 * V;
-  __shared__ float part[WARPS][16 * R][8 * NT + 1];
+__global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) w4_kernel(Args a) {
+  constexpr int G = 32 * V, MX = 8 * NT, ROWS = 16 * R * WARPS;
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float sums[MX][ROWS + 4];
   grid_go();
   grid_wait();
-  if (__syncthreads_or(threadIdx.x == 0 && *a.status != 0)) return;
+  const bool failed = *a.status != 0;      // nothing is stored then; the blocks of a cluster stay together
+  cg::cluster_group cluster = cg::this_cluster();
+  const int split = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q = lane & 3;
-  const int n0 = blockIdx.x * 16 * R, m0 = blockIdx.y * 8 * NT;
-  float acc[R][NT][4] = {};
-  for (int g = warp; g < a.groups; g += WARPS) {
-    uint32_t xf[NT][V][4];
+  const int n_block = blockIdx.x / split * ROWS, m0 = blockIdx.y * MX, rows = min(MX, a.M - m0);
+  const int g_begin = (int)((long long)a.groups * rank / split), g_end = (int)((long long)a.groups * (rank + 1) / split);
+  uint4* const xs = reinterpret_cast<uint4*>(smem);                                             // [round][V][rows][4]
+  float* const ss = reinterpret_cast<float*>(smem + (size_t)a.round * V * rows * 4 * 16);       // [round][ROWS] scales
+
+  const uint8_t* row[2 * R];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const int m = m0 + 8 * j + r;
-      const T* row = reinterpret_cast<const T*>(a.x) + m * a.x_stride;
+  for (int i = 0; i < 2 * R; ++i)
+    row[i] = a.codes + (long long)min(n_block + warp * 16 * R + 8 * i + r, a.N - 1) * a.row_bytes + q * (4 * V);
+  const int last_at = a.row_bytes - 4 * V - q * (4 * V);       // behind the row's end x is 0, and any codes will do
+  auto load = [&](Codes<V, R>& c, int g) {
+    if (g >= g_end) return;
+    const int at = min(g * (16 * V), last_at);
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        uint4 u = make_uint4(0u, 0u, 0u, 0u);
-        if (m < a.M) u = load_x<T>(a, row, g * G + (q * V + v) * 8);
-        xf[j][v][0] = __byte_perm(u.x, u.z, 0x5410);
-        xf[j][v][1] = __byte_perm(u.x, u.z, 0x7632);
-        xf[j][v][2] = __byte_perm(u.y, u.w, 0x5410);
-        xf[j][v][3] = __byte_perm(u.y, u.w, 0x7632);
+    for (int i = 0; i < 2 * R; ++i) {
+      const uint8_t* p = row[i] + at;
+      if constexpr (V == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        c.w[i][0] = u.x; c.w[i][1] = u.y; c.w[i][2] = u.z; c.w[i][3] = u.w;
+      } else if constexpr (V == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        c.w[i][0] = u.x; c.w[i][1] = u.y;
+      } else {
+        c.w[i][0] = *reinterpret_cast<const uint32_t*>(p);
       }
     }
+  };
+  Codes<V, R> next[AHEAD];
 #pragma unroll
-    for (int s = 0; s < R; ++s) {
-      uint32_t w[2][V];
-      float scale[2];
+  for (int i = 0; i < AHEAD; ++i) load(next[i], g_begin + i);
+
+  float acc[R][NT][4] = {};
+  int col[NT];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = n0 + 16 * s + 8 * i + r, at = (g * 4 + q) * (4 * V);
-        const bool in = n < a.N && at < a.row_bytes;
-        const uint8_t* p = a.codes + (long long)n * a.row_bytes + at;
+  for (int j = 0; j < NT; ++j) col[j] = min(8 * j + r, rows - 1) * 4 + q;           // columns without a row are not kept
+  for (int g0 = g_begin; g0 < g_end; g0 += a.round) {
+    const int here = min(a.round, g_end - g0);
+    if (g0 > g_begin) __syncthreads();
+    {
+      const int piece = threadIdx.x % (4 * V), pq = piece & 3, pv = piece >> 2;
+      const int step_m = WARPS * 8 / V % rows, step_g = WARPS * 8 / V / rows;
+      int m = threadIdx.x / (4 * V) % rows, g = threadIdx.x / (4 * V) / rows;
+      while (g < here) {
+        const uint4 u = load_x<T>(a, reinterpret_cast<const T*>(a.x) + (m0 + m) * a.x_stride, (g0 + g) * G + (pq * V + pv) * 8);
+        xs[((g * V + pv) * rows + m) * 4 + pq] = make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632),
+                                                            __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
+        g += step_g;
+        m += step_m;
+        if (m >= rows) {
+          m -= rows;
+          ++g;
+        }
+      }
+    }
+    for (int i = threadIdx.x; i < here * ROWS; i += WARPS * 32) {
+      const int n = i % ROWS, g = i / ROWS;
+      ss[i] = n_block + n < a.N ? __bfloat162float(a.scales[(long long)(n_block + n) * a.groups + g0 + g]) : 0.f;
+    }
+    __syncthreads();
+    const float* const sl = ss + warp * 16 * R + r;
+    for (int gt = 0; gt < here; gt += AHEAD) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) w[i][v] = 0x88888888u;
-        if (in) {
-          if constexpr (V == 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p);
-            w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
-          } else if constexpr (V == 2) {
-            const uint2 u = *reinterpret_cast<const uint2*>(p);
-            w[i][0] = u.x; w[i][1] = u.y;
-          } else {
-            w[i][0] = *reinterpret_cast<const uint32_t*>(p);
+      for (int i = 0; i < AHEAD; ++i) {
+        const int g = gt + i;
+        if (g >= here) break;
+        float d[R][NT][4] = {};
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          uint4 u[NT];
+#pragma unroll
+          for (int j = 0; j < NT; ++j) u[j] = xs[(g * V + v) * rows * 4 + col[j]];
+#pragma unroll
+          for (int k = 0; k < R; ++k) {
+            uint32_t f0[4], f1[4];
+            weights_of<T>(next[i].w[2 * k][v], f0);
+            weights_of<T>(next[i].w[2 * k + 1][v], f1);
+            const uint32_t fa[4] = {f0[0], f1[0], f0[1], f1[1]}, fb[4] = {f0[2], f1[2], f0[3], f1[3]};
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+              mma<T>(d[k][j], fa, u[j].x, u[j].y);
+              mma<T>(d[k][j], fb, u[j].z, u[j].w);
+            }
           }
         }
-        scale[i] = n < a.N ? __bfloat162float(a.scales[(long long)n * a.groups + g]) : 0.f;
-      }
-      float d[NT][4] = {};
+        load(next[i], g0 + g + AHEAD);
 #pragma unroll
-      for (int v = 0; v < V; ++v)
+        for (int k = 0; k < R; ++k) {
+          const float s0 = sl[g * ROWS + 16 * k], s1 = sl[g * ROWS + 16 * k + 8];
 #pragma unroll
-        for (int p = 0; p < 4; p += 2) {
-          const uint32_t f[4] = {weights_of<T>(w[0][v], p), weights_of<T>(w[1][v], p), weights_of<T>(w[0][v], p + 1),
-                                 weights_of<T>(w[1][v], p + 1)};
+          for (int j = 0; j < NT; ++j)
 #pragma unroll
-          for (int j = 0; j < NT; ++j) mma<T>(d[j], f, xf[j][v][p], xf[j][v][p + 1]);
+            for (int e = 0; e < 4; ++e) acc[k][j][e] = fmaf(e < 2 ? s0 : s1, d[k][j][e], acc[k][j][e]);
         }
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[s][j][e] = fmaf(scale[e >> 1], d[j][e], acc[s][j][e]);
+      }
     }
   }
 #pragma unroll
-  for (int s = 0; s < R; ++s)
+  for (int k = 0; k < R; ++k)
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) part[warp][16 * s + 8 * (e >> 1) + r][8 * j + 2 * q + (e & 1)] = acc[s][j][e];
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * R * 8 * NT; i += WARPS * 32) {
-    const int row = i % (16 * R), col = i / (16 * R), n = n0 + row, m = m0 + col;
-    if (n >= a.N || m >= a.M) continue;
+      for (int e = 0; e < 4; ++e) sums[8 * j + 2 * q + (e & 1)][(warp * R + k) * 16 + 8 * (e >> 1) + r] = acc[k][j][e];
+  if (split > 1) cluster.sync();
+  else __syncthreads();
+  const int share = ROWS / split;        // rows that this block finishes
+  for (int i = threadIdx.x; i < share * rows; i += WARPS * 32) {
+    const int at = rank * share + i % share, m = i / share, n = n_block + at;
+    if (n >= a.N || failed) continue;
     float sum = a.bias ? to_f32<T>(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
-#pragma unroll
-    for (int k = 0; k < WARPS; ++k) sum += part[k][row][col];
-    reinterpret_cast<T*>(a.y)[(long long)m * a.N + n] = from_f32<T>(sum);
+    if (split == 1) sum += sums[m][at];
+    else
+      for (int k = 0; k < split; ++k) sum += *cluster.map_shared_rank(&sums[m][at], k);
+    reinterpret_cast<T*>(a.y)[(long long)(m0 + m) * a.N + n] = from_f32<T>(sum);
   }
+  if (split > 1) cluster.sync();         // the others have read this block's sums
 }
 
 // The weights themselves, [N][K], for products of many rows: a thread turns a word of 8 codes into 16 bytes.
@@ -169,16 +233,33 @@ __global__ void __launch_bounds__(256) w4_expand_kernel(const uint8_t* codes, co
 }
 
 template <typename T, int V, int NT, int R>
-int launch(const Args& a, cudaStream_t st) {
-  const dim3 grid((a.N + 16 * R - 1) / (16 * R), (a.M + 8 * NT - 1) / (8 * NT));
-  if (grid.y > 65535) return -2;
-  return launch_after(w4_kernel<T, V, NT, R>, grid, WARPS * 32, 0, st, 1, a) == cudaSuccess ? 0 : -5;
+int launch(Args a, cudaStream_t st) {
+  constexpr int G = 32 * V, MX = 8 * NT, ROWS = 16 * R * WARPS, MOST = 56 * 1024;
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return -5;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(w4_kernel<T, V, NT, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, MOST) != cudaSuccess) return -4;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const long long blocks = (a.N + ROWS - 1LL) / ROWS, chunks = (a.M + MX - 1LL) / MX;
+  if (chunks > 65535) return -2;
+  // shares of the groups until there are three blocks for two SMs; a block keeps four groups, else its start outweighs them
+  int split = 1;
+  while (split < 8 && blocks * chunks * split < 222 && a.groups >= 8 * split) split *= 2;
+  const int rows = a.M < MX ? a.M : MX, group_bytes = G * 2 * rows + 4 * ROWS;
+  const int share = (a.groups + split - 1) / split;
+  a.round = MOST / group_bytes < share ? MOST / group_bytes / AHEAD * AHEAD : share;       // codes are asked for in turns of AHEAD
+  if (blocks * split > 0x7fffffffLL) return -2;
+  return launch_after(w4_kernel<T, V, NT, R>, dim3((unsigned)(blocks * split), (unsigned)chunks), WARPS * 32,
+                      (size_t)a.round * group_bytes, st, split, a) == cudaSuccess ? 0 : -5;
 }
 template <typename T, int V>
 int by_rows(const Args& a, cudaStream_t st) {
   if (a.M <= 8) return launch<T, V, 1, 1>(a, st);
   if (a.M <= 16) return launch<T, V, 2, 2>(a, st);
-  return launch<T, V, 4, 2>(a, st);
+  return launch<T, V, 4, 1>(a, st);
 }
 template <typename T>
 int by_group(const Args& a, int group, cudaStream_t st) {
@@ -193,7 +274,7 @@ extern "C" int atb_w4_linear(const void* x, const void* codes, const void* scale
                              int group, long long x_stride, int wide, int dtype, void* stream, void* status) {
   if (M <= 0 || N <= 0) return 0;
   const Args a{x, (const uint8_t*)codes, (const __nv_bfloat16*)scales, bias, y, M, N, K, (K + 31) / 32 * 16,
-               (K + group - 1) / group, x_stride, wide, (const int*)status};
+               (K + group - 1) / group, x_stride, wide, 0, (const int*)status};
   if (dtype == 0) return by_group<__nv_bfloat16>(a, group, (cudaStream_t)stream);
   if (dtype == 1) return by_group<__half>(a, group, (cudaStream_t)stream);
   return -1;
