@@ -16,7 +16,7 @@ namespace {
 using namespace atb;
 namespace cg = cooperative_groups;
 
-constexpr int WARPS = 8, AHEAD = 3;      // groups of codes asked for ahead
+constexpr int WARPS = 8, AHEAD = 3, BATCH = 4;      // groups of codes asked for ahead; loads of x on their way at once
 
 template <typename T>
 ATB_DEVICE void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -31,13 +31,20 @@ ATB_DEVICE void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t
 }
 ATB_DEVICE uint32_t bits(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 ATB_DEVICE uint32_t bits(__nv_bfloat162 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+// (x & mask) | magic in one operation (left to itself the compiler makes two of them)
+ATB_DEVICE uint32_t and_or(uint32_t x, uint32_t mask, uint32_t magic) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(magic));
+  return y;
+}
 // The codes of a word less 8: pair p holds places p and p + 4.
 template <typename T>
 ATB_DEVICE void weights_of(uint32_t w, uint32_t (&f)[4]) {
   if constexpr (__is_same(T, __half)) {
     const uint32_t magic = 0x64006400u, eight = 0x64086408u, by16 = 0x2c002c00u, less72 = 0xd480d480u;      // 1024, 1032, 1 / 16, -72
     const uint32_t hi = w >> 8;
-    const uint32_t u[4] = {(w & 0x000F000Fu) | magic, (w & 0x00F000F0u) | magic, (hi & 0x000F000Fu) | magic, (hi & 0x00F000F0u) | magic};
+    const uint32_t u[4] = {and_or(w, 0x000F000Fu, magic), and_or(w, 0x00F000F0u, magic), and_or(hi, 0x000F000Fu, magic),
+                           and_or(hi, 0x00F000F0u, magic)};
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
       const __half2 h = *reinterpret_cast<const __half2*>(&u[p]);
@@ -48,7 +55,7 @@ ATB_DEVICE void weights_of(uint32_t w, uint32_t (&f)[4]) {
     const uint32_t magic = 0x43004300u, eight = 0x43084308u;                                                // 128, 136
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
-      const uint32_t u = ((w >> (4 * p)) & 0x000F000Fu) | magic;
+      const uint32_t u = and_or(w >> (4 * p), 0x000F000Fu, magic);
       f[p] = bits(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&eight)));
     }
   }
@@ -139,21 +146,37 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) w4_kernel(Args a)
       const int piece = threadIdx.x % (4 * V), pq = piece & 3, pv = piece >> 2;
       const int step_m = WARPS * 8 / V % rows, step_g = WARPS * 8 / V / rows;
       int m = threadIdx.x / (4 * V) % rows, g = threadIdx.x / (4 * V) / rows;
-      while (g < here) {
-        const uint4 u = load_x<T>(a, reinterpret_cast<const T*>(a.x) + (m0 + m) * a.x_stride, (g0 + g) * G + (pq * V + pv) * 8);
-        xs[((g * V + pv) * rows + m) * 4 + pq] = make_uint4(__byte_perm(u.x, u.z, 0x5410), __byte_perm(u.x, u.z, 0x7632),
-                                                            __byte_perm(u.y, u.w, 0x5410), __byte_perm(u.y, u.w, 0x7632));
-        g += step_g;
-        m += step_m;
-        if (m >= rows) {
-          m -= rows;
-          ++g;
+      while (g < here) {        // several loads are on their way before the first is stored
+        uint4 u[BATCH];
+        int at[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+          at[i] = g < here ? ((g * V + pv) * rows + m) * 4 + pq : -1;
+          if (g < here) u[i] = load_x<T>(a, reinterpret_cast<const T*>(a.x) + (m0 + m) * a.x_stride, (g0 + g) * G + (pq * V + pv) * 8);
+          g += step_g;
+          m += step_m;
+          if (m >= rows) {
+            m -= rows;
+            ++g;
+          }
         }
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+          if (at[i] >= 0)
+            xs[at[i]] = make_uint4(__byte_perm(u[i].x, u[i].z, 0x5410), __byte_perm(u[i].x, u[i].z, 0x7632),
+                                   __byte_perm(u[i].y, u[i].w, 0x5410), __byte_perm(u[i].y, u[i].w, 0x7632));
       }
     }
-    for (int i = threadIdx.x; i < here * ROWS; i += WARPS * 32) {
-      const int n = i % ROWS, g = i / ROWS;
-      ss[i] = n_block + n < a.N ? __bfloat162float(a.scales[(long long)(n_block + n) * a.groups + g0 + g]) : 0.f;
+    for (int i0 = threadIdx.x; i0 < here * ROWS; i0 += BATCH * WARPS * 32) {
+      __nv_bfloat16 v[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const int k = min(i0 + i * WARPS * 32, here * ROWS - 1);
+        v[i] = a.scales[(long long)min(n_block + k % ROWS, a.N - 1) * a.groups + g0 + k / ROWS];
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i)
+        if (i0 + i * WARPS * 32 < here * ROWS) ss[i0 + i * WARPS * 32] = __bfloat162float(v[i]);
     }
     __syncthreads();
     const float* const sl = ss + warp * 16 * R + r;
@@ -201,14 +224,19 @@ __global__ void __launch_bounds__(WARPS * 32, NT == 1 ? 3 : 2) w4_kernel(Args a)
       for (int e = 0; e < 4; ++e) sums[8 * j + 2 * q + (e & 1)][(warp * R + k) * 16 + 8 * (e >> 1) + r] = acc[k][j][e];
   if (split > 1) cluster.sync();
   else __syncthreads();
-  const int share = ROWS / split;        // rows that this block finishes
-  for (int i = threadIdx.x; i < share * rows; i += WARPS * 32) {
-    const int at = rank * share + i % share, m = i / share, n = n_block + at;
+  // the blocks of a cluster finish the rows in turns, by the warp
+  for (int i = warp * split + rank; i < ROWS / 32 * rows; i += WARPS * split) {
+    const int at = i % (ROWS / 32) * 32 + lane, m = i / (ROWS / 32), n = n_block + at;
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < split) v[k] = split == 1 ? sums[m][at] : *cluster.map_shared_rank(&sums[m][at], k);
+    float sum = v[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k)
+      if (k < split) sum += v[k];
     if (n >= a.N || failed) continue;
-    float sum = a.bias ? to_f32<T>(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
-    if (split == 1) sum += sums[m][at];
-    else
-      for (int k = 0; k < split; ++k) sum += *cluster.map_shared_rank(&sums[m][at], k);
+    if (a.bias) sum += to_f32<T>(reinterpret_cast<const T*>(a.bias)[n]);
     reinterpret_cast<T*>(a.y)[(long long)(m0 + m) * a.N + n] = from_f32<T>(sum);
   }
   if (split > 1) cluster.sync();         // the others have read this block's sums
@@ -245,9 +273,10 @@ int launch(Args a, cudaStream_t st) {
   }
   const long long blocks = (a.N + ROWS - 1LL) / ROWS, chunks = (a.M + MX - 1LL) / MX;
   if (chunks > 65535) return -2;
-  // shares of the groups until there are three blocks for two SMs; a block keeps four groups, else its start outweighs them
-  int split = 1;
-  while (split < 8 && blocks * chunks * split < 222 && a.groups >= 8 * split) split *= 2;
+  // as many shares of the groups as keep all blocks on the GPU at once, of four groups at least: less would be outweighed by its
+  // start
+  const long long room = 148 * (NT == 1 ? 3 : 2) / (blocks * chunks);
+  const int most = a.groups / 4, split = room < 2 || most < 2 ? 1 : room < 8 && room < most ? (int)room : most < 8 ? most : 8;
   const int rows = a.M < MX ? a.M : MX, group_bytes = G * 2 * rows + 4 * ROWS;
   const int share = (a.groups + split - 1) / split;
   a.round = MOST / group_bytes < share ? MOST / group_bytes / AHEAD * AHEAD : share;       // codes are asked for in turns of AHEAD
