@@ -166,6 +166,11 @@ def stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def stream_of(device: int) -> int:
+    """Handle of the current stream of the device with this index."""
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
 def stream_ptr() -> ctypes.c_void_p:
     return ctypes.c_void_p(stream())
 

@@ -62,6 +62,20 @@ ATB_DEVICE void store8(T* p, const float (&x)[8]) {
     *reinterpret_cast<uint4*>(p) = u;
   }
 }
+// 8 elements as they lie in memory
+template <typename T>
+struct Piece {
+  uint4 u[sizeof(T) / 2];
+  ATB_DEVICE void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  ATB_DEVICE void get(float (&x)[8]) const {
+    const T* h = reinterpret_cast<const T*>(u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(h[i]);
+  }
+};
 // minimum and maximum that keep a NaN: a token with one stands for NaN, as its values would
 ATB_DEVICE float min_nan(float a, float b) {
   float r;
@@ -74,111 +88,134 @@ ATB_DEVICE float max_nan(float a, float b) {
   return r;
 }
 
+constexpr int SMALL = 128;      // threads of a block of the two kernels below: a few heads of one token
+
 // A head of a token is D / 16 lanes: each has 8 dims of the first half and the 8 of the second half that they turn with.
-// Rotation and codes are computed by separately rounded fp32 operations (no fused multiply-add, true division), so that the
-// codes are those of the formula evaluated operation by operation, and do not depend on how a compiler contracts it. The scale
-// is rounded to bf16 before the codes are taken: the code is the nearest one of the scale that is kept.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const T* qkv, T* q_out, Cache c, const int* seq, const int* pos,
-                                                         const float* cosT, const float* sinT, int positions,
-                                                         long long units, int n_q, long long token_stride, int* status) {
+// The result is that of separately rounded fp32 operations (no fused multiply-add, true division), so that the codes are those of
+// the formula evaluated operation by operation, and do not depend on how a compiler contracts it. The scale is rounded to bf16
+// before the codes are taken: the code is the nearest one of the scale that is kept. Bound by memory where there are many tokens:
+// so a division is a product with the reciprocal, and only a quotient that comes within 1e-5 of the middle of two codes (the
+// product is off by 2e-6 at most) is divided (a true division for each took 78 us for 10900 tokens of 48 heads, ... us now).
+template <typename T, int D, int PER>
+__global__ void __launch_bounds__(SMALL, PER == 1 || sizeof(T) == 4 ? 1 : 7) kv4_append_kernel(const T* qkv, T* q_out, Cache c, const int* seq, const int* pos,
+                                                           const float* cosT, const float* sinT, int positions, int n_q,
+                                                           long long token_stride, int* status) {
   grid_go();
   grid_wait();
-  constexpr int L = D / 16, HALF = D / 2;
-  const int heads = n_q + 2 * c.kv_heads;
-  const long long thread = blockIdx.x * 256ll + threadIdx.x;
-  const long long unit = thread / L;
-  const int l = (int)(thread % L);
-  const bool failed = warp_uniform(*status) != 0;       // one answer for the lanes of a head; asked by all lanes
-  const bool live = unit < units && !failed;
-  const long long t = live ? unit / heads : 0;
-  const int h = live ? (int)(unit - t * heads) : 0;
-  float a[8], b[8];
-  int p = -1, page = -1;
-  if (live) {
-    const T* src = qkv + t * token_stride + (long long)h * D + l * 8;
-    load8<T>(src, a);
-    load8<T>(src + HALF, b);
-    p = pos[t];
-    if (p >= 0) {
-      page = page_of(c, seq ? seq[t] : (int)t, p);
-      if (page < 0 || (cosT && p >= positions)) {
-        atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
-        page = -1;
-        p = -1;
-      }
+  constexpr int L = D / 16, HALF = D / 2, EACH = SMALL / L;
+  const int heads = n_q + 2 * c.kv_heads, l = threadIdx.x % L, h0 = blockIdx.y * (EACH * PER) + threadIdx.x / L;
+  const long long t = blockIdx.x;
+  const int before = *status, row = seq ? seq[t] : (int)t;
+  int p = pos[t], page = -1;
+  Piece<T> x[PER][2];              // 8 dims of the first half of head h0 + j EACH, 8 of the second
+#pragma unroll
+  for (int j = 0; j < PER; ++j)
+    if (h0 + j * EACH < heads) {
+      const T* src = qkv + t * token_stride + (long long)(h0 + j * EACH) * D + l * 8;
+      x[j][0].load(src);
+      x[j][1].load(src + HALF);
+    }
+  if (p >= 0) {
+    page = page_of(c, row, p);
+    if (page < 0 || (cosT && p >= positions)) {
+      atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
+      page = -1;
+      p = -1;
     }
   }
-  if (cosT && p >= 0 && h < n_q + c.kv_heads) {
-    float cs[8], sn[8];
+  float cs[8], sn[8];
+  const bool turn = cosT && p >= 0 && h0 < n_q + c.kv_heads;
+  if (turn) {
     load8<float>(cosT + (long long)p * HALF + l * 8, cs);
     load8<float>(sinT + (long long)p * HALF + l * 8, sn);
+  }
+  const bool failed = warp_uniform(before) != 0;       // one answer for the lanes of a head; every lane has to ask
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = __fsub_rn(__fmul_rn(x, cs[i]), __fmul_rn(y, sn[i]));
-      b[i] = __fadd_rn(__fmul_rn(y, cs[i]), __fmul_rn(x, sn[i]));
+  for (int j = 0; j < PER; ++j) {
+    const int h = h0 + j * EACH;
+    const bool live = h < heads && !failed;
+    float a[8], b[8];
+    x[j][0].get(a);
+    x[j][1].get(b);
+    if (turn && h < n_q + c.kv_heads) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float u = a[i], v = b[i];
+        a[i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(v, sn[i]));
+        b[i] = __fadd_rn(__fmul_rn(v, cs[i]), __fmul_rn(u, sn[i]));
+      }
     }
-  }
-  if (live && h < n_q) {
-    T* dst = q_out + (t * n_q + h) * D + l * 8;
-    store8<T>(dst, a);
-    store8<T>(dst + HALF, b);
-  }
-  float lo = 0.f, hi = 0.f;
-  if (live) {
-    lo = min_nan(a[0], b[0]);
-    hi = max_nan(a[0], b[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) {
-      lo = min_nan(lo, min_nan(a[i], b[i]));
-      hi = max_nan(hi, max_nan(a[i], b[i]));
+    if (live && h < n_q) {
+      T* dst = q_out + (t * n_q + h) * D + l * 8;
+      store8<T>(dst, a);
+      store8<T>(dst + HALF, b);
     }
-  }
+    const bool kept = live && h >= n_q && page >= 0;
+    if (!__any_sync(0xffffffffu, kept)) continue;
+    float lo = 0.f, hi = 0.f;
+    if (kept) {
+      lo = min_nan(a[0], b[0]);
+      hi = max_nan(a[0], b[0]);
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  if (!live || h < n_q || page < 0) return;
-  const __nv_bfloat16 scale = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), low = __float2bfloat16_rn(lo);
-  const float s = __bfloat162float(scale), m = __bfloat162float(low);
-  uint32_t w[2] = {0u, 0u};
-  if (s > 0.f) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(a[i], m), s)), 0.f), 15.f);
-      const float v = fminf(fmaxf(rintf(__fdiv_rn(__fsub_rn(b[i], m), s)), 0.f), 15.f);
-      w[0] |= (uint32_t)u << (4 * i);
-      w[1] |= (uint32_t)v << (4 * i);
+      for (int i = 1; i < 8; ++i) {
+        lo = min_nan(lo, min_nan(a[i], b[i]));
+        hi = max_nan(hi, max_nan(a[i], b[i]));
+      }
     }
-  }
-  const int which = h >= n_q + c.kv_heads, head = h - n_q - (which ? c.kv_heads : 0), slot = p & ((1 << c.page_shift) - 1);
-  uint8_t* dst = codes_at<D>(c, page, which, head, slot) + l * 4;
-  *reinterpret_cast<uint32_t*>(dst) = w[0];
-  *reinterpret_cast<uint32_t*>(dst + HALF / 2) = w[1];
-  if (l == 0) {
-    const __nv_bfloat162 pair = __halves2bfloat162(scale, low);
-    reinterpret_cast<__nv_bfloat162*>(scales_at(c, page, head, slot))[which] = pair;
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (kept) {
+      const __nv_bfloat16 scale = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f)), low = __float2bfloat16_rn(lo);
+      const float s = __bfloat162float(scale), m = __bfloat162float(low);
+      uint32_t w[2] = {0u, 0u};
+      if (s > 0.f) {
+        const float inv = __frcp_rn(s), round = 12582912.f;       // 1.5 * 2^23: adding it leaves the nearest integer, ties to even
+        float off = s < 1e-30f ? 1.f : 0.f;                       // (a reciprocal that is not exact enough, or infinite)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float d = __fsub_rn(i < 8 ? a[i] : b[i - 8], m);
+          const float y = fminf(fmaxf(__fmul_rn(d, inv), 0.f), 15.f);
+          const float r = __fadd_rn(y, round);
+          off = fmaxf(off, fabsf(__fsub_rn(y, __fsub_rn(r, round))));
+          w[i / 8] |= (__float_as_uint(r) & 15u) << (4 * (i % 8));
+        }
+        if (off > 0.49999f) {
+          w[0] = w[1] = 0u;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float d = __fsub_rn(i < 8 ? a[i] : b[i - 8], m);
+            w[i / 8] |= (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(d, s)), 0.f), 15.f) << (4 * (i % 8));
+          }
+        }
+      }
+      const int which = h >= n_q + c.kv_heads, head = h - n_q - (which ? c.kv_heads : 0), slot = p & ((1 << c.page_shift) - 1);
+      uint8_t* dst = codes_at<D>(c, page, which, head, slot) + l * 4;
+      *reinterpret_cast<uint32_t*>(dst) = w[0];
+      *reinterpret_cast<uint32_t*>(dst + HALF / 2) = w[1];
+      if (l == 0) {
+        const __nv_bfloat162 pair = __halves2bfloat162(scale, low);
+        reinterpret_cast<__nv_bfloat162*>(scales_at(c, page, head, slot))[which] = pair;
+      }
+    }
   }
 }
 
 // What the cache stands for at given tokens: a lane turns 8 codes of the keys and of the values into two 16-byte pieces.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(T* k, T* v, Cache c, const int* seq, const int* pos, long long units,
-                                                       int* status) {
+__global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, const int* seq, const int* pos, int* status) {
   grid_go();
   grid_wait();
   constexpr int L = D / 8;
-  const long long thread = blockIdx.x * 256ll + threadIdx.x;
-  const long long unit = thread / L;
-  const int l = (int)(thread % L);
-  if (unit >= units || *status != 0) return;
-  const long long t = unit / c.kv_heads;
-  const int h = (int)(unit - t * c.kv_heads), p = pos[t];
+  const int l = threadIdx.x % L, h = blockIdx.y * (SMALL / L) + threadIdx.x / L;
+  const long long t = blockIdx.x;
+  const int before = *status, p = pos[t], row = seq ? seq[t] : (int)t;
+  if (h >= c.kv_heads || before != 0) return;
   float x[2][8] = {};
   if (p >= 0) {
-    const int page = page_of(c, seq ? seq[t] : (int)t, p), slot = p & ((1 << c.page_shift) - 1);
+    const int page = page_of(c, row, p), slot = p & ((1 << c.page_shift) - 1);
     if (page < 0) {
       atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
     } else {
@@ -192,8 +229,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(T* k, T* v, Cache c, cons
       }
     }
   }
-  store8<T>(k + unit * D + l * 8, x[0]);
-  store8<T>(v + unit * D + l * 8, x[1]);
+  const long long at = (t * c.kv_heads + h) * D + l * 8;
+  store8<T>(k + at, x[0]);
+  store8<T>(v + at, x[1]);
 }
 
 // ----------------------------------------------------------------------------------
@@ -772,18 +810,22 @@ Cache cache_of(void* codes, void* scales, const void* table, long long table_str
 template <typename T, int D>
 int launch_append(const void* qkv, void* q, const Cache& c, const void* seq, const void* pos, const void* cosT, const void* sinT,
                   int positions, int tokens, int n_q, long long stride, cudaStream_t st, int* status) {
-  const long long units = (long long)tokens * (n_q + 2 * c.kv_heads), blocks = (units * (D / 16) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -2;
-  return launch_after(kv4_append_kernel<T, D>, dim3((unsigned)blocks), 256, 0, st, 1, (const T*)qkv, (T*)q, c, (const int*)seq,
-                      (const int*)pos, (const float*)cosT, (const float*)sinT, positions, units, n_q, stride,
-                      status) == cudaSuccess ? 0 : -5;
+  const int each = SMALL / (D / 16), heads = n_q + 2 * c.kv_heads;
+  // where there are more blocks than the GPU holds, a thread has three heads: more loads on their way, one look at the page table
+  // and the angles (one head each: 82 us for 10900 tokens of 48 heads and their reading back, three: ... us)
+  const bool many = (long long)tokens * ((heads + each - 1) / each) > 148 * 16 && heads > each;
+  const int blocks = many ? (heads + 3 * each - 1) / (3 * each) : (heads + each - 1) / each;
+  if (blocks > 65535) return -2;
+  return launch_after(many ? kv4_append_kernel<T, D, 3> : kv4_append_kernel<T, D, 1>, dim3(tokens, blocks), SMALL, 0, st, 1,
+                      (const T*)qkv, (T*)q, c, (const int*)seq, (const int*)pos, (const float*)cosT, (const float*)sinT, positions,
+                      n_q, stride, status) == cudaSuccess ? 0 : -5;
 }
 template <typename T, int D>
 int launch_read(void* k, void* v, const Cache& c, const void* seq, const void* pos, int tokens, cudaStream_t st, int* status) {
-  const long long units = (long long)tokens * c.kv_heads, blocks = (units * (D / 8) + 255) / 256;
-  if (blocks > 0x7fffffffLL) return -2;
-  return launch_after(kv4_read_kernel<T, D>, dim3((unsigned)blocks), 256, 0, st, 1, (T*)k, (T*)v, c, (const int*)seq,
-                      (const int*)pos, units, status) == cudaSuccess ? 0 : -5;
+  const int each = SMALL / (D / 8), blocks = (c.kv_heads + each - 1) / each;
+  if (blocks > 65535) return -2;
+  return launch_after(kv4_read_kernel<T, D>, dim3(tokens, blocks), SMALL, 0, st, 1, (T*)k, (T*)v, c, (const int*)seq,
+                      (const int*)pos, status) == cudaSuccess ? 0 : -5;
 }
 
 template <typename T, int D, int NT>

@@ -58,28 +58,31 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
             raise ValueError(f"finished is bool {(B, W)}, got {finished.dtype} {tuple(finished.shape)}")
         if not 0 <= eos < V:
             raise ValueError(f"finished beams go on with eos, and {eos} is not in the vocabulary")
-    if not (logits.device == scores.device and (finished is None or finished.device == logits.device)):
+    dev = logits.get_device()
+    if scores.get_device() != dev or (finished is not None and finished.get_device() != dev):
         raise ValueError("logits, scores and finished are on several devices")
-    if torch.is_grad_enabled() and (logits.requires_grad or scores.requires_grad):
+    if (logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("a selection has no gradient: call under torch.no_grad()")
-    if not _lib.use_kernels(logits):
+    if dev < 0 or not _lib.use_kernels(logits):
         return beam_select_reference(logits, scores, finished, eos, keep)
     if W > MAX_BEAMS or keep > MAX_BEAMS:
         raise ValueError(f"{W} beams, {keep} kept: the kernels take {MAX_BEAMS}")
-    dev = logits.device
-    if logits.stride(2) != 1 or (B > 1 and W > 1 and logits.stride(0) != W * logits.stride(1)):
-        logits = logits.contiguous()
-    row = logits.stride(1) if W > 1 else logits.stride(0)
-    wide = logits.data_ptr() % 16 == 0 and row * logits.element_size() % 16 == 0
+    step, row, one = logits.stride()
+    if one != 1 or (B > 1 and W > 1 and step != W * row):
+        logits, row, step = logits.contiguous(), V, W * V
+    if W == 1:
+        row = step
+    base = logits.data_ptr()
     scores, finished = scores.contiguous(), None if finished is None else finished.contiguous()
-    best = torch.empty(B * W * keep, dtype=torch.int64, device=dev)
-    out = torch.empty(B, keep, dtype=torch.float32, device=dev)
-    tokens = torch.empty(B, keep, dtype=torch.int64, device=dev)
-    parents = torch.empty(B, keep, dtype=torch.int32, device=dev)
-    ended = torch.empty(B, keep, dtype=torch.bool, device=dev)
-    rc = _lib.lib().atb_beam_select(logits.data_ptr(), scores.data_ptr(), _lib.addr(finished), best.data_ptr(), out.data_ptr(),
-                                    tokens.data_ptr(), parents.data_ptr(), ended.data_ptr(), B, W, V, row, int(wide), int(eos), keep,
-                                    _lib.DT[logits.dtype], _lib.stream(), _lib.status_addr(logits))
+    out = scores.new_empty(B, keep)
+    tokens = torch.empty_like(out, dtype=torch.int64)
+    parents = torch.empty_like(out, dtype=torch.int32)
+    ended = torch.empty_like(out, dtype=torch.bool)
+    best = torch.empty(B * W * keep, dtype=torch.int64, device=logits.device)
+    rc = _lib.lib().atb_beam_select(base, scores.data_ptr(), _lib.addr(finished), best.data_ptr(), out.data_ptr(), tokens.data_ptr(),
+                                    parents.data_ptr(), ended.data_ptr(), B, W, V, row,
+                                    int(base % 16 == 0 and row * logits.element_size() % 16 == 0), int(eos), keep,
+                                    _lib.DT[logits.dtype], _lib.stream_of(dev), _lib.status_addr(logits))
     _lib.check(rc, "atb_beam_select")
     return out, tokens, parents, ended
 
@@ -126,14 +129,15 @@ def beam_reorder(codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Te
         raise ValueError(f"page_table is int32 [{B * W}, pages], its rows contiguous")
     if lengths.dtype is not torch.int32 or lengths.shape != (B * W,):
         raise ValueError(f"lengths are int32 [{B * W}], got {lengths.dtype} {tuple(lengths.shape)}")
-    if len({t.device for t in (codes, scales, page_table, lengths, parents)}) != 1:
+    dev = codes.get_device()
+    if any(t.get_device() != dev for t in (scales, page_table, lengths, parents)):
         raise ValueError("tensors on several devices")
-    if not _lib.use_kernels(codes):
+    if dev < 0 or not _lib.use_kernels(codes):
         return beam_reorder_reference(codes, scales, page_table, lengths, parents)
     if W > MAX_BEAMS or half % 16:
         raise ValueError(f"{W} beams, head_dim {2 * half}: the kernel takes {MAX_BEAMS} and multiples of 32")
     parents, lengths = parents.contiguous(), lengths.contiguous()
     rc = _lib.lib().atb_beam_reorder(codes.data_ptr(), scales.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
                                      parents.data_ptr(), B, W, page_table.shape[1], page_table.stride(0), layers, pages, KV,
-                                     page_size.bit_length() - 1, 2 * half, _lib.stream(), _lib.status_addr(codes))
+                                     page_size.bit_length() - 1, 2 * half, _lib.stream_of(dev), _lib.status_addr(codes))
     _lib.check(rc, "atb_beam_reorder")

@@ -16,7 +16,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -44,42 +44,62 @@ def _check_page_size(n: int) -> None:
         raise ValueError(f"page_size has to be a power of two of 16 or more, got {n}")
 
 
-def _sizes(layer: Layer, page_table: torch.Tensor) -> Tuple[int, int, int, int]:
-    """(pages, kv_heads, page_size, head_dim) of a layer's cache, after the checks that all calls share."""
+class _Cache(NamedTuple):
+    """A layer's cache and page table as the launchers take them."""
+
+    codes: int
+    scales: int
+    table: int
+    pages: int
+    kv_heads: int
+    page_shift: int
+    rows: int
+    width: int
+    table_stride: int
+    head_dim: int
+    device: int          # index; -1: the CPU
+
+
+def _cache(layer: Layer, page_table: torch.Tensor) -> _Cache:
+    """After the checks that all calls share."""
     codes, scales = layer
-    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or codes.dim() != 5 or scales.dim() != 4:
+    shape, table_shape = codes.shape, page_table.shape
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1] != 2 or 0 in shape:
         raise ValueError("a layer's cache is (uint8 [pages, 2, kv_heads, page_size, head_dim / 2], "
-                         "bf16 [pages, kv_heads, page_size, 4])")
-    pages, two, kv_heads, page_size, half = codes.shape
-    if two != 2 or tuple(scales.shape) != (pages, kv_heads, page_size, 4) or pages == 0 or kv_heads == 0 or half == 0:
-        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not one cache")
-    if not (codes.is_contiguous() and scales.is_contiguous()) or (codes.data_ptr() | scales.data_ptr()) % 16:
+                         f"bf16 [pages, kv_heads, page_size, 4]), got {codes.dtype} {tuple(shape)} and {scales.dtype}")
+    pages, _, kv_heads, page_size, half = shape
+    if scales.shape != (pages, kv_heads, page_size, 4):
+        raise ValueError(f"codes {tuple(shape)} and scales {tuple(scales.shape)} are not one cache")
+    codes_at, scales_at, dev = codes.data_ptr(), scales.data_ptr(), codes.get_device()
+    if not (codes.is_contiguous() and scales.is_contiguous()) or (codes_at | scales_at) & 15:
         raise ValueError("the cache has to be contiguous and begin on 16 bytes")
-    _check_page_size(page_size)
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.stride(1) != 1:
+    if page_size < 16 or page_size & (page_size - 1):
+        _check_page_size(page_size)
+    if page_table.dtype is not torch.int32 or len(table_shape) != 2 or page_table.stride(1) != 1:
         raise ValueError("page_table is int32 [sequences, pages], its rows contiguous")
-    return pages, kv_heads, page_size, 2 * half
+    if dev >= 0:
+        if half != 64 and half != 32:
+            raise ValueError(f"head_dim {2 * half}: the kernels take {HEAD_DIMS}")
+        _lib.lib()
+    _same_device(dev, scales, page_table)
+    return _Cache(codes_at, scales_at, page_table.data_ptr(), pages, kv_heads, page_size.bit_length() - 1, table_shape[0],
+                  table_shape[1], page_table.stride(0), 2 * half, dev)
 
 
-def _on_gpu(head_dim: int, *tensors: torch.Tensor) -> bool:
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) != 1:
-        raise ValueError(f"tensors on several devices: {sorted(map(str, devices))}")
-    if not _lib.use_kernels(tensors[0]):
-        return False
-    if head_dim not in HEAD_DIMS:
-        raise ValueError(f"head_dim {head_dim}: the kernels take {HEAD_DIMS}")
-    return True
+def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor on {t.device}, and the cache on {dev if dev >= 0 else 'the CPU'}")
 
 
-def _no_gradient(*tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def _no_gradient(t: torch.Tensor) -> None:
+    if t.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("the 4-bit cache has no gradient: call under torch.no_grad()")
 
 
 def _int32(name: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:
-    if t is None:
-        return None
+    if t is None or (t.dtype is torch.int32 and t.shape == (n,) and t.is_contiguous()):
+        return t
     if t.dtype not in (torch.int32, torch.int64) or t.numel() != n:
         raise ValueError(f"{name}: {n} whole numbers are wanted, got {t.dtype} {tuple(t.shape)}")
     return t.reshape(-1).to(torch.int32).contiguous()
@@ -139,33 +159,36 @@ def kv4_append(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tenso
     position is padding: its token is not kept, its queries come back as they are. Two tokens at one place: either is kept.
 
     The rotation is not rounded before the codes are taken; queries are rounded once."""
-    pages, KV, page_size, D = _sizes(layer, page_table)
-    width = (n_q + 2 * KV) * D
-    if n_q < 0 or qkv.numel() % width or (qkv.shape[-1] != width and qkv.shape[-2:] != (n_q + 2 * KV, D)):
-        raise ValueError(f"qkv {tuple(qkv.shape)}: {n_q} + 2 x {KV} heads of {D} are wanted in a token")
-    if qkv.dtype not in _lib.DT:
+    c = _cache(layer, page_table)
+    KV, D, dev = c.kv_heads, c.head_dim, c.device
+    shape, dtype, width = qkv.shape, _lib.DT.get(qkv.dtype), (n_q + 2 * KV) * D
+    if dtype is None:
         raise ValueError(f"qkv is bf16, fp16 or fp32, got {qkv.dtype}")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    if cos is not None and (cos.dtype is not torch.float32 or cos.shape != sin.shape or sin.dtype is not torch.float32
-                            or cos.dim() != 2 or cos.shape[1] != D // 2):
-        raise ValueError(f"cos and sin are fp32 [positions, {D // 2}]")
-    _no_gradient(qkv)
-    T = qkv.numel() // width
-    seq, pos = _int32("seq", seq, T), _int32("pos", pos, T)
-    if not _on_gpu(D, qkv, *layer, page_table, pos, seq, cos, sin):
-        return kv4_append_reference(layer, page_table, seq, pos, qkv, n_q, cos, sin)
-    x = qkv if qkv.dim() == 2 and qkv.shape[1] == width and qkv.stride(1) == 1 else qkv.reshape(T, width)
-    if x.stride(1) != 1 or not _aligned(x, x.stride(0)):
-        x = x.clone(memory_format=torch.contiguous_format)
-    if cos is not None:
+    if n_q < 0 or (shape[-1:] != (width,) and shape[-2:] != (n_q + 2 * KV, D)):
+        raise ValueError(f"qkv {tuple(shape)}: {n_q} + 2 x {KV} heads of {D} are wanted in a token")
+    positions = 0
+    if cos is not None and sin is not None:
+        positions = cos.shape[0]
+        if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != (positions, D // 2) \
+                or sin.shape != (positions, D // 2):
+            raise ValueError(f"cos and sin are fp32 [positions, {D // 2}]")
         cos, sin = cos.contiguous(), sin.contiguous()
-    q = torch.empty(T, n_q, D, dtype=x.dtype, device=x.device)
-    rc = _lib.lib().atb_kv4_append(
-        x.data_ptr(), q.data_ptr(), layer[0].data_ptr(), layer[1].data_ptr(), page_table.data_ptr(), _lib.addr(seq), pos.data_ptr(),
-        _lib.addr(cos), _lib.addr(sin), 0 if cos is None else cos.shape[0], T, n_q, KV, D, page_size.bit_length() - 1, pages,
-        page_table.shape[0], page_table.shape[1], page_table.stride(0), x.stride(0), _lib.DT[x.dtype], _lib.stream(),
-        _lib.status_addr(x))
+    elif cos is not sin:
+        raise ValueError("cos and sin go together")
+    _no_gradient(qkv)
+    x = qkv if len(shape) == 2 and shape[1] == width else qkv.reshape(qkv.numel() // width, width)
+    T = x.shape[0]
+    seq, pos = _int32("seq", seq, T), _int32("pos", pos, T)
+    _same_device(dev, qkv, pos, seq, cos, sin)
+    if dev < 0:
+        return kv4_append_reference(layer, page_table, seq, pos, qkv, n_q, cos, sin)
+    step, one = x.stride()
+    if one != 1 or not _aligned(x, step):
+        x, step = x.clone(memory_format=torch.contiguous_format), width
+    q = x.new_empty(T, n_q, D)
+    rc = _lib.lib().atb_kv4_append(x.data_ptr(), q.data_ptr(), c.codes, c.scales, c.table, _lib.addr(seq), pos.data_ptr(),
+                                   _lib.addr(cos), _lib.addr(sin), positions, T, n_q, KV, D, c.page_shift, c.pages, c.rows, c.width,
+                                   c.table_stride, step, dtype, _lib.stream_of(dev), _lib.status_addr(x))
     _lib.check(rc, "atb_kv4_append")
     return q
 
@@ -190,18 +213,19 @@ def kv4_read(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tensor]
     """Keys and values ``[T, kv_heads, head_dim]`` that the cache stands for at the positions ``pos`` of the sequences ``seq``
     (as in :func:`kv4_append`); zeros where the position is negative. A prompt's own attention runs on them, so that its tokens
     see the same keys as the tokens after it."""
-    pages, KV, page_size, D = _sizes(layer, page_table)
-    if dtype not in _lib.DT:
+    c = _cache(layer, page_table)
+    kind, dev, T = _lib.DT.get(dtype), c.device, pos.numel()
+    if kind is None:
         raise ValueError(f"dtype is bf16, fp16 or fp32, got {dtype}")
-    T = pos.numel()
     seq, pos = _int32("seq", seq, T), _int32("pos", pos, T)
-    if not _on_gpu(D, *layer, page_table, pos, seq):
+    _same_device(dev, pos, seq)
+    if dev < 0:
         return kv4_read_reference(layer, page_table, seq, pos, dtype)
-    k, v = torch.empty(2, T, KV, D, dtype=dtype, device=pos.device).unbind(0)
-    rc = _lib.lib().atb_kv4_read(
-        k.data_ptr(), v.data_ptr(), layer[0].data_ptr(), layer[1].data_ptr(), page_table.data_ptr(), _lib.addr(seq), pos.data_ptr(),
-        T, KV, D, page_size.bit_length() - 1, pages, page_table.shape[0], page_table.shape[1], page_table.stride(0),
-        _lib.DT[dtype], _lib.stream(), _lib.status_addr(pos))
+    k = pos.new_empty((T, c.kv_heads, c.head_dim), dtype=dtype)
+    v = torch.empty_like(k)
+    rc = _lib.lib().atb_kv4_read(k.data_ptr(), v.data_ptr(), c.codes, c.scales, c.table, _lib.addr(seq), pos.data_ptr(), T, c.kv_heads,
+                                 c.head_dim, c.page_shift, c.pages, c.rows, c.width, c.table_stride, kind, _lib.stream_of(dev),
+                                 _lib.status_addr(pos))
     _lib.check(rc, "atb_kv4_read")
     return k, v
 
@@ -248,28 +272,31 @@ def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengt
     ``i`` sees the keys ``j < lengths - S + i + 1``. Query heads are shared as in :func:`~atorch_b200.ops.attention` (``n_q`` a
     multiple of the cache's heads). Returns ``[sequences, S, n_q, head_dim]``, and with ``return_lse`` the logarithms of the
     denominators, fp32 ``[sequences, n_q, S]``. A query that sees nothing gives zeros (and ``-inf``)."""
-    pages, KV, page_size, D = _sizes(layer, page_table)
+    c = _cache(layer, page_table)
+    KV, D, dev = c.kv_heads, c.head_dim, c.device
     if q.dim() != 4 or q.shape[3] != D or q.shape[2] % KV or q.shape[2] == 0:
         raise ValueError(f"q {tuple(q.shape)}: [sequences, S, a multiple of {KV}, {D}] is wanted")
-    if q.dtype not in (torch.bfloat16, torch.float16):
+    if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise ValueError(f"q is bf16 or fp16, got {q.dtype}")
     B, S, H, _ = q.shape
-    if page_table.shape[0] != B:
-        raise ValueError(f"page_table has {page_table.shape[0]} rows for {B} sequences")
+    if c.rows != B:
+        raise ValueError(f"page_table has {c.rows} rows for {B} sequences")
     _no_gradient(q)
     lengths = _int32("lengths", lengths, B)
-    if not _on_gpu(D, q, *layer, page_table, lengths):
+    _same_device(dev, q, lengths)
+    if dev < 0:
         out, lse = kv4_attention_reference(q, layer, page_table, lengths, softmax_scale)
         return (out, lse) if return_lse else out
-    if q.stride(3) != 1 or q.stride(2) != D or not (_aligned(q, q.stride(0)) and _aligned(q, q.stride(1))):
+    q_batch, q_token, q_head, one = q.stride()
+    if one != 1 or q_head != D or (q.data_ptr() | 2 * q_batch | 2 * q_token) & 15:
         q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty(B, S, H, D, dtype=q.dtype, device=q.device)
+        q_batch, q_token = S * H * D, H * D
+    out = q.new_empty(B, S, H, D)
     lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if return_lse else None
-    partial = torch.empty(_scratch(B, H, KV, S, D), dtype=torch.float32, device=q.device)
+    partial = q.new_empty(_scratch(B, H, KV, S, D), dtype=torch.float32)
     rc = _lib.lib().atb_kv4_attention(
-        q.data_ptr(), out.data_ptr(), _lib.addr(lse), layer[0].data_ptr(), layer[1].data_ptr(), page_table.data_ptr(),
-        lengths.data_ptr(), partial.data_ptr(), S, H, KV, D, page_size.bit_length() - 1, pages, B, page_table.shape[1],
-        page_table.stride(0), q.stride(0), q.stride(1), softmax_scale if softmax_scale is not None else D ** -0.5,
-        _lib.DT[q.dtype], _lib.stream(), _lib.status_addr(q))
+        q.data_ptr(), out.data_ptr(), _lib.addr(lse), c.codes, c.scales, c.table, lengths.data_ptr(), partial.data_ptr(), S, H, KV, D,
+        c.page_shift, c.pages, B, c.width, c.table_stride, q_batch, q_token, softmax_scale if softmax_scale is not None else D ** -0.5,
+        _lib.DT[q.dtype], _lib.stream_of(dev), _lib.status_addr(q))
     _lib.check(rc, "atb_kv4_attention")
     return (out, lse) if return_lse else out

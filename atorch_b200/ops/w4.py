@@ -16,6 +16,7 @@ from .. import _lib
 from .gemm import gemm
 
 GROUPS = (32, 64, 128)
+_LOW = (torch.bfloat16, torch.float16)
 # rows of x from which the weights are expanded to bf16 and multiplied by the GEMM, with bf16 x and K a multiple of 8
 EXPAND_ROWS = 65
 
@@ -52,10 +53,11 @@ def _check_group(group_size: int) -> None:
 
 
 def _check(codes, scales, K, group_size) -> None:
-    _check_group(group_size)
-    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or codes.dim() != 2 or scales.dim() != 2 or K < 1 \
-            or codes.shape[1] != (K + 31) // 32 * 16 or scales.shape[0] != codes.shape[0] \
-            or scales.shape[1] != (K + group_size - 1) // group_size:
+    if group_size not in GROUPS:
+        _check_group(group_size)
+    N = codes.shape[0] if codes.dim() == 2 else -1
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or K < 1 or codes.shape != (N, (K + 31) // 32 * 16) \
+            or scales.shape != (N, (K + group_size - 1) // group_size):
         raise ValueError(f"codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not a "
                          f"weight of {K} columns in groups of {group_size}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
@@ -72,33 +74,35 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
     """``x @ W.T (+ bias)`` for ``x`` ``[..., K]`` in bf16 or fp16 and the weight that ``codes`` and ``scales`` stand for; sums in
     fp32, the result in the type of ``x``. Made for the few rows of a decode step; many bf16 rows expand the weight for the call and
     run the GEMM (the weight is rounded to bf16 there)."""
-    K = x.shape[-1]
+    K, N = x.shape[-1], codes.shape[0]
     _check(codes, scales, K, group_size)
-    if x.dtype not in (torch.bfloat16, torch.float16):
+    if x.dtype not in _LOW:
         raise ValueError(f"x is bf16 or fp16, got {x.dtype}")
-    N = codes.shape[0]
     if bias is not None and (bias.dtype is not x.dtype or bias.shape != (N,)):
         raise ValueError(f"bias is {x.dtype} [{N}], got {bias.dtype} {tuple(bias.shape)}")
-    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("4-bit weights have no gradient: call under torch.no_grad()")
-    if not (x.device == codes.device == scales.device and (bias is None or bias.device == x.device)):
+    dev = x.get_device()
+    if codes.get_device() != dev or scales.get_device() != dev or (bias is not None and bias.get_device() != dev):
         raise ValueError("x, codes, scales and bias are on several devices")
-    if not _lib.use_kernels(x):
+    if dev < 0 or not _lib.use_kernels(x):
         return w4_linear_reference(x, codes, scales, group_size, bias)
-    M = x.numel() // K
-    x2 = x if x.dim() == 2 and x.stride(1) == 1 else x.reshape(M, K)
-    if x2.stride(1) != 1:
-        x2 = x2.contiguous()
+    x2 = x if x.dim() == 2 else x.reshape(x.numel() // K, K)
+    step, one = x2.stride()
+    if one != 1:
+        x2, step = x2.contiguous(), K
+    M = x2.shape[0]
     if M >= EXPAND_ROWS and x.dtype is torch.bfloat16 and K % 8 == 0:
         w = torch.empty(N, K, dtype=x.dtype, device=x.device)
         rc = _lib.lib().atb_w4_expand(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), N, K, group_size, _lib.DT[x.dtype],
-                                      _lib.stream())
+                                      _lib.stream_of(dev))
         _lib.check(rc, "atb_w4_expand")
         return gemm(x2, w, bias=bias).view(*x.shape[:-1], N)
-    y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-    codes_ok = codes if codes.data_ptr() % 16 == 0 else codes.clone()
-    wide = x2.data_ptr() % 16 == 0 and x2.stride(0) % 8 == 0
-    rc = _lib.lib().atb_w4_linear(x2.data_ptr(), codes_ok.data_ptr(), scales.data_ptr(), _lib.addr(bias), y.data_ptr(), M, N, K,
-                                  group_size, x2.stride(0), int(wide), _lib.DT[x.dtype], _lib.stream(), _lib.status_addr(x))
+    y = x.new_empty(*x.shape[:-1], N)
+    base = x2.data_ptr()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    rc = _lib.lib().atb_w4_linear(base, codes.data_ptr(), scales.data_ptr(), _lib.addr(bias), y.data_ptr(), M, N, K, group_size, step,
+                                  int(base % 16 == 0 and step % 8 == 0), _lib.DT[x.dtype], _lib.stream_of(dev), _lib.status_addr(x))
     _lib.check(rc, "atb_w4_linear")
     return y
