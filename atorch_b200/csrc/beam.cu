@@ -2,12 +2,15 @@
 //
 // A continuation of beam w by token v has f = score[w] + (x[w, v] - lse(x[w])), evaluated in fp32 in this order; NaN counts as
 // -inf. The `keep` largest f of a sequence's beams are kept, equal ones by the lower w, then the lower v.
+#include <cooperative_groups.h>
 #include "common.cuh"
 
 namespace {
 using namespace atb;
+namespace cg = cooperative_groups;
 
-constexpr int THREADS = 512, MOST = 32, ROOM = 1024;      // threads of a row, beams, candidates that a row has room for
+// threads of a share of a row, beams, candidates that a share has room for, groups of lanes whose maxima are ranked
+constexpr int THREADS = 256, MOST = 32, ROOM = 512, GROUPS = THREADS / 4;
 
 // A number whose order as an unsigned integer is that of f (both zeros alike), then of the lower index.
 ATB_DEVICE unsigned long long key_of(float f, unsigned index) {
@@ -45,104 +48,139 @@ ATB_DEVICE unsigned long long block_max_key(unsigned long long k, unsigned long 
   return t;
 }
 
-// Calls f(value, index) for the elements of a row that this thread has: 16-byte pieces where the row allows it.
+// Calls f(value, index) for the elements [from, to) of a row that this thread has: 16-byte pieces where the row allows it (`wide`:
+// it begins on 16 bytes; `from` is a multiple of 8).
 template <typename T, typename F>
-ATB_DEVICE void each(const T* row, int V, bool wide, F f) {
+ATB_DEVICE void each(const T* row, int from, int to, bool wide, F f) {
   constexpr int N = 16 / sizeof(T);
-  const int pieces = wide ? V / N : 0;
+  const int pieces = wide ? (to - from) / N : 0;
   for (int i = threadIdx.x; i < pieces; i += THREADS) {
-    const uint4 u = reinterpret_cast<const uint4*>(row)[i];
+    const uint4 u = reinterpret_cast<const uint4*>(row + from)[i];
     const T* h = reinterpret_cast<const T*>(&u);
 #pragma unroll
-    for (int e = 0; e < N; ++e) f(to_f32<T>(h[e]), i * N + e);
+    for (int e = 0; e < N; ++e) f(to_f32<T>(h[e]), from + i * N + e);
   }
-  for (int i = pieces * N + threadIdx.x; i < V; i += THREADS) f(to_f32<T>(row[i]), i);
+  for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) f(to_f32<T>(row[i]), i);
+}
+// Maximum and sum of exponentials relative to it, of two sets
+struct Sum {
+  float top, sum;
+};
+ATB_DEVICE Sum add(Sum a, Sum b) {
+  const float top = fmaxf(a.top, b.top);
+  return Sum{top, a.sum * (a.top == top ? 1.f : expf(a.top - top)) + b.sum * (b.top == top ? 1.f : expf(b.top - top))};
 }
 
-// The `keep` best continuations of one beam (a block), best first, as keys of f and token.
+// The `keep` best continuations of one beam, best first, as keys of f and token. The blocks of a cluster have a share of the
+// vocabulary each: they add up the row's sum of exponentials through each other's shared memory, each picks the best of its share,
+// and the first picks the best of those. The row comes from memory once, and from the first-level cache after that. Bound by
+// latency for a few beams (one block a row, with the row's 64 KB read three times from L2, took 17 us).
 template <typename T>
 __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, const float* scores, const unsigned char* finished,
                                                            unsigned long long* best, int V, long long row_stride, int wide,
                                                            int eos, int keep, const int* status) {
-  __shared__ float red[33];
-  __shared__ unsigned long long red_key[THREADS / 32], room[ROOM], tops[THREADS];
+  __shared__ Sum warp_sums[THREADS / 32], share_sum;
+  __shared__ unsigned long long red_key[THREADS / 32], room[ROOM], tops[GROUPS], mine[MOST];
+  __shared__ float least;
   __shared__ int count;
   grid_go();
   grid_wait();
-  if (__syncthreads_or(threadIdx.x == 0 && *status != 0)) return;
-  const long long row = blockIdx.x;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int shares = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
+  const long long row = blockIdx.x / shares;
+  const bool failed = *status != 0;      // nothing is stored then; the blocks of a cluster stay together
   const float score = scores[row];
+  const bool ended = finished && finished[row];
   unsigned long long* out = best + row * keep;
-  const int n = min(keep, V);                      // what the row has; the rest is below everything
-  for (int i = n + threadIdx.x; i < keep; i += THREADS) out[i] = 0;
-  if (finished && finished[row]) {
-    // only the end token goes on, at no cost; the others are impossible, and stand in their order
-    for (int i = threadIdx.x; i < n; i += THREADS) {
-      if (score == -INFINITY || score != score) out[i] = key_of(-INFINITY, i);
-      else out[i] = i == 0 ? key_of(score, eos) : key_of(-INFINITY, i - 1 < eos ? i - 1 : i);
+  if (ended || score == -INFINITY || score != score) {
+    // the end token alone goes on, at no cost, or nothing; the others are impossible, and stand in their order
+    const bool only = ended && score != -INFINITY && score == score;
+    if (rank == 0 && threadIdx.x < keep && !failed) {
+      const int i = threadIdx.x;
+      out[i] = i >= V ? 0 : !only ? key_of(-INFINITY, i) : i == 0 ? key_of(score, eos) : key_of(-INFINITY, i - 1 < eos ? i - 1 : i);
     }
     return;
   }
-  if (score == -INFINITY || score != score) {
-    for (int i = threadIdx.x; i < n; i += THREADS) out[i] = key_of(-INFINITY, i);
-    return;
-  }
   const T* x = logits + row * row_stride;
-  float top = -INFINITY;
-  bool bad = false;
-  each<T>(x, V, wide, [&](float v, int) {
-    top = fmaxf(top, v);
-    bad = bad || v != v;
-  });
-  const float row_top = block_max(top, red);
-  float sum = 0.f;
-  each<T>(x, V, wide, [&](float v, int) { sum += expf(v - row_top); });
-  sum = block_sum(sum, red);
-  float lse = row_top + logf(sum);
-  if (__syncthreads_or(bad)) lse = __int_as_float(0x7fc00000);      // a NaN makes every f of the row one
-
-  // the n-th largest of the threads' maxima: no fewer than n continuations reach it
-  tops[threadIdx.x] = key_of(total(score, top, lse), threadIdx.x);
+  const int part = ((V + shares - 1) / shares + 7) / 8 * 8, from = min(V, rank * part), to = min(V, from + part);
+  Sum s{-INFINITY, 0.f};
+  each<T>(x, from, to, wide, [&](float v, int) { s.top = fmaxf(s.top, v); });
+  const float ref = s.top == -INFINITY ? 0.f : s.top;
+  each<T>(x, from, to, wide, [&](float v, int) { s.sum += expf(v - ref); });       // (a NaN makes the sum one)
+  const float my_top = s.top;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s = add(s, Sum{__shfl_xor_sync(0xffffffffu, s.top, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
+  if (lane == 0) warp_sums[threadIdx.x >> 5] = s;
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
-  int rank = 0;
-  for (int i = 0; i < THREADS; ++i) rank += tops[i] > tops[threadIdx.x];
-  if (rank == n - 1) red[32] = value_of(tops[threadIdx.x]);
+  if (threadIdx.x == 0) {
+    s = warp_sums[0];
+    for (int i = 1; i < THREADS / 32; ++i) s = add(s, warp_sums[i]);
+    share_sum = s;
+  }
+  cluster.sync();
+  s = *cluster.map_shared_rank(&share_sum, 0);
+  for (int i = 1; i < shares; ++i) s = add(s, *cluster.map_shared_rank(&share_sum, i));
+  const float lse = s.top + logf(s.sum);
+
+  // the n-th largest of the maxima of four lanes: no fewer than n continuations of the share reach it
+  const int n = min(keep, to - from);
+  float group_top = fmaxf(my_top, __shfl_xor_sync(0xffffffffu, my_top, 1));
+  group_top = fmaxf(group_top, __shfl_xor_sync(0xffffffffu, group_top, 2));
+  if ((lane & 3) == 0) tops[threadIdx.x / 4] = key_of(total(score, group_top, lse), threadIdx.x / 4);
   __syncthreads();
-  const float least = red[32];
-  if (least > -INFINITY) {
-    each<T>(x, V, wide, [&](float v, int i) {
+  if (threadIdx.x < GROUPS) {
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < GROUPS; ++i) place += tops[i] > tops[threadIdx.x];
+    if (place == max(n, 1) - 1) least = value_of(tops[threadIdx.x]);
+  }
+  if (threadIdx.x < MOST) mine[threadIdx.x] = 0;
+  __syncthreads();
+  const float reach = least;
+  if (reach > -INFINITY)
+    each<T>(x, from, to, wide, [&](float v, int i) {
       const float f = total(score, v, lse);
-      if (f >= least) {
+      if (f >= reach) {
         const int at = atomicAdd(&count, 1);
         if (at < ROOM) room[at] = key_of(f, i);
       }
     });
-  } else if (threadIdx.x == 0) {
-    count = ROOM + 1;
-  }
   __syncthreads();
   const int have = count;
-  if (have <= ROOM) {
+  if (reach > -INFINITY && have <= ROOM) {
     for (int i = threadIdx.x; i < have; i += THREADS) {
       const unsigned long long k = room[i];
       int place = 0;
       for (int j = 0; j < have; ++j) place += room[j] > k;
-      if (place < n) out[place] = k;
+      if (place < n) mine[place] = k;
     }
-    return;
+  } else {
+    // too many reach it, or too few continuations are possible at all: one after another
+    unsigned long long last = ~0ull;
+    for (int k = 0; k < n; ++k) {
+      unsigned long long most = 0;
+      each<T>(x, from, to, wide, [&](float v, int i) {
+        const unsigned long long key = key_of(total(score, v, lse), i);
+        if (key < last && key > most) most = key;
+      });
+      last = block_max_key(most, red_key);
+      if (threadIdx.x == 0) mine[k] = last;
+    }
   }
-  // too many reach it, or too few continuations are possible at all: one after another
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < n; ++k) {
-    unsigned long long mine = 0;
-    each<T>(x, V, wide, [&](float v, int i) {
-      const unsigned long long key = key_of(total(score, v, lse), i);
-      if (key < last && key > mine) mine = key;
-    });
-    last = block_max_key(mine, red_key);
-    if (threadIdx.x == 0) out[k] = last;
+  cluster.sync();
+  if (rank == 0) {
+    const int all = shares * keep;               // keys of the shares, best first each
+    for (int i = threadIdx.x; i < all; i += THREADS) room[i] = *cluster.map_shared_rank(&mine[i % keep], i / keep);
+    __syncthreads();
+    for (int i = threadIdx.x; i < all; i += THREADS) {
+      const unsigned long long k = room[i];
+      int place = 0;
+      for (int j = 0; j < all; ++j) place += room[j] > k || (room[j] == k && j < i);     // (only what is not there is equal)
+      if (place < keep && !failed) out[place] = k;
+    }
   }
+  cluster.sync();                                // the first has read the others' keys
 }
 
 // The best of a sequence's beams (a block): each of the W keep continuations counts those before it.
@@ -152,7 +190,7 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long
   __shared__ unsigned long long all[MOST * MOST];
   grid_go();
   grid_wait();
-  if (__syncthreads_or(threadIdx.x == 0 && *status != 0)) return;
+  const bool failed = *status != 0;
   const long long b = blockIdx.x;
   const int n = W * keep;
   for (int i = threadIdx.x; i < n; i += 256) all[i] = best[b * n + i];
@@ -167,7 +205,7 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long
       const uint32_t fo = (uint32_t)(o >> 32), fk = (uint32_t)(k >> 32);
       place += fo != fk ? fo > fk : j < i;
     }
-    if (place >= keep || k == 0) continue;
+    if (place >= keep || k == 0 || failed) continue;
     const long long at = b * keep + place;
     scores[at] = value_of(k);
     tokens[at] = index_of(k);
@@ -178,17 +216,18 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long
 
 // The cache follows its beams: row b W + w of the table takes the full pages of row b W + parent[w], and its own last page the
 // tokens of that row's last page. A thread has one place of all W rows and reads them all before it writes any, so the rows may
-// change places. Bound by memory: each token of the last pages that moves is read and written once.
+// change places. Bound by memory: each token of the last pages that moves is read and written once. What it
+// looks up before, lengths, parents and pages, serves several layers.
 template <int MAX_W>
 __global__ void __launch_bounds__(256) beam_reorder_kernel(uint8_t* codes, uint8_t* scales, int* table, const int* lengths,
                                                            const int* parents, int W, int width, long long table_stride,
-                                                           int pages, long long page_bytes, long long scale_bytes,
+                                                           int layers, int pages, long long page_bytes, long long scale_bytes,
                                                            int kv_heads, int page_shift, int token_bytes, int* status) {
   grid_go();
   grid_wait();
   if (__syncthreads_or(threadIdx.x == 0 && *status != 0)) return;
   const long long b = blockIdx.y, first = b * W;
-  const int layer = (int)blockIdx.z - 1, n = lengths[first], full = n >> page_shift, rest = n - (full << page_shift);
+  const int n = lengths[first], full = n >> page_shift, rest = n - (full << page_shift);
   int from[MAX_W];
   bool good = n >= 0 && full + (rest > 0) <= width;
 #pragma unroll
@@ -200,7 +239,7 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(uint8_t* codes, uint8
     if (threadIdx.x == 0) atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
     return;
   }
-  if (layer < 0) {                // the table
+  if (blockIdx.z == gridDim.z - 1) {                // the table
     for (int i = blockIdx.x * 256 + threadIdx.x; i < full; i += gridDim.x * 256) {
       int x[MAX_W];
 #pragma unroll
@@ -232,29 +271,29 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(uint8_t* codes, uint8
   }
   const int per_token = token_bytes / 16, per_head = rest * per_token, code_pieces = 2 * kv_heads * per_head;
   const int head_bytes = token_bytes << page_shift, all = code_pieces + kv_heads * rest;
-  uint8_t* const layer_codes = codes + (long long)layer * pages * page_bytes;
-  uint8_t* const layer_scales = scales + (long long)layer * pages * scale_bytes;
   for (int i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
-    if (i < code_pieces) {
-      const int h = i / per_head;
-      const long long at = (long long)h * head_bytes + (i - h * per_head) * 16;
+    const bool code = i < code_pieces;
+    const int j = code ? i : i - code_pieces, h = j / (code ? per_head : rest);
+    const long long at = code ? (long long)h * head_bytes + (j - h * per_head) * 16 : ((long long)h << (page_shift + 3)) + (j - h * rest) * 8;
+    const long long bytes = code ? page_bytes : scale_bytes;
+    uint8_t* const base = (code ? codes : scales) + at;
+    for (int layer = blockIdx.z; layer < layers; layer += gridDim.z - 1) {
+      uint8_t* const here = base + (long long)layer * pages * bytes;
       uint4 x[MAX_W];
 #pragma unroll
       for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) x[w] = *reinterpret_cast<const uint4*>(layer_codes + source[w] * page_bytes + at);
+        if (w < W && from[w] != w) {
+          const uint8_t* p = here + source[w] * bytes;
+          if (code) x[w] = *reinterpret_cast<const uint4*>(p);
+          else *reinterpret_cast<uint2*>(&x[w]) = *reinterpret_cast<const uint2*>(p);
+        }
 #pragma unroll
       for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) *reinterpret_cast<uint4*>(layer_codes + page[w] * page_bytes + at) = x[w];
-    } else {
-      const int j = i - code_pieces, h = j / rest;
-      const long long at = ((long long)h << (page_shift + 3)) + (j - h * rest) * 8;
-      uint2 x[MAX_W];
-#pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) x[w] = *reinterpret_cast<const uint2*>(layer_scales + source[w] * scale_bytes + at);
-#pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) *reinterpret_cast<uint2*>(layer_scales + page[w] * scale_bytes + at) = x[w];
+        if (w < W && from[w] != w) {
+          uint8_t* p = here + page[w] * bytes;
+          if (code) *reinterpret_cast<uint4*>(p) = x[w];
+          else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&x[w]);
+        }
     }
   }
 }
@@ -264,11 +303,13 @@ extern "C" int atb_beam_select(const void* logits, const void* scores, const voi
                                void* tokens, void* parents, void* ended, int B, int W, int V, long long row_stride, int wide,
                                int eos, int keep, int dtype, void* stream, void* status) {
   if (B <= 0 || keep <= 0) return 0;
-  if (W < 1 || W > MOST || keep > MOST || V < 1 || (long long)B * W > 0x7fffffffLL) return -1;
+  if (W < 1 || W > MOST || keep > MOST || V < 1 || (long long)B * W > 0x7fffffffLL / 8) return -1;
+  int shares = 1;      // of 2000 tokens at least
+  while (shares < 8 && V >= 4000 * shares) shares *= 2;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc = cudaErrorInvalidValue;
 #define ROWS(T)                                                                                                          \
-  rc = launch_after(beam_row_kernel<T>, dim3(B * W), THREADS, 0, st, 1, (const T*)logits, (const float*)scores,           \
+  rc = launch_after(beam_row_kernel<T>, dim3(B * W * shares), THREADS, 0, st, shares, (const T*)logits, (const float*)scores,           \
                     (const unsigned char*)finished, (unsigned long long*)best, V, row_stride, wide, eos, keep, (const int*)status)
   if (dtype == 0) ROWS(__nv_bfloat16);
   if (dtype == 1) ROWS(__half);
@@ -289,11 +330,13 @@ extern "C" int atb_beam_reorder(void* codes, void* scales, void* table, const vo
   const long long page_bytes = (2LL * kv_heads * token_bytes) << page_shift, scale_bytes = (8LL * kv_heads) << page_shift;
   const long long most = (2LL * kv_heads * token_bytes / 16 + kv_heads) << page_shift;
   if (page_bytes > 0x7fffffffLL || most > 0x7fffffffLL) return -2;
-  const dim3 grid((unsigned)((most + 255) / 256), B, layers + 1);
+  // layers in as many shares as give four blocks an SM, and one share for the table
+  const long long blocks = (most + 255) / 256 * B, want = (148 * 4 + blocks - 1) / blocks;
+  const dim3 grid((unsigned)((most + 255) / 256), B, (unsigned)((want < layers ? want : layers) + 1));
   cudaError_t rc;
 #define MOVE(MAX_W)                                                                                                        \
   rc = launch_after(beam_reorder_kernel<MAX_W>, grid, 256, 0, (cudaStream_t)stream, 1, (uint8_t*)codes, (uint8_t*)scales,    \
-                    (int*)table, (const int*)lengths, (const int*)parents, W, width, table_stride, pages, page_bytes,       \
+                    (int*)table, (const int*)lengths, (const int*)parents, W, width, table_stride, layers, pages, page_bytes,       \
                     scale_bytes, kv_heads, page_shift, token_bytes, (int*)status)
   if (W <= 4) MOVE(4);
   else if (W <= 8) MOVE(8);
