@@ -3,6 +3,7 @@
 // A continuation of beam w by token v has f = score[w] + (x[w, v] - lse(x[w])), evaluated in fp32 in this order; NaN counts as
 // -inf. The `keep` largest f of a sequence's beams are kept, equal ones by the lower w, then the lower v.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include "common.cuh"
 
 namespace {
@@ -48,19 +49,33 @@ ATB_DEVICE unsigned long long block_max_key(unsigned long long k, unsigned long 
   return t;
 }
 
-// Calls f(value, index) for the elements [from, to) of a row that this thread has: 16-byte pieces where the row allows it (`wide`:
-// it begins on 16 bytes; `from` is a multiple of 8).
-template <typename T, typename F>
-ATB_DEVICE void each(const T* row, int from, int to, bool wide, F f) {
-  constexpr int N = 16 / sizeof(T);
-  const int pieces = wide ? (to - from) / N : 0;
-  for (int i = threadIdx.x; i < pieces; i += THREADS) {
-    const uint4 u = reinterpret_cast<const uint4*>(row + from)[i];
-    const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int e = 0; e < N; ++e) f(to_f32<T>(h[e]), from + i * N + e);
+// Calls f(values, n, index) for the elements [from, to) of a row that this thread has, in 16-byte pieces where the row allows it
+// (`wide`: it begins on 16 bytes; `from` is a multiple of 8), else one by one, n = 1.
+template <typename T>
+struct Piece {
+  static constexpr int N = 16 / sizeof(T);
+  uint4 u;
+  ATB_DEVICE float operator[](int i) const { return to_f32<T>(reinterpret_cast<const T*>(&u)[i]); }
+  // the largest of the piece; NaNs are passed over. 16-bit values are compared two at a time as they are.
+  ATB_DEVICE float top() const {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf((*this)[0], (*this)[1]), fmaxf((*this)[2], (*this)[3]));
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const T2* h = reinterpret_cast<const T2*>(&u);
+      const T2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      return fmaxf(to_f32<T>(m.x), to_f32<T>(m.y));
+    }
   }
-  for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) f(to_f32<T>(row[i]), i);
+};
+template <typename T, typename F, typename G>
+ATB_DEVICE void each(const T* row, int from, int to, bool wide, F f, G one) {
+  constexpr int N = Piece<T>::N;
+  const int pieces = wide ? (to - from) / N : 0;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < pieces; i += THREADS)
+    f(Piece<T>{reinterpret_cast<const uint4*>(row + from)[i]}, from + i * N);
+  for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) one(to_f32<T>(row[i]), i);
 }
 // Maximum and sum of exponentials relative to it, of two sets
 struct Sum {
@@ -104,9 +119,14 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
   const T* x = logits + row * row_stride;
   const int part = ((V + shares - 1) / shares + 7) / 8 * 8, from = min(V, rank * part), to = min(V, from + part);
   Sum s{-INFINITY, 0.f};
-  each<T>(x, from, to, wide, [&](float v, int) { s.top = fmaxf(s.top, v); });
-  const float ref = s.top == -INFINITY ? 0.f : s.top;
-  each<T>(x, from, to, wide, [&](float v, int) { s.sum += expf(v - ref); });       // (a NaN makes the sum one)
+  each<T>(x, from, to, wide, [&](const Piece<T>& v, int) { s.top = fmaxf(s.top, v.top()); },
+          [&](float v, int) { s.top = fmaxf(s.top, v); });
+  const float ref = s.top == -INFINITY ? 0.f : s.top, log2e = 1.4426950408889634f, ref2 = ref * log2e;
+  // exponentials on the special-function unit, off by 2^-22: a sum of thousands is as near as its fp32 adds
+  each<T>(x, from, to, wide, [&](const Piece<T>& v, int) {
+#pragma unroll
+            for (int e = 0; e < Piece<T>::N; ++e) s.sum += fast_exp2(fmaf(v[e], log2e, -ref2));       // (a NaN makes the sum one)
+          }, [&](float v, int) { s.sum += fast_exp2(fmaf(v, log2e, -ref2)); });
   const float my_top = s.top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s = add(s, Sum{__shfl_xor_sync(0xffffffffu, s.top, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});
@@ -138,14 +158,22 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
   if (threadIdx.x < MOST) mine[threadIdx.x] = 0;
   __syncthreads();
   const float reach = least;
+  // f grows with x; an x whose f may round up to `reach` is not further below its x than a few roundings
+  const float x_reach = (reach - score + lse) - 4.8e-7f * (fabsf(reach) + fabsf(score) + fabsf(lse));
+  auto take = [&](float v, int i) {
+    const float f = total(score, v, lse);
+    if (f >= reach) {
+      const int at = atomicAdd(&count, 1);
+      if (at < ROOM) room[at] = key_of(f, i);
+    }
+  };
   if (reach > -INFINITY)
-    each<T>(x, from, to, wide, [&](float v, int i) {
-      const float f = total(score, v, lse);
-      if (f >= reach) {
-        const int at = atomicAdd(&count, 1);
-        if (at < ROOM) room[at] = key_of(f, i);
-      }
-    });
+    each<T>(x, from, to, wide, [&](const Piece<T>& v, int i) {
+              if (v.top() >= x_reach) {
+#pragma unroll
+                for (int e = 0; e < Piece<T>::N; ++e) take(v[e], i + e);
+              }
+            }, take);
   __syncthreads();
   const int have = count;
   if (reach > -INFINITY && have <= ROOM) {
@@ -160,10 +188,13 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
     unsigned long long last = ~0ull;
     for (int k = 0; k < n; ++k) {
       unsigned long long most = 0;
-      each<T>(x, from, to, wide, [&](float v, int i) {
+      auto look = [&](float v, int i) {
         const unsigned long long key = key_of(total(score, v, lse), i);
         if (key < last && key > most) most = key;
-      });
+      };
+      each<T>(x, from, to, wide, [&](const Piece<T>& v, int i) {
+                for (int e = 0; e < Piece<T>::N; ++e) look(v[e], i + e);
+              }, look);
       last = block_max_key(most, red_key);
       if (threadIdx.x == 0) mine[k] = last;
     }
@@ -304,8 +335,8 @@ extern "C" int atb_beam_select(const void* logits, const void* scores, const voi
                                int eos, int keep, int dtype, void* stream, void* status) {
   if (B <= 0 || keep <= 0) return 0;
   if (W < 1 || W > MOST || keep > MOST || V < 1 || (long long)B * W > 0x7fffffffLL / 8) return -1;
-  int shares = 1;      // of 2000 tokens at least
-  while (shares < 8 && V >= 4000 * shares) shares *= 2;
+  int shares = 1;      // of 2000 tokens at least, as long as all of them are on the GPU at once
+  while (shares < 8 && V >= 4000 * shares && (long long)B * W * shares * 2 <= 4 * 148) shares *= 2;
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc = cudaErrorInvalidValue;
 #define ROWS(T)                                                                                                          \
