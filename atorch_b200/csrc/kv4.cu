@@ -361,7 +361,7 @@ struct AttnArgs {
   long long q_batch, q_token; // strides of q, elements
   int S, heads, group;
   float scale_log2;           // softmax scale * log2(e)
-  int ctas;
+  int ctas;                   // blocks that the work is cut for; 0: a block takes whole sequences (of a head), one after another
   int* status;
 };
 
@@ -409,9 +409,14 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   grid_wait();
   if (__syncthreads_or(threadIdx.x == 0 && *a.status != 0)) return;    // one answer for the block: others may fail meanwhile
   const int columns = a.S * a.group, col_tiles = (columns + COLS - 1) / COLS, per = col_tiles * c.kv_heads;
-  const Plan plan = make_plan(c, a.lengths, per, a.ctas, a.status);
-  if ((int)blockIdx.x >= plan.ctas) return;
-  const long long run = plan.begin(blockIdx.x), run_end = plan.begin(blockIdx.x + 1);
+  Plan plan{};
+  long long u = blockIdx.x, run_end = (long long)c.rows * per;       // whole sequences: their numbers
+  if (a.ctas > 0) {
+    plan = make_plan(c, a.lengths, per, a.ctas, a.status);
+    if ((int)blockIdx.x >= plan.ctas) return;
+    u = plan.begin(blockIdx.x);
+    run_end = plan.begin(blockIdx.x + 1);
+  }
   uint32_t loads = 0;            // tiles that this warp has taken from its ring
 
   // A tile is two pieces of 16 tokens, each in one page, of three copies: keys, values, scales. Lane 3 p + x has copy x of piece p.
@@ -421,22 +426,29 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   const int token_bytes = what < 2 ? D / 2 : 8;
   const int dst_at = (what < 2 ? what * (TILE * D / 2) : TILE * D) + piece * 16 * token_bytes;
 
-  for (long long u = run; u < run_end;) {
-    int b, len;
-    long long first;
-    find_sequence(c, a.lengths, per, u, b, len, first, a.status);
-    const int tiles = tiles_of(len), hc = (int)((u - first) / (START + tiles));
-    const int head = hc % c.kv_heads, col_tile = hc / c.kv_heads;
-    const long long begin = first + (long long)hc * (START + tiles);       // of the sequence, for this head
-    const int t_first = max(0, (int)(u - begin) - START);                  // tiles of this segment
-    const int t_last = (int)min(run_end - begin - START, (long long)tiles);
-    u = begin + START + t_last;
-    if (t_last <= t_first) {      // the run ends before the first tile
-      u = run_end;
-      continue;
+  while (u < run_end) {
+    int b, len, hc, tiles, t_first = 0, t_last;       // the segment: tiles [t_first, t_last) of a sequence
+    long long begin = 0;
+    if (a.ctas > 0) {
+      long long first;
+      find_sequence(c, a.lengths, per, u, b, len, first, a.status);
+      tiles = tiles_of(len);
+      hc = (int)((u - first) / (START + tiles));
+      begin = first + (long long)hc * (START + tiles);
+      t_first = max(0, (int)(u - begin) - START);
+      t_last = (int)min(run_end - begin - START, (long long)tiles);
+      u = begin + START + t_last;
+      if (t_last <= t_first) break;      // the run ends before the first tile
+    } else {
+      b = (int)(u / per);
+      hc = (int)(u - (long long)b * per);
+      len = seen_length(c, a.lengths, b, a.status);
+      t_last = tiles = tiles_of(len);
+      u += gridDim.x;
     }
+    const int head = hc % c.kv_heads, col_tile = hc / c.kv_heads;
     const bool whole = t_first == 0 && t_last == tiles;
-    if (t_first == 0 && threadIdx.x == 0)
+    if (a.ctas > 0 && t_first == 0 && threadIdx.x == 0)
       a.owners[(long long)b * per + hc] = make_int2(blockIdx.x, plan.owner(begin + START + tiles - 1));
     const int mine = len == 0 ? 0 : max(0, (t_last - t_first - warp + WARPS - 1) / WARPS);
     const int* const row = c.table + b * c.table_stride;
@@ -841,14 +853,20 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const long long per = (a.S * a.group + Sh::COLS - 1) / Sh::COLS * (long long)a.c.kv_heads;
-  const long long room = ((long long)a.c.width << a.c.page_shift) / TILE;       // tiles that a sequence can have
+  const long long room = (((long long)a.c.width << a.c.page_shift) + TILE - 1) / TILE;       // tiles that a sequence can have
   const long long most = (START + (room > 1 ? room : 1)) * a.c.rows * per, runs = a.c.rows * per;
   if (runs > 0x7fffffffLL) return -2;
+  // sequences of up to 256 tokens are not cut: two tiles a warp take less than a join and what the cutting needs to know
+  const bool cut = room > 8;
+  if (cut && !a.partial) return -1;
   a.ctas = 148 * Sh::BLOCKS;
-  a.owners = reinterpret_cast<int2*>(a.partial + 2LL * a.ctas * Sh::COLS * (D + 2));
+  if (cut) a.owners = reinterpret_cast<int2*>(a.partial + 2LL * a.ctas * Sh::COLS * (D + 2));
   const unsigned grid = (unsigned)(most < a.ctas ? most : a.ctas);
-  if (launch_after(kv4_attention_kernel<T, D, NT>, dim3(grid), WARPS * 32, Sh::RING, st, 1, a) != cudaSuccess) return -5;
-  if (room <= 1) return 0;                                                         // nothing to cut
+  if (!cut) a.ctas = 0;
+  if (launch_after(kv4_attention_kernel<T, D, NT>, dim3(cut || runs > grid ? grid : (unsigned)runs), WARPS * 32, Sh::RING, st, 1, a) !=
+      cudaSuccess)
+    return -5;
+  if (!cut) return 0;
   return launch_after(kv4_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per) == cudaSuccess ? 0 : -5;
 }
 }  // namespace
@@ -902,6 +920,7 @@ extern "C" int atb_kv4_attention(const void* q, void* out, void* lse, void* code
   a.lengths = (const int*)lengths;
   a.q = q;
   a.out = out;
+  a.owners = nullptr;
   a.lse = (float*)lse;
   a.partial = (float*)partial;
   a.q_batch = q_batch;

@@ -24,6 +24,7 @@ from .. import _lib
 
 Layer = Tuple[torch.Tensor, torch.Tensor]
 HEAD_DIMS = (64, 128)          # of the kernels; the CPU path takes any even one
+WHOLE = 256                    # tokens up to which the kernel never cuts a sequence, and needs no workspace (csrc/kv4.cu)
 
 
 class KV4Cache:
@@ -293,9 +294,9 @@ def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengt
         q_batch, q_token = S * H * D, H * D
     out = q.new_empty(B, S, H, D)
     lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if return_lse else None
-    partial = q.new_empty(_scratch(B, H, KV, S, D), dtype=torch.float32)
+    partial = None if c.width << c.page_shift <= WHOLE else torch.empty(_scratch(B, H, KV, S, D), dtype=torch.float32, device=q.device)
     rc = _lib.lib().atb_kv4_attention(
-        q.data_ptr(), out.data_ptr(), _lib.addr(lse), c.codes, c.scales, c.table, lengths.data_ptr(), partial.data_ptr(), S, H, KV, D,
+        q.data_ptr(), out.data_ptr(), _lib.addr(lse), c.codes, c.scales, c.table, lengths.data_ptr(), _lib.addr(partial), S, H, KV, D,
         c.page_shift, c.pages, B, c.width, c.table_stride, q_batch, q_token, softmax_scale if softmax_scale is not None else D ** -0.5,
         _lib.DT[q.dtype], _lib.stream_of(dev), _lib.status_addr(q))
     _lib.check(rc, "atb_kv4_attention")

@@ -1,0 +1,148 @@
+"""Generation with the 4-bit cache on the CPU: greedy, beams, sampling, 4-bit weights."""
+import pytest
+import torch
+
+from atorch_b200 import ops
+from atorch_b200.models.generate import CachedSampler, Generator, generate
+from atorch_b200.models.llama import LlamaConfig, LlamaModel
+from atorch_b200.modules.w4_linear import W4Linear, quantize_linears
+
+
+def _model(seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = LlamaConfig(**{**dict(vocab_size=40, hidden_size=64, intermediate_size=96, num_hidden_layers=2, num_attention_heads=4,
+                                num_key_value_heads=2, max_position_embeddings=128, initializer_range=0.1), **kw})
+    return LlamaModel(cfg).bfloat16().eval()
+
+
+def _alone(model, ids, rows=1, steps=0, seed=0):
+    """A cache of its own for ``rows`` copies of a sequence, its pages in no order, after the pass over the prompt in row 0: generator,
+    cache, table, angles, logits of all tokens."""
+    g = Generator(model)
+    S, n, dev = g.page_size, len(ids), ids.device
+    width = -(-(n + steps) // S)
+    table = torch.randperm(rows * width, generator=torch.Generator().manual_seed(seed)).to(torch.int32).view(rows, width).to(dev)
+    cache = ops.KV4Cache(model.config.num_hidden_layers, rows * width, S, model.layers[0].n_kv, model.config.head_dim, dev)
+    cos, sin = model.rope(n + steps, dev)
+    seq, pos = torch.zeros(n, dtype=torch.int32, device=dev), torch.arange(n, dtype=torch.int32, device=dev)
+
+    def attend(q, layer):
+        k, v = ops.kv4_read(layer, table, seq, pos, q.dtype)
+        return ops.attention(q[None], k[None], v[None], causal=True, cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=dev))
+
+    with torch.no_grad():
+        logits = g._run(ids, cache, table, seq, pos, cos, sin, attend)
+    return g, cache, table, cos, sin, logits
+
+
+def _step_is_the_prompt(model, ids, places):
+    """A step over what the prompt left in the cache gives the prompt's logits. Only the step's own token is computed anew: some ten
+    roundings of 2^-9 a layer, in another order, and its own codes."""
+    g, cache, table, cos, sin, logits = _alone(model, ids)
+    kept = cache.codes.clone(), cache.scales.clone()
+    for t in places:
+        cache.codes.copy_(kept[0]), cache.scales.copy_(kept[1])
+        with torch.no_grad():
+            got = g._step(ids[t: t + 1], cache, table, torch.tensor([t], dtype=torch.int32, device=ids.device), cos, sin)[0]
+        off = (got.float() - logits[t].float()).norm() / logits[t].float().norm()
+        assert off < 0.05, (t, off)
+
+
+def _beams_with_pages_of_their_own(model, ids, beams, steps, eos=None):
+    """The same search with a whole copy of the cache for every beam, moved by indexing."""
+    g, cache, table, cos, sin, logits = _alone(model, ids, beams, steps, seed=1)
+    n, pages = len(ids), table.long()
+    cache.codes[:, pages[1:].flatten()] = cache.codes[:, pages[:1].expand(beams - 1, -1).flatten()]
+    cache.scales[:, pages[1:].flatten()] = cache.scales[:, pages[:1].expand(beams - 1, -1).flatten()]
+    with torch.no_grad():
+        logits = g._prompts([ids], cache, table, [0], cos, sin)       # (the logits that a search begins with, in their shape)
+        scores, tokens, parents, done = ops.beam_select_reference(logits.view(1, 1, -1), torch.zeros(1, 1, device=ids.device), None,
+                                                                  -1 if eos is None else eos, beams)
+        sequences = tokens.view(beams, 1)
+        for i in range(1, steps):
+            if eos is not None and bool(done.all()):
+                break
+            logits = g._step(tokens.view(-1), cache, table, torch.full((beams,), n + i - 1, dtype=torch.int32, device=ids.device), cos, sin)
+            scores, tokens, parents, done = ops.beam_select_reference(logits.view(1, beams, -1), scores, None if eos is None else done,
+                                                                      -1 if eos is None else eos)
+            parent = parents[0].long()
+            sequences = torch.cat([sequences[parent], tokens.view(beams, 1)], 1)
+            cache.codes[:, pages.flatten()] = cache.codes[:, pages[parent].flatten()]
+            cache.scales[:, pages.flatten()] = cache.scales[:, pages[parent].flatten()]
+    return torch.cat([ids, sequences[0]])
+
+
+def test_a_step_continues_the_prompt():
+    _step_is_the_prompt(_model(), torch.randint(0, 40, (70,), generator=torch.Generator().manual_seed(1)), (1, 15, 16, 40, 69))
+
+
+def test_greedy_is_one_step_after_another():
+    m = _model()
+    ids = torch.randint(0, 40, (21,), generator=torch.Generator().manual_seed(2))
+    g, cache, table, cos, sin, logits = _alone(m, ids, 1, 15)
+    with torch.no_grad():
+        token, want = g._prompts([ids], cache, table, [0], cos, sin).argmax(-1), []
+        for i in range(15):
+            want.append(token)
+            token = g._step(token, cache, table, torch.tensor([21 + i], dtype=torch.int32), cos, sin).argmax(-1) if i < 14 else token
+    assert torch.equal(generate(m, [ids], 15)[0], torch.cat([ids, *want]))
+
+
+@pytest.mark.parametrize("beams,n,eos", [(2, 5, None), (4, 16, None), (5, 39, 3), (3, 15, 0)])
+def test_beams_share_pages_and_nothing_else(beams, n, eos):
+    m = _model(vocab_size=12)
+    ids = torch.randint(0, 12, (n,), generator=torch.Generator().manual_seed(n))
+    want = _beams_with_pages_of_their_own(m, ids, beams, 25, eos)
+    if eos is not None and (want[n:] == eos).any():
+        want = want[: n + int((want[n:] == eos).nonzero()[0]) + 1]
+    assert torch.equal(generate(m, [ids], 25, beams=beams, eos=eos)[0], want)
+
+
+def test_end_token_and_shapes():
+    m = _model(vocab_size=6)
+    prompts = torch.randint(0, 6, (3, 7), generator=torch.Generator().manual_seed(3))
+    for kw in (dict(), dict(beams=3), dict(temperature=1.0), dict(beams=2, length_penalty=1.0)):
+        torch.manual_seed(0)
+        for p, o in zip(prompts, generate(m, prompts, 12, eos=4, **kw)):
+            new = o[7:]
+            assert torch.equal(o[:7], p) and 1 <= len(new) <= 12
+            assert (new[:-1] != 4).all() and (len(new) == 12 or new[-1] == 4)
+    assert torch.equal(generate(m, prompts, 0)[1], prompts[1])
+    with pytest.raises(ValueError):
+        generate(m, prompts, 4, beams=2, temperature=1.0)
+    with pytest.raises(ValueError):
+        generate(m, [torch.tensor([], dtype=torch.long)], 4)
+    with pytest.raises(ValueError):
+        Generator(m.float())
+    with pytest.raises(ValueError):
+        CachedSampler(_model(), temperature=0.0)
+
+
+def test_sampler_follows_the_distribution():
+    m = _model(vocab_size=4)
+    ids = torch.randint(0, 4, (5,), generator=torch.Generator().manual_seed(4))
+    want = torch.softmax(_alone(m, ids)[-1][-1].float() / 0.7, -1)
+    torch.manual_seed(5)
+    out = CachedSampler(m, max_new_tokens=1, temperature=0.7)(None, ids.expand(4000, 5))
+    assert out.shape == (4000, 6)
+    got = torch.bincount(out[:, -1], minlength=4) / 4000
+    # five standard deviations, and what the sums of a batch in bf16 are rounded by
+    assert ((got - want).abs() < 5 * (want * (1 - want) / 4000).sqrt() + 0.01).all()
+
+
+def test_quantised_linears():
+    m = _model()
+    before = m.layers[0].qkv_proj.weight.detach().clone()
+    quantize_linears(m, 32, lambda name, lin: "lm_head" not in name)
+    assert type(m.lm_head) is torch.nn.Linear
+    lin = m.layers[0].qkv_proj
+    assert type(lin) is W4Linear and lin.in_features == 64 and lin.out_features == before.shape[0]
+    w = ops.w4_dequantize(lin.codes, lin.scales, 64, 32)
+    assert (w - before.float()).abs().max() <= float(lin.scales.max()) * 0.55
+    x = torch.randn(3, 64).bfloat16()
+    assert torch.allclose(lin(x).float(), x.float() @ w.t(), atol=2e-2, rtol=1e-2)
+    out = generate(m, [torch.tensor([1, 2, 3])], 6)[0]
+    assert len(out) == 9
+    tied = _model(tie_word_embeddings=True)
+    quantize_linears(tied)
+    assert type(tied.lm_head) is torch.nn.Linear and type(tied.layers[1].o_proj) is W4Linear

@@ -1,0 +1,116 @@
+"""Generation on the GPU: the operators together, against one another's plain implementations and layouts."""
+import pytest
+import torch
+
+from atorch_b200 import _lib, ops
+from atorch_b200.models.generate import CachedSampler, Generator
+from atorch_b200.models.llama import LlamaConfig, LlamaModel
+from atorch_b200.modules.w4_linear import quantize_linears
+
+pytestmark = pytest.mark.gpu
+
+
+def _model(seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = LlamaConfig(**{**dict(vocab_size=1000, hidden_size=512, intermediate_size=768, num_hidden_layers=3, num_attention_heads=4,
+                                num_key_value_heads=2, max_position_embeddings=512, initializer_range=0.04), **kw})
+    return LlamaModel(cfg).bfloat16().cuda().eval()
+
+
+def _alone(model, ids, rows=1, steps=0, seed=0):
+    """A cache of its own for ``rows`` copies of a sequence, its pages in no order, after the pass over the prompt in row 0: generator,
+    cache, table, angles, logits of all tokens."""
+    g = Generator(model)
+    S, n, dev = g.page_size, len(ids), ids.device
+    width = -(-(n + steps) // S)
+    table = torch.randperm(rows * width, generator=torch.Generator().manual_seed(seed)).to(torch.int32).view(rows, width).to(dev)
+    cache = ops.KV4Cache(model.config.num_hidden_layers, rows * width, S, model.layers[0].n_kv, model.config.head_dim, dev)
+    cos, sin = model.rope(n + steps, dev)
+    seq, pos = torch.zeros(n, dtype=torch.int32, device=dev), torch.arange(n, dtype=torch.int32, device=dev)
+
+    def attend(q, layer):
+        k, v = ops.kv4_read(layer, table, seq, pos, q.dtype)
+        return ops.attention(q[None], k[None], v[None], causal=True, cu_seqlens=torch.tensor([0, n], dtype=torch.int32, device=dev))
+
+    with torch.no_grad():
+        logits = g._run(ids, cache, table, seq, pos, cos, sin, attend)
+    return g, cache, table, cos, sin, logits
+
+
+def _step_is_the_prompt(model, ids, places):
+    """A step over what the prompt left in the cache gives the prompt's logits. Only the step's own token is computed anew: some ten
+    roundings of 2^-9 a layer, in another order, and its own codes."""
+    g, cache, table, cos, sin, logits = _alone(model, ids)
+    kept = cache.codes.clone(), cache.scales.clone()
+    for t in places:
+        cache.codes.copy_(kept[0]), cache.scales.copy_(kept[1])
+        with torch.no_grad():
+            got = g._step(ids[t: t + 1], cache, table, torch.tensor([t], dtype=torch.int32, device=ids.device), cos, sin)[0]
+        off = (got.float() - logits[t].float()).norm() / logits[t].float().norm()
+        assert off < 0.05, (t, off)
+
+
+def _beams_with_pages_of_their_own(model, ids, beams, steps, eos=None):
+    """The same search with a whole copy of the cache for every beam, moved by indexing."""
+    g, cache, table, cos, sin, logits = _alone(model, ids, beams, steps, seed=1)
+    n, pages = len(ids), table.long()
+    cache.codes[:, pages[1:].flatten()] = cache.codes[:, pages[:1].expand(beams - 1, -1).flatten()]
+    cache.scales[:, pages[1:].flatten()] = cache.scales[:, pages[:1].expand(beams - 1, -1).flatten()]
+    with torch.no_grad():
+        logits = g._prompts([ids], cache, table, [0], cos, sin)       # (the logits that a search begins with, in their shape)
+        scores, tokens, parents, done = ops.beam_select_reference(logits.view(1, 1, -1), torch.zeros(1, 1, device=ids.device), None,
+                                                                  -1 if eos is None else eos, beams)
+        sequences = tokens.view(beams, 1)
+        for i in range(1, steps):
+            if eos is not None and bool(done.all()):
+                break
+            logits = g._step(tokens.view(-1), cache, table, torch.full((beams,), n + i - 1, dtype=torch.int32, device=ids.device), cos, sin)
+            scores, tokens, parents, done = ops.beam_select_reference(logits.view(1, beams, -1), scores, None if eos is None else done,
+                                                                      -1 if eos is None else eos)
+            parent = parents[0].long()
+            sequences = torch.cat([sequences[parent], tokens.view(beams, 1)], 1)
+            cache.codes[:, pages.flatten()] = cache.codes[:, pages[parent].flatten()]
+            cache.scales[:, pages.flatten()] = cache.scales[:, pages[parent].flatten()]
+    return torch.cat([ids, sequences[0]])
+
+
+@pytest.mark.parametrize("kw,weights", [(dict(), None), (dict(num_attention_heads=8, num_key_value_heads=8), None), (dict(), 128),
+                                        (dict(num_attention_heads=8, num_key_value_heads=4), 64)])
+def test_a_step_continues_the_prompt(kw, weights):
+    m = _model(**kw)
+    if weights:
+        quantize_linears(m, weights)
+    launches = _lib.launch_count
+    _step_is_the_prompt(m, torch.randint(0, 1000, (300,), generator=torch.Generator().manual_seed(1)).cuda(), (1, 16, 100, 255, 299))
+    assert _lib.launch_count > launches + 5 * 3 * 2
+
+
+def test_prompts_of_several_lengths():
+    """Every sequence begins with its prompt, and goes on with the token that its prompt alone gives, or one as likely."""
+    m = _model()
+    g = torch.Generator().manual_seed(2)
+    prompts = [torch.randint(0, 1000, (n,), generator=g).cuda() for n in (1, 16, 45, 130)]
+    for p, o in zip(prompts, Generator(m).generate(prompts, 24)):
+        assert torch.equal(o[: len(p)], p) and len(o) == len(p) + 24
+        logits = _alone(m, p)[-1][-1].float()
+        assert logits[o[len(p)]] >= logits.max() - 0.05 * logits.norm()
+
+
+@pytest.mark.parametrize("beams,n,eos", [(2, 5, None), (4, 16, None), (7, 40, 3), (16, 31, None)])
+def test_beams_share_pages_and_nothing_else(beams, n, eos):
+    m = _model(vocab_size=64)
+    ids = torch.randint(0, 64, (n,), generator=torch.Generator().manual_seed(n)).cuda()
+    want = _beams_with_pages_of_their_own(m, ids, beams, 40, eos)
+    if eos is not None and (want[n:] == eos).any():
+        want = want[: n + int((want[n:] == eos).nonzero()[0]) + 1]
+    assert torch.equal(Generator(m).generate([ids], 40, beams=beams, eos=eos)[0], want)
+
+
+def test_sampler_and_end_token():
+    m = _model(vocab_size=50)
+    prompt = torch.randint(0, 50, (8, 9), generator=torch.Generator().manual_seed(3)).cuda()
+    torch.manual_seed(0)
+    out = CachedSampler(m, max_new_tokens=12)(None, prompt)
+    assert out.shape == (8, 21) and torch.equal(out[:, :9], prompt) and (out < 50).all()
+    for o in Generator(m).generate(prompt, 30, eos=7, temperature=1.5):
+        assert (o[9:-1] != 7).all() and (o[-1] == 7 or len(o) == 39)
