@@ -2,6 +2,7 @@
 //
 // A continuation of beam w by token v has f = score[w] + (x[w, v] - lse(x[w])), evaluated in fp32 in this order; NaN counts as
 // -inf. The `keep` largest f of a sequence's beams are kept, equal ones by the lower w, then the lower v.
+#include <atomic>
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "common.cuh"
@@ -24,6 +25,15 @@ ATB_DEVICE float value_of(unsigned long long key) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 ATB_DEVICE unsigned index_of(unsigned long long key) { return 0xffffffffu - (uint32_t)key; }
+
+// The same with the beam before the index: the order of a sequence's continuations. 0 is below all of them.
+constexpr int INDEX_BITS = 27;
+ATB_DEVICE unsigned long long with_beam(unsigned long long key, int beam) {
+  if (key == 0) return 0;
+  return (key >> 32 << 32) | ((uint32_t)(MOST - 1 - beam) << INDEX_BITS) | ((1u << INDEX_BITS) - 1 - index_of(key));
+}
+ATB_DEVICE int beam_of(unsigned long long key) { return MOST - 1 - (int)((uint32_t)key >> INDEX_BITS); }
+ATB_DEVICE unsigned token_of(unsigned long long key) { return (1u << INDEX_BITS) - 1 - ((uint32_t)key & ((1u << INDEX_BITS) - 1)); }
 
 ATB_DEVICE float total(float score, float x, float lse) {
   const float f = __fadd_rn(score, __fsub_rn(x, lse));
@@ -89,7 +99,7 @@ struct Share {
       for (int k = 0; k < P; ++k)
         if ((int)threadIdx.x + k * THREADS < pieces) f(kept[k], from + ((int)threadIdx.x + k * THREADS) * N);
     } else {
-#pragma unroll 2
+#pragma unroll 4
       for (int i = threadIdx.x; i < pieces; i += THREADS)
         f(Piece<T>{reinterpret_cast<const uint4*>(row + from)[i]}, from + i * N);
     }
@@ -105,15 +115,37 @@ ATB_DEVICE Sum add(Sum a, Sum b) {
   return Sum{top, a.sum * (a.top == top ? 1.f : expf(a.top - top)) + b.sum * (b.top == top ? 1.f : expf(b.top - top))};
 }
 
-// The `keep` best continuations of one beam, best first, as keys of f and token. The blocks of a cluster have a share of the
+struct Out {
+  float* scores;
+  long long* tokens;
+  int* parents;
+  unsigned char* ended;
+};
+// `key`: with its beam
+ATB_DEVICE void write_out(const Out& out, long long at, unsigned long long key, const unsigned char* ended, int eos) {
+  out.scores[at] = value_of(key);
+  out.tokens[at] = token_of(key);
+  out.parents[at] = beam_of(key);
+  out.ended[at] = (ended && ended[beam_of(key)]) || (int)token_of(key) == eos;
+}
+// Place of key number i among n of them (only those that are 0 are equal)
+ATB_DEVICE int place_of(const unsigned long long* keys, int n, int i) {
+  const unsigned long long k = keys[i];
+  int place = 0;
+#pragma unroll 4
+  for (int j = 0; j < n; ++j) place += keys[j] > k || (keys[j] == k && j < i);
+  return place;
+}
+
+// The `keep` best continuations of one beam, best first, as keys of f and token; or, where the blocks of all W beams of a sequence
+// fit into a cluster (`best` is null, `beams` = W and not 1), those of the sequence at once. The blocks of a cluster have a share of a beam's
 // vocabulary each: they add up the row's sum of exponentials through each other's shared memory, each picks the best of its share,
-// and the first picks the best of those. The row comes from memory once, and from registers or the first-level
-// cache after that. Bound by
-// latency for a few beams (one block a row, with the row's 64 KB read three times from L2, took 17 us).
+// and the first picks the best of those. The row comes from memory once, and from registers or the first-level cache after that.
+// Bound by latency for a few beams (one block a row, with the row's 64 KB read three times from L2, took 17 us).
 template <typename T, int P>
 __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, const float* scores, const unsigned char* finished,
-                                                           unsigned long long* best, int V, long long row_stride, int wide,
-                                                           int eos, int keep, const int* status) {
+                                                           unsigned long long* best, Out final, int beams, int V,
+                                                           long long row_stride, int wide, int eos, int keep, const int* status) {
   __shared__ Sum warp_sums[THREADS / 32], share_sum;
   __shared__ unsigned long long red_key[THREADS / 32], room[ROOM], tops[GROUPS], mine[MOST];
   __shared__ float least;
@@ -121,23 +153,16 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
   grid_go();
   grid_wait();
   cg::cluster_group cluster = cg::this_cluster();
-  const int shares = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
-  const long long row = blockIdx.x / shares;
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
+  const int shares = blocks / beams, share_rank = rank % shares, first_rank = rank - share_rank;
+  const long long item = blockIdx.x / blocks, row = item * beams + rank / shares;
   const bool failed = *status != 0;      // nothing is stored then; the blocks of a cluster stay together
   const float score = scores[row];
   const bool ended = finished && finished[row];
-  unsigned long long* out = best + row * keep;
-  if (ended || score == -INFINITY || score != score) {
-    // the end token alone goes on, at no cost, or nothing; the others are impossible, and stand in their order
-    const bool only = ended && score != -INFINITY && score == score;
-    if (rank == 0 && threadIdx.x < keep && !failed) {
-      const int i = threadIdx.x;
-      out[i] = i >= V ? 0 : !only ? key_of(-INFINITY, i) : i == 0 ? key_of(score, eos) : key_of(-INFINITY, i - 1 < eos ? i - 1 : i);
-    }
-    return;
-  }
+  // a beam that is not looked at: the end token alone goes on, at no cost, or nothing
+  const bool known = ended || score == -INFINITY || score != score;
   const T* x = logits + row * row_stride;
-  const int part = ((V + shares - 1) / shares + 7) / 8 * 8, from = min(V, rank * part), to = min(V, from + part);
+  const int part = ((V + shares - 1) / shares + 7) / 8 * 8, from = min(V, share_rank * part), to = known ? from : min(V, from + part);
   const Share<T, P> share(x, from, to, wide);
   Sum s{-INFINITY, 0.f};
   share.each([&](const Piece<T>& v, int) { s.top = fmaxf(s.top, v.top()); },
@@ -160,8 +185,8 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
     share_sum = s;
   }
   cluster.sync();
-  s = *cluster.map_shared_rank(&share_sum, 0);
-  for (int i = 1; i < shares; ++i) s = add(s, *cluster.map_shared_rank(&share_sum, i));
+  s = *cluster.map_shared_rank(&share_sum, first_rank);
+  for (int i = 1; i < shares; ++i) s = add(s, *cluster.map_shared_rank(&share_sum, first_rank + i));
   const float lse = s.top + logf(s.sum);
 
   // the n-th largest of the maxima of four lanes: no fewer than n continuations of the share reach it
@@ -176,11 +201,20 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
     for (int i = 0; i < GROUPS; ++i) place += tops[i] > tops[threadIdx.x];
     if (place == max(n, 1) - 1) least = value_of(tops[threadIdx.x]);
   }
-  if (threadIdx.x < MOST) mine[threadIdx.x] = 0;
+  if (threadIdx.x < MOST) {
+    const int i = threadIdx.x;
+    unsigned long long k = 0;
+    if (known && share_rank == 0 && i < min(keep, V)) {      // the others are impossible, and stand in their order
+      const bool only = ended && score != -INFINITY && score == score;
+      k = !only ? key_of(-INFINITY, i) : i == 0 ? key_of(score, eos) : key_of(-INFINITY, i - 1 < eos ? i - 1 : i);
+    }
+    mine[i] = k;
+  }
   __syncthreads();
-  const float reach = least;
+  const float reach = known ? -INFINITY : least;
   // f grows with x; an x whose f may round up to `reach` is not further below its x than a few roundings
-  const float x_reach = (reach - score + lse) - 4.8e-7f * (fabsf(reach) + fabsf(score) + fabsf(lse));
+  float x_reach = (reach - score + lse) - 4.8e-7f * (fabsf(reach) + fabsf(score) + fabsf(lse));
+  if (!(x_reach <= 3.4e38f)) x_reach = -INFINITY;          // (a score of +inf)
   auto take = [&](float v, int i) {
     const float f = total(score, v, lse);
     if (f >= reach) {
@@ -222,47 +256,38 @@ __global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, cons
   }
   cluster.sync();
   if (rank == 0) {
-    const int all = shares * keep;               // keys of the shares, best first each
-    for (int i = threadIdx.x; i < all; i += THREADS) room[i] = *cluster.map_shared_rank(&mine[i % keep], i / keep);
+    const int all = blocks * keep;               // keys of the shares, best first each
+    for (int i = threadIdx.x; i < all; i += THREADS)
+      room[i] = with_beam(*cluster.map_shared_rank(&mine[i % keep], i / keep), i / keep / shares);
     __syncthreads();
     for (int i = threadIdx.x; i < all; i += THREADS) {
-      const unsigned long long k = room[i];
-      int place = 0;
-      for (int j = 0; j < all; ++j) place += room[j] > k || (room[j] == k && j < i);     // (only what is not there is equal)
-      if (place < keep && !failed) out[place] = k;
+      const int place = place_of(room, all, i);
+      if (place >= keep || failed) continue;
+      if (best != nullptr) best[row * keep + place] = room[i];
+      else if (room[i] != 0) write_out(final, item * keep + place, room[i], finished ? finished + item * beams : nullptr, eos);
     }
   }
   cluster.sync();                                // the first has read the others' keys
 }
 
 // The best of a sequence's beams (a block): each of the W keep continuations counts those before it.
-__global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long* best, const unsigned char* finished,
-                                                        float* scores, long long* tokens, int* parents,
-                                                        unsigned char* ended, int W, int keep, int eos, const int* status) {
+__global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long* best, const unsigned char* finished, Out final,
+                                                        int W, int keep, int eos, const int* status) {
   __shared__ unsigned long long all[MOST * MOST];
   grid_go();
   grid_wait();
   const bool failed = *status != 0;
   const long long b = blockIdx.x;
   const int n = W * keep;
-  for (int i = threadIdx.x; i < n; i += 256) all[i] = best[b * n + i];
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const unsigned long long k = best[b * n + i];          // (of beam 0, as its cluster knew it)
+    all[i] = k == 0 ? 0 : k - ((unsigned long long)(i / keep) << INDEX_BITS);
+  }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += 256) {
-    const unsigned long long k = all[i];
-    const int w = i / keep;
-    int place = 0;
-    for (int j = 0; j < n && place < keep; ++j) {
-      // by f, then beam, then token (the low half of a key); within a beam the list is in order
-      const unsigned long long o = all[j];
-      const uint32_t fo = (uint32_t)(o >> 32), fk = (uint32_t)(k >> 32);
-      place += fo != fk ? fo > fk : j < i;
-    }
-    if (place >= keep || k == 0 || failed) continue;
-    const long long at = b * keep + place;
-    scores[at] = value_of(k);
-    tokens[at] = index_of(k);
-    parents[at] = w;
-    ended[at] = (finished && finished[b * W + w]) || (int)index_of(k) == eos;
+    const int place = place_of(all, n, i);
+    if (place < keep && all[i] != 0 && !failed)
+      write_out(final, b * keep + place, all[i], finished ? finished + b * W : nullptr, eos);
   }
 }
 
@@ -349,21 +374,44 @@ __global__ void __launch_bounds__(256) beam_reorder_kernel(uint8_t* codes, uint8
     }
   }
 }
+// Blocks of a cluster that has all beams of a sequence: more than the 8 that need no leave
+constexpr int ONE = 16;
+template <typename T, int P>
+bool large_clusters() {
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have them
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return false;
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    if (cudaFuncSetAttribute(beam_row_kernel<T, P>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  return true;
+}
 }  // namespace
 
+// `best`: workspace, a key for each of B W keep; null: the beams of a sequence are one cluster (W up to 16), which needs none.
 extern "C" int atb_beam_select(const void* logits, const void* scores, const void* finished, void* best, void* out_scores,
                                void* tokens, void* parents, void* ended, int B, int W, int V, long long row_stride, int wide,
                                int eos, int keep, int dtype, void* stream, void* status) {
   if (B <= 0 || keep <= 0) return 0;
-  if (W < 1 || W > MOST || keep > MOST || V < 1 || (long long)B * W > 0x7fffffffLL / 8) return -1;
+  if (W < 1 || W > MOST || keep > MOST || V < 1 || V > 1 << INDEX_BITS || (long long)B * W > 0x7fffffffLL / ONE) return -1;
   int shares = 1;      // of 2000 tokens at least, as long as all of them are on the GPU at once
-  while (shares < 8 && V >= 4000 * shares && (long long)B * W * shares * 2 <= 4 * 148) shares *= 2;
+  const bool fused = best == nullptr;
+  while (shares < (fused ? ONE : 8) && V >= 4000 * shares && (long long)B * W * shares * 2 <= 4 * 148) shares *= 2;
+  if (fused) {
+    if (W > ONE) return -1;
+    while (shares * W > ONE) shares /= 2;
+  }
+  const int cluster = fused ? shares * W : shares;
+  const Out final{(float*)out_scores, (long long*)tokens, (int*)parents, (unsigned char*)ended};
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc = cudaErrorInvalidValue;
   const long long part = (V + shares - 1) / shares + 7, pieces = (part * (dtype == 2 ? 4 : 2) / 16 + THREADS - 1) / THREADS;
 #define ROWS_OF(T, P)                                                                                                    \
-  rc = launch_after(beam_row_kernel<T, P>, dim3(B * W * shares), THREADS, 0, st, shares, (const T*)logits, (const float*)scores, \
-                    (const unsigned char*)finished, (unsigned long long*)best, V, row_stride, wide, eos, keep, (const int*)status)
+  rc = cluster > 8 && !large_clusters<T, P>() ? cudaErrorInvalidValue : launch_after(beam_row_kernel<T, P>, dim3(B * W * shares), THREADS, 0, st, cluster, (const T*)logits, (const float*)scores, \
+                    (const unsigned char*)finished, (unsigned long long*)best, final, fused ? W : 1, V, row_stride, wide, eos, keep, \
+                    (const int*)status)
 #define ROWS(T)                                 \
   if (!wide || pieces > 4) ROWS_OF(T, 0);       \
   else if (pieces > 2) ROWS_OF(T, 4);           \
@@ -374,9 +422,9 @@ extern "C" int atb_beam_select(const void* logits, const void* scores, const voi
 #undef ROWS_OF
 #undef ROWS
   if (rc != cudaSuccess) return -5;
-  return launch_after(beam_join_kernel, dim3(B), 256, 0, st, 1, (const unsigned long long*)best, (const unsigned char*)finished,
-                      (float*)out_scores, (long long*)tokens, (int*)parents, (unsigned char*)ended, W, keep, eos,
-                      (const int*)status) == cudaSuccess ? 0 : -5;
+  if (fused) return 0;
+  return launch_after(beam_join_kernel, dim3(B), 256, 0, st, 1, (const unsigned long long*)best, (const unsigned char*)finished, final,
+                      W, keep, eos, (const int*)status) == cudaSuccess ? 0 : -5;
 }
 
 extern "C" int atb_beam_reorder(void* codes, void* scales, void* table, const void* lengths, const void* parents, int B, int W,

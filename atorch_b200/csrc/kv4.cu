@@ -203,35 +203,50 @@ __global__ void __launch_bounds__(SMALL, PER == 1 || sizeof(T) == 4 ? 1 : 7) kv4
   }
 }
 
-// What the cache stands for at given tokens: a lane turns 8 codes of the keys and of the values into two 16-byte pieces.
-template <typename T, int D>
-__global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, const int* seq, const int* pos, int* status) {
+// What the cache stands for at given tokens: a lane turns 8 codes of the keys and of the values of PER tokens into two 16-byte
+// pieces each. Positions, pages and codes follow one another, so the tokens' are asked for side by side.
+template <typename T, int D, int PER>
+__global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, const int* seq, const int* pos, int tokens,
+                                                         int* status) {
   grid_go();
   grid_wait();
   constexpr int L = D / 8;
-  const int l = threadIdx.x % L, h = blockIdx.y * (SMALL / L) + threadIdx.x / L;
-  const long long t = blockIdx.x;
-  const int before = *status, p = pos[t], row = seq ? seq[t] : (int)t;
+  const int l = threadIdx.x % L, h = blockIdx.y * (SMALL / L) + threadIdx.x / L, t0 = blockIdx.x * PER;
+  const int before = *status;
+  int p[PER], page[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) p[j] = t0 + j < tokens ? pos[t0 + j] : -1;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) page[j] = p[j] >= 0 ? page_of(c, seq ? seq[t0 + j] : t0 + j, p[j]) : -1;
   if (h >= c.kv_heads || before != 0) return;
-  float x[2][8] = {};
-  if (p >= 0) {
-    const int page = page_of(c, row, p), slot = p & ((1 << c.page_shift) - 1);
-    if (page < 0) {
+  uint2 sc[PER];
+  uint32_t w[PER][2];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    sc[j] = make_uint2(0u, 0u);
+    w[j][0] = w[j][1] = 0u;
+    if (page[j] >= 0) {
+      const int slot = p[j] & ((1 << c.page_shift) - 1);
+      sc[j] = *reinterpret_cast<const uint2*>(scales_at(c, page[j], h, slot));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) w[j][i] = *reinterpret_cast<const uint32_t*>(codes_at<D>(c, page[j], i, h, slot) + l * 4);
+    } else if (p[j] >= 0) {
       atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
-    } else {
-      const uint2 sc = *reinterpret_cast<const uint2*>(scales_at(c, page, h, slot));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(codes_at<D>(c, page, i, h, slot) + l * 4);
-        const float2 f = unpack_bf16x2(i ? sc.y : sc.x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = (float)((w >> (4 * e)) & 15u) * f.x + f.y;
-      }
     }
   }
-  const long long at = (t * c.kv_heads + h) * D + l * 8;
-  store8<T>(k + at, x[0]);
-  store8<T>(v + at, x[1]);
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    if (t0 + j >= tokens) break;
+    const long long at = ((long long)(t0 + j) * c.kv_heads + h) * D + l * 8;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = unpack_bf16x2(i ? sc[j].y : sc[j].x);
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)((w[j][i] >> (4 * e)) & 15u) * f.x + f.y;
+      store8<T>((i ? v : k) + at, x);
+    }
+  }
 }
 
 // ----------------------------------------------------------------------------------
@@ -836,8 +851,9 @@ template <typename T, int D>
 int launch_read(void* k, void* v, const Cache& c, const void* seq, const void* pos, int tokens, cudaStream_t st, int* status) {
   const int each = SMALL / (D / 8), blocks = (c.kv_heads + each - 1) / each;
   if (blocks > 65535) return -2;
-  return launch_after(kv4_read_kernel<T, D>, dim3(tokens, blocks), SMALL, 0, st, 1, (T*)k, (T*)v, c, (const int*)seq,
-                      (const int*)pos, status) == cudaSuccess ? 0 : -5;
+  const bool many = (long long)tokens * blocks > 148 * 16 * 2;
+  return launch_after(many ? kv4_read_kernel<T, D, 4> : kv4_read_kernel<T, D, 1>, dim3(many ? (tokens + 3) / 4 : tokens, blocks), SMALL,
+                      0, st, 1, (T*)k, (T*)v, c, (const int*)seq, (const int*)pos, tokens, status) == cudaSuccess ? 0 : -5;
 }
 
 template <typename T, int D, int NT>

@@ -14,6 +14,9 @@ from .. import _lib
 from .kv4 import _check_page_size
 
 MAX_BEAMS = 32
+# continuations of a sequence up to which one cluster of blocks selects among them (in one launch); above, each beam has a cluster of
+# its own and a second kernel joins them: 4 beams of 32000 tokens ... us in one, ... in two
+ONE_CLUSTER = 1 << 17
 
 
 def beam_select_reference(logits, scores, finished=None, eos=-1, keep=None):
@@ -78,8 +81,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     tokens = torch.empty_like(out, dtype=torch.int64)
     parents = torch.empty_like(out, dtype=torch.int32)
     ended = torch.empty_like(out, dtype=torch.bool)
-    best = torch.empty(B * W * keep, dtype=torch.int64, device=logits.device)
-    rc = _lib.lib().atb_beam_select(base, scores.data_ptr(), _lib.addr(finished), best.data_ptr(), out.data_ptr(), tokens.data_ptr(),
+    best = None if W * V <= ONE_CLUSTER and W <= 16 else torch.empty(B * W * keep, dtype=torch.int64, device=logits.device)
+    rc = _lib.lib().atb_beam_select(base, scores.data_ptr(), _lib.addr(finished), _lib.addr(best), out.data_ptr(), tokens.data_ptr(),
                                     parents.data_ptr(), ended.data_ptr(), B, W, V, row,
                                     int(base % 16 == 0 and row * logits.element_size() % 16 == 0), int(eos), keep,
                                     _lib.DT[logits.dtype], _lib.stream_of(dev), _lib.status_addr(logits))
