@@ -16,7 +16,7 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
-from typing import NamedTuple, Optional, Tuple
+from typing import Optional, Tuple
 
 import torch
 
@@ -45,26 +45,12 @@ def _check_page_size(n: int) -> None:
         raise ValueError(f"page_size has to be a power of two of 16 or more, got {n}")
 
 
-class _Cache(NamedTuple):
-    """A layer's cache and page table as the launchers take them."""
-
-    codes: int
-    scales: int
-    table: int
-    pages: int
-    kv_heads: int
-    page_shift: int
-    rows: int
-    width: int
-    table_stride: int
-    head_dim: int
-    device: int          # index; -1: the CPU
-
-
-def _cache(layer: Layer, page_table: torch.Tensor) -> _Cache:
-    """After the checks that all calls share."""
+def _cache(layer: Layer, page_table: torch.Tensor) -> Tuple[int, ...]:
+    """A layer's cache and page table as the launchers take them, after the checks that all calls share: addresses of codes, scales
+    and table, pages, kv_heads, page_shift, sequences, pages of a sequence, stride of the table; then head_dim and the index of the
+    device (-1: the CPU)."""
     codes, scales = layer
-    shape, table_shape = codes.shape, page_table.shape
+    shape = codes.shape
     if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or len(shape) != 5 or shape[1] != 2 or 0 in shape:
         raise ValueError("a layer's cache is (uint8 [pages, 2, kv_heads, page_size, head_dim / 2], "
                          f"bf16 [pages, kv_heads, page_size, 4]), got {codes.dtype} {tuple(shape)} and {scales.dtype}")
@@ -76,15 +62,16 @@ def _cache(layer: Layer, page_table: torch.Tensor) -> _Cache:
         raise ValueError("the cache has to be contiguous and begin on 16 bytes")
     if page_size < 16 or page_size & (page_size - 1):
         _check_page_size(page_size)
-    if page_table.dtype is not torch.int32 or len(table_shape) != 2 or page_table.stride(1) != 1:
+    steps = page_table.stride()
+    if page_table.dtype is not torch.int32 or len(steps) != 2 or steps[1] != 1:
         raise ValueError("page_table is int32 [sequences, pages], its rows contiguous")
-    if dev >= 0:
-        if half != 64 and half != 32:
-            raise ValueError(f"head_dim {2 * half}: the kernels take {HEAD_DIMS}")
-        _lib.lib()
-    _same_device(dev, scales, page_table)
-    return _Cache(codes_at, scales_at, page_table.data_ptr(), pages, kv_heads, page_size.bit_length() - 1, table_shape[0],
-                  table_shape[1], page_table.stride(0), 2 * half, dev)
+    if dev >= 0 and half != 64 and half != 32:
+        raise ValueError(f"head_dim {2 * half}: the kernels take {HEAD_DIMS}")
+    if scales.get_device() != dev or page_table.get_device() != dev:
+        _same_device(dev, scales, page_table)
+    rows, width = page_table.shape
+    return (codes_at, scales_at, page_table.data_ptr(), pages, kv_heads, page_size.bit_length() - 1, rows, width, steps[0], 2 * half,
+            dev)
 
 
 def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
@@ -108,7 +95,7 @@ def _int32(name: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tenso
 
 def _aligned(t: torch.Tensor, row: int) -> bool:
     """Whether rows of ``t`` that are ``row`` elements apart can be read in 16-byte pieces."""
-    return t.data_ptr() % 16 == 0 and row * t.element_size() % 16 == 0
+    return (t.data_ptr() | row * t.element_size()) & 15 == 0
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -160,8 +147,7 @@ def kv4_append(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tenso
     position is padding: its token is not kept, its queries come back as they are. Two tokens at one place: either is kept.
 
     The rotation is not rounded before the codes are taken; queries are rounded once."""
-    c = _cache(layer, page_table)
-    KV, D, dev = c.kv_heads, c.head_dim, c.device
+    codes, scales, table, pages, KV, shift, rows, most, stride, D, dev = _cache(layer, page_table)
     shape, dtype, width = qkv.shape, _lib.DT.get(qkv.dtype), (n_q + 2 * KV) * D
     if dtype is None:
         raise ValueError(f"qkv is bf16, fp16 or fp32, got {qkv.dtype}")
@@ -187,9 +173,9 @@ def kv4_append(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tenso
     if one != 1 or not _aligned(x, step):
         x, step = x.clone(memory_format=torch.contiguous_format), width
     q = x.new_empty(T, n_q, D)
-    rc = _lib.lib().atb_kv4_append(x.data_ptr(), q.data_ptr(), c.codes, c.scales, c.table, _lib.addr(seq), pos.data_ptr(),
-                                   _lib.addr(cos), _lib.addr(sin), positions, T, n_q, KV, D, c.page_shift, c.pages, c.rows, c.width,
-                                   c.table_stride, step, dtype, _lib.stream_of(dev), _lib.status_addr(x))
+    rc = _lib.lib().atb_kv4_append(x.data_ptr(), q.data_ptr(), codes, scales, table, _lib.addr(seq), pos.data_ptr(), _lib.addr(cos),
+                                   _lib.addr(sin), positions, T, n_q, KV, D, shift, pages, rows, most, stride, step, dtype,
+                                   _lib.stream_of(dev), _lib.status_addr(x))
     _lib.check(rc, "atb_kv4_append")
     return q
 
@@ -214,19 +200,18 @@ def kv4_read(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tensor]
     """Keys and values ``[T, kv_heads, head_dim]`` that the cache stands for at the positions ``pos`` of the sequences ``seq``
     (as in :func:`kv4_append`); zeros where the position is negative. A prompt's own attention runs on them, so that its tokens
     see the same keys as the tokens after it."""
-    c = _cache(layer, page_table)
-    kind, dev, T = _lib.DT.get(dtype), c.device, pos.numel()
+    codes, scales, table, pages, KV, shift, rows, most, stride, D, dev = _cache(layer, page_table)
+    kind, T = _lib.DT.get(dtype), pos.numel()
     if kind is None:
         raise ValueError(f"dtype is bf16, fp16 or fp32, got {dtype}")
     seq, pos = _int32("seq", seq, T), _int32("pos", pos, T)
     _same_device(dev, pos, seq)
     if dev < 0:
         return kv4_read_reference(layer, page_table, seq, pos, dtype)
-    k = pos.new_empty((T, c.kv_heads, c.head_dim), dtype=dtype)
+    k = pos.new_empty((T, KV, D), dtype=dtype)
     v = torch.empty_like(k)
-    rc = _lib.lib().atb_kv4_read(k.data_ptr(), v.data_ptr(), c.codes, c.scales, c.table, _lib.addr(seq), pos.data_ptr(), T, c.kv_heads,
-                                 c.head_dim, c.page_shift, c.pages, c.rows, c.width, c.table_stride, kind, _lib.stream_of(dev),
-                                 _lib.status_addr(pos))
+    rc = _lib.lib().atb_kv4_read(k.data_ptr(), v.data_ptr(), codes, scales, table, _lib.addr(seq), pos.data_ptr(), T, KV, D, shift, pages,
+                                 rows, most, stride, kind, _lib.stream_of(dev), _lib.status_addr(pos))
     _lib.check(rc, "atb_kv4_read")
     return k, v
 
@@ -273,15 +258,14 @@ def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengt
     ``i`` sees the keys ``j < lengths - S + i + 1``. Query heads are shared as in :func:`~atorch_b200.ops.attention` (``n_q`` a
     multiple of the cache's heads). Returns ``[sequences, S, n_q, head_dim]``, and with ``return_lse`` the logarithms of the
     denominators, fp32 ``[sequences, n_q, S]``. A query that sees nothing gives zeros (and ``-inf``)."""
-    c = _cache(layer, page_table)
-    KV, D, dev = c.kv_heads, c.head_dim, c.device
+    codes, scales, table, pages, KV, shift, rows, most, stride, D, dev = _cache(layer, page_table)
     if q.dim() != 4 or q.shape[3] != D or q.shape[2] % KV or q.shape[2] == 0:
         raise ValueError(f"q {tuple(q.shape)}: [sequences, S, a multiple of {KV}, {D}] is wanted")
     if q.dtype is not torch.bfloat16 and q.dtype is not torch.float16:
         raise ValueError(f"q is bf16 or fp16, got {q.dtype}")
     B, S, H, _ = q.shape
-    if c.rows != B:
-        raise ValueError(f"page_table has {c.rows} rows for {B} sequences")
+    if rows != B:
+        raise ValueError(f"page_table has {rows} rows for {B} sequences")
     _no_gradient(q)
     lengths = _int32("lengths", lengths, B)
     _same_device(dev, q, lengths)
@@ -294,10 +278,10 @@ def kv4_attention(q: torch.Tensor, layer: Layer, page_table: torch.Tensor, lengt
         q_batch, q_token = S * H * D, H * D
     out = q.new_empty(B, S, H, D)
     lse = torch.empty(B, H, S, dtype=torch.float32, device=q.device) if return_lse else None
-    partial = None if c.width << c.page_shift <= WHOLE else torch.empty(_scratch(B, H, KV, S, D), dtype=torch.float32, device=q.device)
+    partial = None if most << shift <= WHOLE else torch.empty(_scratch(B, H, KV, S, D), dtype=torch.float32, device=q.device)
     rc = _lib.lib().atb_kv4_attention(
-        q.data_ptr(), out.data_ptr(), _lib.addr(lse), c.codes, c.scales, c.table, lengths.data_ptr(), _lib.addr(partial), S, H, KV, D,
-        c.page_shift, c.pages, B, c.width, c.table_stride, q_batch, q_token, softmax_scale if softmax_scale is not None else D ** -0.5,
-        _lib.DT[q.dtype], _lib.stream_of(dev), _lib.status_addr(q))
+        q.data_ptr(), out.data_ptr(), _lib.addr(lse), codes, scales, table, lengths.data_ptr(), _lib.addr(partial), S, H, KV, D, shift,
+        pages, B, most, stride, q_batch, q_token, D ** -0.5 if softmax_scale is None else softmax_scale, _lib.DT[q.dtype],
+        _lib.stream_of(dev), _lib.status_addr(q))
     _lib.check(rc, "atb_kv4_attention")
     return (out, lse) if return_lse else out
