@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, co
 // in place; of the others, the run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins in
 // the order of the blocks.
 constexpr int WARPS = 4, TILE = 32, START = 8;
-constexpr float SLACK = 8.f;       // powers of two by which a score may exceed the maximum that is kept
+constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
 
 ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
   const int n = lengths[b], most = c.width << c.page_shift;
@@ -384,16 +384,19 @@ struct AttnArgs {
 // code needs no conversion: its 4 bits, alone in the low bits of a half, are the fp16 number code * 2^-24, and four places
 // further up code * 2^-20; so eight codes cost four ANDs and a shift. The other operand takes the powers of two and everything
 // else that a value has:
-//   s[t, n]  = ks[t] (q[n] . code[t]) + km[t] sum(q[n])        o[d, n] = sum_t (p[t, n] vs[t]) code[t, d] + sum_t p[t, n] vm[t]
+//   s[t, n] = ks[t] (q[n] . code[t]) + km[t] sum(q[n])
+//   o[d, n] = sum_t (p[t, n] vs[t]) (code[t, d] - 8) + sum_t p[t, n] (vm[t] + 8 vs[t])
 // q is scaled by a power of two to at most 2^15 before it is rounded to fp16 (bf16 and fp16 values stay exact down to 2^-29 of
-// the largest), p vs by 2^(7 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
-// 11 bits of it are kept, which is what the products with 4-bit codes can use. Sums, maxima and denominators are fp32.
+// the largest), p vs by 2^(11 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
+// 11 bits of it are kept. The 8s are taken off as
+// products of the same rounded numbers (a row of 8s in the place of codes), so that their rounding errors weigh as much as a value
+// and not as a code: fp16 results were off by 3.6e-4 without it, of 2.1e-4 that fp16 takes. Sums, maxima and denominators are fp32.
 //
 // A warp has every fourth tile of a segment. Its tiles come through a ring of its own in shared memory, filled by the copy unit
 // STAGES tiles ahead. What bounds the kernel beside memory is the integer pipe: 5 operations for 8 codes of a key, 6 of a value.
 // So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and
 // only the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by
-// 2^8 before everything is rescaled: a warp sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its values'
+// 2^4 before everything is rescaled: a warp sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its values'
 // words without a bank conflict worse than two ways.
 template <int D, int NT>
 struct Shape {
@@ -552,13 +555,15 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
 
     // running maximum of the scores (m), sums of p, of p times the values' minima and of p times their scaled codes; `ref` is what
     // scores are taken relative to: m, or 0 where there is none yet
-    float o_acc[NT][MT][4], m[NT][2], ref[NT][2], l[NT][2], z[NT][2];
+    float o_acc[NT][MT][4], eights[NT][4], m[NT][2], ref[NT][2], l[NT][2], z[NT][2];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o_acc[j][i][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) eights[j][e] = 0.f;
 #pragma unroll
       for (int o = 0; o < 2; ++o) {
         m[j][o] = -INFINITY;
@@ -651,6 +656,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o_acc[n][i][e] *= f[e & 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eights[n][e] *= f[e & 1];
         }
       }
       const float up = __int_as_float((268 - (int)SLACK - top_e) << 23);      // 2^(15 - SLACK) / 2^(exponent + 1)
@@ -660,7 +667,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = 16 * p + order(r) + 8 * i;
-          const float scale = vs[2 * p + i].x * up, low = vs[2 * p + i].y;
+          const float scale = vs[2 * p + i].x * up, middle = fmaf(8.f, vs[2 * p + i].x, vs[2 * p + i].y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float pv[2];
@@ -669,12 +676,15 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
               const float w = fast_exp2(s[p][n][2 * i + o]);
               const bool seen = !MASK || t0 + t < limit[n][o];
               l[n][o] += w;
-              z[n][o] = seen ? fmaf(w, low, z[n][o]) : z[n][o];
+              z[n][o] = seen ? fmaf(w, middle, z[n][o]) : z[n][o];
               pv[o] = seen ? w * scale : 0.f;
             }
             pf[n][i] = transpose_8x8(pack_f16x2(pv[0], pv[1]));
           }
         }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          mma_f16(eights[n], 0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u, pf[n][0], pf[n][1]);
         Words<VW> vc[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -727,7 +737,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           *reinterpret_cast<float2*>(&sh_o[warp][col][r * (D / 8) + 2 * i]) =
-              make_float2(o_acc[j][i][o] * (16.f * f) + z[j][o], o_acc[j][i][2 + o] * f + z[j][o]);
+              make_float2((o_acc[j][i][o] - eights[j][o]) * (16.f * f) + z[j][o],
+                          fmaf(o_acc[j][i][2 + o], f, fmaf(-16.f * f, eights[j][o], z[j][o])));
       }
     }
     __syncthreads();
