@@ -16,7 +16,7 @@ from .. import _lib
 from .gemm import gemm
 
 GROUPS = (32, 64, 128)
-_LOW = (torch.bfloat16, torch.float16)
+_LOW = {torch.bfloat16: 0, torch.float16: 1}
 # rows of x from which the weights are expanded to bf16 and multiplied by the GEMM, with bf16 x and K a multiple of 8
 EXPAND_ROWS = 65
 
@@ -52,16 +52,19 @@ def _check_group(group_size: int) -> None:
         raise ValueError(f"group_size is one of {GROUPS}, got {group_size}")
 
 
-def _check(codes, scales, K, group_size) -> None:
+def _check(codes, scales, K, group_size) -> int:
+    """Rows of a weight of K columns."""
     if group_size not in GROUPS:
         _check_group(group_size)
-    N = codes.shape[0] if codes.dim() == 2 else -1
-    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or K < 1 or codes.shape != (N, (K + 31) // 32 * 16) \
+    shape = codes.shape
+    N = shape[0] if len(shape) == 2 else -1
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.bfloat16 or K < 1 or shape[1:] != ((K + 31) // 32 * 16,) \
             or scales.shape != (N, (K + group_size - 1) // group_size):
-        raise ValueError(f"codes {codes.dtype} {tuple(codes.shape)} and scales {scales.dtype} {tuple(scales.shape)} are not a "
+        raise ValueError(f"codes {codes.dtype} {tuple(shape)} and scales {scales.dtype} {tuple(scales.shape)} are not a "
                          f"weight of {K} columns in groups of {group_size}")
     if not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError("codes and scales have to be contiguous")
+    return N
 
 
 def w4_linear_reference(x, codes, scales, group_size=128, bias=None):
@@ -74,35 +77,39 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
     """``x @ W.T (+ bias)`` for ``x`` ``[..., K]`` in bf16 or fp16 and the weight that ``codes`` and ``scales`` stand for; sums in
     fp32, the result in the type of ``x``. Made for the few rows of a decode step; many bf16 rows expand the weight for the call and
     run the GEMM (the weight is rounded to bf16 there)."""
-    K, N = x.shape[-1], codes.shape[0]
-    _check(codes, scales, K, group_size)
-    if x.dtype not in _LOW:
+    shape, kind = x.shape, _LOW.get(x.dtype)
+    K, N = shape[-1], _check(codes, scales, shape[-1], group_size)
+    if kind is None:
         raise ValueError(f"x is bf16 or fp16, got {x.dtype}")
-    if bias is not None and (bias.dtype is not x.dtype or bias.shape != (N,)):
-        raise ValueError(f"bias is {x.dtype} [{N}], got {bias.dtype} {tuple(bias.shape)}")
+    dev = x.get_device()
+    if bias is not None:
+        if bias.dtype is not x.dtype or bias.shape != (N,):
+            raise ValueError(f"bias is {x.dtype} [{N}], got {bias.dtype} {tuple(bias.shape)}")
+        if bias.get_device() != dev:
+            raise ValueError(f"bias is on {bias.device}, and x on {x.device}")
+        bias = bias.contiguous()
     if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
         raise RuntimeError("4-bit weights have no gradient: call under torch.no_grad()")
-    dev = x.get_device()
-    if codes.get_device() != dev or scales.get_device() != dev or (bias is not None and bias.get_device() != dev):
-        raise ValueError("x, codes, scales and bias are on several devices")
-    if dev < 0 or not _lib.use_kernels(x):
+    if codes.get_device() != dev or scales.get_device() != dev:
+        raise ValueError(f"x is on {x.device}, and its weights on {codes.device} and {scales.device}")
+    if dev < 0:
         return w4_linear_reference(x, codes, scales, group_size, bias)
-    x2 = x if x.dim() == 2 else x.reshape(x.numel() // K, K)
+    x2 = x if len(shape) == 2 else x.reshape(x.numel() // K, K)
+    M = x2.shape[0]
     step, one = x2.stride()
     if one != 1:
         x2, step = x2.contiguous(), K
-    M = x2.shape[0]
     if M >= EXPAND_ROWS and x.dtype is torch.bfloat16 and K % 8 == 0:
         w = torch.empty(N, K, dtype=x.dtype, device=x.device)
-        rc = _lib.lib().atb_w4_expand(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), N, K, group_size, _lib.DT[x.dtype],
+        rc = _lib.lib().atb_w4_expand(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), N, K, group_size, kind,
                                       _lib.stream_of(dev))
         _lib.check(rc, "atb_w4_expand")
-        return gemm(x2, w, bias=bias).view(*x.shape[:-1], N)
-    y = x.new_empty(*x.shape[:-1], N)
+        return gemm(x2, w, bias=bias).view(*shape[:-1], N)
+    y = x.new_empty(M, N) if x2 is x else x.new_empty(*shape[:-1], N)
     base = x2.data_ptr()
     if codes.data_ptr() % 16:
         codes = codes.clone()
     rc = _lib.lib().atb_w4_linear(base, codes.data_ptr(), scales.data_ptr(), _lib.addr(bias), y.data_ptr(), M, N, K, group_size, step,
-                                  int(base % 16 == 0 and step % 8 == 0), _lib.DT[x.dtype], _lib.stream_of(dev), _lib.status_addr(x))
+                                  int((base | 2 * step) & 15 == 0), kind, _lib.stream_of(dev), _lib.status_addr(x))
     _lib.check(rc, "atb_w4_linear")
     return y
