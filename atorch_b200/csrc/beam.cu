@@ -408,23 +408,27 @@ extern "C" int atb_beam_select(const void* logits, const void* scores, const voi
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t rc = cudaErrorInvalidValue;
   const long long part = (V + shares - 1) / shares + 7, pieces = (part * (dtype == 2 ? 4 : 2) / 16 + THREADS - 1) / THREADS;
-#define ROWS_OF(T, P)                                                                                                    \
-  rc = cluster > 8 && !large_clusters<T, P>() ? cudaErrorInvalidValue : launch_after(beam_row_kernel<T, P>, dim3(B * W * shares), THREADS, 0, st, cluster, (const T*)logits, (const float*)scores, \
-                    (const unsigned char*)finished, (unsigned long long*)best, final, fused ? W : 1, V, row_stride, wide, eos, keep, \
-                    (const int*)status)
-#define ROWS(T)                                 \
-  if (!wide || pieces > 4) ROWS_OF(T, 0);       \
-  else if (pieces > 2) ROWS_OF(T, 4);           \
-  else ROWS_OF(T, 2)
-  if (dtype == 0) { ROWS(__nv_bfloat16); }
-  if (dtype == 1) { ROWS(__half); }
-  if (dtype == 2) { ROWS(float); }
+#define ROWS_OF(T, P)                                                                                                      \
+  {                                                                                                                        \
+    if (cluster <= 8 || large_clusters<T, P>())                                                                            \
+      rc = launch_after(beam_row_kernel<T, P>, dim3(B * W * shares), THREADS, 0, st, cluster, (const T*)logits,             \
+                        (const float*)scores, (const unsigned char*)finished, (unsigned long long*)best, final,             \
+                        fused ? W : 1, V, row_stride, wide, eos, keep, (const int*)status);                                 \
+  }
+#define ROWS(T)                              \
+  {                                          \
+    if (!wide || pieces > 4) ROWS_OF(T, 0)   \
+    else if (pieces > 2) ROWS_OF(T, 4)       \
+    else ROWS_OF(T, 2)                       \
+  }
+  if (dtype == 0) ROWS(__nv_bfloat16)
+  if (dtype == 1) ROWS(__half)
+  if (dtype == 2) ROWS(float)
 #undef ROWS_OF
 #undef ROWS
-  if (rc != cudaSuccess) return -5;
-  if (fused) return 0;
-  return launch_after(beam_join_kernel, dim3(B), 256, 0, st, 1, (const unsigned long long*)best, (const unsigned char*)finished, final,
-                      W, keep, eos, (const int*)status) == cudaSuccess ? 0 : -5;
+  if (rc != cudaSuccess || fused) return launched(rc);
+  return launched(launch_after(beam_join_kernel, dim3(B), 256, 0, st, 1, (const unsigned long long*)best, (const unsigned char*)finished, final,
+                      W, keep, eos, (const int*)status));
 }
 
 extern "C" int atb_beam_reorder(void* codes, void* scales, void* table, const void* lengths, const void* parents, int B, int W,
@@ -449,5 +453,5 @@ extern "C" int atb_beam_reorder(void* codes, void* scales, void* table, const vo
   else if (W <= 16) MOVE(16);
   else MOVE(32);
 #undef MOVE
-  return rc == cudaSuccess ? 0 : -5;
+  return launched(rc);
 }

@@ -592,6 +592,12 @@ ATB_DEVICE __half from_f32<__half>(float v) { return __float2half_rn(v); }
 #include <cstdio>
 #include <utility>
 namespace atb {
+// What a launcher returns; an error does not stay behind for others to find.
+inline int launched(cudaError_t rc) {
+  if (rc == cudaSuccess) return 0;
+  cudaGetLastError();
+  return -5;
+}
 // Launch that may start before the kernel in front has ended (see grid_wait), in clusters of `cluster` CTAs.
 template <typename... P, typename... A>
 inline cudaError_t launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster,

@@ -95,7 +95,8 @@ constexpr int SMALL = 128;      // threads of a block of the two kernels below: 
 // the formula evaluated operation by operation, and do not depend on how a compiler contracts it. The scale is rounded to bf16
 // before the codes are taken: the code is the nearest one of the scale that is kept. Bound by memory where there are many tokens:
 // so a division is a product with the reciprocal, and only a quotient that comes within 1e-5 of the middle of two codes (the
-// product is off by 2e-6 at most) is divided (a true division for each took 78 us for 10900 tokens of 48 heads, ... us now).
+// product is off by 2e-6 at most) is divided (a true division for each took 78 us for 10900 tokens of 48 heads, 53 us
+// now: 4.4 TB/s).
 template <typename T, int D, int PER>
 __global__ void __launch_bounds__(SMALL, PER == 1 || sizeof(T) == 4 ? 1 : 7) kv4_append_kernel(const T* qkv, T* q_out, Cache c, const int* seq, const int* pos,
                                                            const float* cosT, const float* sinT, int positions, int n_q,
@@ -388,16 +389,20 @@ struct AttnArgs {
 //   o[d, n] = sum_t (p[t, n] vs[t]) (code[t, d] - 8) + sum_t p[t, n] (vm[t] + 8 vs[t])
 // q is scaled by a power of two to at most 2^15 before it is rounded to fp16 (bf16 and fp16 values stay exact down to 2^-29 of
 // the largest), p vs by 2^(11 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
-// 11 bits of it are kept. The 8s are taken off as
-// products of the same rounded numbers (a row of 8s in the place of codes), so that their rounding errors weigh as much as a value
-// and not as a code: fp16 results were off by 3.6e-4 without it, of 2.1e-4 that fp16 takes. Sums, maxima and denominators are fp32.
+// 11 bits of it are kept. The 8s are taken off as products of the same rounded numbers (a row of 8s in the place of codes), so that
+// their rounding errors weigh as much as a value and not as a code: fp16 results of 5 tokens, 64-wide heads, were off by 3.6e-4
+// without it, 2.3e-4 now, of which rounding to fp16 takes 2.1e-4. Sums, maxima and denominators are fp32.
 //
 // A warp has every fourth tile of a segment. Its tiles come through a ring of its own in shared memory, filled by the copy unit
 // STAGES tiles ahead. What bounds the kernel beside memory is the integer pipe: 5 operations for 8 codes of a key, 6 of a value.
-// So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and
-// only the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by
-// 2^4 before everything is rescaled: a warp sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its values'
-// words without a bank conflict worse than two ways.
+// So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and only
+// the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by 2^4 before everything is rescaled: a warp
+// sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its
+// values' words without a bank conflict worse than two ways.
+// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 60 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 31 us. The
+// copies alone would take 32 and 10: the warps issue every other clock, the integer pipe is busy 57 % of the time. Loading tiles
+// into registers a warp's tile at a time took 99 and 51 us; queries in shared memory, a fifth block an SM, or the products of the
+// next tile beside the sums of this one were no faster.
 template <int D, int NT>
 struct Shape {
   static constexpr int COLS = 8 * NT, STAGE = TILE * D + TILE * 8, STAGES = NT == 1 ? 2 : 4, RING = WARPS * STAGES * STAGE;
@@ -850,21 +855,21 @@ int launch_append(const void* qkv, void* q, const Cache& c, const void* seq, con
                   int positions, int tokens, int n_q, long long stride, cudaStream_t st, int* status) {
   const int each = SMALL / (D / 16), heads = n_q + 2 * c.kv_heads;
   // where there are more blocks than the GPU holds, a thread has three heads: more loads on their way, one look at the page table
-  // and the angles (one head each: 82 us for 10900 tokens of 48 heads and their reading back, three: ... us)
+  // and the angles (one head each: 82 us for 10900 tokens of 48 heads and their reading back, three: 70)
   const bool many = (long long)tokens * ((heads + each - 1) / each) > 148 * 16 && heads > each;
   const int blocks = many ? (heads + 3 * each - 1) / (3 * each) : (heads + each - 1) / each;
   if (blocks > 65535) return -2;
-  return launch_after(many ? kv4_append_kernel<T, D, 3> : kv4_append_kernel<T, D, 1>, dim3(tokens, blocks), SMALL, 0, st, 1,
+  return launched(launch_after(many ? kv4_append_kernel<T, D, 3> : kv4_append_kernel<T, D, 1>, dim3(tokens, blocks), SMALL, 0, st, 1,
                       (const T*)qkv, (T*)q, c, (const int*)seq, (const int*)pos, (const float*)cosT, (const float*)sinT, positions,
-                      n_q, stride, status) == cudaSuccess ? 0 : -5;
+                      n_q, stride, status));
 }
 template <typename T, int D>
 int launch_read(void* k, void* v, const Cache& c, const void* seq, const void* pos, int tokens, cudaStream_t st, int* status) {
   const int each = SMALL / (D / 8), blocks = (c.kv_heads + each - 1) / each;
   if (blocks > 65535) return -2;
   const bool many = (long long)tokens * blocks > 148 * 16 * 2;
-  return launch_after(many ? kv4_read_kernel<T, D, 4> : kv4_read_kernel<T, D, 1>, dim3(many ? (tokens + 3) / 4 : tokens, blocks), SMALL,
-                      0, st, 1, (T*)k, (T*)v, c, (const int*)seq, (const int*)pos, tokens, status) == cudaSuccess ? 0 : -5;
+  return launched(launch_after(many ? kv4_read_kernel<T, D, 4> : kv4_read_kernel<T, D, 1>, dim3(many ? (tokens + 3) / 4 : tokens, blocks), SMALL,
+                      0, st, 1, (T*)k, (T*)v, c, (const int*)seq, (const int*)pos, tokens, status));
 }
 
 template <typename T, int D, int NT>
@@ -872,11 +877,11 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   using Sh = Shape<D, NT>;
   static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
   int device = 0;
-  if (cudaGetDevice(&device) != cudaSuccess) return -5;
+  if (cudaGetDevice(&device) != cudaSuccess) return launched(cudaErrorInvalidDevice);
   const unsigned long long bit = 1ull << (device & 63);
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    if (cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::RING) != cudaSuccess)
-      return -4;
+    const int rc = launched(cudaFuncSetAttribute(kv4_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Sh::RING));
+    if (rc != 0) return rc;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   const long long per = (a.S * a.group + Sh::COLS - 1) / Sh::COLS * (long long)a.c.kv_heads;
@@ -890,11 +895,10 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   if (cut) a.owners = reinterpret_cast<int2*>(a.partial + 2LL * a.ctas * Sh::COLS * (D + 2));
   const unsigned grid = (unsigned)(most < a.ctas ? most : a.ctas);
   if (!cut) a.ctas = 0;
-  if (launch_after(kv4_attention_kernel<T, D, NT>, dim3(cut || runs > grid ? grid : (unsigned)runs), WARPS * 32, Sh::RING, st, 1, a) !=
-      cudaSuccess)
-    return -5;
-  if (!cut) return 0;
-  return launch_after(kv4_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per) == cudaSuccess ? 0 : -5;
+  const int rc = launched(launch_after(kv4_attention_kernel<T, D, NT>, dim3(cut || runs > grid ? grid : (unsigned)runs), WARPS * 32,
+                                       Sh::RING, st, 1, a));
+  if (rc != 0 || !cut) return rc;
+  return launched(launch_after(kv4_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per));
 }
 }  // namespace
 

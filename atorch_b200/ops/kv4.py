@@ -70,6 +70,8 @@ def _cache(layer: Layer, page_table: torch.Tensor) -> Tuple[int, ...]:
     if scales.get_device() != dev or page_table.get_device() != dev:
         _same_device(dev, scales, page_table)
     rows, width = page_table.shape
+    if width * page_size > 0x7fffffff:
+        raise ValueError(f"{width} pages of {page_size} tokens a sequence: positions have 31 bits")
     return (codes_at, scales_at, page_table.data_ptr(), pages, kv_heads, page_size.bit_length() - 1, rows, width, steps[0], 2 * half,
             dev)
 
@@ -144,7 +146,7 @@ def kv4_append(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tenso
     projection of ``T`` tokens; token ``t`` goes to position ``pos[t]`` of sequence ``seq[t]`` (``seq=None``: of sequence ``t``).
     With ``cos`` / ``sin`` (fp32 ``[positions, head_dim / 2]``, see :func:`~atorch_b200.ops.rope_tables`) the query and key
     heads are turned to the position first. Returns the query heads ``[T, n_q, head_dim]`` in the type of ``qkv``. A negative
-    position is padding: its token is not kept, its queries come back as they are. Two tokens at one place: either is kept.
+    position is padding: its token is not kept, its queries come back as they are. What two tokens at one place leave there is not defined.
 
     The rotation is not rounded before the codes are taken; queries are rounded once."""
     codes, scales, table, pages, KV, shift, rows, most, stride, D, dev = _cache(layer, page_table)

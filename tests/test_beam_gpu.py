@@ -163,3 +163,23 @@ def test_refusals():
                    (4, ok[4].long()), (4, ok[4][0]), (2, ok[2].cpu())):
         with pytest.raises(ValueError):
             ops.beam_reorder(*[bad if j == i else t for j, t in enumerate(ok)])
+
+
+@pytest.mark.parametrize("B,W,V,keep", [(2, 3, 20000, None), (1, 6, 9000, None), (3, 7, 18000, 5), (1, 4, 32000, 32), (1, 11, 5000, None),
+                                        (2, 16, 8192, 16), (1, 16, 8193, 16), (40, 5, 4100, None), (1, 1, 131072, 9), (1, 17, 300, None),
+                                        (1, 1, 200003, 3)])
+def test_select_by_one_cluster_or_by_several(B, W, V, keep):
+    """Sizes on both sides of the rule that joins a sequence's beams in one cluster, and clusters of every size."""
+    g = _gen(V + W)
+    scores = torch.randn(B, W, generator=g, device=DEV) - 5
+    for dtype in (torch.bfloat16, torch.float32):
+        logits = (torch.randn(B, W, V, generator=g, device=DEV) * 3).to(dtype)
+        _check(logits, scores, keep=keep)
+        _check(logits, scores, torch.rand(B, W, generator=g, device=DEV) < 0.3, 0, keep)
+
+
+def test_an_infinite_score():
+    """A sum that is infinite whatever follows: the first tokens."""
+    logits = torch.randn(1, 2, 3000, generator=_gen(9), device=DEV)
+    got = ops.beam_select(logits, torch.tensor([[0.0, math.inf]], device=DEV), keep=4)
+    assert (got[0] == math.inf).all() and (got[2] == 1).all() and torch.equal(got[1], torch.arange(4, device=DEV)[None])
