@@ -259,10 +259,11 @@ __global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, co
 // The work is one row of units: the tiles of 32 tokens of a sequence, once per head and column tile, one sequence behind another.
 // Every block takes an equal run of it, which it finds for itself from the lengths on the device (they need not be known on the
 // host), so that long and short sequences fill the GPU alike. A run is cut into segments where a sequence (of a head) ends;
-// what a segment costs beside its tiles counts as START units before the first. A segment that is a whole sequence is finished
+// what a segment costs beside its tiles counts as START units before the first (5, 8 and 12 of them: 32 sequences of up to 4096
+// tokens 33.9, 32.0 and 32.0 us, 19 of up to 1800 15.4, 15.1 and 14.6). A segment that is a whole sequence is finished
 // in place; of the others, the run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins in
 // the order of the blocks.
-constexpr int WARPS = 4, TILE = 32, START = 8;
+constexpr int WARPS = 4, TILE = 32, START = 12;
 constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
 
 ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
@@ -394,15 +395,16 @@ struct AttnArgs {
 // without it, 2.3e-4 now, of which rounding to fp16 takes 2.1e-4. Sums, maxima and denominators are fp32.
 //
 // A warp has every fourth tile of a segment. Its tiles come through a ring of its own in shared memory, filled by the copy unit
-// STAGES tiles ahead. What bounds the kernel beside memory is the integer pipe: 5 operations for 8 codes of a key, 6 of a value.
+// STAGES tiles ahead. Beside the copies the integer pipe has most to do: 5 operations for 8 codes of a key, 6 of a value.
 // So the rest of a tile is kept short: scores are taken relative to the running maximum, which is looked at by one vote, and only
 // the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by 2^4 before everything is rescaled: a warp
 // sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its
 // values' words without a bank conflict worse than two ways.
-// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 60 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 31 us. The
-// copies alone would take 32 and 10: the warps issue every other clock, the integer pipe is busy 57 % of the time. Loading tiles
-// into registers a warp's tile at a time took 99 and 51 us; queries in shared memory, a fifth block an SM, or the products of the
-// next tile beside the sums of this one were no faster.
+// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 58 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 32 us. With
+// the arithmetic left out, the copies, waits and starts take 50 and 23 us, and a library's sum over as many bytes 41 and 20: memory
+// bounds the kernel, and of the arithmetic (an instruction every other clock, the integer pipe busy 57 % of the time) what a block
+// does while it has no copies on their way. Loading tiles into registers a warp's tile at a time took 99 and 51 us; a third stage,
+// queries in shared memory, a fifth block an SM, or the products of the next tile beside the sums of this one were no faster.
 template <int D, int NT>
 struct Shape {
   static constexpr int COLS = 8 * NT, STAGE = TILE * D + TILE * 8, STAGES = NT == 1 ? 2 : 4, RING = WARPS * STAGES * STAGE;
@@ -443,9 +445,11 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   uint32_t loads = 0;            // tiles that this warp has taken from its ring
 
   // A tile is two pieces of 16 tokens, each in one page, of three copies: keys, values, scales. Lane 3 p + x has copy x of piece p.
+  // Where a page holds a whole tile, the first piece's copies bring both (two sequences of 100k tokens: 60.3 us, now 58.9).
   const int piece = lane / 3, what = lane - 3 * piece;
   const bool copies = lane < 6;
   const long long page_stride = ((what < 2 ? (long long)c.kv_heads * D : c.kv_heads * 8LL) << c.page_shift);
+  const bool whole_tiles = (1 << c.page_shift) >= TILE;
   const int token_bytes = what < 2 ? D / 2 : 8;
   const int dst_at = (what < 2 ? what * (TILE * D / 2) : TILE * D) + piece * 16 * token_bytes;
 
@@ -500,9 +504,10 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
       const bool both = t - piece * 16 + 16 < len;         // the second piece may lie behind the sequence, and have no page
       if (lane == 0) mbar_expect_tx(&bars[warp][s], both ? Sh::STAGE : Sh::STAGE / 2);
       __syncwarp();
-      if (copies && t < len)
+      const int tokens = both && whole_tiles ? TILE : 16;
+      if (copies && t < len && (tokens == 16 || piece == 0))
         bulk_load(ring + s * Sh::STAGE + dst_at, src_at + page * page_stride + (t & ((1 << c.page_shift) - 1)) * token_bytes,
-                  16 * token_bytes, &bars[warp][s]);
+                  tokens * token_bytes, &bars[warp][s]);
     };
     for (int j = 0; j < STAGES; ++j) fetch(j);
 
