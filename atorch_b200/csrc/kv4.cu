@@ -432,16 +432,17 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   mbar_fence_init();
   grid_go();
   grid_wait();
-  if (__syncthreads_or(threadIdx.x == 0 && *a.status != 0)) return;    // one answer for the block: others may fail meanwhile
+  const int failed = threadIdx.x == 0 ? *a.status : 0;       // on its way beside the lengths
   const int columns = a.S * a.group, col_tiles = (columns + COLS - 1) / COLS, per = col_tiles * c.kv_heads;
   Plan plan{};
   long long u = blockIdx.x, run_end = (long long)c.rows * per;       // whole sequences: their numbers
   if (a.ctas > 0) {
     plan = make_plan(c, a.lengths, per, a.ctas, a.status);
-    if ((int)blockIdx.x >= plan.ctas) return;
     u = plan.begin(blockIdx.x);
     run_end = plan.begin(blockIdx.x + 1);
   }
+  if (__syncthreads_or(failed != 0)) return;       // one answer for the block: others may fail meanwhile
+  if (a.ctas > 0 && (int)blockIdx.x >= plan.ctas) return;
   uint32_t loads = 0;            // tiles that this warp has taken from its ring
 
   // A tile is two pieces of 16 tokens, each in one page, of three copies: keys, values, scales. Lane 3 p + x has copy x of piece p.
