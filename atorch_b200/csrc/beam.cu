@@ -292,85 +292,112 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long
 }
 
 // The cache follows its beams: row b W + w of the table takes the full pages of row b W + parent[w], and its own last page the
-// tokens of that row's last page. A thread has one place of all W rows and reads them all before it writes any, so the rows may
-// change places. Bound by memory: each token of the last pages that moves is read and written once. What it
-// looks up before, lengths, parents and pages, serves several layers.
-template <int MAX_W>
+// tokens of that row's last page. A warp has the same places of all rows that move, as many as give its lanes EACH of them, and
+// reads them all before it writes any, so the rows may change places. Bound by memory: each token of the last pages that moves
+// is read and written once. Measured with 32 layers, 8 heads of 128, 10 tokens in the last page: 24 sequences of 8 beams (57 MB
+// written) 28 us, 4.1 TB/s both ways; 48 of 4 26 us; 6 of 32 34 us. Two places a lane took 31, 28 and 47; eight 36, 32 and 37; a
+// block in the place of the warp 33, 30 and 36; a thread with its place of all rows 32, 25 and 59.
+constexpr int EACH = 4;
 __global__ void __launch_bounds__(256) beam_reorder_kernel(uint8_t* codes, uint8_t* scales, int* table, const int* lengths,
                                                            const int* parents, int W, int width, long long table_stride,
                                                            int layers, int pages, long long page_bytes, long long scale_bytes,
                                                            int kv_heads, int page_shift, int token_bytes, int* status) {
+  __shared__ int2 sh_rows[MOST], sh_pages[MOST];       // of the rows that move: from and to
+  __shared__ int sh_moving;
   grid_go();
   grid_wait();
-  if (__syncthreads_or(threadIdx.x == 0 && *status != 0)) return;
-  const long long b = blockIdx.y, first = b * W;
+  const int failed = threadIdx.x == 0 ? *status : 0;
+  const long long first = (long long)blockIdx.y * W;
   const int n = lengths[first], full = n >> page_shift, rest = n - (full << page_shift);
-  int from[MAX_W];
-  bool good = n >= 0 && full + (rest > 0) <= width;
-#pragma unroll
-  for (int w = 0; w < MAX_W; ++w) {
-    from[w] = w < W ? parents[first + w] : w;
-    good = good && (w >= W || (from[w] >= 0 && from[w] < W && lengths[first + w] == n));
+  bool good = true;
+  if (threadIdx.x < 32) {
+    const int w = threadIdx.x, own = w < W ? lengths[first + w] : n, from = w < W ? parents[first + w] : w;
+    good = n >= 0 && own == n && full + (rest > 0) <= width && from >= 0 && (from < W || w >= W);
+    int2 page = make_int2(0, 0);
+    if (good && w < W && rest > 0) {
+      page = make_int2(table[(first + from) * table_stride + full], table[(first + w) * table_stride + full]);
+      good = min(page.x, page.y) >= 0 && max(page.x, page.y) < pages;
+    }
+    const unsigned moving = __ballot_sync(0xffffffffu, from != w);
+    const int place = __popc(moving & ((1u << w) - 1));
+    if (from != w) {
+      sh_rows[place] = make_int2(from, w);
+      sh_pages[place] = page;
+    }
+    if (w == 0) sh_moving = __popc(moving);
   }
-  if (!good) {
+  if (__syncthreads_or(failed != 0)) return;
+  if (__syncthreads_or(!good)) {
     if (threadIdx.x == 0) atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
     return;
   }
-  if (blockIdx.z == gridDim.z - 1) {                // the table
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < full; i += gridDim.x * 256) {
-      int x[MAX_W];
+  const int moving = sh_moving, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (moving == 0) return;
+  const unsigned per_token = token_bytes / 16, per_head = rest * per_token, code_pieces = 2 * kv_heads * per_head;
+  const unsigned head_bytes = token_bytes << page_shift;
+  const bool is_table = blockIdx.x == gridDim.x - 1;
+  // a round is `span` places, of all rows that move
+  const unsigned all = is_table ? full : code_pieces + kv_heads * rest;
+  if (all == 0) return;
+  const unsigned most = EACH * 32 / moving / 4 * 4, rounds = (all + most - 1) / most, span = ((all + rounds - 1) / rounds + 3) / 4 * 4;
+  unsigned mine[EACH];            // row and place in the round, of this thread
 #pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W) x[w] = table[(first + from[w]) * table_stride + i];
+  for (int k = 0; k < EACH; ++k) {
+    const unsigned slot = k * 32 + lane, m = slot / span;
+    mine[k] = m << 16 | (slot - m * span);
+  }
+  if (is_table) {
+    for (unsigned round = warp; round < rounds; round += 8) {
+      int x[EACH];
 #pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) table[(first + w) * table_stride + i] = x[w];
+      for (int k = 0; k < EACH; ++k) {
+        const unsigned m = mine[k] >> 16, i = round * span + (mine[k] & 0xffff);
+        if (m < (unsigned)moving && i < all) x[k] = table[(first + sh_rows[m].x) * table_stride + i];
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const unsigned m = mine[k] >> 16, i = round * span + (mine[k] & 0xffff);
+        if (m < (unsigned)moving && i < all) table[(first + sh_rows[m].y) * table_stride + i] = x[k];
+      }
     }
     return;
   }
-  if (rest == 0) return;
-  int page[MAX_W];
+  // the warps of a sequence take the rounds of all layers in turn
+  const unsigned step = (gridDim.x - 1) * 8;
+  unsigned layer = (blockIdx.x * 8 + warp) / rounds, round = (blockIdx.x * 8 + warp) % rounds;
+  while (layer < (unsigned)layers) {
+    uint8_t* const code_page = codes + (long long)layer * pages * page_bytes;
+    uint8_t* const scale_page = scales + (long long)layer * pages * scale_bytes;
+    uint4 x[EACH];
+    unsigned at[EACH];
 #pragma unroll
-  for (int w = 0; w < MAX_W; ++w) {
-    page[w] = w < W ? table[(first + w) * table_stride + full] : 0;
-    good = good && page[w] >= 0 && page[w] < pages;
-  }
-  if (!good) {
-    if (threadIdx.x == 0) atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
-    return;
-  }
-  int source[MAX_W];              // page of the parent
+    for (int k = 0; k < EACH; ++k) {
+      const unsigned m = mine[k] >> 16, i = round * span + (mine[k] & 0xffff);
+      if (m >= (unsigned)moving || i >= all) continue;
+      if (i < code_pieces) {
+        const unsigned h = i / per_head;
+        at[k] = h * head_bytes + (i - h * per_head) * 16;
+        x[k] = *reinterpret_cast<const uint4*>(code_page + sh_pages[m].x * page_bytes + at[k]);
+      } else {
+        const unsigned j = i - code_pieces, h = j / rest;
+        at[k] = ((h << page_shift) + j - h * rest) * 8;
+        *reinterpret_cast<uint2*>(&x[k]) = *reinterpret_cast<const uint2*>(scale_page + sh_pages[m].x * scale_bytes + at[k]);
+      }
+    }
+    __syncwarp();
 #pragma unroll
-  for (int w = 0; w < MAX_W; ++w) {
-    source[w] = 0;
-#pragma unroll
-    for (int o = 0; o < MAX_W; ++o) source[w] = from[w] == o ? page[o] : source[w];
-  }
-  const int per_token = token_bytes / 16, per_head = rest * per_token, code_pieces = 2 * kv_heads * per_head;
-  const int head_bytes = token_bytes << page_shift, all = code_pieces + kv_heads * rest;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < all; i += gridDim.x * 256) {
-    const bool code = i < code_pieces;
-    const int j = code ? i : i - code_pieces, h = j / (code ? per_head : rest);
-    const long long at = code ? (long long)h * head_bytes + (j - h * per_head) * 16 : ((long long)h << (page_shift + 3)) + (j - h * rest) * 8;
-    const long long bytes = code ? page_bytes : scale_bytes;
-    uint8_t* const base = (code ? codes : scales) + at;
-    for (int layer = blockIdx.z; layer < layers; layer += gridDim.z - 1) {
-      uint8_t* const here = base + (long long)layer * pages * bytes;
-      uint4 x[MAX_W];
-#pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) {
-          const uint8_t* p = here + source[w] * bytes;
-          if (code) x[w] = *reinterpret_cast<const uint4*>(p);
-          else *reinterpret_cast<uint2*>(&x[w]) = *reinterpret_cast<const uint2*>(p);
-        }
-#pragma unroll
-      for (int w = 0; w < MAX_W; ++w)
-        if (w < W && from[w] != w) {
-          uint8_t* p = here + page[w] * bytes;
-          if (code) *reinterpret_cast<uint4*>(p) = x[w];
-          else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&x[w]);
-        }
+    for (int k = 0; k < EACH; ++k) {
+      const unsigned m = mine[k] >> 16, i = round * span + (mine[k] & 0xffff);
+      if (m >= (unsigned)moving || i >= all) continue;
+      if (i < code_pieces) *reinterpret_cast<uint4*>(code_page + sh_pages[m].y * page_bytes + at[k]) = x[k];
+      else *reinterpret_cast<uint2*>(scale_page + sh_pages[m].y * scale_bytes + at[k]) = *reinterpret_cast<const uint2*>(&x[k]);
+    }
+    layer += step / rounds;
+    round += step % rounds;
+    if (round >= rounds) {
+      round -= rounds;
+      ++layer;
     }
   }
 }
@@ -440,18 +467,10 @@ extern "C" int atb_beam_reorder(void* codes, void* scales, void* table, const vo
   const long long page_bytes = (2LL * kv_heads * token_bytes) << page_shift, scale_bytes = (8LL * kv_heads) << page_shift;
   const long long most = (2LL * kv_heads * token_bytes / 16 + kv_heads) << page_shift;
   if (page_bytes > 0x7fffffffLL || most > 0x7fffffffLL) return -2;
-  // layers in as many shares as give four blocks an SM, and one share for the table
-  const long long blocks = (most + 255) / 256 * B, want = (148 * 4 + blocks - 1) / blocks;
-  const dim3 grid((unsigned)((most + 255) / 256), B, (unsigned)((want < layers ? want : layers) + 1));
-  cudaError_t rc;
-#define MOVE(MAX_W)                                                                                                        \
-  rc = launch_after(beam_reorder_kernel<MAX_W>, grid, 256, 0, (cudaStream_t)stream, 1, (uint8_t*)codes, (uint8_t*)scales,    \
-                    (int*)table, (const int*)lengths, (const int*)parents, W, width, table_stride, layers, pages, page_bytes,       \
-                    scale_bytes, kv_heads, page_shift, token_bytes, (int*)status)
-  if (W <= 4) MOVE(4);
-  else if (W <= 8) MOVE(8);
-  else if (W <= 16) MOVE(16);
-  else MOVE(32);
-#undef MOVE
-  return launched(rc);
+  // eight blocks an SM where there is work for them, and one of a sequence for the table
+  const long long places = EACH * 32 / W / 4 * 4, rounds = (most + places - 1) / places * layers / 8 + 1, want = (148 * 8 + B - 1) / B;
+  return launched(launch_after(beam_reorder_kernel, dim3((unsigned)(want < rounds ? want : rounds) + 1, B), 256, 0, (cudaStream_t)stream,
+                               1, (uint8_t*)codes, (uint8_t*)scales, (int*)table, (const int*)lengths, (const int*)parents, W,
+                               width, table_stride, layers, pages, page_bytes, scale_bytes, kv_heads, page_shift, token_bytes,
+                               (int*)status));
 }
