@@ -79,7 +79,8 @@ struct Piece {
   }
 };
 // P pieces of a thread stay in registers, all asked for at once; P = 0: they are read (from the first-level cache) every time. Two
-// and four pay (4 beams of 32000 tokens 12.9 -> 11.9 us with what follows); eight leave room for two blocks an SM (192 beams 15 -> 22).
+// and four pay (4 beams of 32000 tokens 12.9 -> 11.9 us with what follows); eight leave room for three blocks an SM and pay as long as
+// there are no more (192 beams 17.5 -> 14.5 us; with two blocks an SM, in two turns, 22).
 template <typename T, int P>
 struct Share {
   static constexpr int N = Piece<T>::N;
@@ -143,7 +144,7 @@ ATB_DEVICE int place_of(const unsigned long long* keys, int n, int i) {
 // and the first picks the best of those. The row comes from memory once, and from registers or the first-level cache after that.
 // Bound by latency for a few beams (one block a row, with the row's 64 KB read three times from L2, took 17 us).
 template <typename T, int P>
-__global__ void __launch_bounds__(THREADS) beam_row_kernel(const T* logits, const float* scores, const unsigned char* finished,
+__global__ void __launch_bounds__(THREADS, P == 8 ? 3 : 1) beam_row_kernel(const T* logits, const float* scores, const unsigned char* finished,
                                                            unsigned long long* best, Out final, int beams, int V,
                                                            long long row_stride, int wide, int eos, int keep, const int* status) {
   __shared__ Sum warp_sums[THREADS / 32], share_sum;
@@ -444,7 +445,8 @@ extern "C" int atb_beam_select(const void* logits, const void* scores, const voi
   }
 #define ROWS(T)                              \
   {                                          \
-    if (!wide || pieces > 4) ROWS_OF(T, 0)   \
+    if (!wide || pieces > 8 || (pieces > 4 && (long long)B * W * shares > 3 * 148)) ROWS_OF(T, 0) \
+    else if (pieces > 4) ROWS_OF(T, 8)       \
     else if (pieces > 2) ROWS_OF(T, 4)       \
     else ROWS_OF(T, 2)                       \
   }

@@ -183,3 +183,22 @@ def test_an_infinite_score():
     logits = torch.randn(1, 2, 3000, generator=_gen(9), device=DEV)
     got = ops.beam_select(logits, torch.tensor([[0.0, math.inf]], device=DEV), keep=4)
     assert (got[0] == math.inf).all() and (got[2] == 1).all() and torch.equal(got[1], torch.arange(4, device=DEV)[None])
+
+
+@pytest.mark.parametrize("B,W,V,keep", [(24, 8, 20000, None), (1, 3, 100003, 7), (2, 12, 10900, None), (74, 3, 16001, 4)])
+def test_select_with_a_whole_row_in_registers(B, W, V, keep):
+    """Five to eight pieces of 16 bytes a thread, as clusters of a beam and of a sequence, and sizes just beyond."""
+    g = _gen(V)
+    scores = torch.randn(B, W, generator=g, device=DEV) - 5
+    for dtype in (torch.bfloat16, torch.float16):
+        logits = (torch.randn(B, W, V, generator=g, device=DEV) * 3).to(dtype)
+        logits[:, 0, V // 2:] = -math.inf
+        _check(logits, scores, keep=keep)
+        _check(logits, scores, torch.rand(B, W, generator=g, device=DEV) < 0.3, 0, keep)
+
+
+@pytest.mark.parametrize("B,W,length,page,KV,D,layers", [(24, 8, 410, 16, 8, 128, 4), (2, 3, 1000, 2048, 1, 64, 2), (70, 2, 33, 16, 1, 64, 1),
+                                                         (1, 16, 1603, 16, 2, 64, 3), (1, 32, 1601, 16, 1, 64, 40), (3, 31, 63, 64, 3, 128, 5)])
+def test_reorder_in_many_rounds(B, W, length, page, KV, D, layers):
+    """More places, pages or layers than the warps of a sequence take at a time."""
+    test_reorder(B, W, length, page, KV, D, layers)
