@@ -400,7 +400,7 @@ struct AttnArgs {
 // the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by 2^4 before everything is rescaled: a warp
 // sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its
 // values' words without a bank conflict worse than two ways.
-// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 58 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 32 us. With
+// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 58 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 31 us. With
 // the arithmetic left out, the copies, waits and starts take 50 and 23 us, and a library's sum over as many bytes 41 and 20: memory
 // bounds the kernel, and of the arithmetic (an instruction every other clock, the integer pipe busy 57 % of the time) what a block
 // does while it has no copies on their way. Loading tiles into registers a warp's tile at a time took 99 and 51 us; a third stage,
