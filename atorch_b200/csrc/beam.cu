@@ -168,12 +168,13 @@ __global__ void __launch_bounds__(THREADS, P == 8 ? 3 : 1) beam_row_kernel(const
   Sum s{-INFINITY, 0.f};
   share.each([&](const Piece<T>& v, int) { s.top = fmaxf(s.top, v.top()); },
              [&](float v, int) { s.top = fmaxf(s.top, v); });
-  const float ref = s.top == -INFINITY ? 0.f : s.top, log2e = 1.4426950408889634f, ref2 = ref * log2e;
-  // exponentials on the special-function unit, off by 2^-22: a sum of thousands is as near as its fp32 adds
+  const float ref = s.top == -INFINITY ? 0.f : s.top, log2e = 1.4426950408889634f;
+  // exponentials on the special-function unit, off by 2^-22: a sum of thousands is as near as its fp32 adds. The difference comes
+  // before the factor: it is exactly 0 at the maximum, however large that is (rows masked by a type's lowest value).
   share.each([&](const Piece<T>& v, int) {
 #pragma unroll
-            for (int e = 0; e < Piece<T>::N; ++e) s.sum += fast_exp2(fmaf(v[e], log2e, -ref2));       // (a NaN makes the sum one)
-          }, [&](float v, int) { s.sum += fast_exp2(fmaf(v, log2e, -ref2)); });
+            for (int e = 0; e < Piece<T>::N; ++e) s.sum += fast_exp2((v[e] - ref) * log2e);       // (a NaN makes the sum one)
+          }, [&](float v, int) { s.sum += fast_exp2((v - ref) * log2e); });
   const float my_top = s.top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s = add(s, Sum{__shfl_xor_sync(0xffffffffu, s.top, o), __shfl_xor_sync(0xffffffffu, s.sum, o)});

@@ -202,3 +202,43 @@ def test_select_with_a_whole_row_in_registers(B, W, V, keep):
 def test_reorder_in_many_rounds(B, W, length, page, KV, D, layers):
     """More places, pages or layers than the warps of a sequence take at a time."""
     test_reorder(B, W, length, page, KV, D, layers)
+
+
+@pytest.mark.parametrize("B,W,V,keep", [(2, 3, 40, 4), (1, 4, 32000, None), (3, 8, 4001, 5), (2, 17, 1003, 6), (1, 2, 131072, None), (24, 8, 20000, None)])
+@pytest.mark.parametrize("dtype,mask", [(torch.bfloat16, torch.finfo(torch.bfloat16).min), (torch.float32, torch.finfo(torch.float32).min),
+                                        (torch.bfloat16, -1e30), (torch.float32, -1e20), (torch.float32, -1e10), (torch.float16, -65504.0)])
+def test_finite_masks(B, W, V, keep, dtype, mask):
+    """Tokens masked by a large finite number, most of a row of them or all: the others go on as if the masked were not there."""
+    g, keep = _gen(V), keep or W
+    logits = (torch.randn(B, W, V, generator=g, device=DEV) * 2).to(dtype)
+    scores = torch.randn(B, W, generator=g, device=DEV) - 5
+    for pattern in ("few", "end", "one row", "a token each"):
+        x, masked = logits.clone(), torch.zeros(B, W, V, dtype=torch.bool, device=DEV)
+        if pattern == "few":
+            masked |= torch.arange(V, device=DEV) % 13 != 5
+        elif pattern == "end":
+            masked[..., V // 3:] = True
+        elif pattern == "one row":
+            masked[:, W - 1] = True
+        else:
+            masked |= torch.arange(V, device=DEV) != V - 1
+        x[masked] = mask
+        got, tokens, parents, _ = ops.beam_select(x, scores, keep=keep)
+        lse = torch.logsumexp(x.double(), -1)
+        f = (scores.double().unsqueeze(-1) + (x.double() - lse.unsqueeze(-1))).flatten(1)
+        at = parents.long() * V + tokens
+        row = lambda t: t.gather(1, parents.long())  # noqa: E731
+        # an fp32 sum of exponentials, its logarithm, two differences, of the numbers that enter the kept score
+        tol = 2.0 ** -21 * (row(scores).double().abs() + row(lse).abs() + x.flatten(1).gather(1, at).double().abs() + 12)
+        assert (torch.isfinite(got) & ((got.double() - f.gather(1, at)).abs() <= tol)).all(), pattern
+        assert ((got.double() - f.topk(keep, -1).values).abs() <= tol).all(), pattern
+        hit = masked.flatten(1).gather(1, at)
+        if pattern == "one row":       # masked alike, none is better than another: the row is one more distribution
+            hit = hit & (parents != W - 1)
+        allowed = V if pattern == "one row" else int((~masked[0]).sum())
+        assert (hit.sum(1) == max(0, keep - allowed)).all(), pattern
+        if pattern == "a token each" and abs(mask) > 1e9:       # what is left is alike in 32 bits: by the index
+            rest = max(0, keep - W)
+            assert torch.equal(tokens[:, keep - rest:], torch.arange(rest, device=DEV).expand(B, -1))
+            assert (parents[:, keep - rest:] == 0).all()
+    _lib.check_status(got.device)
