@@ -265,6 +265,7 @@ __global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, co
 // the order of the blocks.
 constexpr int WARPS = 4, TILE = 32, START = 12;
 constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
+constexpr int LEAST_E = 24, AHEAD_E = 12;      // exponent fields of value scales: the least, and how far one may lie above what its weight leaves
 
 ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
   const int n = lengths[b], most = c.width << c.page_shift;
@@ -389,8 +390,10 @@ struct AttnArgs {
 //   s[t, n] = ks[t] (q[n] . code[t]) + km[t] sum(q[n])
 //   o[d, n] = sum_t (p[t, n] vs[t]) (code[t, d] - 8) + sum_t p[t, n] (vm[t] + 8 vs[t])
 // q is scaled by a power of two to at most 2^15 before it is rounded to fp16 (bf16 and fp16 values stay exact down to 2^-29 of
-// the largest), p vs by 2^(11 - e) with e the largest exponent of a value's scale so far, as the maximum of a softmax runs:
-// 11 bits of it are kept. The 8s are taken off as products of the same rounded numbers (a row of 8s in the place of codes), so that
+// the largest, and in range below 2^117), p vs by a power of two that runs with the softmax, for each column its own: by the largest
+// exponent of a value's scale so far, as long as that is not 2^12 above the largest p vs (a token without weight, however large its
+// values, takes no bits from the others; nor does one that a column does not see). 11 bits of p vs are kept, and absolutely
+// 2^-20 of the largest at least. The 8s are taken off as products of the same rounded numbers (a row of 8s in the place of codes), so that
 // their rounding errors weigh as much as a value and not as a code: fp16 results of 5 tokens, 64-wide heads, were off by 3.6e-4
 // without it, 2.3e-4 now, of which rounding to fp16 takes 2.1e-4. Sums, maxima and denominators are fp32.
 //
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
       }
-      const int e = top > 0.f ? min(max((__float_as_int(top) >> 23) - 127, -100), 100) : 0;   // top < 2^(e + 1)
+      const int e = top > 0.f ? min(max((__float_as_int(top) >> 23) - 127, -100), 116) : 0;   // top < 2^(e + 1)
       const float up = pow2(14 - e);
 #pragma unroll
       for (int k = 0; k < KW; ++k)
@@ -581,7 +584,9 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
         ref[j][o] = l[j][o] = z[j][o] = 0.f;
       }
     }
-    int top_e = 24;        // exponent field of the largest value scale so far
+    int top_e[NT][2], least_e = LEAST_E;       // exponent fields that p vs is scaled by, and the lane's least one
+#pragma unroll
+    for (int j = 0; j < NT; ++j) top_e[j][0] = top_e[j][1] = LEAST_E;
     bool unset = true;     // whether a column has no maximum yet
 
     auto tile = [&](const uint8_t* src, int t0, auto masked) {
@@ -627,17 +632,26 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
             }
         }
       }
-      if (__any_sync(0xffffffffu, over > SLACK || (int)(most_scale >> 7) > top_e || unset)) {
-        int e_new = top_e;
+      if (__any_sync(0xffffffffu, over > SLACK || (int)(most_scale >> 7) > least_e || unset)) {
+        uint32_t range = 0;            // the largest exponent, and 255 less the least of those that are not 0
+        int e_vs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = (__float_as_int(vs[i].x) >> 23) & 255;
-          e_new = max(e_new, e == 255 ? 0 : e);       // an infinity is not for the queries that do not see it
+          e_vs[i] = e == 255 ? 0 : e;       // an infinity is not for the queries that do not see it
+          range = __vmaxu2(range, e_vs[i] > 0 ? e_vs[i] | (255 - e_vs[i]) << 16 : 0);
         }
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, o));
-        const float down = __int_as_float((127 + max(top_e - e_new, -126)) << 23);
-        top_e = e_new;
+        for (int o = 4; o < 32; o <<= 1) range = __vmaxu2(range, __shfl_xor_sync(0xffffffffu, range, o));
+        const int e_most = range & 0xffff, e_min = 255 - (int)(range >> 16);
+        bool apart = false;            // whether exponents of a column lie so far apart that the weights have to be looked at
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int o = 0; o < 2; ++o)
+            apart = apart || max(top_e[n][o], e_most) - (m[n][o] == -INFINITY ? e_min : min(top_e[n][o], e_min)) > AHEAD_E;
+        apart = __any_sync(0xffffffffu, apart);
+        least_e = 255;
         unset = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -650,18 +664,30 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
             const float to = fmaxf(m[n][o], ref[n][o] + most), by = (to == -INFINITY ? 0.f : to) - ref[n][o];
-            f[o] = m[n][o] == -INFINITY ? 0.f : fast_exp2(-by);
+            const bool first = m[n][o] == -INFINITY;
+            f[o] = first ? 0.f : fast_exp2(-by);
             m[n][o] = to;
             ref[n][o] += by;
             unset = unset || to == -INFINITY;
             l[n][o] *= f[o];
             z[n][o] *= f[o];
-            f[o] *= down;
 #pragma unroll
-            for (int p = 0; p < 2; ++p) {
-              s[p][n][o] -= by;
-              s[p][n][2 + o] -= by;
+            for (int i = 0; i < 4; ++i) s[i >> 1][n][2 * (i & 1) + o] -= by;
+            int e = max(top_e[n][o], e_most);
+            if (apart) {
+              int weighed = first ? -1000 : top_e[n][o] - __float2int_rd(by);       // p vs so far is below 2^(this - 126)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float v = s[i >> 1][n][2 * (i & 1) + o];
+                if (v > -INFINITY) weighed = max(weighed, e_vs[i] + __float2int_ru(fmaxf(v, -300.f)));
+              }
+#pragma unroll
+              for (int k = 4; k < 32; k <<= 1) weighed = max(weighed, __shfl_xor_sync(0xffffffffu, weighed, k));
+              e = max(LEAST_E, min(e, weighed + AHEAD_E));
             }
+            f[o] *= __int_as_float((127 + max(min(top_e[n][o] - e, 126), -126)) << 23);
+            top_e[n][o] = e;
+            least_e = min(least_e, e);
           }
 #pragma unroll
           for (int i = 0; i < MT; ++i)
@@ -671,14 +697,18 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           for (int e = 0; e < 4; ++e) eights[n][e] *= f[e & 1];
         }
       }
-      const float up = __int_as_float((268 - (int)SLACK - top_e) << 23);      // 2^(15 - SLACK) / 2^(exponent + 1)
+      float up[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int o = 0; o < 2; ++o) up[n][o] = pow2(137 + 4 - (int)SLACK - top_e[n][o]);      // 2^(15 - SLACK) / 2^(exponent + 1)
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
         uint32_t pf[NT][2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = 16 * p + order(r) + 8 * i;
-          const float scale = vs[2 * p + i].x * up, middle = fmaf(8.f, vs[2 * p + i].x, vs[2 * p + i].y);
+          const float scale = vs[2 * p + i].x, middle = fmaf(8.f, vs[2 * p + i].x, vs[2 * p + i].y);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             float pv[2];
@@ -688,7 +718,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
               const bool seen = !MASK || t0 + t < limit[n][o];
               l[n][o] += w;
               z[n][o] = seen ? fmaf(w, middle, z[n][o]) : z[n][o];
-              pv[o] = seen ? w * scale : 0.f;
+              pv[o] = seen ? w * scale * up[n][o] : 0.f;      // (w scale is in range, scale up need not be)
             }
             pf[n][i] = transpose_8x8(pack_f16x2(pv[0], pv[1]));
           }
@@ -744,12 +774,13 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
           sh_m[warp][col] = m[j][o];
           sh_l[warp][col] = l[j][o];
         }
-        const float f = pow2(min(top_e - 121 + (int)SLACK, 127));      // of the odd places: 2^20 over what p was scaled by
+        // what p vs was scaled by, taken back; codes stand at 2^-24, the odd places at 2^-20 (two factors: neither overflows alone)
+        const float f = pow2(top_e[j][o] - 137 - 4 + (int)SLACK);
 #pragma unroll
         for (int i = 0; i < MT; ++i)
           *reinterpret_cast<float2*>(&sh_o[warp][col][r * (D / 8) + 2 * i]) =
-              make_float2((o_acc[j][i][o] - eights[j][o]) * (16.f * f) + z[j][o],
-                          fmaf(o_acc[j][i][2 + o], f, fmaf(-16.f * f, eights[j][o], z[j][o])));
+              make_float2(fmaf((o_acc[j][i][o] - eights[j][o]) * 16777216.f, f, z[j][o]),
+                          fmaf(fmaf(-16.f, eights[j][o], o_acc[j][i][2 + o]) * 1048576.f, f, z[j][o]));
       }
     }
     __syncthreads();

@@ -329,3 +329,76 @@ def test_refusals():
     with pytest.raises(ValueError):
         ops.KV4Cache(1, 4, 24, 2, 64, DEV)
     assert kv4.HEAD_DIMS == (64, 128)
+
+
+def _check_weighted(q, layer, table, lengths, scale):
+    """As :func:`_check`, with a tolerance that goes by what the weights leave of the values: a token without weight adds nothing to it,
+    however large its values are."""
+    out = ops.kv4_attention(q, layer, table, torch.tensor(lengths, dtype=torch.int32, device=DEV), scale)
+    want, _, _ = _attention(q, layer, table, lengths, scale)
+    B, S, H, D = q.shape
+    unit = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11
+    for b, n in enumerate(lengths):
+        k, v, sc = (t.repeat_interleave(H // layer[0].shape[2], 0) for t in _values(layer, table, b, n))
+        for i in range(S):
+            m = n - S + i + 1
+            p = torch.softmax(torch.einsum("hd,htd->ht", q[b, i].double(), k[:, :m]) * scale, -1)
+            # p vs is rounded to 11 bits and meets codes up to 15; a score is an fp32 sum, its exponential off by 2^-22, and the weights'
+            # sums with the minima are fp32
+            score = (q[b, i].double().abs()[:, None] * k[:, :m].abs()).sum(-1).amax(-1) * scale
+            tol = 2.0 ** -11 * 15 * (p * sc[:, :m, 2].abs()).sum(-1) + (4 * score + 64) * 2.0 ** -20 * (p * v[:, :m].abs().amax(-1)).sum(-1)
+            off = (out[b, i].double() - want[b, i]).abs() - unit * want[b, i].abs() - tol[:, None]
+            assert torch.isfinite(out[b, i]).all() and (off <= 0).all(), (b, i, float(off.max()))
+    _lib.check_status(out.device)
+
+
+@pytest.mark.parametrize("heads,S", [(1, 1), (4, 1), (4, 4)])
+@pytest.mark.parametrize("apart", [12, 28, 45, 100])
+def test_values_of_little_weight_do_not_blur_the_others(apart, heads, S):
+    """Value scales 2^12 to 2^100 apart, the large ones at tokens whose weights make up for it, many times over or just."""
+    page, D, n = 16, 64, 700
+    t = torch.arange(n, device=DEV)
+    for steps, large in ((1.0, t % 5 == 4), (1.0, t < 200), (1.0, t >= 640), (0.0, t % 50 == 49), (0.0, t < 3)):
+        cache = ops.KV4Cache(1, 44, page, 1, D, DEV)
+        codes, scales = layer = cache.layer(0)
+        _fill(codes, scales, seed=21)
+        table = _table(1, 44, 44)
+        page_of, slot = table[0, t // page].long(), t % page
+        # keys of equal dims: with a query of ones and a scale of 1 / D a score is the key's minimum. Large values stand 2^apart above the others,
+        # their weights as far below them (steps 0), or twice as far and a little (steps 1)
+        codes[page_of, 0, 0, slot] = 0
+        scales[page_of, 0, slot, 0] = 0
+        scales[page_of, 0, slot, 1] = torch.where(large, -apart * (1 + steps) * math.log(2) - 3 * steps, -0.01 * (t % 7)).bfloat16()
+        size = torch.where(large, 2.0 ** (apart // 2), 2.0 ** (apart // 2 - apart)).bfloat16()
+        scales[page_of, 0, slot, 2] = size
+        scales[page_of, 0, slot, 3] = (-7.5 * size.float()).bfloat16()
+        q = torch.ones(1, S, heads, D, device=DEV).bfloat16()
+        _check_weighted(q, layer, table, [n], 1 / D)
+
+
+@pytest.mark.parametrize("S,apart", [(2, 20), (3, 30), (5, 60)])
+def test_values_that_a_query_does_not_see_do_not_blur_its_others(S, apart):
+    """The newest token has huge values; the queries before it do not see them."""
+    page, D, KV, n = 32, 128, 2, 333
+    cache = ops.KV4Cache(1, 11, page, KV, D, DEV)
+    codes, scales = layer = cache.layer(0)
+    _fill(codes, scales, seed=22)
+    table = _table(1, 11, 11)
+    at = table[0, (n - 1) // page].long(), 1, (n - 1) % page
+    scales[at[0], at[1], at[2], 2] = 2.0 ** apart
+    scales[at[0], at[1], at[2], 3] = -7 * 2.0 ** apart
+    q = torch.randn(1, S, 4, D, generator=_gen(23), device=DEV).bfloat16()
+    _check_weighted(q, layer, table, [n], D ** -0.5)
+
+
+def test_the_largest_values_and_queries():
+    """Values up to 10^37, which bf16 holds, and queries of 10^34 against keys that are as small."""
+    page, D = 16, 128
+    cache = ops.KV4Cache(1, 20, page, 1, D, DEV)
+    codes, scales = layer = cache.layer(0)
+    table = _table(1, 20, 20)
+    _fill(codes, scales, seed=24, v_scale=2.0 ** 119)
+    q = torch.randn(1, 1, 8, D, generator=_gen(25), device=DEV).bfloat16()
+    _check_weighted(q, layer, table, [311], D ** -0.5)
+    _fill(codes, scales, seed=24, k_scale=0.4e-34)
+    _check_weighted(q * 1e34, layer, table, [311], D ** -0.5)
