@@ -99,6 +99,8 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
     step, one = x2.stride()
     if one != 1:
         x2, step = x2.contiguous(), K
+    if codes.data_ptr() % 16:          # both kernels read them in words
+        codes = codes.clone()
     if M >= EXPAND_ROWS and x.dtype is torch.bfloat16 and K % 8 == 0:
         w = torch.empty(N, K, dtype=x.dtype, device=x.device)
         rc = _lib.lib().atb_w4_expand(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), N, K, group_size, kind,
@@ -107,8 +109,6 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
         return gemm(x2, w, bias=bias).view(*shape[:-1], N)
     y = x.new_empty(M, N) if x2 is x else x.new_empty(*shape[:-1], N)
     base = x2.data_ptr()
-    if codes.data_ptr() % 16:
-        codes = codes.clone()
     rc = _lib.lib().atb_w4_linear(base, codes.data_ptr(), scales.data_ptr(), _lib.addr(bias), y.data_ptr(), M, N, K, group_size, step,
                                   int((base | 2 * step) & 15 == 0), kind, _lib.stream_of(dev), _lib.status_addr(x))
     _lib.check(rc, "atb_w4_linear")

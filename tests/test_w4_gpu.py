@@ -128,3 +128,13 @@ def test_refusals():
     with torch.no_grad():
         ops.w4_linear(x.clone().requires_grad_(), codes, scales)
     assert w4.GROUPS == (32, 64, 128)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 4, 8])
+@pytest.mark.parametrize("M", [64, 72, 300])
+def test_codes_off_their_alignment(M, offset):
+    codes, scales, g = _weights(104, 264, 64)
+    x = torch.randn(M, 264, generator=g, device=DEV).bfloat16()
+    pad = torch.zeros(codes.numel() + offset, dtype=torch.uint8, device=DEV)[offset:].view_as(codes)
+    pad.copy_(codes)
+    assert torch.equal(_check(x, pad, scales, 64, weight_rounded=M > 64), ops.w4_linear(x, codes, scales, 64))
