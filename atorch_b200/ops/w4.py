@@ -102,11 +102,17 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
     if codes.data_ptr() % 16:          # both kernels read them in words
         codes = codes.clone()
     if M >= EXPAND_ROWS and x.dtype is torch.bfloat16 and K % 8 == 0:
-        w = torch.empty(N, K, dtype=x.dtype, device=x.device)
+        if step < K or (x2.data_ptr() | 2 * step) & 15:
+            x2 = x2.clone(memory_format=torch.contiguous_format)
+        wide = (N + 7) // 8 * 8            # the GEMM stores 8 columns at a time; those behind the last are cut off
+        w = torch.empty(wide, K, dtype=x.dtype, device=x.device)
         rc = _lib.lib().atb_w4_expand(codes.data_ptr(), scales.data_ptr(), w.data_ptr(), N, K, group_size, kind,
                                       _lib.stream_of(dev))
         _lib.check(rc, "atb_w4_expand")
-        return gemm(x2, w, bias=bias).view(*shape[:-1], N)
+        if bias is not None and wide != N:
+            bias = torch.nn.functional.pad(bias, (0, wide - N))
+        y = gemm(x2, w, bias=bias)
+        return (y if wide == N else y[:, :N].contiguous()).view(*shape[:-1], N)
     y = x.new_empty(M, N) if x2 is x else x.new_empty(*shape[:-1], N)
     base = x2.data_ptr()
     rc = _lib.lib().atb_w4_linear(base, codes.data_ptr(), scales.data_ptr(), _lib.addr(bias), y.data_ptr(), M, N, K, group_size, step,

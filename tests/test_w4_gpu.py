@@ -138,3 +138,19 @@ def test_codes_off_their_alignment(M, offset):
     pad = torch.zeros(codes.numel() + offset, dtype=torch.uint8, device=DEV)[offset:].view_as(codes)
     pad.copy_(codes)
     assert torch.equal(_check(x, pad, scales, 64, weight_rounded=M > 64), ops.w4_linear(x, codes, scales, 64))
+
+
+@pytest.mark.parametrize("N", [104, 99, 513])
+@pytest.mark.parametrize("M", [65, 72, 300])
+def test_many_rows_of_any_layout(M, N):
+    """Rows off 16 bytes, pitches that are no multiple of 8, one row many times over, outputs of any width: two launches of the package."""
+    codes, scales, g = _weights(N, 256, 64)
+    x = torch.randn(M, 300, generator=g, device=DEV).bfloat16()
+    bias = torch.randn(N + 1, generator=g, device=DEV).bfloat16()[1:]
+    for y in (x[:, :256], x[:, 3: 259], x[:, :259][:, 1: 257], x.view(-1)[: M * 256].view(M, 256), x[:1, :256].expand(M, 256),
+              x.view(-1)[5: M * 261 + 5].view(M, 261)[:, :256]):
+        _lib.lib()
+        before = _lib.launch_count
+        _check(y, codes, scales, 64, bias, weight_rounded=True)
+        assert _lib.launch_count == before + 4
+    assert ops.w4_linear(x[:, :256].reshape(M, 1, 256), codes, scales, 64).shape == (M, 1, N)
