@@ -126,6 +126,8 @@ def beam_reorder(codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Te
             or codes.shape[2] != 2 or scales.shape != (*codes.shape[:2], *codes.shape[3:5], 4) \
             or not (codes.is_contiguous() and scales.is_contiguous()):
         raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not the caches of layers")
+    if (codes.data_ptr() | scales.data_ptr()) & 15:
+        raise ValueError("the cache has to begin on 16 bytes")
     layers, pages, _, KV, page_size, half = codes.shape
     _check_page_size(page_size)
     if parents.dim() != 2 or parents.dtype is not torch.int32:

@@ -65,3 +65,23 @@ def test_reorder_moves_what_the_beams_hold():
             assert torch.equal(k, held[i][parents[0, w]][0]) and torch.equal(v, held[i][parents[0, w]][1])
     with pytest.raises(IndexError):
         ops.beam_reorder(cache.codes, cache.scales, table, torch.full((3,), n, dtype=torch.int32), parents + 1)
+
+
+def test_reorder_refuses_a_cache_off_its_alignment():
+    """The kernel moves codes in pieces of 16 bytes and scales in pieces of 8; a layer's operators refuse the same."""
+    cache = ops.KV4Cache(1, 6, 16, 1, 64)
+    table, lengths = torch.zeros(2, 2, dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    table[1] = 1
+    parents = torch.zeros(1, 2, dtype=torch.int32)
+    ops.beam_reorder(cache.codes, cache.scales, table, lengths, parents)
+
+    def off(t, n):
+        return torch.zeros(t.numel() + 16, dtype=t.dtype)[n: n + t.numel()].view(t.shape)
+
+    for codes, scales in ((off(cache.codes, 1), cache.scales), (off(cache.codes, 8), cache.scales), (cache.codes, off(cache.scales, 1)),
+                          (cache.codes, off(cache.scales, 4))):
+        assert codes.is_contiguous() and scales.is_contiguous()
+        with pytest.raises(ValueError):
+            ops.beam_reorder(codes, scales, table, lengths, parents)
+        with pytest.raises(ValueError):
+            ops.kv4_read((codes[0], scales[0]), table, None, lengths)
