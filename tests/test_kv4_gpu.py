@@ -402,3 +402,21 @@ def test_the_largest_values_and_queries():
     _check_weighted(q, layer, table, [311], D ** -0.5)
     _fill(codes, scales, seed=24, k_scale=0.4e-34)
     _check_weighted(q * 1e34, layer, table, [311], D ** -0.5)
+
+
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_angles_off_their_alignment(offset):
+    """Tables of angles that are contiguous and begin anywhere."""
+    D, n_q, KV, T = 64, 2, 2, 9
+    cos, sin = ops.rope_tables(40, D, device=DEV)
+    x = torch.randn(T, (n_q + 2 * KV) * D, generator=_gen(40), device=DEV).bfloat16()
+    pos = torch.arange(30, 30 + T, dtype=torch.int32, device=DEV)
+    table, seq = torch.tensor([[0, 1, 2]], dtype=torch.int32, device=DEV), torch.zeros(T, dtype=torch.int32, device=DEV)
+    results = []
+    for off in (0, offset):
+        cache = ops.KV4Cache(1, 3, 16, KV, D, DEV)
+        pair = [torch.cat([torch.zeros(off, device=DEV), t.flatten()])[off:].view(t.shape) for t in (cos, sin)]
+        assert all(t.is_contiguous() and t.data_ptr() % 16 == 4 * off for t in pair)
+        results.append((ops.kv4_append(cache.layer(0), table, seq, pos, x, n_q, *pair), cache.codes, cache.scales.view(torch.int16)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    _lib.check_status(x.device)
