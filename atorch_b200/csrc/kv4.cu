@@ -746,10 +746,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
       }
     };
 
+    bool arrived = true;
     for (int j = 0; j < mine; ++j) {
       const uint32_t stage = (loads + j) % STAGES, phase = ((loads + j) / STAGES) & 1;
       const int t0 = (t_first + warp + j * WARPS) * TILE;
-      mbar_wait_warp(&bars[warp][stage], phase, &abort_flag, a.status);
+      arrived = mbar_wait_warp(&bars[warp][stage], phase, &abort_flag, a.status);
+      if (!arrived) break;
       if (t0 + TILE <= all_see) tile(ring + stage * Sh::STAGE, t0, std::false_type());
       else tile(ring + stage * Sh::STAGE, t0, std::true_type());
       __syncwarp();
@@ -759,7 +761,12 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
 
     // the warps' sums, in their order, in the place of the rings: every copy has arrived and been read
     float (*const sh_o)[COLS][D + 4] = reinterpret_cast<float (*)[COLS][D + 4]>(smem);
-    __syncthreads();
+    if (__syncthreads_or(!arrived)) {
+      // a copy did not come in time: nothing more is asked for or stored, and those on their way may land before the block ends
+      const uint64_t t_start = globaltimer_ns();
+      while (globaltimer_ns() - t_start < 200000ull) __nanosleep(1000);
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
