@@ -122,8 +122,16 @@ struct Out {
   int* parents;
   unsigned char* ended;
 };
-// `key`: with its beam
-ATB_DEVICE void write_out(const Out& out, long long at, unsigned long long key, const unsigned char* ended, int eos) {
+// `key`: with its beam. Behind a failed kernel nothing is selected: the first token of the first beam, impossible and ended, so that
+// what goes on from there finds indices in range.
+ATB_DEVICE void write_out(const Out& out, long long at, unsigned long long key, const unsigned char* ended, int eos, bool failed) {
+  if (failed) {
+    out.scores[at] = -INFINITY;
+    out.tokens[at] = 0;
+    out.parents[at] = 0;
+    out.ended[at] = 1;
+    return;
+  }
   out.scores[at] = value_of(key);
   out.tokens[at] = token_of(key);
   out.parents[at] = beam_of(key);
@@ -157,7 +165,7 @@ __global__ void __launch_bounds__(THREADS, P == 8 ? 3 : 1) beam_row_kernel(const
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
   const int shares = blocks / beams, share_rank = rank % shares, first_rank = rank - share_rank;
   const long long item = blockIdx.x / blocks, row = item * beams + rank / shares;
-  const bool failed = *status != 0;      // nothing is stored then; the blocks of a cluster stay together
+  const bool failed = *status != 0;      // (the blocks of a cluster stay together)
   const float score = scores[row];
   const bool ended = finished && finished[row];
   // a beam that is not looked at: the end token alone goes on, at no cost, or nothing
@@ -264,9 +272,9 @@ __global__ void __launch_bounds__(THREADS, P == 8 ? 3 : 1) beam_row_kernel(const
     __syncthreads();
     for (int i = threadIdx.x; i < all; i += THREADS) {
       const int place = place_of(room, all, i);
-      if (place >= keep || failed) continue;
+      if (place >= keep) continue;
       if (best != nullptr) best[row * keep + place] = room[i];
-      else if (room[i] != 0) write_out(final, item * keep + place, room[i], finished ? finished + item * beams : nullptr, eos);
+      else if (room[i] != 0) write_out(final, item * keep + place, room[i], finished ? finished + item * beams : nullptr, eos, failed);
     }
   }
   cluster.sync();                                // the first has read the others' keys
@@ -288,8 +296,8 @@ __global__ void __launch_bounds__(256) beam_join_kernel(const unsigned long long
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += 256) {
     const int place = place_of(all, n, i);
-    if (place < keep && all[i] != 0 && !failed)
-      write_out(final, b * keep + place, all[i], finished ? finished + b * W : nullptr, eos);
+    if (place < keep && all[i] != 0)
+      write_out(final, b * keep + place, all[i], finished ? finished + b * W : nullptr, eos, failed);
   }
 }
 

@@ -84,6 +84,8 @@ class Generator:
             return prompts
         m, cfg, S = self.model, self.model.config, self.page_size
         dev, B, W = m.embed_tokens.weight.device, len(prompts), beams
+        if dev.type == "cuda":
+            _lib.check_status(dev)           # behind a failed kernel the operators store nothing
         longest = max(len(p) for p in prompts) + max_new_tokens
         cos, sin = m.rope(longest, dev)
 

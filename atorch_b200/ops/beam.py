@@ -48,7 +48,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     ``-inf``. A beam with ``finished`` set goes on with ``eos`` alone, at its score.
 
     Returns scores fp32, tokens int64, parents int32 (the beam that a continuation goes on from) and finished bool (the parent
-    was, or the token is ``eos``), each ``[B, keep]``, best first."""
+    was, or the token is ``eos``), each ``[B, keep]``, best first. Behind a failed kernel (see ``_lib.check_status``) nothing is
+    selected: scores of ``-inf``, tokens and parents 0, all finished."""
     if logits.dim() != 3 or logits.dtype not in _lib.DT or logits.shape[2] == 0 or logits.shape[1] == 0:
         raise ValueError(f"logits are bf16, fp16 or fp32 [B, beams, vocabulary], got {logits.dtype} {tuple(logits.shape)}")
     B, W, V = logits.shape

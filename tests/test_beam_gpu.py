@@ -242,3 +242,20 @@ def test_finite_masks(B, W, V, keep, dtype, mask):
             assert torch.equal(tokens[:, keep - rest:], torch.arange(rest, device=DEV).expand(B, -1))
             assert (parents[:, keep - rest:] == 0).all()
     _lib.check_status(got.device)
+
+
+@pytest.mark.parametrize("B,W,V,keep", [(2, 3, 1000, 4), (1, 4, 32000, None), (3, 17, 500, 20), (2, 32, 8000, None), (1, 1, 200003, 3)])
+def test_behind_a_failed_kernel(B, W, V, keep):
+    """Nothing is selected, and what comes back are tokens and parents all the same: they go on as indices."""
+    logits = torch.randn(B, W, V, generator=_gen(V), device=DEV)
+    scores, n = torch.randn(B, W, generator=_gen(W), device=DEV), keep or W
+    _lib.check_status(logits.device)
+    used = [torch.full((B, n), 1 << 40, dtype=t, device=DEV) if t is torch.int64 else torch.full((B, n), 99, dtype=t, device=DEV)
+            for t in (torch.float32, torch.int64, torch.int32, torch.uint8) for _ in range(3)]
+    del used                                 # what the outputs find in their place
+    _lib.status_word(logits.device).fill_(5)
+    got, tokens, parents, ended = ops.beam_select(logits, scores, eos=7, keep=keep)
+    assert (got == -math.inf).all() and (tokens == 0).all() and (parents == 0).all() and ended.all()
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status(logits.device)
+    _check(logits, scores, eos=7, keep=keep)

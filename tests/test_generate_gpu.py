@@ -114,3 +114,17 @@ def test_sampler_and_end_token():
     assert out.shape == (8, 21) and torch.equal(out[:, :9], prompt) and (out < 50).all()
     for o in Generator(m).generate(prompt, 30, eos=7, temperature=1.5):
         assert (o[9:-1] != 7).all() and (o[-1] == 7 or len(o) == 39)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(beams=3), dict(temperature=1.0)])
+def test_a_failed_kernel_is_reported_before_the_first_token(kw, monkeypatch):
+    m = _model(vocab_size=50)
+    prompt = torch.randint(0, 50, (2, 9), generator=torch.Generator().manual_seed(4)).cuda()
+    run, calls = Generator._run, []
+    monkeypatch.setattr(Generator, "_run", lambda self, *a: calls.append(1))
+    _lib.status_word(prompt.device).fill_(1)
+    with pytest.raises(_lib.KernelError):
+        Generator(m).generate(prompt, 4, **kw)
+    assert not calls
+    monkeypatch.setattr(Generator, "_run", run)
+    assert len(Generator(m).generate(prompt, 4, **kw)[1]) == 13
