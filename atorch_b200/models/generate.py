@@ -122,7 +122,9 @@ class Generator:
         got, done = [], None
         for i in range(steps):
             if temperature > 0:
-                tokens = torch.multinomial(torch.softmax(logits.float() / temperature, -1), 1).squeeze(1)
+                # the first to arrive of exponential waiting times: what multinomial draws, without its assertion on the device
+                weights = torch.softmax(logits.float() / temperature, -1)
+                tokens = (weights / torch.empty_like(weights).exponential_()).argmax(-1)
             else:
                 tokens = logits.argmax(-1)
             got.append(tokens)

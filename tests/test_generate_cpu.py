@@ -146,3 +146,20 @@ def test_quantised_linears():
     tied = _model(tie_word_embeddings=True)
     quantize_linears(tied)
     assert type(tied.lm_head) is torch.nn.Linear and type(tied.layers[1].o_proj) is W4Linear
+
+
+def test_sampling_is_that_of_multinomial_and_outlives_nan(monkeypatch):
+    """The same tokens for a seed; logits that hold NaN (weights that have diverged) give a token of the vocabulary."""
+    m = _model(vocab_size=30)
+    ids = torch.randint(0, 30, (6, 5), generator=torch.Generator().manual_seed(6))
+    logits = torch.randn(6, 30, generator=torch.Generator().manual_seed(7)).bfloat16()
+    monkeypatch.setattr(Generator, "_run", lambda self, *a: logits)
+    torch.manual_seed(8)
+    want = torch.stack([torch.multinomial(torch.softmax(logits.float() / 0.8, -1), 1).squeeze(1) for _ in range(3)], 1)
+    torch.manual_seed(8)
+    assert torch.equal(torch.stack(generate(m, ids, 3, temperature=0.8))[:, 5:], want)
+    logits[2] = float("nan")
+    logits[3, 4:9] = float("nan")
+    logits[4] = -float("inf")
+    out = torch.stack(generate(m, ids, 3, temperature=0.8))[:, 5:]
+    assert (out >= 0).all() and (out < 30).all()

@@ -128,3 +128,20 @@ def test_a_failed_kernel_is_reported_before_the_first_token(kw, monkeypatch):
     assert not calls
     monkeypatch.setattr(Generator, "_run", run)
     assert len(Generator(m).generate(prompt, 4, **kw)[1]) == 13
+
+
+def test_sampling_is_that_of_multinomial_and_outlives_nan(monkeypatch):
+    """The same tokens for a seed; logits that hold NaN give a token of the vocabulary, and no assertion on the device."""
+    m = _model(vocab_size=300)
+    ids = torch.randint(0, 300, (40, 5), generator=torch.Generator().manual_seed(6)).cuda()
+    logits = torch.randn(40, 300, generator=torch.Generator().manual_seed(7)).bfloat16().cuda()
+    monkeypatch.setattr(Generator, "_run", lambda self, *a: logits)
+    torch.manual_seed(8)
+    want = torch.stack([torch.multinomial(torch.softmax(logits.float() / 0.8, -1), 1).squeeze(1) for _ in range(4)], 1)
+    torch.manual_seed(8)
+    assert torch.equal(torch.stack(Generator(m).generate(ids, 4, temperature=0.8))[:, 5:], want)
+    logits[2] = float("nan")
+    logits[3, 4:9] = float("nan")
+    logits[4] = -float("inf")
+    out = torch.stack(Generator(m).generate(ids, 4, temperature=0.8))[:, 5:]
+    assert (out >= 0).all() and (out < 300).all()
