@@ -92,6 +92,8 @@ def _int32(name: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tenso
         return t
     if t.dtype not in (torch.int32, torch.int64) or t.numel() != n:
         raise ValueError(f"{name}: {n} whole numbers are wanted, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype is torch.int64:       # what is out of range stays so
+        t = t.clamp(-1 << 31, (1 << 31) - 1)
     return t.reshape(-1).to(torch.int32).contiguous()
 
 

@@ -67,3 +67,26 @@ def test_what_is_not_there_is_refused():
         ops.kv4_append(cache.layer(0), table, None, one, x.clone().requires_grad_(), 4)
     with pytest.raises(ValueError):
         ops.KV4Cache(1, 4, 8, 2, 32)
+
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 5, 1 << 40, (1 << 63) - 1, -(1 << 32) + 5, -(1 << 63)])
+def test_whole_numbers_of_64_bits_are_not_cut(far):
+    """What is out of range in 64 bits stays out of range: skipped where it is negative, refused where it is not."""
+    cache, table, _ = _filled()
+    layer, x = cache.layer(0), torch.randn(1, 8 * 32)
+    place, one = torch.tensor([far]), torch.zeros(1, dtype=torch.int64)
+    if far < 0:
+        ops.kv4_append(layer, table, one, place, x, 4)
+        assert all((t == 0).all() for t in ops.kv4_read(layer, table, one, place))
+        out, lse = ops.kv4_attention(torch.randn(2, 1, 4, 32).half(), layer, table, torch.tensor([far, 0]), return_lse=True)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    else:
+        with pytest.raises(IndexError):
+            ops.kv4_append(layer, table, one, place, x, 4)
+        with pytest.raises(IndexError):
+            ops.kv4_read(layer, table, one, place)
+        with pytest.raises(IndexError):
+            ops.kv4_attention(torch.randn(2, 1, 4, 32).half(), layer, table, torch.tensor([1, far]))
+    with pytest.raises(IndexError):
+        ops.kv4_append(layer, table, place, one, x, 4)
+    assert (cache.codes == 0).all() and (cache.scales == 0).all()

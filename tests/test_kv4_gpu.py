@@ -420,3 +420,32 @@ def test_angles_off_their_alignment(offset):
         results.append((ops.kv4_append(cache.layer(0), table, seq, pos, x, n_q, *pair), cache.codes, cache.scales.view(torch.int16)))
     assert all(torch.equal(a, b) for a, b in zip(*results))
     _lib.check_status(x.device)
+
+
+@pytest.mark.parametrize("far", [1 << 32, (1 << 32) + 5, (1 << 63) - 1, -(1 << 32) + 5, -(1 << 63)])
+def test_whole_numbers_of_64_bits_are_not_cut(far):
+    """What is out of range in 64 bits stays out of range: skipped where it is negative, reported where it is not."""
+    D, KV = 64, 2
+    cache = ops.KV4Cache(1, 4, 16, KV, D, DEV)
+    layer, table = cache.layer(0), torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    place, one = torch.tensor([far], device=DEV), torch.zeros(1, dtype=torch.int64, device=DEV)
+    x, q = torch.randn(1, (2 + 2 * KV) * D, device=DEV).bfloat16(), torch.randn(2, 1, 4, D, device=DEV).bfloat16()
+    dev = x.device
+
+    def is_reported(wanted):
+        if not wanted:
+            return _lib.check_status(dev)
+        with pytest.raises(_lib.KernelError):
+            _lib.check_status(dev)
+
+    ops.kv4_append(layer, table, one, place, x, 2)
+    is_reported(far > 0)
+    k, v = ops.kv4_read(layer, table, one, place)
+    is_reported(far > 0)
+    assert far > 0 or ((k == 0).all() and (v == 0).all())
+    out = ops.kv4_attention(q, layer, table, torch.tensor([far, 0], device=DEV))
+    is_reported(far > 0)
+    assert far > 0 or (out == 0).all()
+    ops.kv4_append(layer, table, place, one, x, 2)
+    is_reported(True)
+    assert (cache.codes == 0).all() and (cache.scales == 0).all()
