@@ -98,6 +98,15 @@ class LlamaConfig:
 _NOT_PLAIN = {"dropout_p", "additive_mask", "additive_bias"}
 
 
+def linear_of(mod: nn.Module, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`ops.linear` on the module's weight; a module that has none (its weights are held in 4 bits) runs its own forward."""
+    weight = getattr(mod, "weight", None)
+    if weight is not None:
+        return ops.linear(x, weight, residual=residual)
+    y = mod(x)
+    return y if residual is None else residual + y
+
+
 class RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float = 1e-5):
         super().__init__()
@@ -221,7 +230,7 @@ class LlamaModel(nn.Module):
             else:
                 h = layer(h, cos, sin, positions, attn_kwargs)
         h = self.norm(h)
-        logits = ops.linear(h, self.lm_head.weight)
+        logits = linear_of(self.lm_head, h)
         loss = None
         if labels is not None:
             loss = causal_lm_loss(logits, labels)

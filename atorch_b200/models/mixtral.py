@@ -16,7 +16,7 @@ import torch.nn as nn
 from .. import ops
 from ..modules.moe import Grouped_GEMM_MoE, TopNRouter
 from ..utils.checkpoint import checkpoint_module
-from .llama import LlamaConfig, RMSNorm, causal_lm_loss
+from .llama import LlamaConfig, RMSNorm, causal_lm_loss, linear_of
 
 
 @dataclass
@@ -83,12 +83,16 @@ class MixtralDecoderLayer(nn.Module):
         B, S, _ = h.shape
         d = self.config.head_dim
         x = self.input_layernorm(h)
-        qkv = ops.linear_rope(x, self.qkv_proj.weight, cos, sin, self.n_q + self.n_kv, d, positions,
-                              inplace_grad=True)      # a temporary of the attention backward
+        weight = getattr(self.qkv_proj, "weight", None)
+        if weight is not None:
+            qkv = ops.linear_rope(x, weight, cos, sin, self.n_q + self.n_kv, d, positions,
+                                  inplace_grad=True)      # a temporary of the attention backward
+        else:
+            qkv = ops.rope(self.qkv_proj(x), cos, sin, self.n_q + self.n_kv, d, positions, inplace=True)
         qkv = qkv.view(B, S, self.n_q + 2 * self.n_kv, d)
         a = ops.attention(qkv[:, :, : self.n_q], qkv[:, :, self.n_q: self.n_q + self.n_kv],
                           qkv[:, :, self.n_q + self.n_kv:], **(attn_kwargs or {"causal": True}))
-        h = ops.linear(a.reshape(B, S, self.n_q * d), self.o_proj.weight, residual=h)
+        h = linear_of(self.o_proj, a.reshape(B, S, self.n_q * d), h)
         return h + self.block_sparse_moe(self.post_attention_layernorm(h))
 
 
@@ -129,7 +133,7 @@ class MixtralModel(nn.Module):
                 h = checkpoint_module(layer, h, cos, sin)
             else:
                 h = layer(h, cos, sin)
-        logits = ops.linear(self.norm(h), self.lm_head.weight)
+        logits = linear_of(self.lm_head, self.norm(h))
         loss = None
         if labels is not None:
             loss = causal_lm_loss(logits, labels) + self.aux_loss()

@@ -57,7 +57,8 @@ class TopkGate(nn.Module):
         self.min_capacity, self.noisy_gate_policy = min_capacity, noisy_gate_policy
 
     def forward(self, x: torch.Tensor):
-        logits = self.wg(x.float() if self.wg.weight.dtype == torch.float32 else x)
+        weight = getattr(self.wg, "weight", None)         # (none where it is held in 4 bits)
+        logits = self.wg(x.float() if weight is not None and weight.dtype == torch.float32 else x)
         if self.noisy_gate_policy == "Jitter" and self.training:
             logits = logits * torch.empty_like(logits).uniform_(0.99, 1.01)
         cf = self.capacity_factor if self.training else self.eval_capacity_factor

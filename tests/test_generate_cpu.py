@@ -1,4 +1,6 @@
 """Generation with the 4-bit cache on the CPU: greedy, beams, sampling, 4-bit weights."""
+import copy
+
 import pytest
 import torch
 
@@ -163,3 +165,47 @@ def test_sampling_is_that_of_multinomial_and_outlives_nan(monkeypatch):
     logits[4] = -float("inf")
     out = torch.stack(generate(m, ids, 3, temperature=0.8))[:, 5:]
     assert (out >= 0).all() and (out < 30).all()
+
+
+def _dequantised(model):
+    """The same model with the weights that the codes stand for in its ``nn.Linear`` modules."""
+    for m in list(model.modules()):
+        for child, lin in list(m.named_children()):
+            if type(lin) is W4Linear:
+                plain = torch.nn.Linear(lin.in_features, lin.out_features, bias=lin.bias is not None)
+                plain.weight.data = ops.w4_dequantize(lin.codes, lin.scales, lin.in_features, lin.group_size)
+                if lin.bias is not None:
+                    plain.bias.data = lin.bias.float()
+                setattr(m, child, plain)
+    return model.float()
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_a_quantised_model_runs_its_own_forward(tied):
+    """As a reference or reward model does: head and all, against the weights that the codes stand for."""
+    m = quantize_linears(_model(tie_word_embeddings=tied), 32)
+    assert type(m.lm_head) is (torch.nn.Linear if tied else W4Linear)
+    ids = torch.randint(0, 40, (3, 17), generator=torch.Generator().manual_seed(9))
+    with torch.no_grad():
+        loss, logits = m(ids, labels=ids)
+        want_loss, want = _dequantised(copy.deepcopy(m))(ids, labels=ids)
+    # some twenty roundings to bf16 in series, each of 2^-9
+    assert (logits.float() - want).norm() < 20 * 2 ** -9 * want.norm() and abs(float(loss) - float(want_loss)) < 0.05 * float(want_loss)
+
+
+def test_a_quantised_mixture_of_experts_runs_its_own_forward():
+    from atorch_b200.models.mixtral import MixtralConfig, MixtralModel
+    from atorch_b200.modules.moe.gating import TopkGate
+
+    torch.manual_seed(3)
+    m = MixtralModel(MixtralConfig.tiny_moe()).bfloat16().eval()
+    quantize_linears(m, 32, lambda name, lin: "router" not in name)
+    assert type(m.lm_head) is W4Linear and type(m.layers[1].qkv_proj) is W4Linear
+    ids = torch.randint(0, 256, (2, 12), generator=torch.Generator().manual_seed(9))
+    with torch.no_grad():
+        _, logits = m(ids)
+        _, want = _dequantised(copy.deepcopy(m)).bfloat16()(ids)
+    assert (logits.float() - want.float()).norm() < 0.1 * want.float().norm()
+    gate = quantize_linears(TopkGate(64, 4).bfloat16(), 32)
+    with torch.no_grad():
+        assert torch.isfinite(gate(torch.randn(10, 64).bfloat16())[0])

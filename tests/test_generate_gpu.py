@@ -5,7 +5,7 @@ import torch
 from atorch_b200 import _lib, ops
 from atorch_b200.models.generate import CachedSampler, Generator
 from atorch_b200.models.llama import LlamaConfig, LlamaModel
-from atorch_b200.modules.w4_linear import quantize_linears
+from atorch_b200.modules.w4_linear import W4Linear, quantize_linears
 
 pytestmark = pytest.mark.gpu
 
@@ -145,3 +145,22 @@ def test_sampling_is_that_of_multinomial_and_outlives_nan(monkeypatch):
     logits[4] = -float("inf")
     out = torch.stack(Generator(m).generate(ids, 4, temperature=0.8))[:, 5:]
     assert (out >= 0).all() and (out < 300).all()
+
+
+@pytest.mark.parametrize("shape", [(1, 5), (2, 60), (3, 100)])
+def test_a_quantised_model_runs_its_own_forward(shape):
+    """As a reference or reward model does, against the weights that the codes stand for, in 32 bits on the CPU."""
+    m = quantize_linears(_model(), 64)
+    ids = torch.randint(0, 1000, shape, generator=torch.Generator().manual_seed(9))
+    plain = LlamaModel(m.config)
+    plain.load_state_dict({n: t.float().cpu() for n, t in m.state_dict().items() if not n.endswith(("codes", "scales"))}, strict=False)
+    for name, lin in m.named_modules():
+        if type(lin) is W4Linear:
+            w = ops.w4_dequantize(lin.codes, lin.scales, lin.in_features, lin.group_size).cpu()
+            plain.get_submodule(name).weight.data = w
+    with torch.no_grad():
+        loss, logits = m(ids.cuda(), labels=ids.cuda())
+        want_loss, want = plain(ids, labels=ids)
+    # some thirty roundings to bf16 in series, each of 2^-9
+    assert (logits.float().cpu() - want).norm() < 30 * 2 ** -9 * want.norm()
+    assert abs(float(loss) - float(want_loss)) < 0.05 * float(want_loss)
