@@ -7,6 +7,7 @@ was cut into prompt and generated tokens.
 """
 from __future__ import annotations
 
+import contextlib
 import math
 from typing import List, Optional, Sequence, Union
 
@@ -69,12 +70,30 @@ class Generator:
         return self._run(tokens, cache, table, None, lengths, cos, sin,
                          lambda q, layer: ops.kv4_attention(q.unsqueeze(1), layer, table, now))
 
+    @contextlib.contextmanager
+    def _whole_parameters(self):
+        """All parameters in their place for the whole call: the layers' parts are called directly, past the forwards at which a
+        sharded engine (``parallel/fsdp.py``) gathers them."""
+        engines = {}
+        for p in self.model.parameters():
+            unit = getattr(p, "_atb_unit", None)
+            if unit is not None:
+                engines[id(unit.engine)] = unit.engine
+        with contextlib.ExitStack() as stack:
+            for engine in engines.values():
+                stack.enter_context(engine.summon_full_params())
+            for name, p in self.model.named_parameters():
+                if p.numel() and p.untyped_storage().nbytes() == 0:
+                    raise ValueError(f"parameter {name} is not in memory: it is sharded by something that generation does not know")
+            yield
+
     @torch.no_grad()
     def generate(self, prompts: Union[torch.Tensor, Sequence[torch.Tensor]], max_new_tokens: int, eos: Optional[int] = None,
                  temperature: float = 0.0, beams: int = 1, length_penalty: float = 0.0) -> List[torch.Tensor]:
         """``prompts``: token ids, ``[B, T]`` or one tensor a sequence. Greedy with ``temperature`` 0, sampling above; with ``beams``
         above 1 a beam search, whose best sequence by ``score / new tokens ** length_penalty`` is returned. Sequences come back with
-        their prompts, up to ``eos`` where there is one."""
+        their prompts, up to ``eos`` where there is one. Where the parameters are sharded (``parallel/fsdp.py``) every rank has to
+        call it, each with prompts of its own; they are gathered once for the call."""
         prompts = [p.reshape(-1) for p in prompts]
         if not prompts or min(len(p) for p in prompts) == 0:
             raise ValueError("prompts have one token at least")
@@ -82,6 +101,10 @@ class Generator:
             raise ValueError("a beam search does not sample")
         if max_new_tokens < 1:
             return prompts
+        with self._whole_parameters():
+            return self._generate(prompts, max_new_tokens, eos, temperature, beams, length_penalty)
+
+    def _generate(self, prompts, max_new_tokens, eos, temperature, beams, length_penalty):
         m, cfg, S = self.model, self.model.config, self.page_size
         dev, B, W = m.embed_tokens.weight.device, len(prompts), beams
         if dev.type == "cuda":
