@@ -21,6 +21,11 @@ class Generator:
     """Holds nothing between calls but the model; every :meth:`generate` has a cache of its own."""
 
     def __init__(self, model: LlamaModel, page_size: int = 16):
+        # (by what is used of them: a layer may be wrapped by something that hands its attributes on)
+        if not all(hasattr(model, n) for n in ("embed_tokens", "layers", "norm", "lm_head", "rope", "config")) \
+                or not all(hasattr(layer, n) for layer in model.layers for n in ("qkv_proj", "gate_up_proj", "down_proj", "n_kv", "_proj")):
+            raise TypeError("generation runs a LlamaModel with its LlamaDecoderLayers (the model inside a wrapper, not the wrapper), and "
+                            f"this is a {type(model).__name__}")
         self.model, self.page_size = model, page_size
         self.dtype = model.embed_tokens.weight.dtype
         if self.dtype not in (torch.bfloat16, torch.float16):

@@ -209,3 +209,27 @@ def test_a_quantised_mixture_of_experts_runs_its_own_forward():
     gate = quantize_linears(TopkGate(64, 4).bfloat16(), 32)
     with torch.no_grad():
         assert torch.isfinite(gate(torch.randn(10, 64).bfloat16())[0])
+
+
+def test_models_that_the_generator_does_not_know_are_refused():
+    from atorch_b200.models.mixtral import MixtralConfig, MixtralModel
+
+    m = _model()
+    wrapped = torch.nn.Module()
+    wrapped.module = m
+    other = _model()
+    other.layers[1] = MixtralModel(MixtralConfig.tiny_moe()).bfloat16().layers[0]
+    for bad in (MixtralModel(MixtralConfig.tiny_moe()).bfloat16(), wrapped, other):
+        with pytest.raises(TypeError):
+            Generator(bad)
+        with pytest.raises(TypeError):
+            CachedSampler(bad)
+
+
+def test_layers_in_a_wrapper_that_hands_on_their_attributes():
+    from atorch_b200.modules.distributed_modules.activation_checkpointing import TPCheckpointWrapper
+
+    m, ids = _model(), torch.randint(0, 40, (2, 9), generator=torch.Generator().manual_seed(4))
+    want = generate(m, ids, 5)
+    m.layers[1] = TPCheckpointWrapper(m.layers[1])
+    assert all(torch.equal(a, b) for a, b in zip(generate(m, ids, 5), want))
