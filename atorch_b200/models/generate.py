@@ -67,6 +67,17 @@ class Generator:
             k, v = ops.kv4_read(layer, table, seq, pos, q.dtype)
             return ops.attention(q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0), causal=True, cu_seqlens=cu)
 
+        def attend_over_cache(q, layer):
+            # the flash kernels take bf16; dense scores of all prompts' tokens by all tokens would be 34 GB for 16 prompts of 1024 and 32 heads
+            if len(set(sizes.tolist())) == 1:
+                return ops.kv4_attention(q.view(len(prompts), -1, *q.shape[1:]), layer, table[rows], lengths)
+            return torch.cat([ops.kv4_attention(one.unsqueeze(0), layer, table[row: row + 1], lengths[i: i + 1])[0]
+                              for i, (row, one) in enumerate(zip(rows, q.split(sizes.tolist())))])
+
+        lengths = sizes.to(torch.int32).to(dev)
+        if self.dtype is not torch.bfloat16 and dev.type == "cuda":
+            attend = attend_over_cache
+
         return self._run(torch.cat([p.to(dev) for p in prompts]), cache, table, seq, pos, cos, sin, attend, last)
 
     def _step(self, tokens, cache, table, lengths, cos, sin):
