@@ -9,8 +9,10 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
+from .function import refuse_gradient
 from .kv4 import _check_page_size
 
 MAX_BEAMS = 32
@@ -68,8 +70,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, finished: Optional[t
     dev = logits.get_device()
     if scores.get_device() != dev or (finished is not None and finished.get_device() != dev):
         raise ValueError("logits, scores and finished are on several devices")
-    if (logits.requires_grad or scores.requires_grad) and torch.is_grad_enabled():
-        raise RuntimeError("a selection has no gradient: call under torch.no_grad()")
+    if logits.requires_grad or scores.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradient("a selection has no gradient: call under torch.no_grad()", logits, scores)
     if dev < 0 or not _lib.use_kernels(logits):
         return beam_select_reference(logits, scores, finished, eos, keep)
     if W > MAX_BEAMS or keep > MAX_BEAMS:

@@ -18,6 +18,14 @@ def watched(*ts: Optional[torch.Tensor]) -> bool:
                    or forward_ad.unpack_dual(t).tangent is not None for t in ts if t is not None))
 
 
+def refuse_gradient(message: str, *ts: Optional[torch.Tensor]) -> None:
+    """RuntimeError where something asks for a gradient of an operator that has none: a tensor that requires it, or one with a
+    tangent, which ``torch.no_grad`` leaves as it is."""
+    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)) \
+            or (forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in ts)):
+        raise RuntimeError(message)
+
+
 class _NoGradContext:
     """What ``forward`` finds in place of its autograd context: no input needs a gradient, nothing is kept."""
 

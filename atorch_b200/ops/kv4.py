@@ -19,8 +19,10 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
+from .function import refuse_gradient
 
 Layer = Tuple[torch.Tensor, torch.Tensor]
 HEAD_DIMS = (64, 128)          # of the kernels; the CPU path takes any even one
@@ -83,8 +85,8 @@ def _same_device(dev: int, *tensors: Optional[torch.Tensor]) -> None:
 
 
 def _no_gradient(t: torch.Tensor) -> None:
-    if t.requires_grad and torch.is_grad_enabled():
-        raise RuntimeError("the 4-bit cache has no gradient: call under torch.no_grad()")
+    if t.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradient("the 4-bit cache has no gradient: call under torch.no_grad()", t)
 
 
 def _int32(name: str, t: Optional[torch.Tensor], n: int) -> Optional[torch.Tensor]:

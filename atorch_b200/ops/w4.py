@@ -11,8 +11,10 @@ from __future__ import annotations
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
+from .function import refuse_gradient
 from .gemm import gemm
 
 GROUPS = (32, 64, 128)
@@ -88,8 +90,8 @@ def w4_linear(x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, group_
         if bias.get_device() != dev:
             raise ValueError(f"bias is on {bias.device}, and x on {x.device}")
         bias = bias.contiguous()
-    if (x.requires_grad or (bias is not None and bias.requires_grad)) and torch.is_grad_enabled():
-        raise RuntimeError("4-bit weights have no gradient: call under torch.no_grad()")
+    if x.requires_grad or (bias is not None and bias.requires_grad) or forward_ad._current_level >= 0:
+        refuse_gradient("4-bit weights have no gradient: call under torch.no_grad()", x, bias)
     if codes.get_device() != dev or scales.get_device() != dev:
         raise ValueError(f"x is on {x.device}, and its weights on {codes.device} and {scales.device}")
     if dev < 0:

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from atorch_b200 import ops
 
@@ -85,3 +86,40 @@ def test_reorder_refuses_a_cache_off_its_alignment():
             ops.beam_reorder(codes, scales, table, lengths, parents)
         with pytest.raises(ValueError):
             ops.kv4_read((codes[0], scales[0]), table, None, lengths)
+
+
+def _calls(dev):
+    """Each operator on tensors of a device, by name: the tensors that a gradient could be asked of, and the call."""
+    g = torch.Generator().manual_seed(2)
+    cache = ops.KV4Cache(1, 4, 16, 2, 64, dev)
+    table, n = torch.tensor([[0, 1]], dtype=torch.int32, device=dev), torch.tensor([20], dtype=torch.int32, device=dev)
+    qkv, q = torch.randn(1, 8 * 64, generator=g).to(dev), torch.randn(1, 1, 4, 64, generator=g).half().to(dev)
+    codes, scales = (t.to(dev) for t in ops.w4_quantize(torch.randn(16, 64, generator=g), 64))
+    x, bias = torch.randn(3, 64, generator=g).bfloat16().to(dev), torch.randn(16, generator=g).bfloat16().to(dev)
+    logits, scores = torch.randn(1, 2, 50, generator=g).to(dev), torch.randn(1, 2, generator=g).to(dev)
+    return {"append": ([qkv], lambda t: ops.kv4_append(cache.layer(0), table, None, n, t, 4)),
+            "attention": ([q], lambda t: ops.kv4_attention(t, cache.layer(0), table, n)),
+            "w4_linear": ([x, bias], lambda t, b: ops.w4_linear(t, codes, scales, 64, b)),
+            "beam_select": ([logits, scores], lambda t, s: ops.beam_select(t, s))}
+
+
+def check_gradients_are_refused(dev):
+    for name, (tensors, call) in _calls(dev).items():
+        with torch.no_grad():
+            call(*tensors)
+        for i in range(len(tensors)):
+            asks = [t.clone().requires_grad_() if j == i else t for j, t in enumerate(tensors)]
+            with pytest.raises(RuntimeError, match="gradient"):
+                call(*asks)
+            with torch.no_grad():
+                call(*asks)
+            with forward_ad.dual_level():
+                dual = [forward_ad.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(tensors)]
+                for off in (False, True):           # gradients that are switched off leave tangents as they are
+                    with torch.set_grad_enabled(not off), pytest.raises(RuntimeError, match="gradient"):
+                        call(*dual)
+                call(*tensors)
+
+
+def test_gradients_and_tangents_are_refused():
+    check_gradients_are_refused("cpu")

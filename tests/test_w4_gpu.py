@@ -154,3 +154,9 @@ def test_many_rows_of_any_layout(M, N):
         _check(y, codes, scales, 64, bias, weight_rounded=True)
         assert _lib.launch_count == before + 4
     assert ops.w4_linear(x[:, :256].reshape(M, 1, 256), codes, scales, 64).shape == (M, 1, N)
+
+
+def test_gradients_and_tangents_are_refused():
+    from tests.test_w4_beam_cpu import check_gradients_are_refused
+
+    check_gradients_are_refused(DEV)
