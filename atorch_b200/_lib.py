@@ -167,7 +167,11 @@ def stream() -> int:
 
 
 def stream_of(device: int) -> int:
-    """Handle of the current stream of the device with this index."""
+    """Handle of the current stream of the device with this index, which has to be the current one: launchers launch there, and a
+    stream's handle alone does not tell them where it belongs."""
+    if torch._C._cuda_getDevice() != device:
+        raise ValueError(f"tensors on cuda:{device}, and the current device is cuda:{torch._C._cuda_getDevice()}: call under "
+                         f"torch.cuda.device({device})")
     return torch._C._cuda_getCurrentRawStream(device)
 
 

@@ -117,7 +117,8 @@ class Generator:
             raise ValueError("a beam search does not sample")
         if max_new_tokens < 1:
             return prompts
-        with self._whole_parameters():
+        dev = self.model.embed_tokens.weight.device
+        with torch.cuda.device(dev) if dev.type == "cuda" else contextlib.nullcontext(), self._whole_parameters():
             return self._generate(prompts, max_new_tokens, eos, temperature, beams, length_penalty)
 
     def _generate(self, prompts, max_new_tokens, eos, temperature, beams, length_penalty):

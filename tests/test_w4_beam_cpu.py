@@ -123,3 +123,17 @@ def check_gradients_are_refused(dev):
 
 def test_gradients_and_tangents_are_refused():
     check_gradients_are_refused("cpu")
+
+
+def test_launches_are_on_the_current_device(monkeypatch):
+    """The launchers launch on the current device: the stream of another one is refused."""
+    from atorch_b200 import _lib
+
+    current = [0]
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 1000 + device, raising=False)
+    assert _lib.stream_of(0) == 1000
+    with pytest.raises(ValueError, match="cuda:1"):
+        _lib.stream_of(1)
+    current[0] = 1
+    assert _lib.stream_of(1) == 1001
