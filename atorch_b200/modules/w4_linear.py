@@ -21,6 +21,13 @@ class W4Linear(nn.Module):
         self.register_buffer("scales", scales)
         self.register_buffer("bias", bias)
 
+    def _apply(self, fn, recurse: bool = True):
+        scales = self.scales
+        super()._apply(fn, recurse)
+        if self.scales.dtype is not scales.dtype:      # the model is cast: scales stay what the codes were taken for
+            self.scales = scales.to(self.codes.device)
+        return self
+
     @classmethod
     def from_linear(cls, linear: nn.Linear, group_size: int = 128) -> "W4Linear":
         codes, scales = w4_quantize(linear.weight, group_size)

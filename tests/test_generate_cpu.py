@@ -233,3 +233,19 @@ def test_layers_in_a_wrapper_that_hands_on_their_attributes():
     want = generate(m, ids, 5)
     m.layers[1] = TPCheckpointWrapper(m.layers[1])
     assert all(torch.equal(a, b) for a, b in zip(generate(m, ids, 5), want))
+
+
+def test_scales_keep_their_type():
+    """A model that is cast keeps its scales in bf16, as its codes were taken for; the bias goes with the model."""
+    lin = torch.nn.Linear(64, 24)
+    w4 = W4Linear.from_linear(lin.bfloat16(), 32)
+    codes, scales, state = w4.codes.clone(), w4.scales.clone(), w4.state_dict().keys()
+    model = torch.nn.Sequential(torch.nn.LayerNorm(64), w4)
+    for cast in (lambda m: m.half(), lambda m: m.float(), lambda m: m.to(torch.float16), lambda m: m.double().bfloat16()):
+        model = cast(model)
+        assert w4.scales.dtype is torch.bfloat16 and torch.equal(w4.scales, scales) and torch.equal(w4.codes, codes)
+        assert w4.bias.dtype is model[0].weight.dtype and w4.state_dict().keys() == state
+        if w4.bias.dtype is not torch.float32:
+            with torch.no_grad():
+                assert w4(torch.randn(3, 64).to(w4.bias.dtype)).dtype is w4.bias.dtype
+    assert copy.deepcopy(w4).to("meta").scales.is_meta
