@@ -165,8 +165,8 @@ def kv4_append(layer: Layer, page_table: torch.Tensor, seq: Optional[torch.Tenso
         if cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.shape != (positions, D // 2) \
                 or sin.shape != (positions, D // 2):
             raise ValueError(f"cos and sin are fp32 [positions, {D // 2}]")
-        cos, sin = (t if t.is_contiguous() and t.data_ptr() & 15 == 0 else t.clone(memory_format=torch.contiguous_format)
-                    for t in (cos, sin))         # read in pieces of 16 bytes
+        if not (cos.is_contiguous() and sin.is_contiguous()) or (cos.data_ptr() | sin.data_ptr()) & 15:      # read in pieces of 16 bytes
+            cos, sin = (t.clone(memory_format=torch.contiguous_format) for t in (cos, sin))
     elif cos is not sin:
         raise ValueError("cos and sin go together")
     _no_gradient(qkv)
