@@ -19,8 +19,13 @@ from .gemm import gemm
 
 GROUPS = (32, 64, 128)
 _LOW = {torch.bfloat16: 0, torch.float16: 1}
-# rows of x from which the weights are expanded to bf16 and multiplied by the GEMM, with bf16 x and K a multiple of 8
-EXPAND_ROWS = 65
+# Rows of x from which the weights are expanded to bf16 and multiplied by the GEMM, with bf16 x and K a multiple of 8. The kernel for few
+# rows keeps the weights exact (up to 12 bits; bf16 has 8), so it stays until it is the slower one. Kernel, expansion and GEMM, in us:
+#    outputs x inputs      33 rows      65 rows      96 rows     128 rows     256 rows
+#    22016 x 4096         58,  95      89,  95      97,  95     125,  97     240, 106
+#    4096 x 11008         34,  94      58,  94      71,  94      64,  95     121,  65
+#    2048 x 2048          10,  18      10,  17      10,  17      10,  18      17,  17
+EXPAND_ROWS = 97
 
 
 def w4_quantize(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -131,17 +131,17 @@ def test_refusals():
 
 
 @pytest.mark.parametrize("offset", [1, 2, 4, 8])
-@pytest.mark.parametrize("M", [64, 72, 300])
+@pytest.mark.parametrize("M", [64, 72, 104, 300])
 def test_codes_off_their_alignment(M, offset):
     codes, scales, g = _weights(104, 264, 64)
     x = torch.randn(M, 264, generator=g, device=DEV).bfloat16()
     pad = torch.zeros(codes.numel() + offset, dtype=torch.uint8, device=DEV)[offset:].view_as(codes)
     pad.copy_(codes)
-    assert torch.equal(_check(x, pad, scales, 64, weight_rounded=M > 64), ops.w4_linear(x, codes, scales, 64))
+    assert torch.equal(_check(x, pad, scales, 64, weight_rounded=M >= w4.EXPAND_ROWS), ops.w4_linear(x, codes, scales, 64))
 
 
 @pytest.mark.parametrize("N", [104, 99, 513])
-@pytest.mark.parametrize("M", [65, 72, 300])
+@pytest.mark.parametrize("M", [97, 104, 300])
 def test_many_rows_of_any_layout(M, N):
     """Rows off 16 bytes, pitches that are no multiple of 8, one row many times over, outputs of any width: two launches of the package."""
     codes, scales, g = _weights(N, 256, 64)
@@ -160,3 +160,10 @@ def test_gradients_and_tangents_are_refused():
     from tests.test_w4_beam_cpu import check_gradients_are_refused
 
     check_gradients_are_refused(DEV)
+
+
+@pytest.mark.parametrize("M", [65, 96])
+def test_weights_are_exact_below_the_expansion(M):
+    codes, scales, g = _weights(200, 512, 128)
+    assert M < w4.EXPAND_ROWS
+    _check(torch.randn(M, 512, generator=g, device=DEV).bfloat16(), codes, scales, 128)
