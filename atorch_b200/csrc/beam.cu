@@ -59,8 +59,7 @@ ATB_DEVICE unsigned long long block_max_key(unsigned long long k, unsigned long 
   return t;
 }
 
-// Calls f(values, n, index) for the elements [from, to) of a row that this thread has, in 16-byte pieces where the row allows it
-// (`wide`: it begins on 16 bytes; `from` is a multiple of 8), else one by one, n = 1.
+// 16 bytes of a row
 template <typename T>
 struct Piece {
   static constexpr int N = 16 / sizeof(T);
@@ -78,6 +77,8 @@ struct Piece {
     }
   }
 };
+// The elements [from, to) of a row that a thread has: `each` calls f(piece, index of its first) for those in 16-byte pieces, where the
+// row allows it (`wide`: it begins on 16 bytes; `from` is a multiple of 8), and one(value, index) for the others.
 // P pieces of a thread stay in registers, all asked for at once; P = 0: they are read (from the first-level cache) every time. Two
 // and four pay (4 beams of 32000 tokens 12.9 -> 11.9 us with what follows); eight leave room for three blocks an SM and pay as long as
 // there are no more (192 beams 17.5 -> 14.5 us; with two blocks an SM, in two turns, 22).

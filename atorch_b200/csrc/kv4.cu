@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(SMALL) kv4_read_kernel(T* k, T* v, Cache c, co
 // Every block takes an equal run of it, which it finds for itself from the lengths on the device (they need not be known on the
 // host), so that long and short sequences fill the GPU alike. A run is cut into segments where a sequence (of a head) ends;
 // what a segment costs beside its tiles counts as START units before the first (5, 8 and 12 of them: 32 sequences of up to 4096
-// tokens 33.9, 32.0 and 32.0 us, 19 of up to 1800 15.4, 15.1 and 14.6). A segment that is a whole sequence is finished
+// tokens 32.0, 30.3 and 30.3 us, two of 100k 60.3, 58.6 and 58.6). A segment that is a whole sequence is finished
 // in place; of the others, the run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins in
 // the order of the blocks.
 constexpr int WARPS = 4, TILE = 32, START = 12;
@@ -403,7 +403,7 @@ struct AttnArgs {
 // the tiles at a sequence's end are masked. The maximum that is kept may be exceeded by 2^4 before everything is rescaled: a warp
 // sees few enough tiles for a new maximum in half of them. Row i of 16 tokens' products is token order(i): a lane then reads its
 // values' words without a bank conflict worse than two ways.
-// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 58 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 31 us. With
+// Measured, 32 query heads on 8 of 128: two sequences of 100k tokens (207 MB) 58.6 us, 3.5 TB/s; 32 of up to 4096 (64 MB) 30.3 us. With
 // the arithmetic left out, the copies, waits and starts take 50 and 23 us, and a library's sum over as many bytes 41 and 20: memory
 // bounds the kernel, and of the arithmetic (an instruction every other clock, the integer pipe busy 57 % of the time) what a block
 // does while it has no copies on their way. Loading tiles into registers a warp's tile at a time took 99 and 51 us; a third stage,
@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   uint32_t loads = 0;            // tiles that this warp has taken from its ring
 
   // A tile is two pieces of 16 tokens, each in one page, of three copies: keys, values, scales. Lane 3 p + x has copy x of piece p.
-  // Where a page holds a whole tile, the first piece's copies bring both (two sequences of 100k tokens: 60.3 us, now 58.9).
+  // Where a page holds a whole tile, the first piece's copies bring both (two sequences of 100k tokens: 60.3 us without, 58.6).
   const int piece = lane / 3, what = lane - 3 * piece;
   const bool copies = lane < 6;
   const long long page_stride = ((what < 2 ? (long long)c.kv_heads * D : c.kv_heads * 8LL) << c.page_shift);

@@ -6,12 +6,12 @@
 // Bound by the codes, N K / 2 bytes, for as many rows as a decode step has. The products run on the warp's matrix instruction
 // (16 x 8 x 16, fp32 sums) with 16 weight rows as its tall operand and 8 rows of x as the other. Two codes become code - 8 in the
 // type of x by one AND-OR and one packed operation, exactly: 128 + code is a bf16 number with the code in its last bits, 1024 +
-// code and 1024 + 16 code are such fp16 numbers. Products are exact in fp32, sums are fp32, and the scale of a row and group
-// multiplies the sum of the group.
-// Measured: 16 x 4096 x 22016 (47 MB) 23.6 us, 2 TB/s; 1 x 11008 x 4096 (23 MB) 12.1. A third of it is a block's start and the sum
-// over a cluster; in the products the warps issue at half the clock, four operations of ten on the integer pipe (7 for 8 codes in
-// bf16). Persistent blocks with equal runs of (strip, group) for every warp took 35 and 12 us, a prefetch of whole rows into L2
-// nothing off.
+// code and 1024 + 16 code are such fp16 numbers (the known way of building small integers into the mantissa of a power of two). Products
+// are exact in fp32, sums are fp32, and the scale of a row and group multiplies the sum of the group.
+// Measured: 16 x 4096 x 22016 (47 MB) 24.3 us, 21.3 with x and a part of the codes in L2; 1 x 11008 x 4096 (23 MB) 13.1 and 11.9.
+// Latency bounds it: the warps (14 of an SM, 80 and 128 registers) use 33 % and 27 % of the issue slots, and wait for loads first, then
+// for operations on one another; a block stages its x and scales before its first product, and its cluster meets for the sum. Persistent
+// blocks with equal runs of (strip, group) for every warp took 35 and 12 us, a prefetch of whole rows into L2 nothing off.
 #include <atomic>
 #include <cooperative_groups.h>
 #include "common.cuh"
