@@ -136,7 +136,8 @@ def beam_reorder(codes: torch.Tensor, scales: torch.Tensor, page_table: torch.Te
     if parents.dim() != 2 or parents.dtype is not torch.int32:
         raise ValueError(f"parents are int32 [B, beams], got {parents.dtype} {tuple(parents.shape)}")
     B, W = parents.shape
-    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B * W or page_table.stride(1) != 1:
+    if page_table.dtype is not torch.int32 or page_table.dim() != 2 or page_table.shape[0] != B * W \
+            or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
         raise ValueError(f"page_table is int32 [{B * W}, pages], its rows contiguous")
     if lengths.dtype is not torch.int32 or lengths.shape != (B * W,):
         raise ValueError(f"lengths are int32 [{B * W}], got {lengths.dtype} {tuple(lengths.shape)}")

@@ -65,7 +65,7 @@ def _cache(layer: Layer, page_table: torch.Tensor) -> Tuple[int, ...]:
     if page_size < 16 or page_size & (page_size - 1):
         _check_page_size(page_size)
     steps = page_table.stride()
-    if page_table.dtype is not torch.int32 or len(steps) != 2 or steps[1] != 1:
+    if page_table.dtype is not torch.int32 or len(steps) != 2 or (steps[1] != 1 and page_table.shape[1] > 1):
         raise ValueError("page_table is int32 [sequences, pages], its rows contiguous")
     if dev >= 0 and half != 64 and half != 32:
         raise ValueError(f"head_dim {2 * half}: the kernels take {HEAD_DIMS}")

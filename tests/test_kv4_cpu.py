@@ -90,3 +90,19 @@ def test_whole_numbers_of_64_bits_are_not_cut(far):
     with pytest.raises(IndexError):
         ops.kv4_append(layer, table, place, one, x, 4)
     assert (cache.codes == 0).all() and (cache.scales == 0).all()
+
+
+def test_a_table_of_one_column_may_have_any_stride_there():
+    cache, table, g = _filled()
+    wide = table.repeat_interleave(3, 1)[:, ::3][:, :1]            # one page a sequence, the next column three places on
+    assert wide.shape == (2, 1) and wide.stride(1) == 3
+    x, pos = torch.randn(2, 8 * 32, generator=g), torch.tensor([3, 7])
+    ops.kv4_append(cache.layer(0), wide, None, pos, x, 4)
+    got = ops.kv4_read(cache.layer(0), wide, None, pos)
+    want = ops.kv4_read(cache.layer(0), table, None, pos)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and got[0].any()
+    ops.beam_reorder(cache.codes, cache.scales, wide, torch.full((2,), 9, dtype=torch.int32), torch.tensor([[1, 0]], dtype=torch.int32))
+    after = ops.kv4_read(cache.layer(0), table, torch.tensor([1, 0]), pos)
+    assert all(torch.equal(a, b) for a, b in zip(after, want))
+    with pytest.raises(ValueError):
+        ops.kv4_read(cache.layer(0), table.repeat_interleave(3, 1)[:, ::3], None, pos)
