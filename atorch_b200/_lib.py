@@ -59,12 +59,17 @@ SIGNATURES = {
     "atb_kv4_append": "pppppppppiiiiiiiiillipp",
     "atb_kv4_read": "pppppppiiiiiiilipp",
     "atb_kv4_attention": "ppppppppiiiiiiiilllfipp",
+    "atb_kv_append": "ppppppppppiiiiiiiiillipp",
+    "atb_kv_attention": "ppppppppiiiiiiiillllfipp",
+    "atb_kv_evict": "ppppppiiiiiiilliipp",
+    "atb_sample": "ppppppppiillllliipp",
 }
 _CTYPE = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float}
 
 _ctypes_launches = 0
 _NOT_LAUNCHES = {"atb_norm_bwd_parts", "atb_sumsq_parts", "atb_set_comm_wait_ns", "atb_noalloc_max_n",
-                 "atb_embedding_bwd_scratch", "atb_kv4_attention_scratch"}
+                 "atb_embedding_bwd_scratch", "atb_kv4_attention_scratch",
+                 "atb_kv_attention_scratch"}
 
 
 def __getattr__(name):

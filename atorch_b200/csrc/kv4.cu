@@ -4,30 +4,19 @@
 //   codes  uint8 [pages][2][kv heads][page size][D / 2]    0: keys, 1: values; byte i: dim 2i low, dim 2i + 1 high
 //   scales bf16  [pages][kv heads][page size][4]           scale and minimum of the key, scale and minimum of the value
 // A value is code * scale + minimum, one scale and minimum per token, head and tensor: (D + 8) bytes a token and head where
-// bf16 keeps 4 D. Sequence b's token p lies in page table[b][p / page size], place p % page size.
+// bf16 keeps 4 D.
 #include <atomic>
 #include <type_traits>
-#include "common.cuh"
+#include "paged.cuh"
 
 namespace {
 using namespace atb;
 
-struct Cache {
+struct Cache : Paging {
   uint8_t* codes;
   __nv_bfloat16* scales;
-  const int* table;
-  long long table_stride;
-  int rows, width;       // sequences, pages a sequence may have
-  int pages, kv_heads, page_shift;
 };
 
-// Page of token p of sequence b, or -1 where the table or the sequence does not have it.
-ATB_DEVICE int page_of(const Cache& c, int b, int p) {
-  const int i = p >> c.page_shift;
-  if (b < 0 || b >= c.rows || i >= c.width) return -1;
-  const int page = c.table[b * c.table_stride + i];
-  return page < 0 || page >= c.pages ? -1 : page;
-}
 template <int D>
 ATB_DEVICE uint8_t* codes_at(const Cache& c, int page, int which, int head, int slot) {
   return c.codes + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * (D / 2);
@@ -36,32 +25,6 @@ ATB_DEVICE __nv_bfloat16* scales_at(const Cache& c, int page, int head, int slot
   return c.scales + ((((long long)page * c.kv_heads + head) << c.page_shift) + slot) * 4;
 }
 
-template <typename T>
-ATB_DEVICE void load8(const T* p, float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-  } else {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
-    const T* h = reinterpret_cast<const T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(h[i]);
-  }
-}
-template <typename T>
-ATB_DEVICE void store8(T* p, const float (&x)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
-  } else {
-    uint4 u;
-    T* h = reinterpret_cast<T*>(&u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = from_f32<T>(x[i]);
-    *reinterpret_cast<uint4*>(p) = u;
-  }
-}
 // 8 elements as they lie in memory
 template <typename T>
 struct Piece {
@@ -267,58 +230,7 @@ constexpr int WARPS = 4, TILE = 32, START = 12;
 constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
 constexpr int LEAST_E = 24, AHEAD_E = 12;      // exponent fields of value scales: the least, and how far one may lie above what its weight leaves
 
-ATB_DEVICE int seen_length(const Cache& c, const int* lengths, int b, int* status) {
-  const int n = lengths[b], most = c.width << c.page_shift;
-  if (n > most) atomicCAS(status, 0, (int)ATB_ERR_BAD_INDEX);
-  return max(0, min(n, most));
-}
-ATB_DEVICE int tiles_of(int n) { return max(1, (n + TILE - 1) / TILE); }     // an empty sequence has its zeros written
-ATB_DEVICE long long warp_sum_ll(long long v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
-}
-
-struct Plan {
-  long long units;
-  int ctas;              // blocks with a run: run k is [k units / ctas, (k + 1) units / ctas)
-  ATB_DEVICE long long begin(long long k) const { return k * units / ctas; }
-  ATB_DEVICE int owner(long long u) const { return (int)(((u + 1) * ctas - 1) / units); }
-};
-// `per`: heads x column tiles. A run has a unit for every warp where there are enough.
-ATB_DEVICE Plan make_plan(const Cache& c, const int* lengths, int per, int ctas, int* status) {
-  long long total = 0;
-  for (int b = threadIdx.x & 31; b < c.rows; b += 32) total += START + tiles_of(seen_length(c, lengths, b, status));
-  Plan p;
-  p.units = warp_sum_ll(total) * per;
-  p.ctas = (int)max(1LL, min((long long)ctas, p.units / WARPS));
-  return p;
-}
-// Sequence of unit u, its length and its first unit. Computed by a whole warp.
-ATB_DEVICE void find_sequence(const Cache& c, const int* lengths, int per, long long u, int& b, int& len, long long& first,
-                              int* status) {
-  const int lane = threadIdx.x & 31;
-  long long before = 0;
-  for (int b0 = 0; b0 < c.rows; b0 += 32) {
-    const int n = b0 + lane < c.rows ? seen_length(c, lengths, b0 + lane, status) : 0;
-    const long long mine = b0 + lane < c.rows ? (long long)(START + tiles_of(n)) * per : 0;
-    long long sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x = __shfl_up_sync(0xffffffffu, sum, o);
-      if (lane >= o) sum += x;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, u < before + sum);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      b = b0 + src;
-      len = __shfl_sync(0xffffffffu, n, src);
-      first = before + __shfl_sync(0xffffffffu, sum - mine, src);
-      return;
-    }
-    before += __shfl_sync(0xffffffffu, sum, 31);
-  }
-}
+using Cut = Runs<TILE, START, WARPS>;
 
 // 16-byte pieces from global to shared memory by the copy unit (both addresses and the size multiples of 16)
 ATB_DEVICE void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -337,11 +249,6 @@ ATB_DEVICE void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t 
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-}
-ATB_DEVICE uint32_t transpose_8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
 }
 ATB_DEVICE uint32_t pack_f16x2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
@@ -440,7 +347,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
   Plan plan{};
   long long u = blockIdx.x, run_end = (long long)c.rows * per;       // whole sequences: their numbers
   if (a.ctas > 0) {
-    plan = make_plan(c, a.lengths, per, a.ctas, a.status);
+    plan = Cut::plan(c, a.lengths, per, a.ctas, a.status);
     u = plan.begin(blockIdx.x);
     run_end = plan.begin(blockIdx.x + 1);
   }
@@ -462,8 +369,8 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
     long long begin = 0;
     if (a.ctas > 0) {
       long long first;
-      find_sequence(c, a.lengths, per, u, b, len, first, a.status);
-      tiles = tiles_of(len);
+      Cut::find(c, a.lengths, per, u, b, len, first, a.status);
+      tiles = Cut::tiles_of(len);
       hc = (int)((u - first) / (START + tiles));
       begin = first + (long long)hc * (START + tiles);
       t_first = max(0, (int)(u - begin) - START);
@@ -474,7 +381,7 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv4_attentio
       b = (int)(u / per);
       hc = (int)(u - (long long)b * per);
       len = seen_length(c, a.lengths, b, a.status);
-      t_last = tiles = tiles_of(len);
+      t_last = tiles = Cut::tiles_of(len);
       u += gridDim.x;
     }
     const int head = hc % c.kv_heads, col_tile = hc / c.kv_heads;
@@ -891,7 +798,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(AttnArgs a, int per) {
 
 Cache cache_of(void* codes, void* scales, const void* table, long long table_stride, int rows, int width, int pages,
                int kv_heads, int page_shift) {
-  return Cache{(uint8_t*)codes, (__nv_bfloat16*)scales, (const int*)table, table_stride, rows, width, pages, kv_heads, page_shift};
+  return Cache{{(const int*)table, table_stride, rows, width, pages, kv_heads, page_shift}, (uint8_t*)codes, (__nv_bfloat16*)scales};
 }
 
 template <typename T, int D>
