@@ -1,6 +1,8 @@
 // Paged key/value cache in 16 bits: append with rotation, attention of the newest tokens, eviction of tokens with little weight.
 //
 // One layer's cache is T [pages][2][kv heads][page size][D]: 0: keys, 1: values.
+#include <atomic>
+#include <type_traits>
 #include "paged.cuh"
 
 namespace {
@@ -85,6 +87,20 @@ __global__ void __launch_bounds__(SMALL) kv_append_kernel(const T* qkv, T* q_out
 // ----------------------------------------------------------------------------------
 // Attention
 // ----------------------------------------------------------------------------------
+// Query i of sequence b's S newest tokens sees its keys j < lengths[b] - S + i + 1. The g query heads of a key/value head times
+// the S tokens are the columns of one matrix product: n = i g + h, in tiles of 8, 16 or 32.
+//
+// The work is cut into equal runs over the GPU (paged.cuh). A segment that is a whole sequence (of a head and column tile) is
+// finished in place; of the others, a run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins
+// in the order of the blocks.
+constexpr int WARPS = 4, TILE = 16, START = 12;
+constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
+// Powers of two that the largest weight is held at: fp16 has numbers from 2^-24 to 2^16, and thousands of tokens with 2^-26 of the
+// largest weight count together.
+template <typename T>
+constexpr float LIFT = std::is_same<T, __half>::value ? 11.f : 0.f;
+using Cut = Runs<TILE, START, WARPS>;
+
 struct AttnArgs {
   Cache c;
   const int* lengths;
@@ -92,93 +108,527 @@ struct AttnArgs {
   void* out;
   float* lse;                 // [rows][heads][S] or nullptr
   float* weights;             // [rows][kv heads][places] or nullptr
-  float* partial;
-  long long places, q_batch, q_token;
+  float* partial;             // sums [2 ctas][columns of a tile][D], then maximum and denominators [2 ctas][columns][4]
+  int2* owners;               // first and last block of each [row][head and column tile]
+  float* scores;              // [rows][kv heads][places of the table][columns], in powers of two, where there are weights
+  float* lse2;                // [rows][kv heads][columns], the same
+  long long places, q_batch, q_token; // (strides of q: elements)
   int S, heads, group;
   float scale_log2;           // softmax scale * log2(e)
+  int ctas;                   // blocks that the work is cut for; 0: a block takes whole sequences (of a head), one after another
   int* status;
 };
 
-// One query of one head: a block's warps take its keys in turn, a lane D / 32 dims.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) kv_attention_kernel(AttnArgs a) {
-  constexpr int E = D / 32;
-  __shared__ float sh_o[4][D], sh_m[4], sh_l[4];
-  grid_go();
-  grid_wait();
-  if (__syncthreads_or(*a.status != 0)) return;
-  const Cache& c = a.c;
-  const int h = blockIdx.x % a.heads, i = blockIdx.x / a.heads % a.S, b = blockIdx.x / a.heads / a.S;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, head = h / a.group;
-  const int len = seen_length(c, a.lengths, b, a.status), limit = min(len, len - a.S + i + 1);
-  const T* q = (const T*)a.q + b * a.q_batch + i * a.q_token + h * D + lane * E;
-  float x[E], o[E], m = -INFINITY, l = 0.f;
-  for (int e = 0; e < E; ++e) {
-    x[e] = to_f32<T>(q[e]) * a.scale_log2;
-    o[e] = 0.f;
+template <typename T>
+ATB_DEVICE void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+ATB_DEVICE void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+ATB_DEVICE void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+template <typename T>
+ATB_DEVICE uint32_t pack2(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(a, b);
   }
-  auto score = [&](int t, int& page) {
-    page = page_of(c, b, t);
-    if (page < 0) {
-      atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
-      page = 0;
-    }
-    const T* k = row_at<T, D>(c, page, 0, head, t & ((1 << c.page_shift) - 1)) + lane * E;
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s += x[e] * to_f32<T>(k[e]);
-    return warp_sum(s);
-  };
-  for (int t = warp; t < limit; t += 4) {
-    int page;
-    const float s = score(t, page), to = fmaxf(m, s), ref = to == -INFINITY ? 0.f : to;
-    const float f = exp2f(m - ref), p = exp2f(s - ref);
-    const T* v = row_at<T, D>(c, page, 1, head, t & ((1 << c.page_shift) - 1)) + lane * E;
-    m = to;
-    l = l * f + p;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f + p * to_f32<T>(v[e]);
-  }
-  for (int e = 0; e < E; ++e) sh_o[warp][lane * E + e] = o[e];
-  sh_m[warp] = m;
-  sh_l[warp] = l;
-  __syncthreads();
-  const float top = fmaxf(fmaxf(sh_m[0], sh_m[1]), fmaxf(sh_m[2], sh_m[3])), ref = top == -INFINITY ? 0.f : top;
-  float sum = 0.f;
-  for (int w = 0; w < 4; ++w) sum += sh_l[w] * exp2f(sh_m[w] - ref);
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float y = 0.f;
-    for (int w = 0; w < 4; ++w) y += sh_o[w][d] * exp2f(sh_m[w] - ref);
-    ((T*)a.out)[((long long)(b * a.S + i) * a.heads + h) * D + d] = from_f32<T>(sum == 0.f ? 0.f : y / sum);
-  }
-  if (threadIdx.x == 0 && a.lse) a.lse[((long long)b * a.heads + h) * a.S + i] = (top + log2f(sum)) * 0.69314718056f;
-  if (a.partial)
-    if (threadIdx.x == 0) a.partial[((long long)b * a.heads + h) * a.S + i] = top + log2f(sum);
+}
+// whether one of two 16-bit numbers is an infinity or a NaN
+template <typename T>
+ATB_DEVICE bool endless(uint32_t u) {
+  constexpr uint32_t E = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+  return (u & E) == E || (u >> 16 & E) == E;
 }
 
-// What the queries attended to, one place after another: a warp forms a key's scores again and adds their shares in the order of the
-// queries.
+// Four dims of a column's result, from its maximum, the sum of its weights, that of the rounded ones, and the sums with the values.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv_weights_kernel(AttnArgs a) {
-  constexpr int E = D / 32;
+ATB_DEVICE void finish(const AttnArgs& a, int b, int head, int n, int d, float top, float sum, float rounded, const float (&o)[4]) {
+  const int i = n / a.group, h = head * a.group + n - i * a.group;
+  const float inv = rounded == 0.f ? 0.f : 1.f / rounded;
+  T y[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = from_f32<T>(o[e] * inv);
+  *reinterpret_cast<uint2*>(reinterpret_cast<T*>(a.out) + (((long long)b * a.S + i) * a.heads + h) * D + d) =
+      *reinterpret_cast<const uint2*>(y);
+  if (d != 0) return;
+  const float lse2 = top + (log2f(sum) - LIFT<T>);
+  if (a.lse) a.lse[((long long)b * a.heads + h) * a.S + i] = lse2 * 0.69314718056f;
+  if (a.lse2) a.lse2[((long long)b * a.c.kv_heads + head) * (a.S * a.group) + n] = lse2;
+}
+
+// Both products run on the warp's matrix instruction (16 x 8 x 16, fp32 sums), with the keys and the values as its 16-row operand
+// and the columns as its 8-wide one: s[t, n] = k[t] . q[n], o[d, n] = sum_t v[t, d] p[t, n]. So a group of up to 8 query heads fills it.
+// A tile of 16 tokens lies in one page; the copy unit brings its keys and values into a ring of the warp's own, STAGES tiles ahead, in
+// halves of 64 dims whose rows are 128 bytes, their 16-byte pieces exchanged by the row (the 128-byte swizzle), so that a matrix load
+// of 8 rows meets no bank twice.
+// Weights p are rounded to the cache's 16 bits for their product with the values; what divides the sums is the sum of the rounded
+// weights (a product with ones), so that they add up to 1, and the logarithm of the denominator comes from the unrounded ones.
+// Scores are taken relative to the running maximum, which may be exceeded by 2^SLACK before everything is rescaled; only tiles at a
+// sequence's end are masked. There, what no column sees is put to 0 in shared memory (memory behind a sequence may hold anything), and
+// a value that some columns see and others do not is kept from the others even if it is an infinity or a NaN: column by column then.
+template <int D, int NT>
+struct Shape {
+  static constexpr int COLS = 8 * NT, STAGE = TILE * D * 4, STAGES = 3 * 128 / D, RING = WARPS * STAGES * STAGE;
+  static constexpr int QUERIES = NT == 4 ? COLS * D * 2 : 0;      // bytes of shared memory for them; else they lie in registers
+  static constexpr int SMEM = RING + QUERIES + 1024, BLOCKS = 2;  // of an SM; the ring begins on 1024 bytes
+};
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv_attention_kernel(const __grid_constant__ CUtensorMap map, AttnArgs a) {
+  using Sh = Shape<D, NT>;
+  constexpr int KS = D / 16, COLS = Sh::COLS, STAGES = Sh::STAGES, HALF_BYTES = TILE * 128;
+  constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+  static_assert(WARPS * COLS * (D + 4) * 4 <= Sh::RING, "the warps' sums lie in the place of the ring");
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  __shared__ float sh_m[WARPS][COLS], sh_l[WARPS][COLS], sh_r[WARPS][COLS];
+  __shared__ uint64_t bars[WARPS][STAGES];
+  __shared__ int abort_flag;
+  const Cache& c = a.c;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, q4 = lane & 3;
+  uint8_t* const ring = smem + warp * (STAGES * Sh::STAGE);
+  uint32_t* const sh_q = reinterpret_cast<uint32_t*>(smem + Sh::RING);
+  if (threadIdx.x == 0) abort_flag = 0;
+  if (lane < STAGES) mbar_init(&bars[warp][lane], 1);
+  mbar_fence_init();
+  if (threadIdx.x == 0) tma_prefetch_desc(&map);
   grid_go();
   grid_wait();
-  if (__syncthreads_or(*a.status != 0)) return;
-  const Cache& c = a.c;
-  const int head = blockIdx.y % c.kv_heads, b = blockIdx.y / c.kv_heads, lane = threadIdx.x & 31;
-  const int len = seen_length(c, a.lengths, b, a.status);
-  for (int t = blockIdx.x * 4 + (threadIdx.x >> 5); t < len; t += gridDim.x * 4) {
-    const int page = page_of(c, b, t);
-    if (page < 0) continue;
-    const T* k = row_at<T, D>(c, page, 0, head, t & ((1 << c.page_shift) - 1)) + lane * E;
-    float sum = 0.f;
-    for (int i = max(0, t - len + a.S); i < a.S; ++i)
-      for (int h = head * a.group; h < (head + 1) * a.group; ++h) {
-        const T* q = (const T*)a.q + b * a.q_batch + i * a.q_token + h * D + lane * E;
-        float s = 0.f;
-        for (int e = 0; e < E; ++e) s += to_f32<T>(q[e]) * a.scale_log2 * to_f32<T>(k[e]);
-        const float lse = a.partial[((long long)b * a.heads + h) * a.S + i];
-        if (lse != -INFINITY) sum += exp2f(warp_sum(s) - lse);
+  const int failed = threadIdx.x == 0 ? *a.status : 0;       // on its way beside the lengths
+  const int columns = a.S * a.group, col_tiles = (columns + COLS - 1) / COLS, per = col_tiles * c.kv_heads;
+  Plan plan{};
+  long long u = blockIdx.x, run_end = (long long)c.rows * per;       // whole sequences: their numbers
+  if (a.ctas > 0) {
+    plan = Cut::plan(c, a.lengths, per, a.ctas, a.status);
+    u = plan.begin(blockIdx.x);
+    run_end = plan.begin(blockIdx.x + 1);
+  }
+  if (__syncthreads_or(failed != 0)) return;       // one answer for the block: others may fail meanwhile
+  if (a.ctas > 0 && (int)blockIdx.x >= plan.ctas) return;
+  uint32_t stage_in = 0, stage_out = 0, phase_out = 0;       // of the warp's ring: where the next tile goes, the next one comes from
+
+  // where a lane reads its row of a matrix load in a half of a tile: keys (tokens 0..7, 8..15, then the next 8 dims) and values (the
+  // next 8 dims, then tokens 8..15)
+  const uint32_t k_row = (lane & 15) * 128, k_piece = lane >> 4, v_row = ((lane >> 4) * 8 + (lane & 7)) * 128, v_piece = (lane >> 3) & 1;
+  const uint32_t turn = lane & 7, ring_at = smem_u32(ring);
+
+  while (u < run_end) {
+    int b, len, hc, tiles, t_first = 0, t_last;       // the segment: tiles [t_first, t_last) of a sequence
+    long long begin = 0;
+    if (a.ctas > 0) {
+      long long first;
+      Cut::find(c, a.lengths, per, u, b, len, first, a.status);
+      tiles = Cut::tiles_of(len);
+      hc = (int)((u - first) / (START + tiles));
+      begin = first + (long long)hc * (START + tiles);
+      t_first = max(0, (int)(u - begin) - START);
+      t_last = (int)min(run_end - begin - START, (long long)tiles);
+      u = begin + START + t_last;
+      if (t_last <= t_first) break;      // the run ends before the first tile
+    } else {
+      b = (int)(u / per);
+      hc = (int)(u - (long long)b * per);
+      len = seen_length(c, a.lengths, b, a.status);
+      t_last = tiles = Cut::tiles_of(len);
+      u += gridDim.x;
+    }
+    const int head = hc % c.kv_heads, col_tile = hc / c.kv_heads;
+    const bool whole = t_first == 0 && t_last == tiles;
+    if (a.ctas > 0 && t_first == 0 && threadIdx.x == 0)
+      a.owners[(long long)b * per + hc] = make_int2(blockIdx.x, plan.owner(begin + START + tiles - 1));
+    const int mine = len == 0 ? 0 : max(0, (t_last - t_first - warp + WARPS - 1) / WARPS);
+    const int* const row = c.table + b * c.table_stride;
+
+    // pages of the warp's tiles j to j + 31
+    auto pages_from = [&](int j) {
+      const int t = (t_first + warp + (j + lane) * WARPS) * TILE;
+      int page = 0;
+      if (j + lane < mine) {
+        page = row[t >> c.page_shift];
+        if (page < 0 || page >= c.pages) {
+          atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+          page = 0;
+        }
       }
-    if (lane == 0) a.weights[((long long)b * c.kv_heads + head) * a.places + t] += sum;
+      return page;
+    };
+    int pages = pages_from(0);
+    auto fetch = [&](int j) {      // by the whole warp: tile j into the ring
+      if (j >= mine) return;
+      if (j > 0 && (j & 31) == 0) pages = pages_from(j);
+      const int page = __shfl_sync(0xffffffffu, pages, j & 31);
+      const int t = (t_first + warp + j * WARPS) * TILE;
+      if (lane == 0) mbar_expect_tx(&bars[warp][stage_in], Sh::STAGE);
+      __syncwarp();
+      if (lane < 2)
+        tma_load_3d(ring + stage_in * Sh::STAGE + lane * (Sh::STAGE / 2), &map, &bars[warp][stage_in], 0,
+                    (((page * 2 + lane) * c.kv_heads + head) << c.page_shift) + (t & ((1 << c.page_shift) - 1)), 0);
+      stage_in = stage_in + 1 == STAGES ? 0 : stage_in + 1;
+    };
+    for (int j = 0; j < STAGES; ++j) fetch(j);
+
+    // queries: of column 8 j + r the dims 16 k + 2 q4, + 1 and 8 further
+    uint32_t qf[NT == 4 ? 1 : NT][KS][2];
+    auto query = [&](int n) {
+      const bool live = n < columns;
+      const int i = live ? n / a.group : 0, h = live ? n - i * a.group : 0;
+      return live ? reinterpret_cast<const T*>(a.q) + b * a.q_batch + i * a.q_token + (long long)(head * a.group + h) * D : nullptr;
+    };
+    if constexpr (NT == 4) {
+      // [k][lane][8 words]: those of four column tiles side by side
+      for (int x = threadIdx.x; x < KS * 32 * 4; x += WARPS * 32) {
+        const int j = x & 3, l = x >> 2 & 31, k = x >> 7;
+        const T* q = query(col_tile * COLS + 8 * j + (l >> 2));
+        uint2 w = make_uint2(0u, 0u);
+        if (q) {
+          w.x = *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * (l & 3));
+          w.y = *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * (l & 3) + 8);
+        }
+        *reinterpret_cast<uint2*>(sh_q + (k * 32 + l) * 8 + 2 * j) = w;
+      }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const T* q = query(col_tile * COLS + 8 * j + r);
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) qf[j][k][e] = q ? *reinterpret_cast<const uint32_t*>(q + 16 * k + 2 * q4 + 8 * e) : 0u;
+      }
+    }
+    // the keys that columns 8 j + 2 q4 + {0, 1} see, and that all of the tile see
+    int limit[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int o = 0; o < 2; ++o) limit[j][o] = min(len, len - a.S + (col_tile * COLS + 8 * j + 2 * q4 + o) / a.group + 1);
+    const int all_see = len - a.S + col_tile * COLS / a.group + 1;
+    float* const scores = a.scores ? a.scores + ((long long)b * c.kv_heads + head) * ((long long)c.width << c.page_shift) * columns : nullptr;
+
+    // running maximum of the scores (m), sums of p (l), of its rounded values (ones), and with the values; `ref` is what scores are
+    // taken relative to: m - LIFT, or 0 where there is none yet
+    float o_acc[NT][KS][4], ones[NT][4], m[NT][2], ref[NT][2], l[NT][2];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o_acc[j][i][e] = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) ones[j][e] = 0.f;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        m[j][o] = -INFINITY;
+        ref[j][o] = l[j][o] = 0.f;
+      }
+    }
+    bool unset = true;     // whether a column has no maximum yet
+
+    auto tile = [&](uint32_t keys, int t0, auto masked) {
+      constexpr bool MASK = decltype(masked)::value;
+      const uint32_t values = keys + Sh::STAGE / 2;
+      float s[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.f;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t x[4];
+        ldmatrix(x, keys + (k >> 2) * HALF_BYTES + k_row + (((2 * (k & 3) + k_piece) ^ turn) << 4));
+        if constexpr (NT == 4) {
+          const uint4 u0 = *reinterpret_cast<const uint4*>(sh_q + (k * 32 + lane) * 8), u1 = *reinterpret_cast<const uint4*>(sh_q + (k * 32 + lane) * 8 + 4);
+          mma_16<T>(s[0], x, u0.x, u0.y);
+          mma_16<T>(s[1], x, u0.z, u0.w);
+          mma_16<T>(s[2], x, u1.x, u1.y);
+          mma_16<T>(s[3], x, u1.z, u1.w);
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma_16<T>(s[n], x, qf[n][k][0], qf[n][k][1]);
+        }
+      }
+      float over = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int o = e & 1, t = t0 + r + 4 * (e & 2);
+          float v = s[n][e] * a.scale_log2;
+          if (MASK && t >= limit[n][o]) v = -INFINITY;
+          if (scores) {
+            const int col = col_tile * COLS + 8 * n + 2 * q4 + o;
+            if (col < columns && t < len) scores[(long long)t * columns + col] = v;
+          }
+          s[n][e] = v - ref[n][o];
+          over = fmaxf(over, s[n][e]);
+        }
+      if (__any_sync(0xffffffffu, over > SLACK + LIFT<T> || unset)) {
+        unset = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float f[2];
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            float most = fmaxf(s[n][o], s[n][2 + o]);
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, k));
+            const float to = fmaxf(m[n][o], ref[n][o] + most), by = to == -INFINITY ? 0.f : to - LIFT<T> - ref[n][o];
+            f[o] = m[n][o] == -INFINITY ? (l[n][o] == 0.f ? 0.f : 1.f) : fast_exp2(-by);
+            m[n][o] = to;
+            ref[n][o] += by;
+            unset = unset || to == -INFINITY;
+            l[n][o] *= f[o];
+            s[n][o] -= by;
+            s[n][2 + o] -= by;
+          }
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o_acc[n][i][e] *= f[e & 1];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) ones[n][e] *= f[e & 1];
+        }
+      }
+      uint32_t pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float w0 = fast_exp2(s[n][2 * i]), w1 = fast_exp2(s[n][2 * i + 1]);
+          l[n][0] += w0;
+          l[n][1] += w1;
+          pf[n][i] = transpose_8x8(pack2<T>(w0, w1));
+        }
+      const uint32_t one[4] = {ONES, ONES, ONES, ONES};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma_16<T>(ones[n], one, pf[n][0], pf[n][1]);
+      if constexpr (MASK) {
+        // values from row `from` on become 0
+        auto clear = [&](int from) {
+          for (int x = lane; x < 2 * (D / 64) * 4 * TILE; x += 32) {
+            const int t = x % TILE, piece = x / TILE;
+            if (t >= from)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(values + (piece >> 3) * HALF_BYTES + t * 128 + (piece & 7) * 16), "r"(0u) : "memory");
+          }
+          __syncwarp();
+        };
+        clear(len - t0);
+        bool odd = false;      // an infinity or a NaN that some columns do not see
+        if (a.S > 1)
+          for (int x = lane; x < 2 * (D / 64) * 4 * TILE; x += 32) {
+            const int t = x % TILE, piece = x / TILE;
+            if (t0 + t >= all_see) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(values + (piece >> 3) * HALF_BYTES + t * 128 + (piece & 7) * 16) : "memory");
+              odd = odd || endless<T>(w[0]) || endless<T>(w[1]) || endless<T>(w[2]) || endless<T>(w[3]);
+            }
+          }
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int n = NT - 1; n >= 0; --n)
+#pragma unroll 1
+            for (int col = 7; col >= 0; --col) {
+              clear(len - a.S + (col_tile * COLS + 8 * n + col) / a.group + 1 - t0);
+              const uint32_t p0 = r == col ? pf[n][0] : 0u, p1 = r == col ? pf[n][1] : 0u;
+#pragma unroll
+              for (int i = 0; i < KS; ++i) {
+                uint32_t y[4];
+                ldmatrix_trans(y, values + (i >> 2) * HALF_BYTES + v_row + (((2 * (i & 3) + v_piece) ^ turn) << 4));
+                float z[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_16<T>(z, y, p0, p1);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (2 * q4 + (e & 1) == col) o_acc[n][i][e] += z[e];
+              }
+            }
+          fence_proxy_async_smem();
+          return;
+        }
+        fence_proxy_async_smem();        // the copy unit writes here next
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        uint32_t y[4];
+        ldmatrix_trans(y, values + (i >> 2) * HALF_BYTES + v_row + (((2 * (i & 3) + v_piece) ^ turn) << 4));
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma_16<T>(o_acc[n][i], y, pf[n][0], pf[n][1]);
+      }
+    };
+
+    bool arrived = true;
+    for (int j = 0; j < mine; ++j) {
+      const int t0 = (t_first + warp + j * WARPS) * TILE;
+      arrived = mbar_wait_warp(&bars[warp][stage_out], phase_out, &abort_flag, a.status);
+      if (!arrived) break;
+      if (t0 + TILE <= all_see) tile(ring_at + stage_out * Sh::STAGE, t0, std::false_type());
+      else tile(ring_at + stage_out * Sh::STAGE, t0, std::true_type());
+      if (++stage_out == STAGES) {
+        stage_out = 0;
+        phase_out ^= 1;
+      }
+      __syncwarp();
+      fetch(j + STAGES);
+    }
+
+    // the warps' sums, in their order, in the place of the rings: every copy has arrived and been read
+    float (*const sh_o)[COLS][D + 4] = reinterpret_cast<float (*)[COLS][D + 4]>(smem);
+    if (__syncthreads_or(!arrived)) {
+      // a copy did not come in time: nothing more is asked for or stored, and those on their way may land before the block ends
+      const uint64_t t_start = globaltimer_ns();
+      while (globaltimer_ns() - t_start < 200000ull) __nanosleep(1000);
+      return;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) l[j][o] += __shfl_xor_sync(0xffffffffu, l[j][o], k);
+        const int col = 8 * j + 2 * q4 + o;
+        if (r == 0) {
+          sh_m[warp][col] = m[j][o];
+          sh_l[warp][col] = l[j][o];
+          sh_r[warp][col] = ones[j][o];
+        }
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+          sh_o[warp][col][16 * i + r] = o_acc[j][i][o];
+          sh_o[warp][col][16 * i + r + 8] = o_acc[j][i][2 + o];
+        }
+      }
+    __syncthreads();
+    const long long slot = 2LL * blockIdx.x + (t_first == 0);        // a sequence that goes on, or one that begins, in this block
+    for (int x = threadIdx.x; x < COLS * (D / 4); x += WARPS * 32) {
+      const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
+      if (n >= columns) continue;
+      float top = sh_m[0][col];
+#pragma unroll
+      for (int k = 1; k < WARPS; ++k) top = fmaxf(top, sh_m[k][col]);
+      float sum = 0.f, rounded = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < WARPS; ++k) {
+        const float f = sh_m[k][col] == -INFINITY ? (sh_l[k][col] == 0.f ? 0.f : 1.f) : fast_exp2(sh_m[k][col] - top);
+        const float4 v = *reinterpret_cast<const float4*>(&sh_o[k][col][d]);
+        sum += f * sh_l[k][col];
+        rounded += f * sh_r[k][col];
+        o[0] += f * v.x;
+        o[1] += f * v.y;
+        o[2] += f * v.z;
+        o[3] += f * v.w;
+      }
+      if (!whole) {
+        *reinterpret_cast<float4*>(a.partial + (slot * COLS + col) * D + d) = make_float4(o[0], o[1], o[2], o[3]);
+        if (d == 0)
+          *reinterpret_cast<float4*>(a.partial + 2LL * a.ctas * COLS * D + (slot * COLS + col) * 4) = make_float4(top, sum, rounded, 0.f);
+      } else {
+        finish<T, D>(a, b, head, n, d, top, sum, rounded, o);
+      }
+    }
+    if (u < run_end) {
+      fence_proxy_async_smem();      // the sums were written by the threads, the next tiles come by the copy unit
+      __syncthreads();
+    }
+  }
+}
+
+// Sequences (of a head and a column tile: a block) that several blocks worked on. Bound by latency: the blocks' results are read
+// eight at a time, independent of one another.
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kv_join_kernel(AttnArgs a, int per) {
+  constexpr int COLS = 8 * NT, EACH = 8;
+  grid_go();
+  grid_wait();
+  const int2 own = a.owners[blockIdx.x];
+  const bool failed = *a.status != 0;
+  // (behind a kernel that left early there may be anything)
+  if (__syncthreads_or(failed) || own.x < 0 || own.y >= a.ctas || own.x >= own.y) return;
+  const int columns = a.S * a.group, b = blockIdx.x / per, hc = blockIdx.x - b * per;
+  const int head = hc % a.c.kv_heads, col_tile = hc / a.c.kv_heads;
+  const float* const stats = a.partial + 2LL * a.ctas * COLS * D;
+  for (int x = threadIdx.x; x < COLS * (D / 4); x += 256) {
+    const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
+    if (n >= columns) continue;
+    float top = -INFINITY, sum = 0.f, rounded = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int k0 = own.x; k0 <= own.y; k0 += EACH) {
+      float4 ml[EACH], v[EACH];
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        const long long at = (2LL * min(k0 + k, own.y) + (k0 + k == own.x)) * COLS + col;
+        ml[k] = *reinterpret_cast<const float4*>(stats + 4 * at);
+        v[k] = *reinterpret_cast<const float4*>(a.partial + at * D + d);
+        if (k0 + k > own.y) ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      }
+      float to = top;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) to = fmaxf(to, ml[k].x);
+      const float down = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : fast_exp2(top - to);
+      sum *= down;
+      rounded *= down;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] *= down;
+      top = to;
+#pragma unroll
+      for (int k = 0; k < EACH; ++k) {
+        if (k0 + k > own.y) continue;
+        const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : fast_exp2(ml[k].x - top);
+        sum += f * ml[k].y;
+        rounded += f * ml[k].z;
+        o[0] += f * v[k].x;
+        o[1] += f * v[k].y;
+        o[2] += f * v[k].z;
+        o[3] += f * v[k].w;
+      }
+    }
+    finish<T, D>(a, b, head, n, d, top, sum, rounded, o);
+  }
+}
+
+// What the queries attended to: a place's scores of all columns, as the kernel above has left them, relative to the columns' logarithms,
+// added up in the order of the columns by LANES lanes, and to what is there.
+template <int LANES>
+__global__ void __launch_bounds__(256) kv_weights_kernel(AttnArgs a) {
+  grid_go();
+  grid_wait();
+  const Cache& c = a.c;
+  const int columns = a.S * a.group, b = blockIdx.y / c.kv_heads, lane = threadIdx.x % LANES;
+  const bool failed = *a.status != 0;
+  const int len = seen_length(c, a.lengths, b, a.status);
+  if (__syncthreads_or(failed)) return;
+  const float* const lse2 = a.lse2 + (long long)blockIdx.y * columns;
+  const float* const scores = a.scores + (long long)blockIdx.y * ((long long)c.width << c.page_shift) * columns;
+  float* const weights = a.weights + (long long)blockIdx.y * a.places;
+  const int step = gridDim.x * (256 / LANES);
+  for (int t0 = blockIdx.x * (256 / LANES); t0 < len; t0 += step) {
+    const int t = t0 + threadIdx.x / LANES;
+    float sum = 0.f;
+    if (t < len) {
+      for (int n = lane; n < columns; n += LANES) {
+        const float x = scores[(long long)t * columns + n], y = lse2[n];
+        sum += x == -INFINITY || y == -INFINITY ? 0.f : fast_exp2(x - y);
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (t < len && lane == 0) weights[t] += sum;
   }
 }
 
@@ -314,13 +764,86 @@ int launch_append(const void* qkv, void* q, void* k, const Cache& c, const void*
                                n_q, stride, status));
 }
 
-template <typename T, int D>
-int launch_attention(const AttnArgs& a, cudaStream_t st) {
-  const long long blocks = (long long)a.c.rows * a.S * a.heads;
-  if (blocks > 0x7fffffffLL || (long long)a.c.rows * a.c.kv_heads > 65535) return -2;
-  const int rc = launched(launch_after(kv_attention_kernel<T, D>, dim3((unsigned)blocks), 128, 0, st, 1, a));
+// The cache's rows of D as rows of 64: boxes of TILE rows of all D dims, the halves one behind another.
+template <int D>
+inline bool make_tmap_halves(CUtensorMap* map, void* data, bool half, long long rows) {
+  const PFN_encodeTiled encode = get_encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {64, (cuuint64_t)rows, D / 64}, strides[2] = {D * 2, 128};
+  const cuuint32_t box[3] = {64, TILE, D / 64}, steps[3] = {1, 1, 1};
+  const auto make = [&] {
+    return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, data, dims, strides, box, steps,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = make();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT) {      // the first CUDA work of this host thread
+    cudaFree(nullptr);
+    rc = make();
+  }
+  return rc == CUDA_SUCCESS;
+}
+
+// Floats of the attention's workspace: what blocks leave of the sequences that they share, and with weights the scores.
+struct Workspace {
+  long long partial, owners, lse2, scores, all;
+  int ctas;
+  bool cut;
+};
+inline int column_tiles_of_8(int columns) { return columns <= 8 ? 1 : columns <= 16 ? 2 : 4; }
+inline Workspace workspace(long long rows, int kv_heads, int columns, int D, long long places, bool weighed) {
+  Workspace w;
+  const int nt = column_tiles_of_8(columns);
+  const long long per = (long long)((columns + 8 * nt - 1) / (8 * nt)) * kv_heads;
+  // sequences of up to 256 tokens are not cut: four tiles a warp take less than a join and what the cutting needs to know
+  w.cut = places > 256;
+  w.ctas = w.cut ? 148 * 2 : 0;
+  w.partial = 0;
+  w.owners = 2LL * w.ctas * 8 * nt * (D + 4);
+  w.lse2 = w.owners + (w.cut ? (2 * rows * per + 3) / 4 * 4 : 0);
+  w.scores = w.lse2 + (weighed ? (rows * kv_heads * columns + 3) / 4 * 4 : 0);
+  w.all = w.scores + (weighed ? rows * kv_heads * places * columns : 0);
+  return w;
+}
+
+template <typename T, int D, int NT>
+int launch_attention(AttnArgs a, cudaStream_t st) {
+  using Sh = Shape<D, NT>;
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return launched(cudaErrorInvalidDevice);
+  const unsigned long long bit = 1ull << (device & 63);
+  constexpr int SMEM = Sh::SMEM;
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const int rc = launched(cudaFuncSetAttribute(kv_attention_kernel<T, D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    if (rc != 0) return rc;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const int columns = a.S * a.group;
+  const long long places = (long long)a.c.width << a.c.page_shift;
+  const long long per = (columns + Sh::COLS - 1) / Sh::COLS * (long long)a.c.kv_heads, runs = a.c.rows * per;
+  const long long room = (places + TILE - 1) / TILE, most = (START + (room > 1 ? room : 1)) * runs;
+  if (runs > 0x7fffffffLL) return -2;
+  const Workspace w = workspace(a.c.rows, a.c.kv_heads, columns, D, places, a.weights != nullptr);
+  if (w.all > 0 && !a.partial) return -1;
+  float* const space = a.partial;
+  a.owners = reinterpret_cast<int2*>(space + w.owners);
+  a.lse2 = a.weights ? space + w.lse2 : nullptr;
+  a.scores = a.weights ? space + w.scores : nullptr;
+  a.ctas = w.ctas;
+  CUtensorMap map;
+  if (!make_tmap_halves<D>(&map, a.c.data, std::is_same<T, __half>::value, ((long long)a.c.pages * 2 * a.c.kv_heads) << a.c.page_shift)) return -3;
+  const long long grid = most < 148 * Sh::BLOCKS ? most : 148 * Sh::BLOCKS;
+  int rc = launched(launch_after(kv_attention_kernel<T, D, NT>, dim3((unsigned)(w.cut || runs > grid ? grid : runs)), WARPS * 32, SMEM, st, 1,
+                                 map, a));
+  if (rc == 0 && w.cut) rc = launched(launch_after(kv_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per));
   if (rc != 0 || !a.weights) return rc;
-  return launched(launch_after(kv_weights_kernel<T, D>, dim3(64, a.c.rows * a.c.kv_heads), 128, 0, st, 1, a));
+  const long long heads = (long long)a.c.rows * a.c.kv_heads;
+  if (heads > 65535) return -2;
+  const int lanes = columns <= 4 ? 1 : 8, each = 256 / lanes;
+  const long long chunks = (places + each - 1) / each, enough = 148 * 8 / heads + 1;
+  const dim3 blocks((unsigned)(chunks < enough ? chunks : enough), (unsigned)heads);
+  return launched(lanes == 1 ? launch_after(kv_weights_kernel<1>, blocks, 256, 0, st, 1, a) : launch_after(kv_weights_kernel<8>, blocks, 256, 0, st, 1, a));
 }
 
 template <typename T, int D>
@@ -353,7 +876,7 @@ extern "C" int atb_kv_append(const void* qkv, void* q, void* k, void* data, cons
 
 // Floats of the workspace of atb_kv_attention.
 extern "C" long long atb_kv_attention_scratch(int rows, int heads, int kv_heads, int S, int head_dim, int places, int weighed) {
-  return weighed ? (long long)rows * heads * S : 0;
+  return workspace(rows, kv_heads, heads / kv_heads * S, head_dim, places, weighed != 0).all;
 }
 
 extern "C" int atb_kv_attention(const void* q, void* out, void* lse, void* data, const void* table, const void* lengths, void* weights,
@@ -377,7 +900,11 @@ extern "C" int atb_kv_attention(const void* q, void* out, void* lse, void* data,
   a.group = heads / kv_heads;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.status = (int*)status;
-#define ATTN(T, D) return launch_attention<T, D>(a, (cudaStream_t)stream)
+  const int tiles = column_tiles_of_8(S * a.group);
+#define ATTN(T, D)                                                                 \
+  return tiles == 1   ? launch_attention<T, D, 1>(a, (cudaStream_t)stream)         \
+         : tiles == 2 ? launch_attention<T, D, 2>(a, (cudaStream_t)stream)         \
+                      : launch_attention<T, D, 4>(a, (cudaStream_t)stream)
   ATB_KV_TYPES(ATTN)
 #undef ATTN
   return -1;
