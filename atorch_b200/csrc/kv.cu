@@ -2,11 +2,13 @@
 //
 // One layer's cache is T [pages][2][kv heads][page size][D]: 0: keys, 1: values.
 #include <atomic>
+#include <cooperative_groups.h>
 #include <type_traits>
 #include "paged.cuh"
 
 namespace {
 using namespace atb;
+namespace cg = cooperative_groups;
 
 struct Cache : Paging {
   void* data;
@@ -640,7 +642,9 @@ struct EvictArgs {
   const int* lengths;
   float* weights;
   int* out;
-  int* index;                 // [units][budget + 1]
+  int* first;                 // [units] the first place whose token changes, `budget` where none does
+  int* source;                // [units][budget] place in the pool (page, slot) of the token that a place takes
+  float* kept;                // [units][budget] its weight
   long long places, layer_elements;
   int budget, recent, layers;
   int* status;
@@ -650,7 +654,8 @@ ATB_DEVICE uint32_t rank_of(float f) {
   const uint32_t u = __float_as_uint((f != f ? -INFINITY : f) + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-ATB_DEVICE int block_exclusive(int v, int* red, int* total) {
+// Sum of v over the threads before this one, and over all; `red` is a shared int[32].
+ATB_DEVICE int block_before(int v, int* red, int& all) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int sum = v;
 #pragma unroll
@@ -661,92 +666,235 @@ ATB_DEVICE int block_exclusive(int v, int* red, int* total) {
   __syncthreads();
   if (lane == 31) red[w] = sum;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int i = 0; i < warps; ++i) {
-    if (i < w) before += red[i];
-    all += red[i];
+  const int x = lane < warps ? red[lane] : 0;
+  int up = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, up, o);
+    if (lane >= o) up += y;
   }
-  *total = all;
-  return before + sum - v;
+  all = __shfl_sync(0xffffffffu, up, 31);
+  return __shfl_sync(0xffffffffu, up - x, w) + sum - v;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv_evict_kernel(EvictArgs a) {
-  __shared__ int hist[256], red[8], sh_digit, sh_left;
+// What a unit (a key/value head of a sequence in a layer) keeps: the blocks of a cluster have a share of its places each. The
+// least rank that is kept is found digit by digit, 11, 11 and 10 bits, from counts that the blocks read from each other's shared memory;
+// of the places of that rank the lowest are kept. Then the places that are kept are numbered in their order: that number is where the
+// token goes. Weights are moved through the workspace, so that no block writes what another still reads.
+constexpr int SELECT = 512, BINS = 2048, EACH = 4;
+__global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room) {
+  extern __shared__ float sh_w[];                 // `room` weights of the share; the others are read again
+  __shared__ int hist[2][BINS], red[32], sh_digit, sh_above, sh_counts[2], sh_least, sh_failed;
+  cg::cluster_group cluster = cg::this_cluster();
   grid_go();
   grid_wait();
-  if (__syncthreads_or(*a.status != 0)) return;
-  Cache c = a.c;
-  const int head = blockIdx.x % c.kv_heads, b = blockIdx.x / c.kv_heads % c.rows, layer = blockIdx.x / c.kv_heads / c.rows;
-  c.data = (T*)c.data + layer * a.layer_elements;
-  const int len = seen_length(c, a.lengths, b, a.status);
-  if (layer == 0 && head == 0 && threadIdx.x == 0) a.out[b] = min(a.lengths[b], a.budget);
-  if (len <= a.budget) return;
-  bool good = true;
-  for (int i = threadIdx.x; i << c.page_shift < len; i += 256) good = good && page_of(c, b, i << c.page_shift) >= 0;
-  if (__syncthreads_or(!good)) {
-    if (threadIdx.x == 0) atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+  const Cache& c = a.c;
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const long long unit = blockIdx.x / blocks;
+  const int b = (int)(unit / c.kv_heads % c.rows);
+  const int len = seen_length(c, a.lengths, b, a.status), lane = threadIdx.x & 31;
+  const bool leader = rank == 0 && threadIdx.x == 0;
+  if (leader && unit < (long long)c.rows * c.kv_heads && unit % c.kv_heads == 0) a.out[b] = min(a.lengths[b], a.budget);
+  if (len <= a.budget) {
+    if (leader) a.first[unit] = a.budget;
     return;
   }
-  float* const w = a.weights + (long long)blockIdx.x * a.places;
-  int* const index = a.index + (long long)blockIdx.x * (a.budget + 1);
-  const int n = len - a.recent;
-  int left = a.budget - a.recent;            // of rank `rank`, so many go with the higher ones
-  uint32_t rank = 0;
-  if (left == 0) rank = 0xffffffffu;
-  for (int shift = 24; shift >= 0 && left > 0; shift -= 8) {
-    hist[threadIdx.x] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += 256) {
-      const uint32_t r = rank_of(w[i]);
-      if (shift == 24 || (r >> (shift + 8)) == (rank >> (shift + 8))) atomicAdd(&hist[r >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      int d = 255, k = left;
-      for (; d > 0 && hist[d] < k; --d) k -= hist[d];
-      sh_digit = d;
-      sh_left = k;
-    }
-    __syncthreads();
-    rank |= (uint32_t)sh_digit << shift;
-    left = sh_left;
+  const int part = (((len + blocks - 1) / blocks + 3) & ~3), from = min(len, rank * part), to = min(len, from + part);
+  float* const w = a.weights + unit * a.places;
+  bool bad = false;
+  for (int i = (from >> c.page_shift) + threadIdx.x; i << c.page_shift < to; i += SELECT) bad = bad || page_of(c, b, i << c.page_shift) < 0;
+  const int held = min(to - from, room);
+#pragma unroll 8
+  for (int i = threadIdx.x; i < held; i += SELECT) sh_w[i] = w[from + i];
+  for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = hist[1][i] = 0;
+  if (threadIdx.x == 0) {
+    sh_least = len;
+    sh_failed = *a.status;
   }
-  int kept = 0, ties = 0;
-  for (int i0 = 0; i0 < len; i0 += 256) {
-    const int i = i0 + threadIdx.x;
-    const float f = i < len ? w[i] : 0.f;
-    const uint32_t r = rank_of(f);
-    int all_ties, all_kept;
-    const bool tie = i < n && r == rank;
-    const int tie_before = ties + block_exclusive(tie, red, &all_ties);
-    const bool keep = i < len && (i >= n || r > rank || (tie && tie_before < left));
-    const int at = kept + block_exclusive(keep, red, &all_kept);
-    ties += all_ties;
-    kept += all_kept;
-    __syncthreads();
-    if (keep) {
-      index[at] = i;
-      w[at] = f;
-    }
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0 && bad) {
+    atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+    sh_failed = 1;
   }
-  __syncthreads();
-  for (int i = a.budget + threadIdx.x; i < len; i += 256) w[i] = 0.f;
-  constexpr int L = D / 8, EACH = 256 / L;
-  const int l = threadIdx.x % L, mask = (1 << c.page_shift) - 1;
-  for (int j0 = 0; j0 < a.budget; j0 += EACH) {
-    const int j = j0 + threadIdx.x / L;
-    uint4 x[2];
-    if (j < a.budget) {
-      const int src = index[j], page = page_of(c, b, src);
-      for (int i = 0; i < 2; ++i) x[i] = *reinterpret_cast<const uint4*>(row_at<T, D>(c, page, i, head, src & mask) + l * 8);
+  auto weight = [&](int i) { return i - from < held ? sh_w[i - from] : w[i]; };
+
+  const int n = len - a.recent, mine = min(to, n);      // those from n on stay
+  int left = a.budget - a.recent;            // of rank `least`, so many are kept
+  uint32_t least = left == 0 ? 0xffffffffu : 0u;
+  bool failed = false;
+#pragma unroll 1
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+    int* const h = hist[pass & 1];
+    if (left > 0) {
+#pragma unroll 4
+      for (int i0 = from; i0 < mine; i0 += SELECT) {
+        const int i = i0 + threadIdx.x;
+        const uint32_t r = i < mine ? rank_of(weight(i)) : 0u;
+        const bool in = i < mine && (pass == 0 || (r ^ least) >> (shift + bits) == 0);
+        const int bin = in ? r >> shift & ((1 << bits) - 1) : -1;
+        int same;
+        __match_all_sync(0xffffffffu, bin, &same);       // (many weights alike would wait for one another)
+        if (!same) {
+          if (in) atomicAdd(&h[bin], 1);
+        } else if (in && lane == 0) {
+          atomicAdd(&h[bin], 32);
+        }
+      }
+    }
+    cluster.sync();
+    if (pass == 0)
+      for (int i = 0; i < blocks; ++i) failed = failed || *cluster.map_shared_rank(&sh_failed, i) != 0;
+    if (pass == 1)                           // the first pass's counts have been read by all
+      for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = 0;
+    if (left > 0 && !failed) {
+      // from the highest bin down: four of a thread
+      int count[EACH], sum = 0;
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) count[e] = 0;
+      const int top = BINS - 1 - EACH * (int)threadIdx.x;
+#pragma unroll 4
+      for (int i = 0; i < blocks; ++i) {
+        const int4 v = *reinterpret_cast<const int4*>(cluster.map_shared_rank(h, i) + top - 3);
+        count[0] += v.w;
+        count[1] += v.z;
+        count[2] += v.y;
+        count[3] += v.x;
+      }
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) sum += count[e];
+      int all, above = block_before(sum, red, all);
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        if (above < left && above + count[e] >= left) {
+          sh_digit = top - e;
+          sh_above = above;
+        }
+        above += count[e];
+      }
+      __syncthreads();
+      least |= (uint32_t)sh_digit << shift;
+      left -= sh_above;
     }
     __syncthreads();
-    if (j < a.budget) {
-      const int page = page_of(c, b, j);
-      for (int i = 0; i < 2; ++i) *reinterpret_cast<uint4*>(row_at<T, D>(c, page, i, head, j & mask) + l * 8) = x[i];
+  }
+  // places above and at the border, before the share
+  int above = 0, ties = 0;
+#pragma unroll 4
+  for (int i = from + threadIdx.x; i < to; i += SELECT) {
+    const uint32_t r = rank_of(weight(i));
+    above += i >= n || r > least;
+    ties += i < n && r == least;
+  }
+  int all;
+  block_before(above, red, all);
+  if (threadIdx.x == 0) sh_counts[0] = all;
+  block_before(ties, red, all);
+  if (threadIdx.x == 0) sh_counts[1] = all;
+  cluster.sync();
+  int above_before = 0, ties_before = 0;
+  for (int i = 0; i < rank; ++i) {
+    above_before += cluster.map_shared_rank(sh_counts, i)[0];
+    ties_before += cluster.map_shared_rank(sh_counts, i)[1];
+  }
+  if (!failed) {
+    int* const source = a.source + unit * a.budget;
+    float* const kept = a.kept + unit * a.budget;
+    int first = len;
+    for (int i0 = from; i0 < to; i0 += SELECT * EACH) {
+      const int i1 = i0 + threadIdx.x * EACH;
+      float f[EACH];
+      int count = 0;                        // above in the low half, ties in the high one
+      bool is_above[EACH], is_tie[EACH];
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = i1 + e;
+        f[e] = i < to ? weight(i) : 0.f;
+        const uint32_t r = rank_of(f[e]);
+        is_above[e] = i < to && (i >= n || r > least);
+        is_tie[e] = i < to && i < n && r == least;
+        count += is_above[e] + (is_tie[e] << 16);
+      }
+      const int before = block_before(count, red, all);
+      int g = above_before + (before & 0xffff), t = ties_before + (before >> 16);
+      const int page = i1 < to ? page_of(c, b, i1) : 0;       // (pages have a multiple of EACH places)
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int i = i1 + e;
+        if (is_above[e] || (is_tie[e] && t < left)) {
+          const int at = g + min(t, left);
+          source[at] = (page << c.page_shift) + (i & ((1 << c.page_shift) - 1));
+          kept[at] = f[e];
+        } else if (i < to) {
+          first = min(first, i);
+        }
+        g += is_above[e];
+        t += is_tie[e];
+      }
+      above_before += all & 0xffff;
+      ties_before += all >> 16;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    if (lane == 0) atomicMin(&sh_least, first);
+  }
+  cluster.sync();
+  if (leader) {
+    int first = len;
+    for (int i = 0; i < blocks; ++i) first = min(first, *cluster.map_shared_rank(&sh_least, i));
+    a.first[unit] = failed ? a.budget : min(first, a.budget);
+  }
+  if (!failed)
+    for (int i = from + threadIdx.x; i < to; i += SELECT) w[i] = i < a.budget ? a.kept[unit * a.budget + i] : 0.f;
+  cluster.sync();                                // the first has read the others' words
+}
+
+// The tokens' move: a block has the keys or the values of a unit, or a slab of their dims where there are few units, and takes places in
+// their order, PER rows a thread at a time. A token only moves down, so what a place's token comes from is not written before that place's
+// turn: the reads of a round end before its writes begin, and those of the next round may come before either.
+template <int D, int THREADS, int PER>
+__global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a, int slabs) {
+  grid_go();
+  grid_wait();
+  const Cache& c = a.c;
+  const int slab = blockIdx.x % slabs, which = blockIdx.x / slabs & 1;
+  const long long unit = blockIdx.x / slabs / 2;
+  const int first = a.first[unit];
+  if (first >= a.budget) return;           // (also of a unit that could not be selected from; its weights stay, too)
+  const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
+  const int lanes = D / 8 / slabs, rows = THREADS / lanes;
+  uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + slab * lanes + threadIdx.x % lanes;
+  const int* const source = a.source + unit * a.budget;
+  const int* const row = c.table + b * c.table_stride;
+  auto at = [&](int page, int slot) -> uint4* { return data + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * (D / 8); };
+  uint4 x[2][PER];
+  auto load = [&](uint4 (&y)[PER], int j0) {
+    int src[PER];
+#pragma unroll
+    for (int k = 0; k < PER; ++k) src[k] = j0 + k * rows < a.budget ? source[j0 + k * rows] : -1;
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (src[k] >= 0) y[k] = *at(src[k] >> c.page_shift, src[k] & mask);
+  };
+  auto store = [&](const uint4 (&y)[PER], int j0) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int j = j0 + k * rows;
+      if (j < a.budget) *at(row[j >> c.page_shift], j & mask) = y[k];
+    }
+  };
+  int j0 = first + threadIdx.x / lanes;
+  const int step = rows * PER, end = a.budget + threadIdx.x / lanes;      // the same number of rounds for all threads
+  load(x[0], j0);
+  for (;; j0 += 2 * step) {
     __syncthreads();
+    load(x[1], j0 + step);
+    store(x[0], j0);
+    if (j0 + step >= end) break;
+    __syncthreads();
+    load(x[0], j0 + 2 * step);
+    store(x[1], j0 + step);
+    if (j0 + 2 * step >= end) break;
   }
 }
 
@@ -846,11 +994,32 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   return launched(lanes == 1 ? launch_after(kv_weights_kernel<1>, blocks, 256, 0, st, 1, a) : launch_after(kv_weights_kernel<8>, blocks, 256, 0, st, 1, a));
 }
 
-template <typename T, int D>
+template <int D>
 int launch_evict(const EvictArgs& a, cudaStream_t st) {
-  const long long units = (long long)a.layers * a.c.rows * a.c.kv_heads;
-  if (units > 0x7fffffffLL) return -2;
-  return launched(launch_after(kv_evict_kernel<T, D>, dim3((unsigned)units), 256, 0, st, 1, a));
+  const long long units = (long long)a.layers * a.c.rows * a.c.kv_heads, places = (long long)a.c.width << a.c.page_shift;
+  // a cluster where the GPU has room for it and its blocks have 2048 places each
+  int blocks = 1;
+  while (blocks < 8 && units * blocks * 2 <= 148 && places > 2048LL * blocks) blocks *= 2;
+  constexpr int LARGEST = 16384;
+  const long long share = (places + blocks - 1) / blocks + 4;
+  const int room = (int)(share < LARGEST ? share : LARGEST);
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return launched(cudaErrorInvalidDevice);
+  const unsigned long long bit = 1ull << (device & 63);
+  if (!(allowed.load(std::memory_order_relaxed) & bit)) {
+    const int rc = launched(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LARGEST * 4));
+    if (rc != 0) return rc;
+    allowed.fetch_or(bit, std::memory_order_relaxed);
+  }
+  int slabs = 1;
+  while (slabs < D / 16 && units * 2 * slabs < 148) slabs *= 2;       // rows in pieces of 32 bytes at least
+  if (units * 2 * slabs > 0x7fffffffLL) return -2;
+  const int rc = launched(launch_after(kv_select_kernel, dim3((unsigned)(units * blocks)), SELECT, room * 4, st, blocks, a, room));
+  if (rc != 0) return rc;
+  const unsigned grid = (unsigned)(units * 2 * slabs);
+  return launched(grid < 148 * 2 ? launch_after(kv_move_kernel<D, 1024, 4>, dim3(grid), 1024, 0, st, 1, a, slabs)
+                                 : launch_after(kv_move_kernel<D, 256, 8>, dim3(grid), 256, 0, st, 1, a, slabs));
 }
 }  // namespace
 
@@ -910,7 +1079,7 @@ extern "C" int atb_kv_attention(const void* q, void* out, void* lse, void* data,
   return -1;
 }
 
-extern "C" int atb_kv_evict(void* data, const void* table, const void* lengths, void* weights, void* out, void* index, int layers,
+extern "C" int atb_kv_evict(void* data, const void* table, const void* lengths, void* weights, void* out, void* work, int layers,
                             int kv_heads, int head_dim, int page_shift, int pages, int rows, int width, long long table_stride,
                             long long places, int budget, int recent, void* stream, void* status) {
   if (rows <= 0) return 0;
@@ -919,14 +1088,17 @@ extern "C" int atb_kv_evict(void* data, const void* table, const void* lengths, 
   a.lengths = (const int*)lengths;
   a.weights = (float*)weights;
   a.out = (int*)out;
-  a.index = (int*)index;
+  const long long units = (long long)layers * rows * kv_heads;
+  a.first = (int*)work;
+  a.source = a.first + units;
+  a.kept = (float*)(a.source + units * budget);
   a.places = places;
   a.layer_elements = ((long long)pages * 2 * kv_heads << page_shift) * head_dim;
   a.budget = budget;
   a.recent = recent;
   a.layers = layers;
   a.status = (int*)status;
-  if (head_dim == 64) return launch_evict<__half, 64>(a, (cudaStream_t)stream);      // (16 bits are moved as they are)
-  if (head_dim == 128) return launch_evict<__half, 128>(a, (cudaStream_t)stream);
+  if (head_dim == 64) return launch_evict<64>(a, (cudaStream_t)stream);
+  if (head_dim == 128) return launch_evict<128>(a, (cudaStream_t)stream);
   return -1;
 }

@@ -299,8 +299,9 @@ def kv_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tenso
     out = torch.empty_like(lengths)
     if budget >= most << shift:              # no row of the page table has so many places
         return out.copy_(lengths)
-    index = torch.empty(layers * rows * KV * (budget + 1), dtype=torch.int32, device=lengths.device)
-    rc = _lib.lib().atb_kv_evict(at, table, lengths.data_ptr(), weights.data_ptr(), out.data_ptr(), index.data_ptr(), layers, KV, D, shift,
+    # per layer, sequence and head: the first place that changes, where the tokens come from, their weights
+    work = torch.empty(layers * rows * KV * (2 * budget + 1), dtype=torch.int32, device=lengths.device)
+    rc = _lib.lib().atb_kv_evict(at, table, lengths.data_ptr(), weights.data_ptr(), out.data_ptr(), work.data_ptr(), layers, KV, D, shift,
                                  pages, rows, most, stride, places, budget, recent, _lib.stream_of(dev), _lib.status_addr(weights))
     _lib.check(rc, "atb_kv_evict")
     return out
