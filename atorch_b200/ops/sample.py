@@ -13,7 +13,7 @@ from .. import _lib
 from .function import refuse_gradient
 
 Number = Union[float, int, torch.Tensor]
-MOST = 1 << 27          # tokens of a vocabulary
+MOST = 1 << 19          # tokens of a vocabulary that the kernel takes
 
 
 def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -93,7 +93,7 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
         raise ValueError(f"logits are bf16, fp16 or fp32 [B, vocabulary], got {logits.dtype} {tuple(logits.shape)}")
     B, V = logits.shape
     if V > MOST:
-        raise ValueError(f"a vocabulary of {V}: 2 ** 27 at most")
+        raise ValueError(f"a vocabulary of {V}: 2 ** 19 at most")
     if waiting.dtype is not torch.float32 or waiting.shape != (B, V):
         raise ValueError(f"waiting is fp32 {(B, V)}, got {waiting.dtype} {tuple(waiting.shape)}")
     dev = logits.get_device()
