@@ -28,7 +28,7 @@ def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p
     top = x.amax(-1, keepdim=True)
     best = (x == top).double().argmax(-1, keepdim=True)                    # the lowest of the largest
     below = torch.where(x == top, torch.zeros_like(x), x - top)
-    w = torch.where(x > -math.inf, torch.exp(below / T), torch.zeros_like(x))
+    w = torch.where((x > -math.inf) & (below > -math.inf), torch.exp(below / T), torch.zeros_like(x))
     at = torch.arange(V, device=x.device).expand_as(x)
     w = torch.where(T > 0, w, ((at == best) & (top > -math.inf)).double())
     order = x.sort(dim=-1, descending=True, stable=True).indices
@@ -99,7 +99,7 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
     dev = logits.get_device()
     if waiting.get_device() != dev:
         raise ValueError("logits and waiting are on several devices")
-    t_rows, t = _number("temperature", temperature, B, dev, False, 0.0, 3.0e38)
+    t_rows, t = _number("temperature", temperature, B, dev, False, 0.0, math.inf)
     k_rows, k = _number("top_k", top_k, B, dev, True, 0, float(1 << 62))
     p_rows, p = _number("top_p", top_p, B, dev, False, 0.0, 1.0)
     m_rows, m = _number("min_p", min_p, B, dev, False, 0.0, 1.0)
