@@ -28,9 +28,9 @@ def test_with_a_budget(dtype, monkeypatch):
 def test_sampling_filters():
     m = model("cuda", **SHAPE)
     ids = prompts(m, (6, 6, 6, 6))
-    greedy = Generator(m).generate(ids, 8)
-    for kw in (dict(top_k=1), dict(top_p=1e-6), dict(min_p=1.0)):
-        for a, b in zip(greedy, Generator(m).generate(ids, 8, temperature=1.5, **kw)):
+    first = Generator(m).generate(ids, 8, temperature=1.5, top_k=1)
+    for kw in (dict(top_p=1e-6), dict(top_k=7, top_p=0.0), dict(top_k=1, min_p=1.0)):       # of equal logits the lowest index
+        for a, b in zip(first, Generator(m).generate(ids, 8, temperature=0.5, **kw)):
             assert torch.equal(a, b)
     torch.manual_seed(3)
     whole = Generator(m).generate(ids, 8, temperature=1.0)
