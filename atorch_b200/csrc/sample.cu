@@ -10,9 +10,10 @@ namespace {
 using namespace atb;
 namespace cg = cooperative_groups;
 
-// Threads of a block; bins of a factor of 2 in weight, the last for all that is less; tokens of which one block finds the end of the
-// prefix; bins of a step towards it where there are more
-constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 20, ROOM = 2048, SUB = 512;
+// Threads of a block; bins of a factor of 2 in weight, the last for all that is less; tokens that one block draws from; tokens that it
+// puts in order by counting; parts of a step towards the end of the prefix where there are more
+constexpr int THREADS = 512, WARPS = THREADS / 32, BINS = 20, ROOM = 4096, FEW = 256, SUB = 512;
+constexpr double DOUBT = 1. / (1 << 24);         // of a row's weight: how near to a border sums in 32 bits are not trusted
 constexpr float NOTHING = 1075.f;       // powers of two below the largest weight from which on a weight is 0 in 64 bits
 
 struct Args {
@@ -92,9 +93,9 @@ struct Shared {
   double above, inside;                          // of those above the bin at hand, and in it
   unsigned long long low, high, least_above;     // keys of the bin at hand, and the least above it
   unsigned count[BINS], weight[BINS];            // tokens of a bin, their weights in units of 2^-14 of the bin's largest
-  unsigned sub_count[SUB], sub_low[SUB], sub_high[SUB];
-  int listed;
-  unsigned long long cut;
+  int listed, few_listed;
+  double margin;                                 // how near the target comes to where the prefix might end otherwise
+  unsigned long long few[FEW], cut;
   unsigned long long best_score;                 // fp64 bits
   int best_at;
 };
@@ -103,15 +104,20 @@ struct Shared {
 //
 // The end of the prefix is looked for in this order: a histogram of tokens and weights over the powers of two below the largest weight, where
 // every thread has bins of its own; if no more than ROOM tokens lie in the bins down to the one where the prefix ends, the first block
-// lists and sorts them, finds the end from exact sums in 64 bits, and draws. If there are more, the bin is divided into SUB parts by
-// the tokens' place in the order, the one with the end again, until few enough are left, and every block draws from its share.
-// Weights that are added up are whole numbers (in units below 2^-30 of a bin's largest) or summed in one order, so the result does not depend on
-// which thread comes first. A draw is decided in 64 bits: 32-bit arrival times only say which tokens have to be looked at.
+// lists them, finds the end, and draws. If there are more, all blocks look for the end in that bin, and every block draws from its share.
+// Looking for the end: a few tokens are put in order and added up in 64 bits; of more, the keys' range is divided into SUB parts, and the
+// part with the end again. Weights that several threads add up are whole numbers (2^-46 of the largest of the range), others are
+// summed in one order, so the result does not depend on which thread comes first. Sums of thousands of weights in 32 bits are off by some
+// 2^-26; where that might decide where the prefix ends, they are formed again in 64 bits. A draw is decided in 64 bits: 32-bit arrival
+// times only say which tokens have to be looked at.
 template <typename T, int P>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
-  // [BINS][THREADS]: weights in the low 22 bits, tokens above; then the list of keys
+  // [BINS][THREADS]: weights in the low 22 bits, tokens above; then the list of keys, and behind it [4][SUB]: tokens of a part, its
+  // weights in three limbs of 16 bits
   extern __shared__ __align__(16) unsigned own_bins[];
   unsigned long long* const list = reinterpret_cast<unsigned long long*>(own_bins);
+  unsigned* const parts = own_bins + 2 * ROOM;
+  static_assert(ROOM * 8 + 4 * SUB * 4 <= BINS * THREADS * 4, "they lie in the place of the bins");
   __shared__ Shared sh;
   __shared__ double red_d[32];
   __shared__ int red_i[32];
@@ -120,6 +126,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   grid_go();
   grid_wait();
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), lane = threadIdx.x & 31;
+  const bool leader = rank == 0;
   const long long row = blockIdx.x / blocks;
   const T* const x = (const T*)a.logits + row * a.stride;
   const float* const wait = a.waiting + row * a.wait_stride;
@@ -132,15 +139,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
                }, [&](float v, int i) { f(fmaxf(v, -INFINITY), i); });
   };
   auto again = [&](auto f) {                     // the same from memory, for what happens seldom
+    const bool wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    const int pieces = wide ? (to - from) / Piece<T>::N : 0;
 #pragma unroll 1
-    for (int i0 = from + (int)threadIdx.x * 4; i0 < to; i0 += THREADS * 4)
+    for (int k = threadIdx.x; k < pieces; k += THREADS) {
+      const Piece<T> v{reinterpret_cast<const uint4*>(x + from)[k]};
+#pragma unroll
+      for (int e = 0; e < Piece<T>::N; ++e) f(fmaxf(v[e], -INFINITY), from + k * Piece<T>::N + e);
+    }
 #pragma unroll 1
-      for (int i = i0; i < min(i0 + 4, to); ++i) f(fmaxf(to_f32<T>(x[i]), -INFINITY), i);
+    for (int i = from + pieces * Piece<T>::N + threadIdx.x; i < to; i += THREADS) f(fmaxf(to_f32<T>(x[i]), -INFINITY), i);
   };
   const double temp = a.t_rows ? a.t_rows[row] : a.t, p = a.p_rows ? a.p_rows[row] : a.p, m = a.m_rows ? a.m_rows[row] : a.m;
   int k = a.k_rows ? a.k_rows[row] : a.k;
   if (k < 0 || k >= a.V) k = 0;
-  const bool failed = *a.status != 0;
+  const bool failed = *a.status != 0, by_weight = p < 1., unfiltered = k == 0 && !by_weight && !(m > 0.);
+  if (unfiltered)                                // every waiting time is read: on their way to L2 under the look for the largest logit
+    for (int i = from + (int)threadIdx.x * 32; i < to; i += THREADS * 32)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(__cvta_generic_to_global(wait + i)));
 
   // the largest logit
   float top = -INFINITY;
@@ -153,7 +169,6 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   }
   cluster.sync();
   for (int i = 0; i < blocks; ++i) top = fmaxf(top, cluster.map_shared_rank(&sh, i)->top);
-  const bool leader = rank == 0;
   auto answer = [&](int token, double logprob) {
     a.tokens[row] = failed ? 0 : token;
     a.logprobs[row] = failed ? -INFINITY : (float)logprob;
@@ -161,8 +176,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   if (top == -INFINITY || !(temp > 0.)) {
     int first = a.V;
     if (top > -INFINITY) again([&](float v, int i) { if (v == top) first = min(first, i); });
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) atomicMin(&sh.first, first);
     cluster.sync();
     if (leader && threadIdx.x == 0) {
@@ -175,10 +189,125 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
   }
   const double c = fmin(1.4426950408889634 / temp, 1e38);
   const Scale scale{top, (float)c, (float)(c - (double)(float)c), temp};
+  auto block_min = [&](int v) {
+    v = __reduce_min_sync(0xffffffffu, v);
+    __syncthreads();
+    if (lane == 0) red_i[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return __reduce_min_sync(0xffffffffu, red_i[lane & (WARPS - 1)]);
+  };
+
+  // The end of the prefix among the keys that `keys(f)` calls f(key) with, those in [low, high]: the least key whose predecessors are fewer
+  // than `target` tokens (by count), or weigh less. `before` come in front of them. With LOCAL the first block alone has them all.
+  double margin = 0.;
+  auto end_of_prefix = [&](auto local, auto keys, unsigned long long low, unsigned long long high, int n, bool count, double target, double before) {
+    constexpr bool LOCAL = decltype(local)::value;
+    const int members = LOCAL ? 1 : blocks;
+    auto meet = [&] {
+      if constexpr (LOCAL) __syncthreads();
+      else cluster.sync();
+    };
+    auto of = [&](int i) -> Shared* {
+      if constexpr (LOCAL) return &sh;
+      else return cluster.map_shared_rank(&sh, i);
+    };
+    while (n > FEW && low != high) {
+      const int shift = max(0, 64 - __clzll(high - low) - 9);      // SUB parts at most
+      const int up = 46 + min((int)scale.power(value_of(high)), 900);
+      const double unit = ldexp(1., -up), per = ldexp(1., up);
+      for (int i = threadIdx.x; i < 4 * SUB; i += THREADS) parts[i] = 0;
+      __syncthreads();
+      keys([&](unsigned long long key) {
+        if (key < low || key > high) return;
+        const int s = (int)((high - key) >> shift);
+        atomicAdd(parts + s, 1u);
+        if (count) return;
+        const unsigned long long q = (unsigned long long)(scale.exact(value_of(key)) * per);
+        atomicAdd(parts + 1 * SUB + s, (unsigned)q & 0xffffu);
+        atomicAdd(parts + 2 * SUB + s, (unsigned)(q >> 16) & 0xffffu);
+        atomicAdd(parts + 3 * SUB + s, (unsigned)(q >> 32));
+      });
+      meet();
+      static_assert(SUB == THREADS, "a thread has one part");
+      unsigned mine_n = 0;
+      unsigned long long mine_w = 0;
+      for (int i = 0; i < members; ++i) {
+        const unsigned* s = parts;
+        if constexpr (!LOCAL) s = cluster.map_shared_rank(parts, i);
+        mine_n += s[threadIdx.x];
+        if (!count)
+          mine_w += s[SUB + threadIdx.x] + ((unsigned long long)s[2 * SUB + threadIdx.x] << 16) + ((unsigned long long)s[3 * SUB + threadIdx.x] << 32);
+      }
+      double all;
+      const double mine = count ? (double)mine_n : (double)mine_w * unit, till = block_before(mine, red_d, all) + before;
+      // the first part at whose end the target is reached, or the last that has tokens
+      int hit = block_min(mine_n > 0 && till + mine >= target ? (int)threadIdx.x : SUB);
+      if (hit == SUB) hit = -block_min(mine_n > 0 ? -(int)threadIdx.x : 1);
+      __syncthreads();
+      if ((int)threadIdx.x == hit) {
+        red_d[0] = till;
+        red_i[0] = (int)mine_n;
+      }
+      meet();                                    // (the parts have been read by all)
+      before = red_d[0];
+      n = red_i[0];
+      const unsigned long long top_key = high - ((unsigned long long)max(hit, 0) << shift), width = (1ull << shift) - 1;
+      low = top_key - low > width ? top_key - width : low;
+      high = top_key;
+      __syncthreads();
+    }
+    // few: in their order, by counting those before each
+    if (threadIdx.x == 0) sh.few_listed = 0;
+    __syncthreads();
+    keys([&](unsigned long long key) {
+      if (key < low || key > high) return;
+      const int at = atomicAdd(&sh.few_listed, 1);
+      if (at < FEW) sh.few[at] = key;
+    });
+    meet();
+    if (leader) {
+      n = min(sh.few_listed, FEW);
+      for (int r = 1; r < members; ++r) {
+        const Shared* s = of(r);
+        const int more = s->few_listed;
+        __syncthreads();
+        for (int i = threadIdx.x; i < more && n + i < FEW; i += THREADS) sh.few[n + i] = s->few[i];
+        n = min(n + more, FEW);
+      }
+      __syncthreads();
+      const unsigned long long key = (int)threadIdx.x < n ? sh.few[threadIdx.x] : 0;
+      int place = n;
+      if ((int)threadIdx.x < n) {
+        place = 0;
+#pragma unroll 4
+        for (int i = 0; i < n; ++i) place += sh.few[i] > key;
+      }
+      __syncthreads();
+      if ((int)threadIdx.x < n) sh.few[place] = key;
+      __syncthreads();
+      double all;
+      const double w = (int)threadIdx.x >= n ? 0. : count ? 1. : scale.exact(value_of(sh.few[threadIdx.x]));
+      const double till = block_before(w, red_d, all) + before;
+      const int left = block_min((int)threadIdx.x < n && till >= target ? (int)threadIdx.x : n);
+      if (threadIdx.x == 0) {
+        sh.cut = sh.few[max(left, 1) - 1];
+        sh.margin = INFINITY;
+      }
+      __syncthreads();
+      // (the ends of the token before and of that one: their distances as the bits of numbers that are not negative)
+      if ((int)threadIdx.x < n && ((int)threadIdx.x == left || (int)threadIdx.x == left - 1))
+        atomicMin(reinterpret_cast<unsigned long long*>(&sh.margin),
+                  (unsigned long long)__double_as_longlong(fmin(fabs(till - target), fabs(till + w - target))));
+    }
+    meet();
+    const unsigned long long cut = of(0)->cut;
+    margin = of(0)->margin;
+    meet();
+    return cut;
+  };
 
   unsigned long long cut = 0;                    // tokens with keys of at least this are left
-  const bool by_count = k > 0, by_weight = p < 1.;
-  if (by_count || by_weight) {
+  if (k > 0 || by_weight) {
     // one look at the row: tokens and weights of the bins, and all weights; a token without weight does not count
     for (int i = 0; i < BINS; ++i) own_bins[i * THREADS + threadIdx.x] = 0;
     float sum = 0.f;
@@ -195,8 +324,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     if (threadIdx.x == 0) sh.sum = total_own;
     for (int bin = threadIdx.x >> 5; bin < BINS; bin += WARPS) {
       unsigned n = 0, w = 0;
-      for (int i = lane; i < THREADS; i += 32) {
-        const unsigned u = own_bins[bin * THREADS + i];
+#pragma unroll
+      for (int i = 0; i < THREADS; i += 32) {
+        const unsigned u = own_bins[bin * THREADS + i + lane];
         n += u >> 22;
         w += u & ((1u << 22) - 1);
       }
@@ -208,22 +338,17 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     }
     cluster.sync();
-    double total = 0.;
-    unsigned n_bin = 0;
-    double w_bin = 0.;
+    double total = 0., w_to = 0.;                // tokens and weights down to the lane's bin
+    unsigned n_to = 0;
     for (int i = 0; i < blocks; ++i) {
       const Shared* s = cluster.map_shared_rank(&sh, i);
       total += s->sum;
       if (lane < BINS) {
-        n_bin += s->count[lane];
-        w_bin += s->weight[lane];
+        n_to += s->count[lane];
+        w_to += s->weight[lane];
       }
     }
-    w_bin *= 1. / 16384.;
-    for (int i = 0; i < lane; ++i) w_bin *= 0.5;
-    // tokens and weights down to the lane's bin
-    unsigned n_to = n_bin;
-    double w_to = w_bin;
+    w_to *= (double)__int_as_float((127 - 14 - lane) << 23);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const unsigned u = __shfl_up_sync(0xffffffffu, n_to, o);
@@ -234,9 +359,9 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
       }
     }
     const unsigned counted = __shfl_sync(0xffffffffu, n_to, BINS - 1);
-    const bool counts = by_count && (unsigned)k < counted;       // (fewer have weight: top_k leaves them all)
+    const bool by_count = k > 0 && (unsigned)k < counted;       // (fewer have weight: top_k leaves them all)
     int bin = BINS - 1;                          // the prefix ends in this bin or before
-    if (counts) {
+    if (by_count) {
       bin = __ffs(__ballot_sync(0xffffffffu, lane < BINS && n_to >= (unsigned)k)) - 1;
     } else if (by_weight) {
       // (the bins' weights are rounded: a bin more rather than one too few)
@@ -245,160 +370,150 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     }
     const unsigned listed = __shfl_sync(0xffffffffu, n_to, bin);
 
-    // the end of the prefix among the n listed tokens of the first block, which it sorts: how many are left of them. `before` weighs what
-    // comes before the list.
-    auto sort_list = [&](int n) {
-      int size = 2;
-      while (size < n) size *= 2;
-      for (int i = n + threadIdx.x; i < size; i += THREADS) list[i] = 0;
-      for (int span = 2; span <= size; span *= 2)
-        for (int step = span / 2; step > 0; step /= 2) {
-          __syncthreads();
-          for (int i = threadIdx.x; i < size / 2; i += THREADS) {
-            const int at = 2 * i - (i & (step - 1)), other = at + step;
-            const unsigned long long u = list[at], v = list[other];
-            if ((u < v) == ((at & span) == 0)) {
-              list[at] = v;
-              list[other] = u;
-            }
-          }
+    if (listed <= ROOM) {
+      const float until = bin == BINS - 1 ? NOTHING : (float)(bin + 1);
+      each([&](float v, int i) {
+        if (scale.power(v) < until) {
+          const int at = atomicAdd(&sh.listed, 1);
+          if (at < ROOM) list[at] = key_of(v, i);
         }
-      __syncthreads();
-    };
-    // the blocks' tokens that `want` asks for, one list in the first block; returns how many
-    auto note = [&](float v, int i) {
-      const int at = atomicAdd(&sh.listed, 1);
-      if (at < ROOM) list[at] = key_of(v, i);
-    };
-    auto gather = [&] {
+      });
       cluster.sync();
-      int n = sh.listed;
-      if (leader)
+      if (leader) {
+        int n = sh.listed;
         for (int r = 1; r < blocks; ++r) {
           const int more = cluster.map_shared_rank(&sh, r)->listed;
           const unsigned long long* const other = cluster.map_shared_rank(list, r);
           for (int i = threadIdx.x; i < more && n + i < ROOM; i += THREADS) list[n + i] = other[i];
           n += more;
         }
-      return min(n, ROOM);
-    };
-    constexpr int EACH = ROOM / THREADS;
-
-    if (listed <= ROOM) {
-      const float until = (float)(bin + 1);
-      each([&](float v, int i) {
-        const float y = scale.power(v);
-        if (y < NOTHING && (bin == BINS - 1 || y < until)) note(v, i);
-      });
-      const int n = gather();
-      if (leader) {
-        sort_list(n);
-        double w[EACH], sum = 0., all;
+        n = min(n, ROOM);
+        __syncthreads();
+        auto keys = [&](auto f) {
+          for (int i = threadIdx.x; i < n; i += THREADS) f(list[i]);
+        };
+        unsigned long long low = ~0ull, high = 0;
+        keys([&](unsigned long long key) {
+          low = min(low, key);
+          high = max(high, key);
+        });
 #pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int j = threadIdx.x * EACH + e;
-          w[e] = j < n && !(counts && j >= k) ? scale.exact(value_of(list[j])) : 0.;
-          sum += w[e];
+        for (int o = 16; o > 0; o >>= 1) {
+          low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+          high = max(high, __shfl_xor_sync(0xffffffffu, high, o));
         }
-        const double before = block_before(sum, red_d, all);
-        const double most = p * (counts ? all : total);
-        int left = counts ? min(k, n) : n;
-#pragma unroll
-        for (int e = EACH - 1; e >= 0; --e) {      // the first place that is not left any more
-          const int j = threadIdx.x * EACH + e;
-          double b = before;
-          for (int i = 0; i < e; ++i) b += w[i];
-          if (j < n && j > 0 && ((by_weight && b >= most) || w[e] < m)) left = min(left, j);
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) left = min(left, __shfl_xor_sync(0xffffffffu, left, o));
-        if (lane == 0) red_i[threadIdx.x >> 5] = left;
         if (threadIdx.x == 0) {
+          sh.low = ~0ull;
+          sh.high = 0;
           sh.best_score = 0;
           sh.best_at = a.V;
         }
         __syncthreads();
-        for (int i = 0; i < WARPS; ++i) left = min(left, red_i[i]);
-        sum = 0.;
-        double score = -1.;
+        if (lane == 0) {
+          atomicMin(&sh.low, low);
+          atomicMax(&sh.high, high);
+        }
+        __syncthreads();
+        low = sh.low;
+        high = sh.high;
+        if (by_count) cut = end_of_prefix(std::true_type(), keys, low, high, n, true, (double)k, 0.);
+        if (by_weight) {
+          if (by_count) {
+            double w = 0.;
+            keys([&](unsigned long long key) { if (key >= cut) w += scale.exact(value_of(key)); });
+            total = block_sum(w, red_d);
+          }
+          const unsigned long long from_key = max(low, cut);
+          unsigned long long end = end_of_prefix(std::true_type(), keys, from_key, high, n, false, p * total, 0.);
+          if (!by_count && margin < DOUBT * total) {
+            double w = 0.;
+#pragma unroll 1
+            for (int i = threadIdx.x; i < a.V; i += THREADS) w += scale.exact(fmaxf(to_f32<T>(x[i]), -INFINITY));
+            total = block_sum(w, red_d);
+            end = end_of_prefix(std::true_type(), keys, from_key, high, n, false, p * total, 0.);
+          }
+          cut = max(cut, end);
+        }
+        double all = 0., score = -1.;
         int token = a.V;
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int j = threadIdx.x * EACH + e;
-          if (j >= left || w[e] == 0.) continue;
-          sum += w[e];
-          const int i = (int)index_of(list[j]);
+        keys([&](unsigned long long key) {
+          if (key < cut) return;
+          const double w = scale.exact(value_of(key));
+          if (w < m || w == 0.) return;
+          all += w;
+          const int i = (int)index_of(key);
           const float t = wait[i];
-          const double s = t >= 0.f ? w[e] / (double)t : 0.;
+          const double s = t >= 0.f ? w / (double)t : 0.;
           if (s > score || (s == score && i < token)) {
             score = s;
             token = i;
           }
-        }
-        sum = block_sum(sum, red_d);
+        });
+        all = block_sum(all, red_d);
         if (score >= 0.) atomicMax(&sh.best_score, (unsigned long long)__double_as_longlong(score));
         __syncthreads();
         if (score >= 0. && (unsigned long long)__double_as_longlong(score) == sh.best_score) atomicMin(&sh.best_at, token);
         __syncthreads();
         if (threadIdx.x == 0) {
           const int i = sh.best_at;
-          answer(i, log(scale.exact(to_f32<T>(x[i])) / sum));
+          answer(i, log(scale.exact(to_f32<T>(x[i])) / all));
         }
       }
       cluster.sync();                            // the first has read the others' lists
       return;
     }
 
-    // Too many for one block: the end of the prefix by steps. Tokens with keys in [low, high] hold it; `target` tokens or so much weight
-    // come down to it, `before` of it lie above. Both selections come one after the other where both are asked for.
-    for (int which = counts ? 0 : 1; which < (by_weight ? 2 : 1); ++which) {
+    // Too many for one block. Both selections come one after the other where both are asked for.
+    for (int which = by_count ? 0 : 1; which < (by_weight ? 2 : 1); ++which) {
       const bool count = which == 0;
-      double target = count ? (double)k : p * total, before = 0.;
-      int at_bin = bin;
-      if (!count && counts) {                    // of what top_k has left
+      if (!count && by_count) {                  // of what top_k has left
         float s = 0.f;
         again([&](float v, int i) { if (key_of(v, i) >= cut) s += scale.weight(v, scale.power(v)); });
         const double own = block_sum(s, red_d);
-        cluster.sync();
         if (threadIdx.x == 0) sh.sum = own;
         cluster.sync();
         total = 0.;
         for (int i = 0; i < blocks; ++i) total += cluster.map_shared_rank(&sh, i)->sum;
-        target = p * total;
       }
+      const double target = count ? (double)k : p * total;
+      int at_bin = bin;
       if (!count) {
         const unsigned hit = __ballot_sync(0xffffffffu, lane < BINS - 1 && w_to >= target);
         at_bin = min(bin, hit ? __ffs(hit) - 1 : BINS - 1);
       }
+      double before = 0.;
       unsigned long long low = 0, high = 0, least_above = ~0ull;
+      unsigned inside = 0;
       int way = 0;                               // the bins' rounded weights may be a bin off: up or down from there
       while (true) {
-        float above = 0.f, inside = 0.f;
-        unsigned n_above = 0;
+        float w_above = 0.f, w_inside = 0.f;
+        unsigned n_above = 0, n_inside = 0;
         unsigned long long lo = ~0ull, hi = 0, over = ~0ull;
         again([&](float v, int i) {
-          const unsigned long long key = key_of(v, i);
           const float y = scale.power(v);
-          if (!(y < NOTHING) || key < cut) return;
+          if (!(y < NOTHING)) return;
           const int b = min((int)y, BINS - 1);
-          if (b > at_bin) return;
+          const unsigned long long key = key_of(v, i);
+          if (b > at_bin || key < cut) return;
           const float w = scale.weight(v, y);
           if (b < at_bin) {
-            above += w;
+            w_above += w;
             ++n_above;
             over = min(over, key);
           } else {
-            inside += w;
+            w_inside += w;
+            ++n_inside;
             lo = min(lo, key);
             hi = max(hi, key);
           }
         });
-        const double above_own = count ? block_sum((double)n_above, red_d) : block_sum((double)above, red_d), inside_own = block_sum((double)inside, red_d);
+        const double above_own = block_sum(count ? (double)n_above : (double)w_above, red_d), inside_own = block_sum((double)w_inside, red_d);
         if (threadIdx.x == 0) {
           sh.above = above_own;
           sh.inside = inside_own;
           sh.low = sh.least_above = ~0ull;
           sh.high = 0;
+          sh.listed = 0;
         }
         __syncthreads();
 #pragma unroll
@@ -407,20 +522,24 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
           hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
           over = min(over, __shfl_xor_sync(0xffffffffu, over, o));
         }
+        n_inside = __reduce_add_sync(0xffffffffu, n_inside);
         if (lane == 0) {
           atomicMin(&sh.low, lo);
           atomicMin(&sh.least_above, over);
           atomicMax(&sh.high, hi);
+          atomicAdd(&sh.listed, (int)n_inside);
         }
         cluster.sync();
         double in = 0.;
         before = 0.;
         low = least_above = ~0ull;
         high = 0;
+        inside = 0;
         for (int i = 0; i < blocks; ++i) {
           const Shared* s = cluster.map_shared_rank(&sh, i);
           before += s->above;
           in += s->inside;
+          inside += s->listed;
           low = min(low, s->low);
           high = max(high, s->high);
           least_above = min(least_above, s->least_above);
@@ -441,112 +560,45 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
         if (least_above != ~0ull) cut = max(cut, least_above);
         continue;
       }
-      // units of the weights: 2^-30 of the bin's largest
-      const double unit = ldexp(1., -30 - at_bin);
-      int n_inside = 0;
-      while (true) {
-        const unsigned long long range = high - low;
-        const int shift = max(0, 64 - __clzll(range) - 9);      // SUB parts at most
-        for (int i = threadIdx.x; i < SUB; i += THREADS) sh.sub_count[i] = sh.sub_low[i] = sh.sub_high[i] = 0;
-        __syncthreads();
+      auto keys = [&](auto f) { again([&](float v, int i) { f(key_of(v, i)); }); };
+      unsigned long long end = end_of_prefix(std::false_type(), keys, low, high, (int)inside, count, target, before);
+      if (!count && margin < DOUBT * total) {
+        double w_all = 0., w_above = 0.;
         again([&](float v, int i) {
           const unsigned long long key = key_of(v, i);
-          if (key < low || key > high || key < cut) return;
-          const int s = (int)((high - key) >> shift);
-          atomicAdd(&sh.sub_count[s], 1u);
-          if (!count) {
-            const float y = scale.power(v);
-            const unsigned q = (unsigned)(fminf(scale.weight(v, y) * __int_as_float((127 + at_bin) << 23), 1.f) * 1073741824.f);
-            atomicAdd(&sh.sub_low[s], q & 0xffffu);
-            atomicAdd(&sh.sub_high[s], q >> 16);
-          }
+          if (key < cut) return;
+          const double w = scale.exact(v);
+          w_all += w;
+          if (key > high) w_above += w;
         });
+        w_all = block_sum(w_all, red_d);
+        w_above = block_sum(w_above, red_d);
+        if (threadIdx.x == 0) {
+          sh.sum = w_all;
+          sh.above = w_above;
+        }
         cluster.sync();
-        static_assert(SUB == THREADS, "a thread has one part");
-        unsigned n = 0;
-        unsigned long long w = 0;
+        total = before = 0.;
         for (int i = 0; i < blocks; ++i) {
-          const Shared* s = cluster.map_shared_rank(&sh, i);
-          n += s->sub_count[threadIdx.x];
-          w += s->sub_low[threadIdx.x] + ((unsigned long long)s->sub_high[threadIdx.x] << 16);
+          total += cluster.map_shared_rank(&sh, i)->sum;
+          before += cluster.map_shared_rank(&sh, i)->above;
         }
-        double all;
-        const double mine = count ? (double)n : (double)w * unit, till = block_before(mine, red_d, all) + before;
-        // the first part at whose end the target is reached, or the last that has tokens
-        int hit = n > 0 && till + mine >= target ? (int)threadIdx.x : SUB;
-        int last = n > 0 ? (int)threadIdx.x : -1;
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
-          hit = min(hit, __shfl_xor_sync(0xffffffffu, hit, o));
-          last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-        }
-        __syncthreads();
-        if (lane == 0) {
-          red_i[threadIdx.x >> 5] = hit;
-          red_i[16 + (threadIdx.x >> 5)] = last;
-        }
-        __syncthreads();
-        for (int i = 0; i < WARPS; ++i) {
-          hit = min(hit, red_i[i]);
-          last = max(last, red_i[16 + i]);
-        }
-        if (hit == SUB) hit = last;
-        __syncthreads();
-        if ((int)threadIdx.x == hit) {
-          red_d[0] = till;
-          red_i[0] = (int)n;
-        }
-        __syncthreads();
-        before = red_d[0];
-        n_inside = red_i[0];
-        const unsigned long long top_key = high - ((unsigned long long)hit << shift);
-        const unsigned long long width = (1ull << shift) - 1;
-        low = top_key - low > width ? top_key - width : low;
-        high = top_key;
-        cluster.sync();                          // the parts have been read by all
-        if (n_inside <= ROOM || low == high) break;
+        end = end_of_prefix(std::false_type(), keys, low, high, (int)inside, count, p * total, before);
       }
-      // the few that are left: the last of them that the prefix has
-      if (threadIdx.x == 0) sh.listed = 0;
-      __syncthreads();
-      again([&](float v, int i) {
-        const unsigned long long key = key_of(v, i);
-        if (key >= low && key <= high && key >= cut) note(v, i);
-      });
-      const int n = gather();
-      if (leader) {
-        sort_list(n);
-        double w[EACH], sum = 0., all;
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int j = threadIdx.x * EACH + e;
-          w[e] = j >= n ? 0. : count ? 1. : scale.exact(value_of(list[j]));
-          sum += w[e];
-        }
-        double till = block_before(sum, red_d, all) + before;
-        int left = n;                            // the tokens whose predecessors are less than the target
-#pragma unroll
-        for (int e = 0; e < EACH; ++e) {
-          const int j = threadIdx.x * EACH + e;
-          if (j < n && till >= target) left = min(left, j);
-          till += w[e];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) left = min(left, __shfl_xor_sync(0xffffffffu, left, o));
-        __syncthreads();
-        if (lane == 0) red_i[threadIdx.x >> 5] = left;
-        __syncthreads();
-        for (int i = 0; i < WARPS; ++i) left = min(left, red_i[i]);
-        if (threadIdx.x == 0) sh.cut = list[max(left, 1) - 1];
-      }
-      cluster.sync();
-      cut = max(cut, cluster.map_shared_rank(&sh, 0)->cut);
-      if (threadIdx.x == 0) sh.listed = 0;
-      cluster.sync();
+      cut = max(cut, end);
     }
   }
 
   // The draw: the best arrival in 32 bits, how near the next best of the same thread comes, and the sum of what is left.
+  float sum = 0.f, best = -INFINITY, next = -INFINITY;
+  int at = -1;
+  auto arrival = [&](float y, float t) { return -y - __log2f(t >= 0.f ? t : INFINITY); };
+  auto arrives = [&](float s, int i) {
+    const bool first = at < 0 || s > best;
+    next = at < 0 ? -INFINITY : fmaxf(next, first ? best : s);
+    best = first ? s : best;
+    at = first ? i : at;
+  };
   const double most_below = m > 0. ? -temp * log(m) : INFINITY;       // distance from the largest logit
   const float surely = (float)most_below * (1.f - 1e-6f), never = (float)most_below * (1.f + 1e-6f);
   auto is_left = [&](float v, int i) {
@@ -555,22 +607,36 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a) {
     const float d = scale.below(v);
     return d <= surely || (d <= never && !(scale.exact(v) < m));
   };
-  float sum = 0.f, best = -INFINITY, next = -INFINITY;
-  int at = -1;
-  auto arrival = [&](float y, float t) { return -y - __log2f(t >= 0.f ? t : INFINITY); };
-  each([&](float v, int i) {
-    const float y = scale.power(v);
-    if (!(y < NOTHING) || !is_left(v, i)) return;
-    sum += scale.weight(v, y);
-    const float s = arrival(y, wait[i]);
-    if (s > best || at < 0) {
-      next = at < 0 ? -INFINITY : best;
-      best = s;
-      at = i;
-    } else {
-      next = fmaxf(next, s);
-    }
-  });
+  if (unfiltered) {
+    auto one = [&](float v, float t, int i) {
+      const float y = scale.power(v);
+      sum += scale.weight(v, y);
+      if (y < NOTHING) arrives(arrival(y, t), i);
+    };
+    const bool wide = (reinterpret_cast<uintptr_t>(wait) & 15) == 0;
+    share.each([&](const Piece<T>& v, int i) {
+                 float t[Piece<T>::N];
+                 if (wide) {
+#pragma unroll
+                   for (int e = 0; e < Piece<T>::N; e += 4) {
+                     const float4 u = *reinterpret_cast<const float4*>(wait + i + e);
+                     t[e] = u.x; t[e + 1] = u.y; t[e + 2] = u.z; t[e + 3] = u.w;
+                   }
+                 } else {
+#pragma unroll
+                   for (int e = 0; e < Piece<T>::N; ++e) t[e] = wait[i + e];
+                 }
+#pragma unroll
+                 for (int e = 0; e < Piece<T>::N; ++e) one(fmaxf(v[e], -INFINITY), t[e], i + e);
+               }, [&](float v, int i) { one(fmaxf(v, -INFINITY), wait[i], i); });
+  } else {
+    each([&](float v, int i) {
+      const float y = scale.power(v);
+      if (!(y < NOTHING) || !is_left(v, i)) return;
+      sum += scale.weight(v, y);
+      arrives(arrival(y, wait[i]), i);
+    });
+  }
   const double sum_own = block_sum((double)sum, red_d);
   const float block_best = block_max(at < 0 ? -INFINITY : best, red_f);
   if (threadIdx.x == 0) {
@@ -634,7 +700,7 @@ int launch(const Args& a, int rows, cudaStream_t st) {
   constexpr int N = THREADS * (16 / sizeof(T));      // tokens of a piece for every thread
   // blocks of a row: as long as the GPU holds all of them at once and they have a piece for every thread
   int blocks = 1;
-  while (blocks < 8 && (long long)rows * blocks * 2 <= 148 * 2 && a.V > N * blocks) blocks *= 2;
+  while (blocks < 8 && (long long)rows * blocks * 2 <= 148 * 3 && a.V > N * blocks) blocks *= 2;
   const int part = (a.V + blocks - 1) / blocks + 8;
   // a thread's bins have room for the weights of 255 tokens, a block's parts for those of 65536
   while (blocks < 8 && a.V > blocks * 128 * THREADS) blocks *= 2;
