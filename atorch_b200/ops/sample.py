@@ -23,6 +23,7 @@ def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p
         return logits.new_empty(0, dtype=torch.int64), logits.new_empty(0, dtype=torch.float32)
     T, k, p, m = (torch.as_tensor(v, dtype=torch.float64, device=logits.device).expand(logits.shape[0]).unsqueeze(1)
                   for v in (temperature, top_k, top_p, min_p))
+    m = torch.where(m > 1, torch.ones_like(m), m)
     x = logits.double()
     x = torch.where(torch.isnan(x), torch.full_like(x, -math.inf), x)
     top = x.amax(-1, keepdim=True)
@@ -85,7 +86,8 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
 
     Every parameter is a number or a tensor with one for each row, fp32 (``top_k``: int32 or int64). Numbers out of range are refused; in
     a tensor, which is not looked at on the host, a temperature that is not positive counts as 0, ``top_k`` below 1 as 0, ``top_p``
-    above 1 or NaN as 1 and below 0 as 0 (the first token alone), ``min_p`` above 1 as nothing left but ties of the first, NaN as 0.
+    above 1 or NaN as 1 and below 0 as 0 (the first token alone),
+    ``min_p`` above 1 as 1, NaN as 0.
 
     A NaN logit counts as ``-inf``; of logits of ``+inf`` each weighs 1 and all others nothing; where every logit is ``-inf`` the token
     is 0 and the logarithm ``-inf``. A waiting time below 0 or NaN counts as infinite."""

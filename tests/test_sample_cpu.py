@@ -11,7 +11,7 @@ from atorch_b200 import ops
 def draw(x, wait, T, k, p, m):
     """Token and logarithm of its probability of one row, by the definition, in Python's numbers."""
     x = [-math.inf if v != v else v for v in x]
-    top = max(x)
+    top, m = max(x), 1.0 if m > 1 else m
     if top == -math.inf:
         return 0, -math.inf
     if not T > 0:
@@ -89,7 +89,7 @@ def test_parameters_of_rows():
     g = torch.Generator().manual_seed(3)
     x, wait = torch.randn(6, 300, generator=g) * 2, torch.empty(6, 300).exponential_(generator=g)
     T, k = torch.tensor([0.5, 0.0, -1.0, 2.0, 1.0, 1.0]), torch.tensor([3, 0, 5, -2, 400, 1 << 40])
-    p, m = torch.tensor([0.5, 0.9, 1.0, 1.5, float("nan"), -0.5]), torch.tensor([0.0, 0.5, float("nan"), 0.01, 0.2, 0.0])
+    p, m = torch.tensor([0.5, 0.9, 1.0, 1.5, float("nan"), -0.5]), torch.tensor([0.0, 0.5, float("nan"), 0.01, 1.5, -0.5])
     whole = check(x, wait, temperature=T, top_k=k, top_p=p, min_p=m)
     for b in range(6):
         one = ops.sample(x[b: b + 1], wait[b: b + 1], T[b: b + 1], k[b: b + 1], p[b: b + 1], m[b: b + 1])

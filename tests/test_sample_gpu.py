@@ -79,7 +79,7 @@ def test_strides_offsets_and_rows_of_parameters():
     g = torch.Generator().manual_seed(5)
     x, wait = torch.randn(6, 3007, generator=g) * 2, torch.empty(6, 3007).exponential_(generator=g)
     kw = dict(temperature=torch.tensor([0.5, 0.0, -1.0, 2.0, 1.0, 1.0]), top_k=torch.tensor([3, 0, 5, -2, 400, 1 << 40]),
-              top_p=torch.tensor([0.5, 0.9, 1.0, 1.5, float("nan"), -0.5]), min_p=torch.tensor([0.0, 0.5, float("nan"), 0.01, 0.2, 0.0]))
+              top_p=torch.tensor([0.5, 0.9, 1.0, 1.5, float("nan"), -0.5]), min_p=torch.tensor([0.0, 0.5, float("nan"), 0.01, 1.5, -0.5]))
     for dtype in (torch.float32, torch.bfloat16):
         want = check(x.to(dtype), wait, DEV, **kw)
         kd = {k: v.to(DEV) for k, v in kw.items()}
