@@ -167,30 +167,35 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
   const long long row = blockIdx.x / blocks;
   const T* const x = (const T*)a.logits + row * a.stride;
   const float* const wait = a.waiting + row * a.wait_stride;
-  const int part = ((a.V + blocks - 1) / blocks + 7) / 8 * 8, from = min(a.V, rank * part), to = min(a.V, from + part);
+  // shares begin where the row is aligned to 16 bytes; the first one has what is in front of that
+  constexpr int N = Piece<T>::N;
+  const int part = ((a.V + blocks - 1) / blocks + 7) / 8 * 8, ahead = (int)(-reinterpret_cast<uintptr_t>(x) & 15) / (int)sizeof(T);
+  const int from = rank == 0 ? 0 : min(a.V, rank * part + ahead), to = rank == blocks - 1 ? a.V : min(a.V, (rank + 1) * part + ahead);
+  const int body = rank == 0 ? min(ahead, to) : from, pieces = (to - body) / N;
   const double temp = a.t_rows ? a.t_rows[row] : a.t, p = a.p_rows ? a.p_rows[row] : a.p;
   double m = a.m_rows ? a.m_rows[row] : a.m;
   if (m > 1.) m = 1.;
   int k = a.k_rows ? a.k_rows[row] : a.k;
   if (k < 0 || k >= a.V) k = 0;
   const bool failed = *a.status != 0, by_weight = p < 1., unfiltered = k == 0 && !by_weight && !(m > 0.) && temp > 0.;
-  // The share's pieces, where the row begins on 16 bytes; in shared memory behind the first look, unless there are too many. (From the
-  // first-level cache, or L2, every look waited for them anew: 3 us a look where a thread has 8.)
-  constexpr int N = Piece<T>::N;
-  const int pieces = (reinterpret_cast<uintptr_t>(x) & 15) == 0 ? (to - from) / N : 0;
+  // The share's pieces are in shared memory behind the first look, unless there are too many. (From the first-level cache, or L2, every
+  // look waited for them anew: 3 us a look where a thread has 8.)
   const bool staged = pieces <= room && !unfiltered;
   uint4* const held = reinterpret_cast<uint4*>(own_bins + BINS * THREADS);
-  const uint4* const src = reinterpret_cast<const uint4*>(x + from);
+  const uint4* const src = reinterpret_cast<const uint4*>(x + body);
+  auto each_odd = [&](auto f) {                  // what lies in no piece: a few at the ends
+    const int i = threadIdx.x < 16 ? from + (int)threadIdx.x : body + pieces * N + (int)threadIdx.x - 16;
+    if (threadIdx.x < 32 && i < (threadIdx.x < 16 ? body : to)) f(to_f32<T>(x[i]), i);
+  };
   auto each_piece = [&](auto f, auto one) {      // f(piece, index of its first), one(logit, index)
     if (staged) {
 #pragma unroll 1
-      for (int i = threadIdx.x; i < pieces; i += THREADS) f(Piece<T>{held[i]}, from + i * N);
+      for (int i = threadIdx.x; i < pieces; i += THREADS) f(Piece<T>{held[i]}, body + i * N);
     } else {
 #pragma unroll 2
-      for (int i = threadIdx.x; i < pieces; i += THREADS) f(Piece<T>{src[i]}, from + i * N);
+      for (int i = threadIdx.x; i < pieces; i += THREADS) f(Piece<T>{src[i]}, body + i * N);
     }
-#pragma unroll 1
-    for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) one(to_f32<T>(x[i]), i);
+    each_odd(one);
   };
   auto each = [&](auto f) {                      // f(logit, index)
     each_piece([&](const Piece<T>& v, int i) {
@@ -228,8 +233,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
     if (staged) held[i] = v.u;
     top = fmaxf(top, v.top());
   }
-#pragma unroll 4
-  for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) top = fmaxf(top, to_f32<T>(x[i]));
+  each_odd([&](float v, int) { top = fmaxf(top, v); });
   top = block_max(top, red_f);
   if (threadIdx.x == 0) {
     sh.top = top;
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
   // Every block draws from its share.
   if (unfiltered) {
     // the block's own largest logit says what weights are relative to; for a logarithm their sum in 32 bits does
-    const bool wide = (reinterpret_cast<uintptr_t>(wait) & 15) == 0;
+    const bool wide = (reinterpret_cast<uintptr_t>(wait + body) & 15) == 0;
     const float bend = -0.69314718f * scale.c_rest;
     float weights = 0.f;
     auto one = [&](float v, float t, int i) {
@@ -696,7 +700,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
     };
 #pragma unroll 4
     for (int k = threadIdx.x; k < pieces; k += THREADS) {
-      const int i = from + k * N;
+      const int i = body + k * N;
       const Piece<T> v{src[k]};
       float t[N];
       if (wide) {
@@ -712,8 +716,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
 #pragma unroll
       for (int e = 0; e < N; ++e) one(v[e], t[e], i + e);
     }
-#pragma unroll 2
-    for (int i = from + pieces * N + threadIdx.x; i < to; i += THREADS) one(to_f32<T>(x[i]), wait[i], i);
+    each_odd([&](float v, int i) { one(v, wait[i], i); });
     sum = weights;
   } else if (in_lists) {
     constexpr int EACH = ROOM / THREADS;
@@ -801,7 +804,7 @@ int launch(const Args& a, int rows, cudaStream_t st) {
   // a thread's bins have room for the weights of 255 tokens, a block's parts for those of 65536
   while (blocks < 8 && a.V > blocks * 128 * THREADS) blocks *= 2;
   if (a.V > 8 * 128 * THREADS || (long long)rows * blocks > 0x7fffffffLL) return -2;
-  const int part = ((a.V + blocks - 1) / blocks + 7) / 8 * 8, bytes = (part * (int)sizeof(T) + 15) / 16 * 16, room = bytes <= MOST ? bytes : 0;
+  const int part = ((a.V + blocks - 1) / blocks + 7) / 8 * 8, bytes = (part + 8) * (int)sizeof(T), room = bytes <= MOST ? bytes : 0;
   return launched(launch_after(sample_kernel<T>, dim3((unsigned)(rows * blocks)), THREADS, BINS_BYTES + room, st, blocks, a, room / 16));
 }
 }  // namespace
