@@ -677,21 +677,29 @@ ATB_DEVICE int block_before(int v, int* red, int& all) {
   return __shfl_sync(0xffffffffu, up - x, w) + sum - v;
 }
 
-// What a unit (a key/value head of a sequence in a layer) keeps: the blocks of a cluster have a share of its places each. The
-// least rank that is kept is found digit by digit, 11, 11 and 10 bits, from counts that the blocks read from each other's shared memory;
-// of the places of that rank the lowest are kept. Then the places that are kept are numbered in their order: that number is where the
-// token goes. Weights are moved through the workspace, so that no block writes what another still reads.
-constexpr int SELECT = 512, BINS = 2048, EACH = 4;
+// What a unit (a key/value head of a sequence in a layer) keeps: the blocks of a cluster have a share of its places each. The least
+// rank that is kept is found digit by digit, 11 bits at a time, from counts that the blocks read from each other's shared memory, until
+// so few are left that each is compared with each; of the places of that rank the lowest are kept. Then the places that are kept are
+// numbered in their order: that number is where the token goes. Weights are moved through the workspace, so that no block writes what
+// another still reads. Bound by latency: reads of lengths, pages and weights one after another, a few meetings of the block.
+constexpr int SELECT = 512, BINS = 2048, EACH = 4, FEW = 256;
 __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room) {
   extern __shared__ float sh_w[];                 // `room` weights of the share; the others are read again
-  __shared__ int hist[2][BINS], red[32], sh_digit, sh_above, sh_counts[2], sh_least, sh_failed;
+  __shared__ int hist[2][BINS], red[32], sh_digit, sh_above, sh_in, sh_counts[2], sh_least, sh_failed, sh_n;
+  __shared__ uint32_t few[FEW], few_all[FEW], sh_rank;
   cg::cluster_group cluster = cg::this_cluster();
+  for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = hist[1][i] = 0;
   grid_go();
   grid_wait();
   const Cache& c = a.c;
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const long long unit = blockIdx.x / blocks;
   const int b = (int)(unit / c.kv_heads % c.rows);
+  auto meet = [&] {
+    if (blocks == 1) __syncthreads();
+    else cluster.sync();
+  };
+  const int before = threadIdx.x == 0 ? *a.status : 0;       // on its way beside the lengths
   const int len = seen_length(c, a.lengths, b, a.status), lane = threadIdx.x & 31;
   const bool leader = rank == 0 && threadIdx.x == 0;
   if (leader && unit < (long long)c.rows * c.kv_heads && unit % c.kv_heads == 0) a.out[b] = min(a.lengths[b], a.budget);
@@ -701,15 +709,15 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   }
   const int part = (((len + blocks - 1) / blocks + 3) & ~3), from = min(len, rank * part), to = min(len, from + part);
   float* const w = a.weights + unit * a.places;
-  bool bad = false;
-  for (int i = (from >> c.page_shift) + threadIdx.x; i << c.page_shift < to; i += SELECT) bad = bad || page_of(c, b, i << c.page_shift) < 0;
   const int held = min(to - from, room);
 #pragma unroll 8
   for (int i = threadIdx.x; i < held; i += SELECT) sh_w[i] = w[from + i];
-  for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = hist[1][i] = 0;
+  bool bad = false;
+  for (int i = (from >> c.page_shift) + threadIdx.x; i << c.page_shift < to; i += SELECT) bad = bad || page_of(c, b, i << c.page_shift) < 0;
   if (threadIdx.x == 0) {
     sh_least = len;
-    sh_failed = *a.status;
+    sh_failed = before;
+    sh_n = 0;
   }
   bad = __syncthreads_or(bad);
   if (threadIdx.x == 0 && bad) {
@@ -722,9 +730,11 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   int left = a.budget - a.recent;            // of rank `least`, so many are kept
   uint32_t least = left == 0 ? 0xffffffffu : 0u;
   bool failed = false;
+  int shift = 32;                            // digits above this are known
 #pragma unroll 1
-  for (int pass = 0; pass < 3; ++pass) {
-    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+  for (int pass = 0; pass < 3 && shift > 0; ++pass) {
+    const int bits = shift == 10 ? 10 : 11;
+    shift -= bits;
     int* const h = hist[pass & 1];
     if (left > 0) {
 #pragma unroll 4
@@ -742,7 +752,7 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
         }
       }
     }
-    cluster.sync();
+    meet();
     if (pass == 0)
       for (int i = 0; i < blocks; ++i) failed = failed || *cluster.map_shared_rank(&sh_failed, i) != 0;
     if (pass == 1)                           // the first pass's counts have been read by all
@@ -769,40 +779,77 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
         if (above < left && above + count[e] >= left) {
           sh_digit = top - e;
           sh_above = above;
+          sh_in = count[e];
         }
         above += count[e];
       }
       __syncthreads();
       least |= (uint32_t)sh_digit << shift;
       left -= sh_above;
+      if (sh_in <= FEW && shift > 0) {
+        // few with these digits: every block gets the ranks of all, and finds the left-th largest
+#pragma unroll 4
+        for (int i = from + threadIdx.x; i < mine; i += SELECT) {
+          const uint32_t r = rank_of(weight(i));
+          if ((r ^ least) >> shift == 0) few[atomicAdd(&sh_n, 1)] = r;
+        }
+        meet();
+        int total = 0;
+        for (int i = 0; i < blocks; ++i) {
+          const int m = *cluster.map_shared_rank(&sh_n, i);
+          const uint32_t* const other = cluster.map_shared_rank(few, i);
+          if ((int)threadIdx.x < m) few_all[total + threadIdx.x] = other[threadIdx.x];
+          total += m;
+        }
+        __syncthreads();
+        if ((int)threadIdx.x < total) {
+          const uint32_t r = few_all[threadIdx.x];
+          int greater = 0, same = 0;
+#pragma unroll 4
+          for (int i = 0; i < total; ++i) {
+            greater += few_all[i] > r;
+            same += few_all[i] == r;
+          }
+          if (greater < left && greater + same >= left) {      // (all that are alike say the same)
+            sh_rank = r;
+            sh_above = greater;
+          }
+        }
+        __syncthreads();
+        least = sh_rank;
+        left -= sh_above;
+        shift = 0;
+      }
     }
     __syncthreads();
   }
   // places above and at the border, before the share
-  int above = 0, ties = 0;
+  int all, above_before = 0, ties_before = 0;
+  if (blocks > 1) {
+    int above = 0, ties = 0;
 #pragma unroll 4
-  for (int i = from + threadIdx.x; i < to; i += SELECT) {
-    const uint32_t r = rank_of(weight(i));
-    above += i >= n || r > least;
-    ties += i < n && r == least;
-  }
-  int all;
-  block_before(above, red, all);
-  if (threadIdx.x == 0) sh_counts[0] = all;
-  block_before(ties, red, all);
-  if (threadIdx.x == 0) sh_counts[1] = all;
-  cluster.sync();
-  int above_before = 0, ties_before = 0;
-  for (int i = 0; i < rank; ++i) {
-    above_before += cluster.map_shared_rank(sh_counts, i)[0];
-    ties_before += cluster.map_shared_rank(sh_counts, i)[1];
+    for (int i = from + threadIdx.x; i < to; i += SELECT) {
+      const uint32_t r = rank_of(weight(i));
+      above += i >= n || r > least;
+      ties += i < n && r == least;
+    }
+    block_before(above, red, all);
+    if (threadIdx.x == 0) sh_counts[0] = all;
+    block_before(ties, red, all);
+    if (threadIdx.x == 0) sh_counts[1] = all;
+    cluster.sync();
+    for (int i = 0; i < rank; ++i) {
+      above_before += cluster.map_shared_rank(sh_counts, i)[0];
+      ties_before += cluster.map_shared_rank(sh_counts, i)[1];
+    }
   }
   if (!failed) {
     int* const source = a.source + unit * a.budget;
     float* const kept = a.kept + unit * a.budget;
-    int first = len;
+    int first = len, page = from + (int)threadIdx.x * EACH < to ? page_of(c, b, from + threadIdx.x * EACH) : 0;
     for (int i0 = from; i0 < to; i0 += SELECT * EACH) {
       const int i1 = i0 + threadIdx.x * EACH;
+      const int next = i1 + SELECT * EACH < to ? page_of(c, b, i1 + SELECT * EACH) : 0;       // (pages have a multiple of EACH places)
       float f[EACH];
       int count = 0;                        // above in the low half, ties in the high one
       bool is_above[EACH], is_tie[EACH];
@@ -815,9 +862,8 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
         is_tie[e] = i < to && i < n && r == least;
         count += is_above[e] + (is_tie[e] << 16);
       }
-      const int before = block_before(count, red, all);
-      int g = above_before + (before & 0xffff), t = ties_before + (before >> 16);
-      const int page = i1 < to ? page_of(c, b, i1) : 0;       // (pages have a multiple of EACH places)
+      const int before_me = block_before(count, red, all);
+      int g = above_before + (before_me & 0xffff), t = ties_before + (before_me >> 16);
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const int i = i1 + e;
@@ -833,45 +879,53 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
       }
       above_before += all & 0xffff;
       ties_before += all >> 16;
+      page = next;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+    first = __reduce_min_sync(0xffffffffu, first);
     if (lane == 0) atomicMin(&sh_least, first);
   }
-  cluster.sync();
+  meet();
   if (leader) {
     int first = len;
     for (int i = 0; i < blocks; ++i) first = min(first, *cluster.map_shared_rank(&sh_least, i));
     a.first[unit] = failed ? a.budget : min(first, a.budget);
   }
-  if (!failed)
-    for (int i = from + threadIdx.x; i < to; i += SELECT) w[i] = i < a.budget ? a.kept[unit * a.budget + i] : 0.f;
-  cluster.sync();                                // the first has read the others' words
+  if (!failed) {
+    const float* const kept = a.kept + unit * a.budget;
+#pragma unroll 4
+    for (int i = from + threadIdx.x; i < to; i += SELECT) w[i] = i < a.budget ? kept[i] : 0.f;
+  }
+  if (blocks > 1) cluster.sync();                // the first has read the others' words
 }
 
-// The tokens' move: a block has the keys or the values of a unit, or a slab of their dims where there are few units, and takes places in
-// their order, PER rows a thread at a time. A token only moves down, so what a place's token comes from is not written before that place's
-// turn: the reads of a round end before its writes begin, and those of the next round may come before either.
+// The tokens' move: a block has the keys or the values of a unit, or a cluster of blocks where there are few units, and takes places in
+// their order, PER pieces of 16 bytes a thread in a round. A token only moves down, so what a place's token comes from is not written
+// before that place's turn: the reads of a round end before its writes begin, and those of the next round may come before either. Bound by memory.
 template <int D, int THREADS, int PER>
-__global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a, int slabs) {
+__global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
+  cg::cluster_group cluster = cg::this_cluster();
   grid_go();
   grid_wait();
   const Cache& c = a.c;
-  const int slab = blockIdx.x % slabs, which = blockIdx.x / slabs & 1;
-  const long long unit = blockIdx.x / slabs / 2;
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int which = blockIdx.x / blocks & 1;
+  const long long unit = blockIdx.x / blocks / 2;
   const int first = a.first[unit];
   if (first >= a.budget) return;           // (also of a unit that could not be selected from; its weights stay, too)
   const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
-  const int lanes = D / 8 / slabs, rows = THREADS / lanes;
-  uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + slab * lanes + threadIdx.x % lanes;
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
+  uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + threadIdx.x % LANES;
   const int* const source = a.source + unit * a.budget;
   const int* const row = c.table + b * c.table_stride;
-  auto at = [&](int page, int slot) -> uint4* { return data + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * (D / 8); };
+  auto at = [&](int page, int slot) -> uint4* { return data + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * LANES; };
+  const int own = (rank * PER) * ROWS + threadIdx.x / LANES, step = blocks * PER * ROWS;       // this thread's first row of a round
   uint4 x[2][PER];
-  auto load = [&](uint4 (&y)[PER], int j0) {
-    int src[PER];
+  int src[PER];
+  auto ask = [&](int j0) {                 // where the round's rows come from
 #pragma unroll
-    for (int k = 0; k < PER; ++k) src[k] = j0 + k * rows < a.budget ? source[j0 + k * rows] : -1;
+    for (int k = 0; k < PER; ++k) src[k] = j0 + own + k * ROWS < a.budget ? source[j0 + own + k * ROWS] : -1;
+  };
+  auto load = [&](uint4 (&y)[PER]) {
 #pragma unroll
     for (int k = 0; k < PER; ++k)
       if (src[k] >= 0) y[k] = *at(src[k] >> c.page_shift, src[k] & mask);
@@ -879,22 +933,28 @@ __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a, int slabs
   auto store = [&](const uint4 (&y)[PER], int j0) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int j = j0 + k * rows;
+      const int j = j0 + own + k * ROWS;
       if (j < a.budget) *at(row[j >> c.page_shift], j & mask) = y[k];
     }
   };
-  int j0 = first + threadIdx.x / lanes;
-  const int step = rows * PER, end = a.budget + threadIdx.x / lanes;      // the same number of rounds for all threads
-  load(x[0], j0);
-  for (;; j0 += 2 * step) {
-    __syncthreads();
-    load(x[1], j0 + step);
+  auto meet = [&] {
+    if (blocks == 1) __syncthreads();
+    else cluster.sync();
+  };
+  ask(first);
+  load(x[0]);
+  ask(first + step);
+  for (int j0 = first;; j0 += 2 * step) {
+    meet();
+    load(x[1]);
+    ask(j0 + 2 * step);
     store(x[0], j0);
-    if (j0 + step >= end) break;
-    __syncthreads();
-    load(x[0], j0 + 2 * step);
+    if (j0 + step >= a.budget) break;
+    meet();
+    load(x[0]);
+    ask(j0 + 3 * step);
     store(x[1], j0 + step);
-    if (j0 + 2 * step >= end) break;
+    if (j0 + 2 * step >= a.budget) break;
   }
 }
 
@@ -1012,14 +1072,14 @@ int launch_evict(const EvictArgs& a, cudaStream_t st) {
     if (rc != 0) return rc;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  int slabs = 1;
-  while (slabs < D / 16 && units * 2 * slabs < 148) slabs *= 2;       // rows in pieces of 32 bytes at least
-  if (units * 2 * slabs > 0x7fffffffLL) return -2;
   const int rc = launched(launch_after(kv_select_kernel, dim3((unsigned)(units * blocks)), SELECT, room * 4, st, blocks, a, room));
   if (rc != 0) return rc;
-  const unsigned grid = (unsigned)(units * 2 * slabs);
-  return launched(grid < 148 * 2 ? launch_after(kv_move_kernel<D, 1024, 4>, dim3(grid), 1024, 0, st, 1, a, slabs)
-                                 : launch_after(kv_move_kernel<D, 256, 8>, dim3(grid), 256, 0, st, 1, a, slabs));
+  int movers = 1;
+  while (movers < 8 && units * 2 * movers * 2 <= 148) movers *= 2;
+  if (units * 2 * movers > 0x7fffffffLL) return -2;
+  const unsigned grid = (unsigned)(units * 2 * movers);
+  return launched(grid < 148 * 2 ? launch_after(kv_move_kernel<D, 1024, 4>, dim3(grid), 1024, 0, st, movers, a)
+                                 : launch_after(kv_move_kernel<D, 256, 8>, dim3(grid), 256, 0, st, movers, a));
 }
 }  // namespace
 
