@@ -94,8 +94,9 @@ __global__ void __launch_bounds__(SMALL) kv_append_kernel(const T* qkv, T* q_out
 //
 // The work is cut into equal runs over the GPU (paged.cuh). A segment that is a whole sequence (of a head and column tile) is
 // finished in place; of the others, a run's first and last, a block leaves sums, maximum and denominator, which a second kernel joins
-// in the order of the blocks.
-constexpr int WARPS = 4, TILE = 16, START = 12;
+// in the order of the blocks. (START of 6, 12, 24 and 40 tiles: 32 sequences of up to 4096 59.0, 45.7, 44.8 and 46.2 us, one of 1531 10.0,
+// 9.9, 9.2 and 9.1, 19 of up to 1801 with 31 queries 71.5, 60.4, 52.6 and 54.6.)
+constexpr int WARPS = 4, TILE = 16, START = 24;
 constexpr float SLACK = 4.f;       // powers of two by which a score may exceed the maximum that is kept
 // Powers of two that the largest weight is held at: fp16 has numbers from 2^-24 to 2^16, and thousands of tokens with 2^-26 of the
 // largest weight count together.
@@ -376,11 +377,29 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv_attention
           const int o = e & 1, t = t0 + r + 4 * (e & 2);
           float v = s[n][e] * a.scale_log2;
           if (MASK && t >= limit[n][o]) v = -INFINITY;
-          if (scores) {
-            const int col = col_tile * COLS + 8 * n + 2 * q4 + o;
-            if (col < columns && t < len) scores[(long long)t * columns + col] = v;
+          s[n][e] = v;
+        }
+      if (scores) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int col = col_tile * COLS + 8 * n + 2 * q4, t = t0 + r + 8 * i;
+            if (MASK && t >= len) continue;
+            float* const dst = scores + (long long)t * columns + col;
+            if (columns % 2 == 0) {
+              if (col < columns) *reinterpret_cast<float2*>(dst) = make_float2(s[n][2 * i], s[n][2 * i + 1]);
+            } else {
+              if (col < columns) dst[0] = s[n][2 * i];
+              if (col + 1 < columns) dst[1] = s[n][2 * i + 1];
+            }
           }
-          s[n][e] = v - ref[n][o];
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[n][e] -= ref[n][e & 1];
           over = fmaxf(over, s[n][e]);
         }
       if (__any_sync(0xffffffffu, over > SLACK + LIFT<T> || unset)) {
@@ -552,85 +571,137 @@ __global__ void __launch_bounds__(WARPS * 32, Shape<D, NT>::BLOCKS) kv_attention
   }
 }
 
-// Sequences (of a head and a column tile: a block) that several blocks worked on. Bound by latency: the blocks' results are read
-// eight at a time, independent of one another.
-template <typename T, int D, int NT>
-__global__ void __launch_bounds__(256) kv_join_kernel(AttnArgs a, int per) {
-  constexpr int COLS = 8 * NT, EACH = 8;
-  grid_go();
-  grid_wait();
-  const int2 own = a.owners[blockIdx.x];
-  const bool failed = *a.status != 0;
-  // (behind a kernel that left early there may be anything)
-  if (__syncthreads_or(failed) || own.x < 0 || own.y >= a.ctas || own.x >= own.y) return;
-  const int columns = a.S * a.group, b = blockIdx.x / per, hc = blockIdx.x - b * per;
-  const int head = hc % a.c.kv_heads, col_tile = hc / a.c.kv_heads;
+// Maximum and sums of a column of a sequence that several blocks worked on, and with V its four dims from d: the blocks' results are read
+// eight at a time, independent of one another, and joined in the order of the blocks.
+template <int D, int COLS, bool V>
+ATB_DEVICE void join_column(const AttnArgs& a, int2 own, int col, int d, float& top, float& sum, float& rounded, float (&o)[4]) {
+  constexpr int EACH = 8;
   const float* const stats = a.partial + 2LL * a.ctas * COLS * D;
-  for (int x = threadIdx.x; x < COLS * (D / 4); x += 256) {
-    const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
-    if (n >= columns) continue;
-    float top = -INFINITY, sum = 0.f, rounded = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int k0 = own.x; k0 <= own.y; k0 += EACH) {
-      float4 ml[EACH], v[EACH];
+  top = -INFINITY;
+  sum = rounded = o[0] = o[1] = o[2] = o[3] = 0.f;
+  for (int k0 = own.x; k0 <= own.y; k0 += EACH) {
+    float4 ml[EACH], v[V ? EACH : 1];
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        const long long at = (2LL * min(k0 + k, own.y) + (k0 + k == own.x)) * COLS + col;
-        ml[k] = *reinterpret_cast<const float4*>(stats + 4 * at);
-        v[k] = *reinterpret_cast<const float4*>(a.partial + at * D + d);
-        if (k0 + k > own.y) ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
-      }
-      float to = top;
+    for (int k = 0; k < EACH; ++k) {
+      const long long at = (2LL * min(k0 + k, own.y) + (k0 + k == own.x)) * COLS + col;
+      ml[k] = *reinterpret_cast<const float4*>(stats + 4 * at);
+      if constexpr (V) v[k] = *reinterpret_cast<const float4*>(a.partial + at * D + d);
+      if (k0 + k > own.y) ml[k] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    }
+    float to = top;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) to = fmaxf(to, ml[k].x);
-      const float down = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : fast_exp2(top - to);
-      sum *= down;
-      rounded *= down;
+    for (int k = 0; k < EACH; ++k) to = fmaxf(to, ml[k].x);
+    const float down = top == -INFINITY ? (sum == 0.f ? 0.f : 1.f) : fast_exp2(top - to);
+    sum *= down;
+    rounded *= down;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] *= down;
-      top = to;
+    for (int e = 0; e < 4; ++e) o[e] *= down;
+    top = to;
 #pragma unroll
-      for (int k = 0; k < EACH; ++k) {
-        if (k0 + k > own.y) continue;
-        const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : fast_exp2(ml[k].x - top);
-        sum += f * ml[k].y;
-        rounded += f * ml[k].z;
+    for (int k = 0; k < EACH; ++k) {
+      if (k0 + k > own.y) continue;
+      const float f = ml[k].x == -INFINITY ? (ml[k].y == 0.f ? 0.f : 1.f) : fast_exp2(ml[k].x - top);
+      sum += f * ml[k].y;
+      rounded += f * ml[k].z;
+      if constexpr (V) {
         o[0] += f * v[k].x;
         o[1] += f * v[k].y;
         o[2] += f * v[k].z;
         o[3] += f * v[k].w;
       }
     }
+  }
+}
+ATB_DEVICE bool shared_by_blocks(const AttnArgs& a, int2 own) {       // (behind a kernel that left early there may be anything)
+  return own.x >= 0 && own.y < a.ctas && own.x < own.y;
+}
+// The join of one sequence, head and column tile (a block). Bound by latency.
+template <typename T, int D, int NT>
+ATB_DEVICE void join(const AttnArgs& a, int item, int per) {
+  constexpr int COLS = 8 * NT;
+  const int2 own = a.owners[item];
+  if (!shared_by_blocks(a, own)) return;
+  const int columns = a.S * a.group, b = item / per, hc = item - b * per;
+  const int head = hc % a.c.kv_heads, col_tile = hc / a.c.kv_heads;
+  for (int x = threadIdx.x; x < COLS * (D / 4); x += 256) {
+    const int col = x / (D / 4), d = (x - col * (D / 4)) * 4, n = col_tile * COLS + col;
+    if (n >= columns) continue;
+    float top, sum, rounded, o[4];
+    join_column<D, COLS, true>(a, own, col, d, top, sum, rounded, o);
     finish<T, D>(a, b, head, n, d, top, sum, rounded, o);
   }
 }
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(256) kv_join_kernel(AttnArgs a, int per) {
+  grid_go();
+  grid_wait();
+  if (__syncthreads_or(*a.status != 0)) return;
+  join<T, D, NT>(a, blockIdx.x, per);
+}
 
 // What the queries attended to: a place's scores of all columns, as the kernel above has left them, relative to the columns' logarithms,
-// added up in the order of the columns by LANES lanes, and to what is there.
-template <int LANES>
-__global__ void __launch_bounds__(256) kv_weights_kernel(AttnArgs a) {
+// added up by LANES lanes in one order, and to what is there. Logarithms of sequences that several blocks worked on are
+// joined here, MOST columns at a time; the last blocks of a head's row do the join of the results beside it.
+template <typename T, int D, int NT, int LANES>
+__global__ void __launch_bounds__(256, 3) kv_weights_kernel(AttnArgs a, int per, int chunks) {
+  constexpr int COLS = 8 * NT, MOST = 128;
+  __shared__ float lse2[MOST];
   grid_go();
   grid_wait();
   const Cache& c = a.c;
-  const int columns = a.S * a.group, b = blockIdx.y / c.kv_heads, lane = threadIdx.x % LANES;
-  const bool failed = *a.status != 0;
+  const int columns = a.S * a.group, b = blockIdx.y / c.kv_heads, head = blockIdx.y - b * c.kv_heads, lane = threadIdx.x % LANES;
+  const bool failed = threadIdx.x == 0 && *a.status != 0;
   const int len = seen_length(c, a.lengths, b, a.status);
   if (__syncthreads_or(failed)) return;
-  const float* const lse2 = a.lse2 + (long long)blockIdx.y * columns;
+  if ((int)blockIdx.x >= chunks) {
+    join<T, D, NT>(a, b * per + ((int)blockIdx.x - chunks) * c.kv_heads + head, per);
+    return;
+  }
   const float* const scores = a.scores + (long long)blockIdx.y * ((long long)c.width << c.page_shift) * columns;
   float* const weights = a.weights + (long long)blockIdx.y * a.places;
-  const int step = gridDim.x * (256 / LANES);
-  for (int t0 = blockIdx.x * (256 / LANES); t0 < len; t0 += step) {
-    const int t = t0 + threadIdx.x / LANES;
-    float sum = 0.f;
-    if (t < len) {
-      for (int n = lane; n < columns; n += LANES) {
-        const float x = scores[(long long)t * columns + n], y = lse2[n];
-        sum += x == -INFINITY || y == -INFINITY ? 0.f : fast_exp2(x - y);
+  const int step = chunks * (256 / LANES);
+  for (int n0 = 0; n0 < columns; n0 += MOST) {
+    const int n1 = min(columns - n0, MOST);
+    __syncthreads();
+    if ((int)threadIdx.x < n1) {
+      const int n = n0 + threadIdx.x, col_tile = n / COLS;
+      const int2 own = a.ctas > 0 ? a.owners[(long long)b * per + col_tile * c.kv_heads + head] : make_int2(0, 0);
+      float x;
+      if (shared_by_blocks(a, own)) {
+        float top, sum, rounded, o[4];
+        join_column<D, COLS, false>(a, own, n - col_tile * COLS, 0, top, sum, rounded, o);
+        x = top + (log2f(sum) - LIFT<T>);
+      } else {
+        x = a.lse2[(long long)blockIdx.y * columns + n];
+      }
+      lse2[threadIdx.x] = x;
+    }
+    __syncthreads();
+    // (several places of a thread at once: their scores and what is there are on their way together)
+    constexpr int U = LANES == 1 ? 4 : 2, C = LANES == 1 ? 4 : 16;       // C LANES columns in a go
+    for (int t0 = blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t0 - (int)threadIdx.x / LANES < len; t0 += U * step) {
+      float x[U][C], old[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * step;
+        old[u] = t < len ? weights[t] : 0.f;
+#pragma unroll
+        for (int k = 0; k < C; ++k) x[u][k] = t < len && lane + k * LANES < n1 ? scores[(long long)t * columns + n0 + lane + k * LANES] : -INFINITY;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * step;
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < C; ++k) {
+          const float y = lane + k * LANES < n1 ? lse2[lane + k * LANES] : -INFINITY;
+          sum += x[u][k] == -INFINITY || y == -INFINITY ? 0.f : fast_exp2(x[u][k] - y);
+        }
+#pragma unroll
+        for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (t < len && lane == 0) weights[t] = old[u] + sum;
       }
     }
-#pragma unroll
-    for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (t < len && lane == 0) weights[t] += sum;
   }
 }
 
@@ -678,17 +749,18 @@ ATB_DEVICE int block_before(int v, int* red, int& all) {
 }
 
 // What a unit (a key/value head of a sequence in a layer) keeps: the blocks of a cluster have a share of its places each. The least
-// rank that is kept is found digit by digit, 11 bits at a time, from counts that the blocks read from each other's shared memory, until
+// rank that is kept is found digit by digit, 8 bits at a time, from counts that the blocks read from each other's shared memory, until
 // so few are left that each is compared with each; of the places of that rank the lowest are kept. Then the places that are kept are
 // numbered in their order: that number is where the token goes. Weights are moved through the workspace, so that no block writes what
 // another still reads. Bound by latency: reads of lengths, pages and weights one after another, a few meetings of the block.
-constexpr int SELECT = 512, BINS = 2048, EACH = 4, FEW = 256;
+constexpr int BINS = 256, EACH = 4, FEW = 256;
+template <int SELECT>
 __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room) {
-  extern __shared__ float sh_w[];                 // `room` weights of the share; the others are read again
-  __shared__ int hist[2][BINS], red[32], sh_digit, sh_above, sh_in, sh_counts[2], sh_least, sh_failed, sh_n;
+  extern __shared__ __align__(16) float sh_w[];   // `room` weights of the share; the others are read again
+  __shared__ int hist[3][BINS], red[32], sh_digit, sh_above, sh_in, sh_counts[2], sh_least, sh_failed, sh_n;
   __shared__ uint32_t few[FEW], few_all[FEW], sh_rank;
   cg::cluster_group cluster = cg::this_cluster();
-  for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = hist[1][i] = 0;
+  for (int i = threadIdx.x; i < 3 * BINS; i += SELECT) hist[0][i] = 0;
   grid_go();
   grid_wait();
   const Cache& c = a.c;
@@ -710,7 +782,7 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   const int part = (((len + blocks - 1) / blocks + 3) & ~3), from = min(len, rank * part), to = min(len, from + part);
   float* const w = a.weights + unit * a.places;
   const int held = min(to - from, room);
-#pragma unroll 8
+#pragma unroll 16
   for (int i = threadIdx.x; i < held; i += SELECT) sh_w[i] = w[from + i];
   bool bad = false;
   for (int i = (from >> c.page_shift) + threadIdx.x; i << c.page_shift < to; i += SELECT) bad = bad || page_of(c, b, i << c.page_shift) < 0;
@@ -732,17 +804,16 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   bool failed = false;
   int shift = 32;                            // digits above this are known
 #pragma unroll 1
-  for (int pass = 0; pass < 3 && shift > 0; ++pass) {
-    const int bits = shift == 10 ? 10 : 11;
-    shift -= bits;
-    int* const h = hist[pass & 1];
+  for (int pass = 0; shift > 0; ++pass) {
+    shift -= 8;
+    int* const h = hist[pass % 3];
     if (left > 0) {
 #pragma unroll 4
       for (int i0 = from; i0 < mine; i0 += SELECT) {
         const int i = i0 + threadIdx.x;
         const uint32_t r = i < mine ? rank_of(weight(i)) : 0u;
-        const bool in = i < mine && (pass == 0 || (r ^ least) >> (shift + bits) == 0);
-        const int bin = in ? r >> shift & ((1 << bits) - 1) : -1;
+        const bool in = i < mine && (pass == 0 || (r ^ least) >> (shift + 8) == 0);
+        const int bin = in ? (int)(r >> shift & (BINS - 1)) : -1;
         int same;
         __match_all_sync(0xffffffffu, bin, &same);       // (many weights alike would wait for one another)
         if (!same) {
@@ -755,33 +826,19 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
     meet();
     if (pass == 0)
       for (int i = 0; i < blocks; ++i) failed = failed || *cluster.map_shared_rank(&sh_failed, i) != 0;
-    if (pass == 1)                           // the first pass's counts have been read by all
-      for (int i = threadIdx.x; i < BINS; i += SELECT) hist[0][i] = 0;
+    if (pass == 1 && threadIdx.x < BINS) hist[0][threadIdx.x] = 0;       // the first digit's counts have been read by all
     if (left > 0 && !failed) {
-      // from the highest bin down: four of a thread
-      int count[EACH], sum = 0;
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) count[e] = 0;
-      const int top = BINS - 1 - EACH * (int)threadIdx.x;
-#pragma unroll 4
-      for (int i = 0; i < blocks; ++i) {
-        const int4 v = *reinterpret_cast<const int4*>(cluster.map_shared_rank(h, i) + top - 3);
-        count[0] += v.w;
-        count[1] += v.z;
-        count[2] += v.y;
-        count[3] += v.x;
-      }
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) sum += count[e];
-      int all, above = block_before(sum, red, all);
-#pragma unroll
-      for (int e = 0; e < EACH; ++e) {
-        if (above < left && above + count[e] >= left) {
-          sh_digit = top - e;
-          sh_above = above;
-          sh_in = count[e];
-        }
-        above += count[e];
+      // from the highest bin down: one of a thread
+      static_assert(BINS <= SELECT, "a thread has a bin");
+      const int digit = BINS - 1 - (int)threadIdx.x;
+      int count = 0, all;
+      if (digit >= 0)
+        for (int i = 0; i < blocks; ++i) count += cluster.map_shared_rank(h, i)[digit];
+      const int above = block_before(count, red, all);
+      if (above < left && above + count >= left) {
+        sh_digit = digit;
+        sh_above = above;
+        sh_in = count;
       }
       __syncthreads();
       least |= (uint32_t)sh_digit << shift;
@@ -794,12 +851,17 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
           if ((r ^ least) >> shift == 0) few[atomicAdd(&sh_n, 1)] = r;
         }
         meet();
-        int total = 0;
+        const int theirs = lane < blocks ? *cluster.map_shared_rank(&sh_n, lane) : 0, total = __reduce_add_sync(0xffffffffu, theirs);
+        const int r_of = threadIdx.x >> 5;       // a warp for each block
+        int at = 0;
         for (int i = 0; i < blocks; ++i) {
-          const int m = *cluster.map_shared_rank(&sh_n, i);
-          const uint32_t* const other = cluster.map_shared_rank(few, i);
-          if ((int)threadIdx.x < m) few_all[total + threadIdx.x] = other[threadIdx.x];
-          total += m;
+          const int m = __shfl_sync(0xffffffffu, theirs, i);
+          if (i < r_of) at += m;
+        }
+        if (r_of < blocks) {
+          const uint32_t* const other = cluster.map_shared_rank(few, r_of);
+          const int m = __shfl_sync(0xffffffffu, theirs, r_of);
+          for (int i = lane; i < m; i += 32) few_all[at + i] = other[i];
         }
         __syncthreads();
         if ((int)threadIdx.x < total) {
@@ -851,12 +913,18 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
       const int i1 = i0 + threadIdx.x * EACH;
       const int next = i1 + SELECT * EACH < to ? page_of(c, b, i1 + SELECT * EACH) : 0;       // (pages have a multiple of EACH places)
       float f[EACH];
+      if (i1 - from + EACH <= held) {       // (the share begins on a multiple of EACH)
+        const float4 v = *reinterpret_cast<const float4*>(sh_w + (i1 - from));
+        f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+      } else {
+#pragma unroll
+        for (int e = 0; e < EACH; ++e) f[e] = i1 + e < to ? weight(i1 + e) : 0.f;
+      }
       int count = 0;                        // above in the low half, ties in the high one
       bool is_above[EACH], is_tie[EACH];
 #pragma unroll
       for (int e = 0; e < EACH; ++e) {
         const int i = i1 + e;
-        f[e] = i < to ? weight(i) : 0.f;
         const uint32_t r = rank_of(f[e]);
         is_above[e] = i < to && (i >= n || r > least);
         is_tie[e] = i < to && i < n && r == least;
@@ -892,39 +960,37 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   }
   if (!failed) {
     const float* const kept = a.kept + unit * a.budget;
-#pragma unroll 4
+#pragma unroll 16
     for (int i = from + threadIdx.x; i < to; i += SELECT) w[i] = i < a.budget ? kept[i] : 0.f;
   }
   if (blocks > 1) cluster.sync();                // the first has read the others' words
 }
 
-// The tokens' move: a block has the keys or the values of a unit, or a cluster of blocks where there are few units, and takes places in
-// their order, PER pieces of 16 bytes a thread in a round. A token only moves down, so what a place's token comes from is not written
-// before that place's turn: the reads of a round end before its writes begin, and those of the next round may come before either. Bound by memory.
+// The tokens' move: a block has the keys or the values of a unit and takes places in their order, THREADS PER pieces of 16 bytes in a
+// round. A token only moves down, so what a place's token comes from is not written before that place's turn: the reads of a round end
+// before its writes begin, and those of later rounds may come before either. Bound by memory where there are many units (8 layers of 8
+// sequences, 8 heads: 68 us for 406 MB).
 template <int D, int THREADS, int PER>
 __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
-  cg::cluster_group cluster = cg::this_cluster();
   grid_go();
   grid_wait();
   const Cache& c = a.c;
-  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int which = blockIdx.x / blocks & 1;
-  const long long unit = blockIdx.x / blocks / 2;
+  const int which = blockIdx.x & 1;
+  const long long unit = blockIdx.x / 2;
   const int first = a.first[unit];
   if (first >= a.budget) return;           // (also of a unit that could not be selected from; its weights stay, too)
   const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
-  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES, STEP = ROWS * PER;
   uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + threadIdx.x % LANES;
   const int* const source = a.source + unit * a.budget;
   const int* const row = c.table + b * c.table_stride;
   auto at = [&](int page, int slot) -> uint4* { return data + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * LANES; };
-  const int own = (rank * PER) * ROWS + threadIdx.x / LANES, step = blocks * PER * ROWS;       // this thread's first row of a round
-  uint4 x[2][PER];
   int src[PER];
   auto ask = [&](int j0) {                 // where the round's rows come from
 #pragma unroll
-    for (int k = 0; k < PER; ++k) src[k] = j0 + own + k * ROWS < a.budget ? source[j0 + own + k * ROWS] : -1;
+    for (int k = 0; k < PER; ++k) src[k] = j0 + k * ROWS < a.budget ? source[j0 + k * ROWS] : -1;
   };
+  uint4 x[2][PER];
   auto load = [&](uint4 (&y)[PER]) {
 #pragma unroll
     for (int k = 0; k < PER; ++k)
@@ -933,28 +999,93 @@ __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
   auto store = [&](const uint4 (&y)[PER], int j0) {
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
-      const int j = j0 + own + k * ROWS;
+      const int j = j0 + k * ROWS;
       if (j < a.budget) *at(row[j >> c.page_shift], j & mask) = y[k];
     }
   };
-  auto meet = [&] {
-    if (blocks == 1) __syncthreads();
-    else cluster.sync();
-  };
-  ask(first);
+  const int own = threadIdx.x / LANES;
+  ask(first + own);
   load(x[0]);
-  ask(first + step);
-  for (int j0 = first;; j0 += 2 * step) {
-    meet();
+  ask(first + own + STEP);
+  for (int j0 = first;; j0 += 2 * STEP) {  // (as many rounds for all threads)
+    __syncthreads();
     load(x[1]);
-    ask(j0 + 2 * step);
-    store(x[0], j0);
-    if (j0 + step >= a.budget) break;
-    meet();
+    ask(j0 + own + 2 * STEP);
+    store(x[0], j0 + own);
+    if (j0 + STEP >= a.budget) break;
+    __syncthreads();
     load(x[0]);
-    ask(j0 + 3 * step);
-    store(x[1], j0 + step);
-    if (j0 + 2 * step >= a.budget) break;
+    ask(j0 + own + 3 * STEP);
+    store(x[1], j0 + own + STEP);
+    if (j0 + 2 * STEP >= a.budget) break;
+  }
+}
+
+// The same for few units: the blocks of a cluster share the rows of a round. DEEP rounds are on their way in shared memory, and the blocks
+// say that they have their part of the next round before they write this one, so that nobody waits for the meeting. 50000 tokens of 8
+// heads (410 MB): 100 us, bound by the rounds' latency; meetings that wait, one round ahead, took 163, a slab of the rows' 32 bytes for
+// every block, which need not meet, 108, for its many small requests.
+template <int D, int THREADS, int PER, int DEEP>
+__global__ void __launch_bounds__(THREADS) kv_move_cluster_kernel(EvictArgs a) {
+  extern __shared__ uint4 ring[];          // [DEEP][PER][THREADS]: a thread reads what it has asked for itself
+  cg::cluster_group cluster = cg::this_cluster();
+  grid_go();
+  grid_wait();
+  const Cache& c = a.c;
+  const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), which = blockIdx.x / blocks & 1;
+  const long long unit = blockIdx.x / blocks / 2;
+  const int first = a.first[unit];
+  if (first >= a.budget) return;
+  const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
+  constexpr int LANES = D / 8, ROWS = THREADS / LANES;
+  uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + threadIdx.x % LANES;
+  const int* const source = a.source + unit * a.budget;
+  const int* const row = c.table + b * c.table_stride;
+  auto at = [&](int page, int slot) -> uint4* { return data + (((((long long)page * 2 + which) * c.kv_heads + head) << c.page_shift) + slot) * LANES; };
+  const int own = rank * PER * ROWS + threadIdx.x / LANES, step = blocks * PER * ROWS;
+  struct Sources {
+    int at[PER];
+  };
+  auto ask = [&](int j0) {                 // where the round's rows come from
+    Sources s;
+#pragma unroll
+    for (int k = 0; k < PER; ++k) s.at[k] = j0 + own + k * ROWS < a.budget ? source[j0 + own + k * ROWS] : -1;
+    return s;
+  };
+  auto load = [&](int stage, const Sources& s) {
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if (s.at[k] >= 0)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(ring + (stage * PER + k) * THREADS + threadIdx.x)),
+                     "l"(__cvta_generic_to_global(at(s.at[k] >> c.page_shift, s.at[k] & mask))) : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // What the meeting orders are reads that have come, before writes that are not yet made: nothing has to be made visible, and a meeting
+  // that waits for the writes before it (release) takes 5 us a round.
+  auto arrive = [] { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); };
+  Sources next = ask(first), far = ask(first + step);
+  for (int s = 0; s < DEEP; ++s) {
+    load(s, next);
+    next = far;
+    far = ask(first + (s + 2) * step);
+  }
+  asm volatile("cp.async.wait_group %0;" ::"n"(DEEP - 1) : "memory");
+  arrive();
+  cluster.barrier_wait();
+  int stage = 0;
+  for (int j0 = first; j0 < a.budget; j0 += step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEEP - 2) : "memory");      // the next round is here
+    arrive();
+#pragma unroll
+    for (int k = 0; k < PER; ++k) {
+      const int j = j0 + own + k * ROWS;
+      if (j < a.budget) *at(row[j >> c.page_shift], j & mask) = ring[(stage * PER + k) * THREADS + threadIdx.x];
+    }
+    load(stage, next);                     // of the round DEEP further on; an empty group behind the last one
+    next = far;
+    far = ask(j0 + (DEEP + 2) * step);
+    stage = stage + 1 == DEEP ? 0 : stage + 1;
+    cluster.barrier_wait();
   }
 }
 
@@ -1044,42 +1175,49 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   const long long grid = most < 148 * Sh::BLOCKS ? most : 148 * Sh::BLOCKS;
   int rc = launched(launch_after(kv_attention_kernel<T, D, NT>, dim3((unsigned)(w.cut || runs > grid ? grid : runs)), WARPS * 32, SMEM, st, 1,
                                  map, a));
-  if (rc == 0 && w.cut) rc = launched(launch_after(kv_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per));
-  if (rc != 0 || !a.weights) return rc;
+  if (rc != 0) return rc;
+  if (!a.weights) return w.cut ? launched(launch_after(kv_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per)) : 0;
   const long long heads = (long long)a.c.rows * a.c.kv_heads;
   if (heads > 65535) return -2;
   const int lanes = columns <= 4 ? 1 : 8, each = 256 / lanes;
-  const long long chunks = (places + each - 1) / each, enough = 148 * 8 / heads + 1;
-  const dim3 blocks((unsigned)(chunks < enough ? chunks : enough), (unsigned)heads);
-  return launched(lanes == 1 ? launch_after(kv_weights_kernel<1>, blocks, 256, 0, st, 1, a) : launch_after(kv_weights_kernel<8>, blocks, 256, 0, st, 1, a));
+  const long long most_chunks = (places + each - 1) / each, enough = (lanes == 1 ? 148 * 3 : 148 * 6) / heads + 1;
+  const int chunks = (int)(most_chunks < enough ? most_chunks : enough);
+  const dim3 blocks((unsigned)(chunks + (w.cut ? per / a.c.kv_heads : 0)), (unsigned)heads);
+  return launched(lanes == 1 ? launch_after(kv_weights_kernel<T, D, NT, 1>, blocks, 256, 0, st, 1, a, (int)per, chunks)
+                             : launch_after(kv_weights_kernel<T, D, NT, 8>, blocks, 256, 0, st, 1, a, (int)per, chunks));
 }
 
 template <int D>
 int launch_evict(const EvictArgs& a, cudaStream_t st) {
   const long long units = (long long)a.layers * a.c.rows * a.c.kv_heads, places = (long long)a.c.width << a.c.page_shift;
-  // a cluster where the GPU has room for it and its blocks have 2048 places each
+  // few units: a cluster of large blocks for each, where its blocks have 2048 places each
+  const bool few = units < 148;
   int blocks = 1;
   while (blocks < 8 && units * blocks * 2 <= 148 && places > 2048LL * blocks) blocks *= 2;
-  constexpr int LARGEST = 16384;
+  // (16 clusters of 8 blocks are resident at once if two blocks fit on an SM, not with one: 15 then)
+  constexpr int LARGEST = 16384, MOVE = 512, PER = 6, DEEP = 2, RING = MOVE * PER * DEEP * 16;
   const long long share = (places + blocks - 1) / blocks + 4;
   const int room = (int)(share < LARGEST ? share : LARGEST);
-  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernel may have its shared memory
+  static std::atomic<unsigned long long> allowed{0};       // devices on which the kernels may have their shared memory
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return launched(cudaErrorInvalidDevice);
   const unsigned long long bit = 1ull << (device & 63);
   if (!(allowed.load(std::memory_order_relaxed) & bit)) {
-    const int rc = launched(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, LARGEST * 4));
+    int rc = launched(cudaFuncSetAttribute(kv_select_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize, LARGEST * 4));
+    if (rc == 0) rc = launched(cudaFuncSetAttribute(kv_select_kernel<1024>, cudaFuncAttributeMaxDynamicSharedMemorySize, LARGEST * 4));
+    if (rc == 0) rc = launched(cudaFuncSetAttribute(kv_move_cluster_kernel<D, MOVE, PER, DEEP>, cudaFuncAttributeMaxDynamicSharedMemorySize, RING));
     if (rc != 0) return rc;
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
-  const int rc = launched(launch_after(kv_select_kernel, dim3((unsigned)(units * blocks)), SELECT, room * 4, st, blocks, a, room));
+  int members = 1;
+  while (few && members < 8 && units * 2 * members * 2 <= 148) members *= 2;
+  if (units * 2 * members > 0x7fffffffLL) return -2;
+  const dim3 grid((unsigned)(units * blocks)), movers((unsigned)(units * 2 * members));
+  const int rc = launched(few ? launch_after(kv_select_kernel<1024>, grid, 1024, room * 4, st, blocks, a, room)
+                              : launch_after(kv_select_kernel<512>, grid, 512, room * 4, st, blocks, a, room));
   if (rc != 0) return rc;
-  int movers = 1;
-  while (movers < 8 && units * 2 * movers * 2 <= 148) movers *= 2;
-  if (units * 2 * movers > 0x7fffffffLL) return -2;
-  const unsigned grid = (unsigned)(units * 2 * movers);
-  return launched(grid < 148 * 2 ? launch_after(kv_move_kernel<D, 1024, 4>, dim3(grid), 1024, 0, st, movers, a)
-                                 : launch_after(kv_move_kernel<D, 256, 8>, dim3(grid), 256, 0, st, movers, a));
+  return launched(few ? launch_after(kv_move_cluster_kernel<D, MOVE, PER, DEEP>, movers, MOVE, RING, st, members, a)
+                      : launch_after(kv_move_kernel<D, 256, 8>, movers, 256, 0, st, 1, a));
 }
 }  // namespace
 
