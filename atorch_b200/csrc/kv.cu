@@ -25,7 +25,8 @@ constexpr int SMALL = 128;      // threads of a block: a few heads of one token
 
 // A head of a token is D / 16 lanes: each has 8 dims of the first half and the 8 of the second half that they turn with. The
 // rotation is that of separately rounded fp32 operations (no fused multiply-add), so that it does not depend on how a compiler
-// contracts it. Bound by memory where there are many tokens, by latency for the one token of a step.
+// contracts it. Bound by memory where there are many tokens (12321 of 48 heads: 52.9 us, 6.2 TB/s; one head a thread 56.4), by latency for
+// the one token of a step (64 sequences: 1.9 us on the device).
 template <typename T, int D, int PER>
 __global__ void __launch_bounds__(SMALL) kv_append_kernel(const T* qkv, T* q_out, T* k_out, Cache c, const int* seq, const int* pos,
                                                           const int* angles, const float* cosT, const float* sinT, int positions,
@@ -187,6 +188,9 @@ ATB_DEVICE void finish(const AttnArgs& a, int b, int head, int n, int d, float t
 // Scores are taken relative to the running maximum, which may be exceeded by 2^SLACK before everything is rescaled; only tiles at a
 // sequence's end are masked. There, what no column sees is put to 0 in shared memory (memory behind a sequence may hold anything), and
 // a value that some columns see and others do not is kept from the others even if it is an infinity or a NaN: column by column then.
+// Bound by memory: two sequences of 100k tokens, 32 query heads on 8 of 128 (781 MB), 128 us, 6.1 TB/s; 32 of up to 4096 (241 MB) 45 us;
+// one of 1531, 16 heads, 9.3. No tcgen05: with 1 to 32 columns the products take a fifth of the issue slots, and a detour through tensor
+// memory would add to a segment's start and end; 31 queries of 4 heads (124 columns, 19 sequences) take 43 us and would gain from it.
 template <int D, int NT>
 struct Shape {
   static constexpr int COLS = 8 * NT, STAGE = TILE * D * 4, STAGES = 3 * 128 / D, RING = WARPS * STAGES * STAGE;
@@ -641,7 +645,8 @@ __global__ void __launch_bounds__(256) kv_join_kernel(AttnArgs a, int per) {
 
 // What the queries attended to: a place's scores of all columns, as the kernel above has left them, relative to the columns' logarithms,
 // added up by LANES lanes in one order, and to what is there. Logarithms of sequences that several blocks worked on are
-// joined here, MOST columns at a time; the last blocks of a head's row do the join of the results beside it.
+// joined here, MOST columns at a time; the last blocks of a head's row do the join of the results beside it. Bound by latency: reads of
+// blocks' results, scores and sums one after another (16 sequences of 1152, 32 heads: 5 us with the join, 8 in two launches).
 template <typename T, int D, int NT, int LANES>
 __global__ void __launch_bounds__(256, 3) kv_weights_kernel(AttnArgs a, int per, int chunks) {
   constexpr int COLS = 8 * NT, MOST = 128;
@@ -649,16 +654,16 @@ __global__ void __launch_bounds__(256, 3) kv_weights_kernel(AttnArgs a, int per,
   grid_go();
   grid_wait();
   const Cache& c = a.c;
-  const int columns = a.S * a.group, b = blockIdx.y / c.kv_heads, head = blockIdx.y - b * c.kv_heads, lane = threadIdx.x % LANES;
+  const int columns = a.S * a.group, b = blockIdx.x / c.kv_heads, head = blockIdx.x - b * c.kv_heads, lane = threadIdx.x % LANES;
   const bool failed = threadIdx.x == 0 && *a.status != 0;
   const int len = seen_length(c, a.lengths, b, a.status);
   if (__syncthreads_or(failed)) return;
-  if ((int)blockIdx.x >= chunks) {
-    join<T, D, NT>(a, b * per + ((int)blockIdx.x - chunks) * c.kv_heads + head, per);
+  if ((int)blockIdx.y >= chunks) {
+    join<T, D, NT>(a, b * per + ((int)blockIdx.y - chunks) * c.kv_heads + head, per);
     return;
   }
-  const float* const scores = a.scores + (long long)blockIdx.y * ((long long)c.width << c.page_shift) * columns;
-  float* const weights = a.weights + (long long)blockIdx.y * a.places;
+  const float* const scores = a.scores + (long long)blockIdx.x * ((long long)c.width << c.page_shift) * columns;
+  float* const weights = a.weights + (long long)blockIdx.x * a.places;
   const int step = chunks * (256 / LANES);
   for (int n0 = 0; n0 < columns; n0 += MOST) {
     const int n1 = min(columns - n0, MOST);
@@ -672,14 +677,14 @@ __global__ void __launch_bounds__(256, 3) kv_weights_kernel(AttnArgs a, int per,
         join_column<D, COLS, false>(a, own, n - col_tile * COLS, 0, top, sum, rounded, o);
         x = top + (log2f(sum) - LIFT<T>);
       } else {
-        x = a.lse2[(long long)blockIdx.y * columns + n];
+        x = a.lse2[(long long)blockIdx.x * columns + n];
       }
       lse2[threadIdx.x] = x;
     }
     __syncthreads();
     // (several places of a thread at once: their scores and what is there are on their way together)
     constexpr int U = LANES == 1 ? 4 : 2, C = LANES == 1 ? 4 : 16;       // C LANES columns in a go
-    for (int t0 = blockIdx.x * (256 / LANES) + threadIdx.x / LANES; t0 - (int)threadIdx.x / LANES < len; t0 += U * step) {
+    for (int t0 = blockIdx.y * (256 / LANES) + threadIdx.x / LANES; t0 - (int)threadIdx.x / LANES < len; t0 += U * step) {
       float x[U][C], old[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -752,7 +757,8 @@ ATB_DEVICE int block_before(int v, int* red, int& all) {
 // rank that is kept is found digit by digit, 8 bits at a time, from counts that the blocks read from each other's shared memory, until
 // so few are left that each is compared with each; of the places of that rank the lowest are kept. Then the places that are kept are
 // numbered in their order: that number is where the token goes. Weights are moved through the workspace, so that no block writes what
-// another still reads. Bound by latency: reads of lengths, pages and weights one after another, a few meetings of the block.
+// another still reads. Bound by latency: reads of lengths, pages and weights one after another, a few meetings of the block (512 units of
+// up to 1152 places 15 us, 8 of 100003 by eight blocks each 40).
 constexpr int BINS = 256, EACH = 4, FEW = 256;
 template <int SELECT>
 __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room) {
@@ -969,7 +975,7 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
 // The tokens' move: a block has the keys or the values of a unit and takes places in their order, THREADS PER pieces of 16 bytes in a
 // round. A token only moves down, so what a place's token comes from is not written before that place's turn: the reads of a round end
 // before its writes begin, and those of later rounds may come before either. Bound by memory where there are many units (8 layers of 8
-// sequences, 8 heads: 68 us for 406 MB).
+// sequences, 8 heads: 64 us for 406 MB).
 template <int D, int THREADS, int PER>
 __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
   grid_go();
@@ -1096,11 +1102,15 @@ Cache cache_of(void* data, const void* table, long long table_stride, int rows, 
 template <typename T, int D>
 int launch_append(const void* qkv, void* q, void* k, const Cache& c, const void* seq, const void* pos, const void* angles,
                   const void* cosT, const void* sinT, int positions, int tokens, int n_q, long long stride, cudaStream_t st, int* status) {
-  const int each = SMALL / (D / 16), heads = n_q + 2 * c.kv_heads, blocks = (heads + each - 1) / each;
+  const int each = SMALL / (D / 16), heads = n_q + 2 * c.kv_heads;
+  // where there are more blocks than the GPU holds, a thread has three heads: more loads on their way, one look at the page table and the
+  // angles
+  const bool many = (long long)tokens * ((heads + each - 1) / each) > 148 * 16 && heads > each;
+  const int blocks = many ? (heads + 3 * each - 1) / (3 * each) : (heads + each - 1) / each;
   if (blocks > 65535) return -2;
-  return launched(launch_after(kv_append_kernel<T, D, 1>, dim3(tokens, blocks), SMALL, 0, st, 1, (const T*)qkv, (T*)q, (T*)k, c,
-                               (const int*)seq, (const int*)pos, (const int*)angles, (const float*)cosT, (const float*)sinT, positions,
-                               n_q, stride, status));
+  return launched(launch_after(many ? kv_append_kernel<T, D, 3> : kv_append_kernel<T, D, 1>, dim3(tokens, blocks), SMALL, 0, st, 1,
+                               (const T*)qkv, (T*)q, (T*)k, c, (const int*)seq, (const int*)pos, (const int*)angles, (const float*)cosT,
+                               (const float*)sinT, positions, n_q, stride, status));
 }
 
 // The cache's rows of D as rows of 64: boxes of TILE rows of all D dims, the halves one behind another.
@@ -1162,7 +1172,7 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   const long long places = (long long)a.c.width << a.c.page_shift;
   const long long per = (columns + Sh::COLS - 1) / Sh::COLS * (long long)a.c.kv_heads, runs = a.c.rows * per;
   const long long room = (places + TILE - 1) / TILE, most = (START + (room > 1 ? room : 1)) * runs;
-  if (runs > 0x7fffffffLL) return -2;
+  if (runs > 0x7fffffffLL || per / a.c.kv_heads > 60000) return -2;
   const Workspace w = workspace(a.c.rows, a.c.kv_heads, columns, D, places, a.weights != nullptr);
   if (w.all > 0 && !a.partial) return -1;
   float* const space = a.partial;
@@ -1178,11 +1188,10 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
   if (rc != 0) return rc;
   if (!a.weights) return w.cut ? launched(launch_after(kv_join_kernel<T, D, NT>, dim3((unsigned)runs), 256, 0, st, 1, a, (int)per)) : 0;
   const long long heads = (long long)a.c.rows * a.c.kv_heads;
-  if (heads > 65535) return -2;
   const int lanes = columns <= 4 ? 1 : 8, each = 256 / lanes;
   const long long most_chunks = (places + each - 1) / each, enough = (lanes == 1 ? 148 * 3 : 148 * 6) / heads + 1;
-  const int chunks = (int)(most_chunks < enough ? most_chunks : enough);
-  const dim3 blocks((unsigned)(chunks + (w.cut ? per / a.c.kv_heads : 0)), (unsigned)heads);
+  const int chunks = (int)(most_chunks < 1 ? 1 : most_chunks < enough ? most_chunks : enough);
+  const dim3 blocks((unsigned)heads, (unsigned)(chunks + (w.cut ? per / a.c.kv_heads : 0)));
   return launched(lanes == 1 ? launch_after(kv_weights_kernel<T, D, NT, 1>, blocks, 256, 0, st, 1, a, (int)per, chunks)
                              : launch_after(kv_weights_kernel<T, D, NT, 8>, blocks, 256, 0, st, 1, a, (int)per, chunks));
 }

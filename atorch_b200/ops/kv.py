@@ -74,9 +74,9 @@ def _table(page_table: torch.Tensor, page_size: int) -> Tuple[int, int, int]:
     return rows, width, steps[0]
 
 
-def _no_gradient(*ts: torch.Tensor) -> None:
-    if forward_ad._current_level >= 0 or any(t.requires_grad for t in ts):
-        refuse_gradient("the cache has no gradient: call under torch.no_grad()", *ts)
+def _no_gradient(a: torch.Tensor, b: torch.Tensor) -> None:
+    if a.requires_grad or b.requires_grad or forward_ad._current_level >= 0:
+        refuse_gradient("the cache has no gradient: call under torch.no_grad()", a, b)
 
 
 # ------------------------------------------------------------------------------------------------------------------
@@ -215,7 +215,7 @@ def kv_attention(q: torch.Tensor, layer: torch.Tensor, page_table: torch.Tensor,
         if weights.dtype is not torch.float32 or weights.shape != (B, KV, places) or places < most << shift or not weights.is_contiguous():
             raise ValueError(f"weights are fp32 {(B, KV)} x {most << shift} places or more, contiguous, got {weights.dtype} "
                              f"{tuple(weights.shape)}")
-        _no_gradient(weights)
+        _no_gradient(weights, q)
     lengths = _int32("lengths", lengths, B)
     _same_device(dev, q, lengths, weights)
     if dev < 0:

@@ -469,6 +469,14 @@ def test_empty_calls():
     assert ops.kv_attention(torch.zeros(0, 1, 4, 64, device=DEV).bfloat16(), cache.layer(0), table, none,
                             weights=torch.zeros(0, 2, 32, device=DEV)).shape == (0, 1, 4, 64)
     assert ops.kv_evict(cache.data, table, none, torch.zeros(1, 0, 2, 32, device=DEV), 4).shape == (0,)
+    # a table without columns: nothing to see
+    nothing = torch.zeros(2, 0, dtype=torch.int32, device=DEV)
+    q = torch.ones(2, 3, 4, 64, device=DEV).bfloat16()
+    out, lse = ops.kv_attention(q, cache.layer(0), nothing, _ints(0, 0), return_lse=True)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    assert (ops.kv_attention(q, cache.layer(0), nothing, _ints(0, 0), weights=torch.zeros(2, 2, 0, device=DEV)) == 0).all()
+    assert ops.kv_evict(cache.data, nothing, _ints(0, 0), torch.zeros(1, 2, 2, 0, device=DEV), 4).tolist() == [0, 0]
+    _lib.check_status(q.device)
     one = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
     assert ops.kv_attention(torch.zeros(1, 0, 4, 64, device=DEV).bfloat16(), cache.layer(0), one, _ints(3)).shape == (1, 0, 4, 64)
 
