@@ -84,7 +84,7 @@ struct Scale {
     const double c64 = endless ? 0. : fmin(1.4426950408889634 / temp, 1e38);
     c = (float)c64;
     c_rest = (float)(c64 - (double)c);
-    cap = 1e36f / fmaxf(c, 1.f);
+    cap = fminf(3.402823466e38f, 1e36f / c);
     least = endless ? 3.402823466e38f : -INFINITY;
   }
   ATB_DEVICE float below(float v) const { return fminf(top - v, cap); }            // (a NaN: cap)
@@ -363,7 +363,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
     return end;
   };
   // logits, and keys, of which no token so many powers of two below the largest has a greater one, or a lesser one
-  auto floor_at = [&](float y) { return top == INFINITY ? INFINITY : scale.c > 0.f ? scale.top - y / scale.c * 1.00001f : -3.402823466e38f; };
+  auto floor_at = [&](float y) { return top == INFINITY ? INFINITY : scale.c > 0.f ? fmaxf(scale.top - y / scale.c * 1.00001f, -3.402823466e38f) : -3.402823466e38f; };
   auto lowest_at = [&](float y) { return key_of(floor_at(y), 0xffffffffu); };
   auto highest_at = [&](float y) { return key_of(scale.c > 0.f ? scale.top - y / scale.c * 0.99999f : scale.top, 0); };
   auto score_of = [&](double w, float t) { return t >= 0.f ? quotient_of(w, (double)t) : 0.; };
@@ -516,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
 #pragma unroll 2
       for (int i = threadIdx.x; i < own && by_weight; i += THREADS) {
         const float v = __int_as_float(list[i].x), y = scale.power(v);
-        off += scale.weight<T>(v, y) - (double)(y < NOTHING ? scale.rough(v, y) : 0.f);
+        if (y < NOTHING) off += scale.weight<T>(v, y) - (double)scale.rough(v, y);
       }
       off = block_sum(off, red_d);
       if (threadIdx.x == 0) sh.inside = off;

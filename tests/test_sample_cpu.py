@@ -32,7 +32,7 @@ def draw(x, wait, T, k, p, m):
     return token, math.log(w[token] / math.fsum(w[i] for i in left))
 
 
-FILTERS = [dict(), dict(temperature=0.4), dict(temperature=3.0), dict(temperature=math.inf), dict(top_k=1), dict(top_k=7), dict(top_k=5000), dict(top_p=0.9), dict(top_p=1e-9),
+FILTERS = [dict(), dict(temperature=0.4), dict(temperature=3.0), dict(temperature=math.inf), dict(temperature=1e38), dict(temperature=1e38, top_k=9, top_p=0.8), dict(temperature=1e-30, top_p=0.5), dict(top_k=1), dict(top_k=7), dict(top_k=5000), dict(top_p=0.9), dict(top_p=1e-9),
            dict(top_p=0.0), dict(min_p=0.1), dict(min_p=1.0), dict(top_k=20, top_p=0.7, min_p=0.02, temperature=0.8), dict(temperature=0.0),
            dict(top_k=50, top_p=0.999, temperature=1.3)]
 
