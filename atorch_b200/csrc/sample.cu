@@ -117,13 +117,25 @@ struct Scale {
   ATB_DEVICE double exact(float v) const { return !(v > least) ? 0. : top == INFINITY ? 1. : exp_of(((double)v - (double)top) * per_temp); }
 };
 
-// What the blocks of a cluster read from each other
+// What the blocks of a cluster read from each other. A field that others read behind a meeting is written again only behind the next one:
+//   top, count, weight      written once
+//   first                   set to V before the first meeting, lowered behind it, read behind a second, for a temperature of 0 alone
+//   sum                     before the meeting behind the first look, the one behind a sum of what top_k has left (or all, in the whole
+//                           shares), the last one: the meeting of the lists, or those of an end_of_prefix, lie between a reading and the next
+//   inside                  before the meeting of the lists; in the whole shares before that of a bin, which is followed by another
+//   above, low, high, least_above, in_bin      before the meeting of a bin, which is followed by another
+//   listed                  before the meeting of the lists, and not again: nothing meets between its readers and the first look of the
+//                           whole shares
+//   few_listed, few, cut    end_of_prefix, whose readings end with a meeting (the first block's `few` is read by itself)
+//   best_score, best_at     set before the first meeting, changed by the block's own threads, read behind the last one
+// The lists and the parts, in the place of the bins, are read before a meeting that ends their use, too.
 struct Shared {
   float top;
-  int first;                                     // lowest index of the largest logit, for a temperature of 0
+  int first;                                     // lowest index of the largest logit
   double sum;                                    // of the weights that this block has
   double above, inside;                          // of those above the bin at hand, and in it
   unsigned long long low, high, least_above;     // keys of the bin at hand, and the least above it
+  int in_bin;                                    // tokens in it
   unsigned count[BINS], weight[BINS];            // tokens of a bin, their weights in units of 2^-14 of the bin's largest
   int listed, few_listed;
   unsigned long long few[FEW], cut;
@@ -637,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
           sh.inside = inside_own;
           sh.low = sh.least_above = ~0ull;
           sh.high = 0;
-          sh.listed = 0;
+          sh.in_bin = 0;
         }
         __syncthreads();
 #pragma unroll
@@ -651,7 +663,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
           atomicMin(&sh.low, lo);
           atomicMin(&sh.least_above, over);
           atomicMax(&sh.high, hi);
-          atomicAdd(&sh.listed, (int)n_inside);
+          atomicAdd(&sh.in_bin, (int)n_inside);
         }
         cluster.sync();
         const double in = over_blocks(&Shared::inside);
@@ -661,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
         inside = 0;
         for (int i = 0; i < blocks; ++i) {
           const Shared* s = cluster.map_shared_rank(&sh, i);
-          inside += s->listed;
+          inside += s->in_bin;
           low = min(low, s->low);
           high = max(high, s->high);
           least_above = min(least_above, s->least_above);

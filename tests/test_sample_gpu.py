@@ -136,3 +136,28 @@ def test_behind_a_failed_kernel():
 
 def test_refusals():
     check_refusals(DEV)
+
+
+@pytest.mark.parametrize("top_k", [9000, 20000, 30000])
+@pytest.mark.parametrize("B,V", [(1, 32000), (1, 131072), (64, 32000), (64, 131072), (192, 32000)])
+def test_prefixes_longer_than_the_lists(B, V, top_k):
+    """Every block of a row has to take the same way through the whole shares, however far behind the others it is."""
+    g = torch.Generator(device=DEV).manual_seed(V + top_k)
+    x = torch.randn(B, V, generator=g, device=DEV)
+    x[::2] *= 1e-3                                     # nearly flat
+    x[::3] = 0.0
+    for kw in (dict(top_k=top_k), dict(top_k=top_k, top_p=0.7)):
+        for dtype in (torch.float32, torch.bfloat16):
+            logits = x.to(dtype)
+            first = None
+            for repeat in range(12):
+                wait = torch.empty(B, V, device=DEV).exponential_(generator=g)
+                got = ops.sample(logits, wait, **kw)
+                if repeat < 2:
+                    want = ops.sample_reference(logits, wait, **kw)
+                    assert torch.equal(got[0], want[0]) and torch.allclose(got[1], want[1], rtol=2 ** -23, atol=2 ** -20)
+                else:
+                    first = first or (wait, got)
+                    again = ops.sample(logits, first[0], **kw)
+                    assert torch.equal(again[0], first[1][0]) and torch.equal(again[1], first[1][1])
+    _lib.check_status(x.device)
