@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
   auto floor_at = [&](float y) { return top == INFINITY ? INFINITY : scale.c > 0.f ? fmaxf(scale.top - y / scale.c * 1.00001f, -3.402823466e38f) : -3.402823466e38f; };
   auto lowest_at = [&](float y) { return key_of(floor_at(y), 0xffffffffu); };
   auto highest_at = [&](float y) { return key_of(scale.c > 0.f ? scale.top - y / scale.c * 0.99999f : scale.top, 0); };
-  auto score_of = [&](double w, float t) { return t >= 0.f ? quotient_of(w, (double)t) : 0.; };
+  auto score_of = [&](double w, float t) { return t >= 0.f ? quotient_of(w, (double)fabsf(t)) : 0.; };       // (-0 is no time, as 0 is)
   // of the block's threads' tokens the one with the largest score, the lowest of equal ones
   auto best_of_block = [&](double score, int token) {
     if (score >= 0.) atomicMax(&sh.best_score, (unsigned long long)__double_as_longlong(score));
@@ -571,7 +571,8 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
         best_of_block(drawn ? score_of(w, t) : -1., drawn ? (int)index_of(key) : a.V);
         if (threadIdx.x == 0) {
           const int i = sh.best_at;
-          answer(i, log(scale.exact(to_f32<T>(x[i])) / all));
+          if (i < a.V) answer(i, log(scale.exact(to_f32<T>(x[i])) / all));
+          else answer(0, -INFINITY);
         }
       }
       cluster.sync();                            // the first has read the others' lists

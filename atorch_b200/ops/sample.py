@@ -40,7 +40,7 @@ def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p
     left = left & (~(p < 1) | (sums - sorted_w < p * sums[:, -1:]) | (at == 0))
     w = torch.zeros_like(w).scatter(1, order, torch.where(left, sorted_w, torch.zeros_like(w)))
     wait = waiting.double()
-    wait = torch.where(wait >= 0, wait, torch.full_like(wait, math.inf))
+    wait = torch.where(wait >= 0, wait.abs(), torch.full_like(wait, math.inf))          # (-0 is no time, as 0 is)
     score = torch.where(w > 0, w / wait, torch.full_like(w, -1.0))
     first = torch.where(score == score.amax(-1, keepdim=True), at, torch.full_like(at, V)).amin(-1)
     logprobs = torch.log(w.gather(1, first[:, None])[:, 0] / w.sum(-1))

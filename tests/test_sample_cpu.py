@@ -85,6 +85,33 @@ def test_waiting_times_of_zero_infinity_and_nan():
     assert tokens.tolist() == [1, 0, 2, 0, 3] and torch.allclose(logprobs, torch.full((5,), -math.log(4)))
 
 
+def unusual_waits(V, g):
+    """Waiting times at which a draw can go wrong, a row of each kind."""
+    wait = torch.empty(11, V).exponential_(generator=g)
+    odd = torch.tensor([0.0, -0.0, math.inf, float("nan"), -1.0, -math.inf])
+    for i in range(6):
+        wait[i] = odd[i]
+    wait[6] = torch.where(torch.rand(V, generator=g) < 0.5, odd[0], odd[1])
+    wait[7] = odd[torch.randint(0, 6, (V,), generator=g)]
+    wait[8] = odd[torch.randint(2, 6, (V,), generator=g)]
+    wait[9, V // 3] = -0.0
+    mixed = torch.rand(V, generator=g) < 0.5
+    wait[10, mixed] = odd[torch.randint(1, 6, (int(mixed.sum()),), generator=g)]
+    return wait
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=1), dict(top_k=5), dict(top_p=0.5), dict(top_p=0.0), dict(min_p=0.2), dict(temperature=0.0)])
+@pytest.mark.parametrize("V", [1, 3, 200])
+def test_unusual_waiting_times(V, kw):
+    g = torch.Generator().manual_seed(V)
+    check(torch.randn(11, V, generator=g) * 2, unusual_waits(V, g), **kw)
+
+
+def test_a_waiting_time_of_minus_zero():
+    tokens, logprobs = check(torch.tensor([[5.0, 1.0, 0.0]]), torch.tensor([[-0.0, 1.0, 1.0]]), top_k=1)
+    assert tokens.tolist() == [0] and logprobs.tolist() == [0.0]
+
+
 def test_parameters_of_rows():
     g = torch.Generator().manual_seed(3)
     x, wait = torch.randn(6, 300, generator=g) * 2, torch.empty(6, 300).exponential_(generator=g)

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from atorch_b200 import _lib, ops
-from test_sample_cpu import FILTERS, check, check_refusals, draw, special_rows
+from test_sample_cpu import FILTERS, check, check_refusals, draw, special_rows, unusual_waits
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -161,3 +161,23 @@ def test_prefixes_longer_than_the_lists(B, V, top_k):
                     again = ops.sample(logits, first[0], **kw)
                     assert torch.equal(again[0], first[1][0]) and torch.equal(again[1], first[1][1])
     _lib.check_status(x.device)
+
+
+@pytest.mark.parametrize("kw", [dict(), dict(top_k=1), dict(top_k=5), dict(top_p=0.5), dict(top_p=0.0), dict(top_p=0.95), dict(top_k=3000), dict(top_k=5000, top_p=0.9),
+                                dict(min_p=0.01), dict(temperature=0.0)])
+@pytest.mark.parametrize("V", [1, 3, 200, 9001])
+def test_unusual_waiting_times(V, kw):
+    """Prefixes put in order, listed, and drawn from without filters."""
+    g = torch.Generator().manual_seed(V)
+    for dtype in (torch.float32, torch.bfloat16):
+        check((torch.randn(11, V, generator=g) * 2).to(dtype), unusual_waits(V, g), DEV, **kw)
+        if V == 9001:
+            check((torch.randn(11, V, generator=g) * 0.01).to(dtype), unusual_waits(V, g), DEV, **kw)
+    _lib.check_status(torch.device("cuda", 0))
+
+
+def test_unusual_waiting_times_behind_a_prefix_too_long_to_list():
+    V, g = 40000, torch.Generator().manual_seed(1)
+    for b in range(11):
+        check(torch.randn(1, V, generator=g) * 0.01, unusual_waits(V, g)[b: b + 1], DEV, top_k=39000)
+    _lib.check_status(torch.device("cuda", 0))
