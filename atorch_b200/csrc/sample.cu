@@ -97,8 +97,9 @@ struct Scale {
   }
   // The same off by 2^-30: 2^-y = 2^(-n / 32) 2^-r with n / 32 the nearest to y; the rest, with what the difference and the product were
   // rounded by, is in 32 bits off by 2^-30, and 2^-r - 1 four terms of its series, below 0.011. Where a prefix ends is decided by these: a
-  // token at the end of one of thousands weighs 1e-5 of it, and sums of rough weights, off by 1e-8, moved the end in one row of a
-  // thousand. (All tokens' weights in 64 bits took 10 us for the look at 192 rows of 32000, these 8, the rough ones 4.)
+  // token at the end of one of thousands weighs 1e-5 of it, and a total of rough weights added up in 32 bits, off by 5e-8, moved the end
+  // in one or two rows of a thousand. (All tokens' weights in 64 bits took 10 us for the look at 192 rows of 32000, these 8, the rough
+  // ones 4.)
   template <typename T>
   ATB_DEVICE double weight(float v, float y) const {
     const float d = below(v);
@@ -120,10 +121,9 @@ struct Scale {
 // What the blocks of a cluster read from each other. A field that others read behind a meeting is written again only behind the next one:
 //   top, count, weight      written once
 //   first                   set to V before the first meeting, lowered behind it, read behind a second, for a temperature of 0 alone
-//   sum                     before the meeting behind the first look, the one behind a sum of what top_k has left (or all, in the whole
-//                           shares), the last one: the meeting of the lists, or those of an end_of_prefix, lie between a reading and the next
-//   inside                  before the meeting of the lists; in the whole shares before that of a bin, which is followed by another
-//   above, low, high, least_above, in_bin      before the meeting of a bin, which is followed by another
+//   sum                     before the meeting behind the first look, the one behind a sum of what top_k has left, the last one: the meeting of
+//                           the lists, or those of an end_of_prefix, lie between a reading and the next
+//   above, inside, low, high, least_above, in_bin      before the meeting of a bin, which is followed by another
 //   listed                  before the meeting of the lists, and not again: nothing meets between its readers and the first look of the
 //                           whole shares
 //   few_listed, few, cut    end_of_prefix, whose readings end with a meeting (the first block's `few` is read by itself)
@@ -310,7 +310,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
         atomicAdd(parts + s, 1u);
         if (count) return;
         const float v = value_of(key);
-        const unsigned long long q = (unsigned long long)(scale.weight<T>(v, scale.power(v)) * per);
+        const unsigned long long q = __double2ull_rn(scale.weight<T>(v, scale.power(v)) * per);
         atomicAdd(parts + 1 * SUB + s, (unsigned)q & 0xffffu);
         atomicAdd(parts + 2 * SUB + s, (unsigned)(q >> 16) & 0xffffu);
         atomicAdd(parts + 3 * SUB + s, (unsigned)(q >> 32));
@@ -448,21 +448,28 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
   bool in_lists = false;                         // every block has its tokens that may be left in its list, so many
   int listed = 0;
   if (k > 0 || by_weight) {
-    // one look at the row: tokens and weights of the bins, and all weights, roughly; a token without weight does not count
+    // One look at the row: tokens and weights of the bins, roughly, and with top-p the sum of all weights, which says where the prefix ends
+    // as much as the sums in front of a token do; a token without weight does not count.
 #pragma unroll
     for (int i = 0; i < BINS; ++i) own_bins[i * THREADS + threadIdx.x] = 0;
-    float rough_sum = 0.f;
+    double weights = 0.;
     each([&](float v, int) {
       const float y = scale.power(v);
       if (!(y < NOTHING)) return;
       const int bin = min((int)y, BINS - 1);
-      const float w = scale.rough(v, y);
-      rough_sum += w;
+      float w;
+      if (by_weight) {
+        const double exact = scale.weight<T>(v, y);
+        weights += exact;
+        w = (float)exact;
+      } else {
+        w = scale.rough(v, y);
+      }
       // (w 2^bin lies in (1/2, 1], in the last bin below; 768 = 1.5 * 2^(23 - 14): adding it leaves the nearest unit in the low bits)
       const unsigned q = __float_as_uint(w * __int_as_float((127 + bin) << 23) + 768.f) - __float_as_uint(768.f);
       own_bins[bin * THREADS + threadIdx.x] += (1u << 22) + q;
     });
-    const double total_own = block_sum((double)rough_sum, red_d);
+    const double total_own = block_sum(weights, red_d);
     if (threadIdx.x == 0) sh.sum = total_own;
     for (int bin = threadIdx.x >> 5; bin < BINS; bin += WARPS) {
       unsigned n = 0, w = 0;
@@ -522,22 +529,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
       each([&](float v, int i) {
         if (v >= floor) list[put++] = make_int2(__float_as_int(v), i);
       });
-      // the listed tokens' part of the row's weight exactly: what is behind them is little
-      __syncthreads();
-      double off = 0.;
-#pragma unroll 2
-      for (int i = threadIdx.x; i < own && by_weight; i += THREADS) {
-        const float v = __int_as_float(list[i].x), y = scale.power(v);
-        if (y < NOTHING) off += scale.weight<T>(v, y) - (double)scale.rough(v, y);
-      }
-      off = block_sum(off, red_d);
-      if (threadIdx.x == 0) sh.inside = off;
     }
     cluster.sync();
     const int theirs = lane < blocks ? cluster.map_shared_rank(&sh, lane)->listed : 0;
     const int n = __reduce_add_sync(0xffffffffu, theirs);
     in_lists = __reduce_max_sync(0xffffffffu, theirs) <= ROOM;
-    if (in_lists) total += over_blocks(&Shared::inside);
     if (n <= FEW) {
       // in their order in the first block, all filters at once
       if (leader) {
@@ -601,11 +597,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
     // Too many to list: the end in the whole shares.
     for (int which = by_count ? 0 : 1; which < (by_weight ? 2 : 1) && !in_lists; ++which) {
       const bool count = which == 0;
-      if (!count) {                              // of what top_k has left, or of all
+      if (!count && by_count) {                  // of what top_k has left
         double s = 0.;
         each([&](float v, int i) {
           const float y = scale.power(v);
-          if (y < NOTHING && (cut == 0 || key_of(v, i) >= cut)) s += scale.weight<T>(v, y);
+          if (y < NOTHING && key_of(v, i) >= cut) s += scale.weight<T>(v, y);
         });
         const double own = block_sum(s, red_d);
         if (threadIdx.x == 0) sh.sum = own;

@@ -181,3 +181,27 @@ def test_unusual_waiting_times_behind_a_prefix_too_long_to_list():
     for b in range(11):
         check(torch.randn(1, V, generator=g) * 0.01, unusual_waits(V, g)[b: b + 1], DEV, top_k=39000)
     _lib.check_status(torch.device("cuda", 0))
+
+
+@pytest.mark.parametrize("top_p", [0.3, 0.9, 0.95])
+@pytest.mark.parametrize("B,V,spread,dtype", [(192, 32000, 2.5, torch.float32), (192, 32000, 2.5, torch.bfloat16), (512, 12001, 2.5, torch.float32),
+                                              (40, 131072, 2.5, torch.float32), (150, 32000, 0.7, torch.float32)])
+def test_the_end_of_a_nucleus(B, V, spread, dtype, top_p):
+    """Thousands of unlike weights (with little spread too many to list): the end of the prefix is that of sums in 64 bits. A token next
+    to it weighs 1e-5 of what is left, ten times what a logarithm may be off by; in every other batch the last token that is left arrives
+    first, but for the one behind it."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    for batch in range(10):
+        x = torch.randn(B, V, generator=g, device=DEV) * spread
+        x += (9.0 if spread > 1 else 0.0) * (torch.rand(B, V, generator=g, device=DEV) < 8 / V)
+        x = x.to(dtype)
+        wait = torch.empty(B, V, device=DEV).exponential_(generator=g)
+        if batch % 2:
+            w, order = torch.softmax(x.double(), -1).sort(dim=-1, descending=True, stable=True)
+            last = ((w.cumsum(-1) - w) < top_p).sum(-1, keepdim=True) - 1
+            wait.scatter_(1, order.gather(1, last), 1e-12)
+            wait.scatter_(1, order.gather(1, last + 1), 1e-18)
+        got, want = ops.sample(x, wait, top_p=top_p), ops.sample_reference(x, wait, top_p=top_p)
+        other = int((got[0] != want[0]).sum())
+        far = int(((got[1] - want[1]).abs() > 2 ** -20 + 2 ** -23 * want[1].abs()).sum())
+        assert other == 0 and far == 0, (batch, other, far)
