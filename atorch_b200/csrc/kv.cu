@@ -718,13 +718,16 @@ struct EvictArgs {
   const int* lengths;
   float* weights;
   int* out;
-  int* first;                 // [units] the first place whose token changes, `budget` where none does
+  int* first;                 // [units] the first place whose token changes, `budget` where none does, WRONG where nothing may
   int* source;                // [units][budget] place in the pool (page, slot) of the token that a place takes
   float* kept;                // [units][budget] its weight
   long long places, layer_elements;
   int budget, recent, layers;
   int* status;
 };
+// A sequence that is longer than its row of the page table, or whose pages are not all there, is left as it is. That is found by the
+// selection, and recorded by the move: within a launch nobody changes the status word that says whether to begin.
+constexpr int WRONG = -1;
 // A number whose order as an unsigned integer is that of f; both zeros alike, a NaN as -inf.
 ATB_DEVICE uint32_t rank_of(float f) {
   const uint32_t u = __float_as_uint((f != f ? -INFINITY : f) + 0.f);
@@ -778,11 +781,11 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
     else cluster.sync();
   };
   const int before = threadIdx.x == 0 ? *a.status : 0;       // on its way beside the lengths
-  const int len = seen_length(c, a.lengths, b, a.status), lane = threadIdx.x & 31;
-  const bool leader = rank == 0 && threadIdx.x == 0;
-  if (leader && unit < (long long)c.rows * c.kv_heads && unit % c.kv_heads == 0) a.out[b] = min(a.lengths[b], a.budget);
-  if (len <= a.budget) {
-    if (leader) a.first[unit] = a.budget;
+  const int len = a.lengths[b], lane = threadIdx.x & 31;
+  const bool leader = rank == 0 && threadIdx.x == 0, too_long = len > c.width << c.page_shift;
+  if (leader && unit < (long long)c.rows * c.kv_heads && unit % c.kv_heads == 0) a.out[b] = too_long ? len : min(len, a.budget);
+  if (len <= a.budget || too_long) {
+    if (leader) a.first[unit] = too_long ? WRONG : a.budget;
     return;
   }
   const int part = (((len + blocks - 1) / blocks + 3) & ~3), from = min(len, rank * part), to = min(len, from + part);
@@ -794,20 +797,17 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   for (int i = (from >> c.page_shift) + threadIdx.x; i << c.page_shift < to; i += SELECT) bad = bad || page_of(c, b, i << c.page_shift) < 0;
   if (threadIdx.x == 0) {
     sh_least = len;
-    sh_failed = before;
+    sh_failed = before != 0;
     sh_n = 0;
   }
   bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0 && bad) {
-    atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
-    sh_failed = 1;
-  }
+  if (threadIdx.x == 0 && bad) sh_failed |= 2;
   auto weight = [&](int i) { return i - from < held ? sh_w[i - from] : w[i]; };
 
   const int n = len - a.recent, mine = min(to, n);      // those from n on stay
   int left = a.budget - a.recent;            // of rank `least`, so many are kept
   uint32_t least = left == 0 ? 0xffffffffu : 0u;
-  bool failed = false;
+  int failed = 0;
   int shift = 32;                            // digits above this are known
 #pragma unroll 1
   for (int pass = 0; shift > 0; ++pass) {
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
     }
     meet();
     if (pass == 0)
-      for (int i = 0; i < blocks; ++i) failed = failed || *cluster.map_shared_rank(&sh_failed, i) != 0;
+      for (int i = 0; i < blocks; ++i) failed |= *cluster.map_shared_rank(&sh_failed, i);
     if (pass == 1 && threadIdx.x < BINS) hist[0][threadIdx.x] = 0;       // the first digit's counts have been read by all
     if (left > 0 && !failed) {
       // from the highest bin down: one of a thread
@@ -962,7 +962,7 @@ __global__ void __launch_bounds__(SELECT) kv_select_kernel(EvictArgs a, int room
   if (leader) {
     int first = len;
     for (int i = 0; i < blocks; ++i) first = min(first, *cluster.map_shared_rank(&sh_least, i));
-    a.first[unit] = failed ? a.budget : min(first, a.budget);
+    a.first[unit] = failed & 2 ? WRONG : failed ? a.budget : min(first, a.budget);
   }
   if (!failed) {
     const float* const kept = a.kept + unit * a.budget;
@@ -984,7 +984,8 @@ __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
   const int which = blockIdx.x & 1;
   const long long unit = blockIdx.x / 2;
   const int first = a.first[unit];
-  if (first >= a.budget) return;           // (also of a unit that could not be selected from; its weights stay, too)
+  if (first == WRONG && threadIdx.x == 0) atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+  if (first == WRONG || first >= a.budget) return;
   const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
   constexpr int LANES = D / 8, ROWS = THREADS / LANES, STEP = ROWS * PER;
   uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + threadIdx.x % LANES;
@@ -1041,7 +1042,8 @@ __global__ void __launch_bounds__(THREADS) kv_move_cluster_kernel(EvictArgs a) {
   const int blocks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), which = blockIdx.x / blocks & 1;
   const long long unit = blockIdx.x / blocks / 2;
   const int first = a.first[unit];
-  if (first >= a.budget) return;
+  if (first == WRONG && threadIdx.x == 0) atomicCAS(a.status, 0, (int)ATB_ERR_BAD_INDEX);
+  if (first == WRONG || first >= a.budget) return;
   const int head = (int)(unit % c.kv_heads), b = (int)(unit / c.kv_heads % c.rows), mask = (1 << c.page_shift) - 1;
   constexpr int LANES = D / 8, ROWS = THREADS / LANES;
   uint4* const data = reinterpret_cast<uint4*>((__half*)c.data + unit / c.kv_heads / c.rows * a.layer_elements) + threadIdx.x % LANES;
@@ -1092,6 +1094,17 @@ __global__ void __launch_bounds__(THREADS) kv_move_cluster_kernel(EvictArgs a) {
     far = ask(j0 + (DEEP + 2) * step);
     stage = stage + 1 == DEEP ? 0 : stage + 1;
     cluster.barrier_wait();
+  }
+}
+
+// A budget that no sequence can be over: the lengths as they are.
+__global__ void __launch_bounds__(256) kv_lengths_kernel(EvictArgs a) {
+  grid_go();
+  grid_wait();
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b < a.c.rows) {
+    seen_length(a.c, a.lengths, b, a.status);
+    a.out[b] = a.lengths[b];
   }
 }
 
@@ -1199,6 +1212,7 @@ int launch_attention(AttnArgs a, cudaStream_t st) {
 template <int D>
 int launch_evict(const EvictArgs& a, cudaStream_t st) {
   const long long units = (long long)a.layers * a.c.rows * a.c.kv_heads, places = (long long)a.c.width << a.c.page_shift;
+  if (a.budget >= places) return launched(launch_after(kv_lengths_kernel, dim3((unsigned)(a.c.rows + 255) / 256), 256, 0, st, 1, a));
   // few units: a cluster of large blocks for each, where its blocks have 2048 places each
   const bool few = units < 148;
   int blocks = 1;

@@ -269,7 +269,8 @@ def kv_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tenso
     ``recent`` last tokens stay, and of those before them the ``budget - recent`` with the largest ``weights`` (what
     :func:`kv_attention` added up; equal ones go to the lower place, a NaN counts as ``-inf``). They move down into the places
     ``0 ... budget - 1`` in their order, keys, values and weights; the weights of the places behind become 0, their keys and values are
-    left as they are. Sequences within the budget are not touched.
+    left as they are. Sequences within the budget are not touched, nor are those that are longer than their row of the page table or
+    have a page that is not there, which are recorded; the others of the call are cut all the same.
 
     ``cache`` ``[layers, pages, 2, kv_heads, page_size, head_dim]`` (a :class:`KVCache`'s ``data``) with ``weights`` fp32
     ``[layers, sequences, kv_heads, places]``, or one layer of both; ``lengths`` ``[sequences]``. Returns the new lengths, int32. No page
@@ -296,12 +297,13 @@ def kv_evict(cache: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tenso
     _same_device(dev, lengths, weights)
     if dev < 0:
         return kv_evict_reference(cache, page_table, lengths, weights, budget, recent)
-    out = torch.empty_like(lengths)
-    if budget >= most << shift:              # no row of the page table has so many places
-        return out.copy_(lengths)
-    # per layer, sequence and head: the first place that changes, where the tokens come from, their weights
-    work = torch.empty(layers * rows * KV * (2 * budget + 1), dtype=torch.int32, device=lengths.device)
-    rc = _lib.lib().atb_kv_evict(at, table, lengths.data_ptr(), weights.data_ptr(), out.data_ptr(), work.data_ptr(), layers, KV, D, shift,
+    out, work = torch.empty_like(lengths), None
+    if budget >= most << shift:              # no row of the page table has so many places: lengths are looked at, no more
+        budget, recent = most << shift, 0
+    else:
+        # per layer, sequence and head: the first place that changes, where the tokens come from, their weights
+        work = torch.empty(layers * rows * KV * (2 * budget + 1), dtype=torch.int32, device=lengths.device)
+    rc = _lib.lib().atb_kv_evict(at, table, lengths.data_ptr(), weights.data_ptr(), out.data_ptr(), _lib.addr(work), layers, KV, D, shift,
                                  pages, rows, most, stride, places, budget, recent, _lib.stream_of(dev), _lib.status_addr(weights))
     _lib.check(rc, "atb_kv_evict")
     return out

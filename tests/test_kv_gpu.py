@@ -489,3 +489,39 @@ def test_refusals():
     table, q = torch.zeros(1, 2, dtype=torch.int32, device=DEV), torch.zeros(1, 1, 4, 96, device=DEV).bfloat16()
     with pytest.raises(ValueError):
         ops.kv_attention(q, odd.layer(0), table, _ints(1))
+
+
+@pytest.mark.parametrize("layers,KV,width,long", [(1, 2, 4, 65), (3, 40, 4, 1000), (1, 1, 300, 4801), (1, 2, 300, 1 << 30)])
+@pytest.mark.parametrize("wrong", ["length", "page"])
+def test_a_cut_leaves_what_is_out_of_range(layers, KV, width, long, wrong):
+    """A sequence longer than its row, whose pages are all there, or with a page that is not: it stays, whole, and the others are cut."""
+    D, page = 64, 16
+    lengths = [width * page, long if wrong == "length" else width * page, width * page - 3, 20]
+    table = _table(4, width, 4 * width)
+    cache = _filled(layers, 4 * width, page, KV, D, torch.bfloat16)
+    weights = torch.rand(layers, 4, KV, width * page, generator=_gen(1), device=DEV)
+    if wrong == "page":
+        table[1, width - 1] = 4 * width
+    data, kept = cache.data.clone(), weights.clone()
+    got = ops.kv_evict(cache.data, table, _ints(*lengths), weights, 30, 5)
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status(table.device)
+    rest = _ints(0, 2, 3).long()
+    kept_rest = kept[:, rest].contiguous()
+    want = ops.kv_evict_reference(data, table[rest], _ints(*(lengths[b] for b in (0, 2, 3))), kept_rest, 30, 5)
+    assert torch.equal(got[rest], want) and (wrong == "page" or int(got[1]) == long)
+    assert torch.equal(weights[:, rest], kept_rest) and torch.equal(weights[:, 1], kept[:, 1])
+    assert torch.equal(cache.data, data)
+
+
+def test_lengths_out_of_range_under_a_budget_that_no_sequence_is_over():
+    cache = _filled(1, 4, 16, 2, 64, torch.bfloat16)
+    table, weights = _table(2, 2, 4), torch.rand(1, 2, 2, 32, device=DEV)
+    before = cache.data.clone(), weights.clone()
+    for budget in (32, 33, 1 << 40):
+        assert ops.kv_evict(cache.data, table, _ints(32, 5), weights, budget, 3).tolist() == [32, 5]
+        _lib.check_status(table.device)
+        ops.kv_evict(cache.data, table, _ints(5, 33), weights, budget, 3)
+        with pytest.raises(_lib.KernelError):
+            _lib.check_status(table.device)
+    assert torch.equal(cache.data, before[0]) and torch.equal(weights, before[1])
