@@ -27,6 +27,9 @@ from .function import refuse_gradient
 from .kv4 import HEAD_DIMS, _aligned, _check_page_size, _int32, _places, _same_device
 
 DTYPES = (torch.bfloat16, torch.float16)
+# Scores that attention with weights keeps at a time (256 MB). 64 prompts of 8192 tokens, 32 last tokens each, 32 heads (2 GB of scores) took
+# 2947 us at once, 3117 with 1 GB, 3291 with 256 MB and 4397 with 64; 64 of 2048 with 32 heads on 8 (512 MB) 612, 649 with 256, 814 with 64.
+SCORES = 1 << 26
 
 
 class KVCache:
@@ -189,6 +192,26 @@ def _scratch(*sizes: int) -> int:
     return fn(*sizes)
 
 
+def _in_pieces(q, layer, page_table, lengths, softmax_scale, return_lse, weights, each):
+    """Attention with weights whose scores (`each` of a token) are too many at once: some sequences after another, or some tokens of one."""
+    B, S = q.shape[:2]
+    got = []
+    if B > 1:
+        n = max(1, SCORES // (S * each))
+        for b in range(0, B, n):
+            got.append(kv_attention(q[b: b + n], layer, page_table[b: b + n], lengths[b: b + n], softmax_scale, return_lse, weights[b: b + n]))
+    else:
+        n = max(1, SCORES // each)
+        for i in range(0, S, n):
+            behind = max(0, S - i - n)          # tokens that these do not see
+            got.append(kv_attention(q[:, i: i + n], layer, page_table, lengths.clamp(min=0) - behind if behind else lengths, softmax_scale,
+                                    return_lse, weights))
+    along = 0 if B > 1 else 1
+    if not return_lse:
+        return torch.cat(got, along)
+    return torch.cat([out for out, _ in got], along), torch.cat([lse for _, lse in got], 2 * along)
+
+
 def kv_attention(q: torch.Tensor, layer: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
                  softmax_scale: Optional[float] = None, return_lse: bool = False, weights: Optional[torch.Tensor] = None):
     """Attention of the newest tokens over the cache. ``q`` ``[sequences, S, n_q, head_dim]``, in the cache's type, are the queries of the
@@ -199,7 +222,9 @@ def kv_attention(q: torch.Tensor, layer: torch.Tensor, page_table: torch.Tensor,
 
     ``weights`` (fp32 ``[sequences, kv_heads, places]``, contiguous, as many places as a row of the page table has or more) takes up what
     the queries attended to, in place: the softmax weights of the ``S`` tokens and of the heads that share a key/value head are added to
-    it. :func:`kv_evict` goes by them."""
+    it. :func:`kv_evict` goes by them. For them the call keeps a score of 4 bytes for every sequence, query, query head and place of a row of
+    the page table, 256 MB of them at a time (or those of one token of one sequence): above that it goes through sequences, then
+    tokens, in pieces."""
     at, table, pages, KV, shift, rows, most, stride, D, dev = _cache(layer, page_table)
     if q.dim() != 4 or q.shape[3] != D or q.shape[2] % KV or q.shape[2] == 0:
         raise ValueError(f"q {tuple(q.shape)}: [sequences, S, a multiple of {KV}, {D}] is wanted")
@@ -221,6 +246,8 @@ def kv_attention(q: torch.Tensor, layer: torch.Tensor, page_table: torch.Tensor,
     if dev < 0:
         out, lse = kv_attention_reference(q, layer, page_table, lengths, softmax_scale, weights)
         return (out, lse) if return_lse else out
+    if weights is not None and (S > 1 or B > 1) and B * S * H * (most << shift) > SCORES:
+        return _in_pieces(q, layer, page_table, lengths, softmax_scale, return_lse, weights, H * (most << shift))
     q_batch, q_token, q_head, one = q.stride()
     if one != 1 or q_head != D or (q.data_ptr() | 2 * q_batch | 2 * q_token) & 15:
         q = q.clone(memory_format=torch.contiguous_format)

@@ -525,3 +525,48 @@ def test_lengths_out_of_range_under_a_budget_that_no_sequence_is_over():
         with pytest.raises(_lib.KernelError):
             _lib.check_status(table.device)
     assert torch.equal(cache.data, before[0]) and torch.equal(weights, before[1])
+
+
+@pytest.mark.parametrize("room", [1, 4000, 20000, 1 << 20])
+def test_attention_with_weights_in_pieces(room, monkeypatch):
+    """Scores that are too many at once: pieces of sequences, and of the tokens of one, down to one token."""
+    monkeypatch.setattr(ops.kv, "SCORES", room)
+    D, KV, page, S = 64, 2, 16, 9
+    lengths = [0, 1, 5, 9, 10, 300, 77]
+    layer = _filled(1, 7 * 19, page, KV, D, torch.bfloat16).layer(0)
+    table = _table(7, 19, 7 * 19)
+    _poison(layer, table, lengths)
+    q = (torch.randn(7, S, 6, D, generator=_gen(1), device=DEV) * 1.5).bfloat16()
+    before = torch.rand(7, KV, 19 * page + 3, generator=_gen(2), device=DEV)
+    weights = before.clone()
+    out, lse = ops.kv_attention(q, layer, table, _ints(*lengths), return_lse=True, weights=weights)
+    want, tol, want_lse, sums, sums_tol = _exact(q, layer, table, lengths, D ** -0.5)
+    assert out.shape == q.shape and lse.shape == (7, 6, S) and ((out.double() - want).abs() <= tol).all()
+    seen = want_lse > -math.inf
+    assert torch.equal(seen, lse > -math.inf) and ((lse.double() - want_lse).abs()[seen] <= 1e-4).all()
+    # one rounding for every call that adds to a place
+    grown = weights.double()[..., : 19 * page] - before.double()[..., : 19 * page]
+    assert ((grown - sums).abs() <= sums_tol + 2.0 ** -24 * (2 + S + S * 3) * (before[..., : 19 * page].double() + sums)).all()
+    for b, n in enumerate(lengths):
+        assert torch.equal(weights[b, :, n:], before[b, :, n:])
+    _lib.check_status(q.device)
+    # a length out of range is reported from any of them
+    ops.kv_attention(q, layer, table.clamp(min=0), _ints(0, 1, 5, 9, 19 * page + 1, 300, 77), weights=weights)
+    with pytest.raises(_lib.KernelError):
+        _lib.check_status(q.device)
+
+
+def test_the_workspace_of_weights_is_bounded():
+    """16 prompts of up to 32768 tokens, 32 query heads, 32 last tokens each: 2.1 GB of scores."""
+    B, S, H, KV, D, page = 16, 32, 32, 8, 64, 64
+    layer = _filled(1, 64, page, KV, D, torch.bfloat16).layer(0)
+    table = torch.zeros(B, 512, dtype=torch.int32, device=DEV) + torch.arange(512, device=DEV, dtype=torch.int32) % 64
+    lengths = _ints(32768, *range(1, 16))
+    q = torch.randn(B, S, H, D, generator=_gen(1), device=DEV).bfloat16()
+    weights = torch.zeros(B, KV, 32768, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    ops.kv_attention(q, layer, table, lengths, weights=weights)
+    assert torch.cuda.max_memory_allocated() - held < 320 << 20
+    _lib.check_status(q.device)
