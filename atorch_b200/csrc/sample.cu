@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
 
   // Every block draws from its share.
   if (unfiltered) {
-    // the block's own largest logit says what weights are relative to; for a logarithm their sum in 32 bits does
+    // the block's own largest logit says what weights are relative to; for a logarithm rough weights do, a piece's added up in 32 bits
     const bool wide = (reinterpret_cast<uintptr_t>(wait + body) & 15) == 0;
     const float bend = -0.69314718f * scale.c_rest;
     float weights = 0.f;
@@ -725,9 +725,11 @@ __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
       }
 #pragma unroll
       for (int e = 0; e < N; ++e) one(v[e], t[e], i + e);
+      sum += (double)weights;
+      weights = 0.f;
     }
     each_odd([&](float v, int i) { one(v, wait[i], i); });
-    sum = weights;
+    sum += (double)weights;
   } else if (in_lists) {
     constexpr int EACH = ROOM / THREADS;
     float t[EACH];
@@ -811,9 +813,10 @@ int launch(const Args& a, int rows, cudaStream_t st) {
   const bool filtered = a.k_rows || a.p_rows || a.m_rows || a.k > 0 || a.p < 1. || a.m > 0.;
   int blocks = 1;
   while (blocks < 8 && (long long)rows * blocks * 2 <= (filtered ? 3 : 2) * 148 && a.V > N * blocks) blocks *= 2;
-  // a thread's bins have room for the weights of 255 tokens, a block's parts for those of 65536
+  // a thread's bins have room for the weights of 255 tokens, a block's parts for those of 65536; they serve top-k and top-p
   while (blocks < 8 && a.V > blocks * 128 * THREADS) blocks *= 2;
-  if (a.V > 8 * 128 * THREADS || (long long)rows * blocks > 0x7fffffffLL) return -2;
+  const bool binned = a.k_rows || a.p_rows || a.k > 0 || a.p < 1.;
+  if (a.V > (binned ? 8 * 128 * THREADS : 1 << 30) || (long long)rows * blocks > 0x7fffffffLL) return -2;
   const int part = ((a.V + blocks - 1) / blocks + 7) / 8 * 8, bytes = (part + 8) * (int)sizeof(T), room = bytes <= MOST ? bytes : 0;
   return launched(launch_after(sample_kernel<T>, dim3((unsigned)(rows * blocks)), THREADS, BINS_BYTES + room, st, blocks, a, room / 16));
 }

@@ -13,7 +13,8 @@ from .. import _lib
 from .function import refuse_gradient
 
 Number = Union[float, int, torch.Tensor]
-MOST = 1 << 19          # tokens of a vocabulary that the kernel takes
+# tokens of a vocabulary that the kernel takes with top-k or top-p (its counts have room for so many), and without
+MOST, LARGEST = 1 << 19, 1 << 30
 
 
 def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
@@ -32,13 +33,16 @@ def sample_reference(logits, waiting, temperature=1.0, top_k=0, top_p=1.0, min_p
     w = torch.where((x > -math.inf) & (below > -math.inf), torch.exp(below / T), torch.zeros_like(x))
     at = torch.arange(V, device=x.device).expand_as(x)
     w = torch.where(T > 0, w, ((at == best) & (top > -math.inf)).double())
-    order = x.sort(dim=-1, descending=True, stable=True).indices
-    sorted_w = w.gather(1, order)
-    left = ~(sorted_w < m)
-    sorted_w = torch.where((k > 0) & (at >= k), torch.zeros_like(w), sorted_w)
-    sums = sorted_w.cumsum(-1)
-    left = left & (~(p < 1) | (sums - sorted_w < p * sums[:, -1:]) | (at == 0))
-    w = torch.zeros_like(w).scatter(1, order, torch.where(left, sorted_w, torch.zeros_like(w)))
+    if not bool(((k > 0) | (p < 1)).any()):                                # min-p alone needs no order
+        w = torch.where(w < m, torch.zeros_like(w), w)
+    else:
+        order = x.sort(dim=-1, descending=True, stable=True).indices
+        sorted_w = w.gather(1, order)
+        left = ~(sorted_w < m)
+        sorted_w = torch.where((k > 0) & (at >= k), torch.zeros_like(w), sorted_w)
+        sums = sorted_w.cumsum(-1)
+        left = left & (~(p < 1) | (sums - sorted_w < p * sums[:, -1:]) | (at == 0))
+        w = torch.zeros_like(w).scatter(1, order, torch.where(left, sorted_w, torch.zeros_like(w)))
     wait = waiting.double()
     wait = torch.where(wait >= 0, wait.abs(), torch.full_like(wait, math.inf))          # (-0 is no time, as 0 is)
     score = torch.where(w > 0, w / wait, torch.full_like(w, -1.0))
@@ -75,7 +79,7 @@ def _bits(v: float) -> int:
 def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.0, top_k: Number = 0, top_p: Number = 1.0,
            min_p: Number = 0.0) -> Tuple[torch.Tensor, torch.Tensor]:
     """A token of every row of ``logits`` ``[B, V]`` (bf16, fp16 or fp32) and the logarithm of the probability that it was drawn with:
-    int64 and fp32 ``[B]``.
+    int64 and fp32 ``[B]``. With ``top_k`` or ``top_p`` a vocabulary has 2 ** 19 tokens at most.
 
     A token's weight is ``exp((logit - largest logit) / temperature)``; tokens are ordered by weight, equal ones by index. ``top_k`` leaves
     that many first ones (0: all), ``top_p`` of what these weigh together the first ones whose predecessors weigh less than that
@@ -94,8 +98,8 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
     if logits.dim() != 2 or logits.dtype not in _lib.DT or logits.shape[1] == 0:
         raise ValueError(f"logits are bf16, fp16 or fp32 [B, vocabulary], got {logits.dtype} {tuple(logits.shape)}")
     B, V = logits.shape
-    if V > MOST:
-        raise ValueError(f"a vocabulary of {V}: 2 ** 19 at most")
+    if V > LARGEST:
+        raise ValueError(f"a vocabulary of {V}: 2 ** 30 at most")
     if waiting.dtype is not torch.float32 or waiting.shape != (B, V):
         raise ValueError(f"waiting is fp32 {(B, V)}, got {waiting.dtype} {tuple(waiting.shape)}")
     dev = logits.get_device()
@@ -105,6 +109,8 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
     k_rows, k = _number("top_k", top_k, B, dev, True, 0, float(1 << 62))
     p_rows, p = _number("top_p", top_p, B, dev, False, 0.0, 1.0)
     m_rows, m = _number("min_p", min_p, B, dev, False, 0.0, 1.0)
+    if V > MOST and (k_rows is not None or p_rows is not None or k > 0 or p < 1):
+        raise ValueError(f"a vocabulary of {V}: 2 ** 19 at most with top_k or top_p")
     if logits.requires_grad or waiting.requires_grad or forward_ad._current_level >= 0:
         refuse_gradient("a draw has no gradient: call under torch.no_grad()", logits, waiting)
     if dev < 0 or not _lib.use_kernels(logits):

@@ -168,3 +168,23 @@ def check_refusals(dev):
 
 def test_refusals():
     check_refusals("cpu")
+
+
+def test_vocabularies_that_the_filters_do_not_take():
+    V, g = (1 << 19) + 5, torch.Generator().manual_seed(1)
+    x, wait = torch.randn(2, V, generator=g), torch.empty(2, V).exponential_(generator=g)
+    for kw in (dict(), dict(temperature=torch.tensor([0.5, 0.0])), dict(min_p=0.3)):
+        check(x, wait, **kw)
+    whole, row = torch.zeros(2, dtype=torch.int32), torch.ones(2)
+    for kw in (dict(top_k=3), dict(top_p=0.5), dict(top_k=whole), dict(top_p=row)):
+        with pytest.raises(ValueError, match="vocabulary"):
+            ops.sample(x, wait, **kw)
+
+
+def test_drawing_without_an_order_sorts_nothing(monkeypatch):
+    monkeypatch.setattr(torch.Tensor, "sort", None)
+    x, wait = torch.randn(3, 50), torch.empty(3, 50).exponential_()
+    for kw in (dict(), dict(temperature=0.3), dict(min_p=0.1), dict(top_p=torch.ones(3), top_k=torch.zeros(3, dtype=torch.int32))):
+        tokens, _ = ops.sample(x, wait, **kw)
+        want = [draw(a, b, kw.get("temperature", 1.0), 0, 1.0, kw.get("min_p", 0.0))[0] for a, b in zip(x.double().tolist(), wait.double().tolist())]
+        assert tokens.tolist() == want

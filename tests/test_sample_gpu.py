@@ -205,3 +205,15 @@ def test_the_end_of_a_nucleus(B, V, spread, dtype, top_p):
         other = int((got[0] != want[0]).sum())
         far = int(((got[1] - want[1]).abs() > 2 ** -20 + 2 ** -23 * want[1].abs()).sum())
         assert other == 0 and far == 0, (batch, other, far)
+
+
+@pytest.mark.parametrize("B,V,dtype", [(2, (1 << 19) + 5, torch.float32), (1, 5000011, torch.bfloat16), (40, 700001, torch.float16)])
+def test_vocabularies_that_the_filters_do_not_take(B, V, dtype):
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x, wait = (torch.randn(B, V, generator=g, device=DEV) * 2).to(dtype), torch.empty(B, V, device=DEV).exponential_(generator=g)
+    for kw in (dict(), dict(temperature=0.0), dict(min_p=0.05), dict(temperature=torch.full((B,), 0.7, device=DEV))):
+        got, want = ops.sample(x, wait, **kw), ops.sample_reference(x, wait, **kw)
+        assert torch.equal(got[0], want[0]) and torch.allclose(got[1], want[1], rtol=2 ** -23, atol=2 ** -20)
+    with pytest.raises(ValueError, match="vocabulary"):
+        ops.sample(x, wait, top_p=0.5)
+    _lib.check_status(x.device)
