@@ -570,3 +570,25 @@ def test_the_workspace_of_weights_is_bounded():
     ops.kv_attention(q, layer, table, lengths, weights=weights)
     assert torch.cuda.max_memory_allocated() - held < 320 << 20
     _lib.check_status(q.device)
+
+
+@pytest.mark.parametrize("KV,n,budget", [(8, 30011, 15000), (1, 50021, 49000), (18, 9000, 8990)])
+def test_rounds_of_a_cluster_again_and_again(KV, n, budget):
+    """Blocks of a cluster write what others have read a round before: the same tokens every time, with other work beside."""
+    D, page = 128, 64
+    width = -(-n // page)
+    cache, table = _filled(1, width, page, KV, D, torch.bfloat16), _table(1, width, width)
+    weights = torch.randn(1, 1, KV, width * page, generator=_gen(3), device=DEV).exp()
+    data, sums = cache.data.clone(), weights.clone()
+    ops.kv_evict_reference(data, table, _ints(n), sums, budget, 7)
+    filled, kept, beside = cache.data.clone(), weights.clone(), torch.cuda.Stream()
+    for _ in range(15):
+        cache.data.copy_(filled)
+        weights.copy_(kept)
+        beside.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(beside):
+            filled.clone()
+        ops.kv_evict(cache.data, table, _ints(n), weights, budget, 7)
+        assert torch.equal(cache.data, data) and torch.equal(weights, sums)
+    torch.cuda.current_stream().wait_stream(beside)
+    _lib.check_status(table.device)
