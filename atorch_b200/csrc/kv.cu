@@ -1030,7 +1030,7 @@ __global__ void __launch_bounds__(THREADS) kv_move_kernel(EvictArgs a) {
 
 // The same for few units: the blocks of a cluster share the rows of a round. DEEP rounds are on their way in shared memory, and the blocks
 // say that they have their part of the next round before they write this one, so that nobody waits for the meeting. 50000 tokens of 8
-// heads (410 MB): 100 us, bound by the rounds' latency; meetings that wait, one round ahead, took 163, a slab of the rows' 32 bytes for
+// heads (410 MB): 112 us, bound by the rounds' latency; meetings that wait, one round ahead, took 163, a slab of the rows' 32 bytes for
 // every block, which need not meet, 108, for its many small requests.
 template <int D, int THREADS, int PER, int DEEP>
 __global__ void __launch_bounds__(THREADS) kv_move_cluster_kernel(EvictArgs a) {

@@ -154,10 +154,12 @@ struct Shared {
 // part with the end again, until a few tokens are left, which are put in order and added up. Weights that several threads add up are whole
 // numbers (2^-46 of the largest of the range), others are summed in one order, so the result does not depend on which thread comes
 // first. A draw is decided in 64 bits: 32-bit arrival times only say which tokens have to be looked at.
-// Bound by instructions, of which the first look takes 24 a token, where there are many rows (192 of 32000 with top-p 54.7 us on the
-// device, 64 of 100003 without filters 16.2): looks after it only compare a logit, and lists make what follows dense (a look that works on
-// every tenth token costs a warp as much as one that works on all). One row is bound by the cluster's meetings (32000, top-k and top-p:
-// 12.2 us).
+// Bound by latency: what a block does one after another. Of 192 rows of 32000 with top-p (62.5 us on the device, 384 blocks in two rounds)
+// a block takes 5.5 us for its logits and the largest, 7.3 for the first look, 2.2 and 1.5 to count and to list, 8.7 to find the end,
+// 3.7 to draw, 1.8 for the exact look, and 5 in the meetings between; looks after the first only compare a logit, and lists make what
+// follows dense (a look that works on every tenth token costs a warp as much as one that works on all). Of 64 rows of 100003 without
+// filters (16.5 us) the two looks one behind the other take 6.0 and 6.3, the exact one 2.1, the last meeting 2.4. One row of 32000 with top-k and
+// top-p (12.2 us) meets four times, 0.7 to 1.1 us each, and takes 2 us for the first look and as much to count.
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 2) sample_kernel(Args a, int room) {
   // [BINS][THREADS]: weights in the low 22 bits, tokens above; then the list (logit, index), and behind it [4][SUB]: tokens of a part, its
@@ -808,8 +810,11 @@ int launch(const Args& a, int rows, cudaStream_t st) {
     allowed.fetch_or(bit, std::memory_order_relaxed);
   }
   // Blocks of a row: as many as have a piece for every thread, as long as the GPU holds all of them at once (two an SM), or, with
-  // filters, half as many more: 192 rows of 32000 with top-p took 54.8 us with two blocks a row, 78.8 with four, and one has no room for
-  // their lists (123); without filters 16.1 with one, 21.9 with two.
+  // filters, half as many more. Rows of 32000 fp32 with top-p 0.9, us with one, two, four and eight blocks: 1 row 34, 26, 23, 26; 32 rows 85,
+  // 29, 30, 37; 64 rows 87, 36, 32, 72; 150 rows 110, 52, 77, 168; 192 rows 127, 66, 92, 208; with top-k 50 besides (bf16) 192 rows 33, 35,
+  // 50, 95. Without filters (bf16) 64 rows 11.8, 13.2, 10.0, 17; 150 rows 18, 23, 27, 42; 64 rows of 100003 (two, four, eight) 26, 21,
+  // 31. The rule takes one block too early where a list has no room in it: 256 rows with top-p 128, with two 77; 192 rows of 100003 two,
+  // 314, with four 174.
   const bool filtered = a.k_rows || a.p_rows || a.m_rows || a.k > 0 || a.p < 1. || a.m > 0.;
   int blocks = 1;
   while (blocks < 8 && (long long)rows * blocks * 2 <= (filtered ? 3 : 2) * 148 && a.V > N * blocks) blocks *= 2;

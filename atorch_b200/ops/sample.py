@@ -81,7 +81,7 @@ def sample(logits: torch.Tensor, waiting: torch.Tensor, temperature: Number = 1.
     """A token of every row of ``logits`` ``[B, V]`` (bf16, fp16 or fp32) and the logarithm of the probability that it was drawn with:
     int64 and fp32 ``[B]``. With ``top_k`` or ``top_p`` a vocabulary has 2 ** 19 tokens at most.
 
-    A token's weight is ``exp((logit - largest logit) / temperature)``; tokens are ordered by weight, equal ones by index. ``top_k`` leaves
+    A token's weight is ``exp((logit - largest logit) / temperature)`` (with a filter, below ``2 ** -1000`` it may count as none); tokens are ordered by weight, equal ones by index. ``top_k`` leaves
     that many first ones (0: all), ``top_p`` of what these weigh together the first ones whose predecessors weigh less than that
     share, ``min_p`` those of at least that weight, which the first always has. ``waiting`` (fp32 ``[B, V]``, exponentially distributed:
     ``torch.empty(...).exponential_()``) are the random numbers: the token is the first to arrive, that with the largest
